@@ -309,6 +309,79 @@ int mlstm_b200_step_sequence(const void* q, const void* k, const void* v, const 
                              int B, int NH, int T, int DHQK, int DHHV, int dtype, int gate_dtype, float eps,
                              void* stream);
 
+/* ---- the operators around a recurrence -------------------------------------------------------------------------
+ * Layer norm, the short causal convolution and the selective state space scan of a recurrent layer.  The reference
+ * has no counterparts (its layers take them from other packages).  Unlike above, tensors need only be aligned to
+ * their element type, and those that come with strides (host arrays, in elements) may lie anywhere as long as their
+ * last axis is contiguous; workspaces and checkpoints are 16-byte aligned.  Sums, statistics and states are f32.
+ */
+
+/*
+ * Layer norm over the last axis: y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps).
+ *   x (n0,n1,NH,D) at x_strides[3] (of n0, n1, NH); y (n0,n1,NH,D) contiguous; dtype
+ *   weight, bias (NH,D) param_dtype, each may be NULL (ones, zeros).  D <= 16384
+ *   mean, rstd (n0*n1*NH) f32 out, for the backward; both or neither NULL
+ * Backward: dy and dx as x, at strides of their own; dw, db (NH,D) param_dtype out, each may be NULL (workspace is
+ * needed where one is not).  Sums over rows are taken in a fixed order.
+ */
+size_t mlstm_b200_layer_norm_bw_workspace_bytes(long long rows, int NH, int D);   /* rows = n0 * n1 */
+int mlstm_b200_layer_norm_fw(const void* x, const long long* x_strides, const void* weight, const void* bias, void* y,
+                             float* mean, float* rstd, long long n0, long long n1, int NH, int D, int dtype,
+                             int param_dtype, float eps, void* stream);
+int mlstm_b200_layer_norm_bw(const void* x, const long long* x_strides, const void* weight, const float* mean,
+                             const float* rstd, const void* dy, const long long* dy_strides, void* dx,
+                             const long long* dx_strides, void* dw, void* db, void* workspace, size_t workspace_bytes,
+                             long long n0, long long n1, int NH, int D, int dtype, int param_dtype, void* stream);
+
+/*
+ * Causal convolution of every channel with its own W taps (2 to 4), the last of them on the token itself:
+ *   u_t = bias + sum_j weight[j] x_{t-W+1+j};  y = u, or u sigmoid(u) with silu != 0
+ *   x (B,S,D) at x_strides[2] (of B, S); weight (D,W), bias (D) or NULL, w_dtype; y (B,S,D) dtype out
+ *   x_initial (B,W-1,D) dtype: the tokens before the first, NULL = zeros; x_last the same for a call that goes on, or NULL
+ * Backward: dy at dy_strides[2]; dx_last (B,W-1,D) or NULL; dx (B,S,D) out; dx_initial, dw (D,W), db (D) out, each may be
+ * NULL (workspace is needed where dw or db is not).
+ * Step: one token, x and y (B,D); state, state_new (B,W-1,D) are x_initial and x_last (may be the same memory).
+ */
+size_t mlstm_b200_short_conv_bw_workspace_bytes(int B, int S, int D, int W);
+int mlstm_b200_short_conv_fw(const void* x, const long long* x_strides, const void* x_initial, const void* weight,
+                             const void* bias, void* y, void* x_last, int B, int S, int D, int W, int silu, int dtype,
+                             int w_dtype, void* stream);
+int mlstm_b200_short_conv_bw(const void* x, const long long* x_strides, const void* x_initial, const void* weight,
+                             const void* bias, const void* dy, const long long* dy_strides, const void* dx_last, void* dx,
+                             void* dx_initial, void* dw, void* db, void* workspace, size_t workspace_bytes, int B, int S,
+                             int D, int W, int silu, int dtype, int w_dtype, void* stream);
+int mlstm_b200_short_conv_step(const void* x, const void* state, const void* weight, const void* bias, void* y,
+                               void* state_new, int B, int D, int W, int silu, int dtype, int w_dtype, void* stream);
+
+/*
+ * Selective state space scan: every channel has N states (1 to 128) of its own,
+ *   step_t = softplus(dt_t + dt_bias) with softplus != 0, else dt_t + dt_bias
+ *   h_t[n] = exp(step_t a[n]) h_{t-1}[n] + step_t x_t b_t[n];  y_t = (sum_n c_t[n] h_t[n] + skip x_t) z_t sigmoid(z_t)
+ *   x, dt, z (B,S,D), b, c (B,S,G,N) dtype, group g for the channels g D/G ... (g+1) D/G - 1; z NULL = no gate
+ *   strides[12]: x (B, S), dt (B, S), z (B, S), b (B, S, G), c (B, S, G)
+ *   a (D,N), skip (D), dt_bias (D), h_initial (B,D,N) f32; skip, dt_bias, h_initial may be NULL (zeros)
+ *   y (B,S,D) dtype out; h_last (B,D,N) f32 out or NULL
+ *   checkpoints: mlstm_b200_ssm_checkpoint_bytes(), what the backward needs of the forward, or NULL
+ * Backward: dy at dy_strides[2], dh_last (B,D,N) f32 or NULL; dx, ddt, dz (B,S,D), db, dc (B,S,G,N) contiguous, dtype, out
+ * (dz NULL without z); da (D,N) f32 out; dskip, ddt_bias (D), dh_initial (B,D,N) f32 out, each may be NULL.
+ * Step: one token, x, dt, z, y (B,D), b, c (B,G,N) contiguous; h_new may be h.
+ * workspace: mlstm_b200_ssm_workspace_bytes() for the forward (backward = 0; may be none) and the backward (1).
+ */
+size_t mlstm_b200_ssm_checkpoint_bytes(int B, int S, int D, int N);
+size_t mlstm_b200_ssm_workspace_bytes(int B, int S, int D, int N, int G, int backward);
+int mlstm_b200_ssm_scan_fw(const void* x, const void* dt, const float* a, const void* b, const void* c, const float* skip,
+                           const void* z, const float* dt_bias, const float* h_initial, const long long* strides, void* y,
+                           float* h_last, void* checkpoints, void* workspace, size_t workspace_bytes, int B, int S, int D,
+                           int N, int G, int softplus, int dtype, void* stream);
+int mlstm_b200_ssm_scan_bw(const void* x, const void* dt, const float* a, const void* b, const void* c, const float* skip,
+                           const void* z, const float* dt_bias, const long long* strides, const void* checkpoints,
+                           const void* dy, const long long* dy_strides, const float* dh_last, void* dx, void* ddt, float* da,
+                           void* db, void* dc, float* dskip, void* dz, float* ddt_bias, float* dh_initial, void* workspace,
+                           size_t workspace_bytes, int B, int S, int D, int N, int G, int softplus, int dtype, void* stream);
+int mlstm_b200_ssm_step(const void* x, const void* dt, const float* a, const void* b, const void* c, const float* skip,
+                        const void* z, const float* dt_bias, const float* h, void* y, float* h_new, int B, int D, int N, int G,
+                        int softplus, int dtype, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

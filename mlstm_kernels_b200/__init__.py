@@ -1,6 +1,7 @@
 """B200-native (sm_100a) kernels for the mLSTM hot path: chunkwise forward / backward for the
 exponential and sigmoid input gate, and the recurrent decode step, behind the PyTorch-facing
-interface of NX-AI/mlstm_kernels.  All compute runs in hand-written CUDA loaded from
+interface of NX-AI/mlstm_kernels, and the operators around such a recurrence (layer norm, short
+causal convolution, selective state space scan).  All compute runs in hand-written CUDA loaded from
 libmlstm_b200.so through its C ABI (include/mlstm_b200.h); there is no CPU or PyTorch fallback."""
 
 from .chunkwise import (
@@ -13,6 +14,13 @@ from .chunkwise import (
     mlstm_siging_chunkwise__b200_xl_chunk,
     select_chunk_size,
     tcgen05_applies,
+)
+from .layers import (
+    layer_norm__b200,
+    short_conv__b200,
+    short_conv_step__b200,
+    ssm_scan__b200,
+    ssm_step__b200,
 )
 from .recurrent import (
     mlstm_recurrent_sequence__b200,
@@ -27,6 +35,11 @@ __all__ = [
     "mlstm_recurrent_step__b200",
     "mlstm_recurrent_step__b200_fw",
     "mlstm_recurrent_sequence__b200",
+    "layer_norm__b200",
+    "short_conv__b200",
+    "short_conv_step__b200",
+    "ssm_scan__b200",
+    "ssm_step__b200",
     "chunkwise_fw_raw",
     "chunkwise_bw_raw",
     "chunkwise_states_raw",

@@ -21,6 +21,7 @@ _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _CODE_DTYPE = {v: k for k, v in _DTYPE_CODE.items()}
 
 _vp, _fp, _i, _f, _sz = C.c_void_p, C.c_void_p, C.c_int, C.c_float, C.c_size_t
+_ll, _llp = C.c_longlong, C.POINTER(C.c_longlong)
 
 # name -> (restype, argtypes); must list every symbol declared in include/mlstm_b200.h
 SIGNATURES = {
@@ -57,6 +58,19 @@ SIGNATURES = {
     "mlstm_b200_chunkwise_dc_summary": (_i, [_vp, _vp, _fp, _vp, _sz, _fp, _vp, _sz] + [_i] * 6 + [_i, _i, _i, _f, _vp]),
     "mlstm_b200_step": (_i, [_vp] * 12 + [_i] * 7 + [_f, _vp]),
     "mlstm_b200_step_sequence": (_i, [_vp] * 12 + [_i] * 7 + [_f, _vp]),
+    "mlstm_b200_layer_norm_bw_workspace_bytes": (_sz, [_ll, _i, _i]),
+    "mlstm_b200_layer_norm_fw": (_i, [_vp, _llp, _vp, _vp, _vp, _fp, _fp, _ll, _ll, _i, _i, _i, _i, _f, _vp]),
+    "mlstm_b200_layer_norm_bw": (_i, [_vp, _llp, _vp, _fp, _fp, _vp, _llp, _vp, _llp, _vp, _vp, _vp, _sz, _ll, _ll, _i, _i,
+                                      _i, _i, _vp]),
+    "mlstm_b200_short_conv_bw_workspace_bytes": (_sz, [_i] * 4),
+    "mlstm_b200_short_conv_fw": (_i, [_vp, _llp] + [_vp] * 5 + [_i] * 7 + [_vp]),
+    "mlstm_b200_short_conv_bw": (_i, [_vp, _llp] + [_vp] * 4 + [_llp] + [_vp] * 6 + [_sz] + [_i] * 7 + [_vp]),
+    "mlstm_b200_short_conv_step": (_i, [_vp] * 6 + [_i] * 6 + [_vp]),
+    "mlstm_b200_ssm_checkpoint_bytes": (_sz, [_i] * 4),
+    "mlstm_b200_ssm_workspace_bytes": (_sz, [_i] * 6),
+    "mlstm_b200_ssm_scan_fw": (_i, [_vp] * 9 + [_llp] + [_vp] * 4 + [_sz] + [_i] * 7 + [_vp]),
+    "mlstm_b200_ssm_scan_bw": (_i, [_vp] * 8 + [_llp, _vp, _vp, _llp] + [_vp] * 11 + [_sz] + [_i] * 7 + [_vp]),
+    "mlstm_b200_ssm_step": (_i, [_vp] * 11 + [_i] * 6 + [_vp]),
 }
 
 _lib = None

@@ -170,3 +170,164 @@ def _(q, k, v, i, f, c_initial, n_initial, m_initial, eps):
     DHHV = v.shape[-1]
     return (torch.empty_like(v, memory_format=torch.contiguous_format), q.new_empty((B, NH, DHQK, DHHV), dtype=_F32),
             q.new_empty((B, NH, DHQK), dtype=_F32), q.new_empty((B, NH, 1), dtype=_F32))
+
+
+# ---- the operators around a recurrence ----------------------------------------------------------------------------
+# (their checks of arguments are the native host module's, made when an operator runs)
+def _contig(t: Tensor) -> Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("mlstm_b200::layer_norm", mutates_args=(), device_types="cuda")
+def layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    """(y, mean, rstd)"""
+    return _lib.host().layer_norm_fw(x, weight, bias, eps)
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps):
+    rows = 1
+    for n in x.shape[:-1]:
+        rows = rows * n
+    return _contig(x), x.new_empty((rows,), dtype=_F32), x.new_empty((rows,), dtype=_F32)
+
+
+@torch.library.custom_op("mlstm_b200::layer_norm_bw", mutates_args=(), device_types="cuda")
+def layer_norm_bw(x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, dy: Tensor, heads: bool,
+                  param_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    dx, dw, db = _lib.host().layer_norm_bw(x, weight, mean, rstd, dy, heads, param_dtype, True, True)
+    return dx.contiguous(), dw, db
+
+
+@layer_norm_bw.register_fake
+def _(x, weight, mean, rstd, dy, heads, param_dtype):
+    p = x.new_empty(x.shape[-2:] if heads else x.shape[-1:], dtype=param_dtype)
+    return _contig(x), p, torch.empty_like(p)
+
+
+def _norm_setup_context(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    p = weight if weight is not None else bias
+    ctx.save_for_backward(x, weight, output[1], output[2])
+    ctx.cfg = (p is not None and p.dim() == 2, _F32 if p is None else p.dtype, weight is not None, bias is not None)
+
+
+def _norm_backward(ctx, dy, _dmean, _drstd):
+    x, weight, mean, rstd = ctx.saved_tensors
+    heads, pdt, has_w, has_b = ctx.cfg
+    dx, dw, db = layer_norm_bw(x, weight, mean, rstd, dy, heads, pdt)
+    return dx, dw if has_w else None, db if has_b else None, None
+
+
+torch.library.register_autograd("mlstm_b200::layer_norm", _norm_backward, setup_context=_norm_setup_context)
+
+
+@torch.library.custom_op("mlstm_b200::short_conv", mutates_args=(), device_types="cuda")
+def short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], x_initial: Optional[Tensor], want_last: bool, silu: bool
+               ) -> tuple[Tensor, Tensor]:
+    y, last = _lib.host().short_conv(x, weight, bias, x_initial, want_last, silu)
+    return y, last if want_last else x.new_empty((0,))
+
+
+@short_conv.register_fake
+def _(x, weight, bias, x_initial, want_last, silu):
+    return _contig(x), x.new_empty((x.shape[0], weight.shape[1] - 1, x.shape[2]) if want_last else (0,))
+
+
+@torch.library.custom_op("mlstm_b200::short_conv_bw", mutates_args=(), device_types="cuda")
+def short_conv_bw(x: Tensor, weight: Tensor, bias: Optional[Tensor], x_initial: Optional[Tensor], dy: Optional[Tensor],
+                  dlast: Optional[Tensor], silu: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    dx, dw, db, d0 = _lib.host().short_conv_bw(x, weight, bias, x_initial, dy, dlast, silu, True, bias is not None,
+                                               x_initial is not None)
+    none = x.new_empty((0,))
+    return dx, dw, none if db is None else db, none.clone() if d0 is None else d0
+
+
+@short_conv_bw.register_fake
+def _(x, weight, bias, x_initial, dy, dlast, silu):
+    return (_contig(x), _contig(weight), x.new_empty((0,)) if bias is None else _contig(bias),
+            x.new_empty((0,)) if x_initial is None else _contig(x_initial))
+
+
+def _conv_setup_context(ctx, inputs, output):
+    x, weight, bias, x_initial, want_last, silu = inputs
+    ctx.save_for_backward(x, weight, bias, x_initial)
+    ctx.cfg = (want_last, silu)
+
+
+def _conv_backward(ctx, dy, dlast):
+    x, weight, bias, x_initial = ctx.saved_tensors
+    want_last, silu = ctx.cfg
+    dx, dw, db, d0 = short_conv_bw(x, weight, bias, x_initial, dy, dlast if want_last else None, silu)
+    return dx, dw, None if bias is None else db, None if x_initial is None else d0, None, None
+
+
+torch.library.register_autograd("mlstm_b200::short_conv", _conv_backward, setup_context=_conv_setup_context)
+
+
+@torch.library.custom_op("mlstm_b200::short_conv_step", mutates_args=(), device_types="cuda")
+def short_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool) -> tuple[Tensor, Tensor]:
+    return _lib.host().short_conv_step(x, state, weight, bias, silu, None)
+
+
+@short_conv_step.register_fake
+def _(x, state, weight, bias, silu):
+    return _contig(x), _contig(state)
+
+
+@torch.library.custom_op("mlstm_b200::ssm_scan", mutates_args=(), device_types="cuda")
+def ssm_scan(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, skip: Optional[Tensor], z: Optional[Tensor],
+             dt_bias: Optional[Tensor], softplus: bool, h_initial: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
+    """(y, h_last, checkpoints)"""
+    return _lib.host().ssm_scan_fw(x, dt, a, b, c, skip, z, dt_bias, h_initial, softplus)
+
+
+@ssm_scan.register_fake
+def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial):
+    B, S, D = x.shape
+    N = a.shape[1]
+    n = _lib.load().mlstm_b200_ssm_checkpoint_bytes(B, S, D, N)
+    return _contig(x), x.new_empty((B, D, N), dtype=_F32), x.new_empty((max(n, 256),), dtype=torch.uint8)
+
+
+@torch.library.custom_op("mlstm_b200::ssm_scan_bw", mutates_args=(), device_types="cuda")
+def ssm_scan_bw(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, skip: Optional[Tensor], z: Optional[Tensor],
+                dt_bias: Optional[Tensor], softplus: bool, h_initial: Optional[Tensor], checkpoints: Tensor,
+                dy: Optional[Tensor], dh_last: Optional[Tensor]
+                ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    g = _lib.host().ssm_scan_bw(x, dt, a, b, c, skip, z, dt_bias, h_initial, softplus, checkpoints, dy, dh_last)
+    return tuple(x.new_empty((0,)) if t is None else t for t in g)
+
+
+@ssm_scan_bw.register_fake
+def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, checkpoints, dy, dh_last):
+    like = lambda t: x.new_empty((0,)) if t is None else _contig(t)  # noqa: E731
+    return tuple(like(t) for t in (x, dt, a, b, c, skip, z, dt_bias, h_initial))
+
+
+def _ssm_setup_context(ctx, inputs, output):
+    x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial = inputs
+    ctx.save_for_backward(x, dt, a, b, c, skip, z, dt_bias, h_initial, output[2])
+    ctx.softplus = softplus
+
+
+def _ssm_backward(ctx, dy, dh_last, _dck):
+    x, dt, a, b, c, skip, z, dt_bias, h_initial, checkpoints = ctx.saved_tensors
+    dx, ddt, da, db, dc, dskip, dz, dbias, dh0 = ssm_scan_bw(x, dt, a, b, c, skip, z, dt_bias, ctx.softplus, h_initial,
+                                                             checkpoints, dy, dh_last)
+    return (dx, ddt, da, db, dc, None if skip is None else dskip, None if z is None else dz, None if dt_bias is None else dbias,
+            None, None if h_initial is None else dh0)
+
+
+torch.library.register_autograd("mlstm_b200::ssm_scan", _ssm_backward, setup_context=_ssm_setup_context)
+
+
+@torch.library.custom_op("mlstm_b200::ssm_step", mutates_args=(), device_types="cuda")
+def ssm_step(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, h: Tensor, skip: Optional[Tensor], z: Optional[Tensor],
+             dt_bias: Optional[Tensor], softplus: bool) -> tuple[Tensor, Tensor]:
+    return _lib.host().ssm_step(x, dt, a, b, c, skip, z, dt_bias, h, softplus, None)
+
+
+@ssm_step.register_fake
+def _(x, dt, a, b, c, h, skip, z, dt_bias, softplus):
+    return _contig(x), h.new_empty(h.shape, dtype=_F32)

@@ -21,7 +21,9 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libmlstm_b200.so")
 HOST = os.path.join(PKG, "_host.so")
-SOURCES = ["api.cu", "gates.cu", "step.cu", "chunkwise_simt.cu", "chunkwise_sm100.cu", "chunkwise_bw_sm100.cu", "noalloc.cu"]
+SOURCES = ["api.cu", "gates.cu", "step.cu", "chunkwise_simt.cu", "chunkwise_sm100.cu", "chunkwise_bw_sm100.cu", "noalloc.cu",
+           "api_layers.cu", "layer_norm.cu", "short_conv.cu", "ssm_fw.cu", "ssm_bw.cu"]
+HOST_SOURCES = ["host.cpp", "host_layers.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--use_fast_math=false", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -42,17 +44,21 @@ def _deps_mtime() -> float:
     return max(os.path.getmtime(h) for h in hdrs)
 
 
-def _host_command() -> list[str]:
+def _host_commands() -> tuple[list[list[str]], list[str]]:
+    """What compiles each source of _host.so, and what links them."""
     import torch
     from torch.utils import cpp_extension
 
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     inc = [*cpp_extension.include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc),
-            os.path.join(CSRC, "host.cpp"), "-o", HOST, f"-L{PKG}", "-l:libmlstm_b200.so", "-Wl,-rpath,$ORIGIN",
+    objs = [os.path.join(OBJ, s.replace(".cpp", ".o")) for s in HOST_SOURCES]
+    compiles = [["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc),
+                 "-c", os.path.join(CSRC, s), "-o", o] for s, o in zip(HOST_SOURCES, objs)]
+    link = ["g++", "-shared", *objs, "-o", HOST, f"-L{PKG}", "-l:libmlstm_b200.so", "-Wl,-rpath,$ORIGIN",
             f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    return compiles, link
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -75,7 +81,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+            raise RuntimeError("build failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
         return r.stderr
 
     if jobs:
@@ -85,9 +91,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
                     print(out)
     if jobs or not os.path.exists(LIB):
         run([nvcc, "-shared", "-o", LIB, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-lcuda"])
-    host_src = os.path.join(CSRC, "host.cpp")
-    if force or not os.path.exists(HOST) or os.path.getmtime(HOST) < max(os.path.getmtime(host_src), hdr_t):
-        run(_host_command())
+    host_t = max(hdr_t, *(os.path.getmtime(os.path.join(CSRC, s)) for s in HOST_SOURCES))
+    if force or not os.path.exists(HOST) or os.path.getmtime(HOST) < host_t:
+        compiles, link = _host_commands()
+        with ThreadPoolExecutor(max_workers=len(compiles)) as ex:
+            list(ex.map(run, compiles))
+        run(link)
     return LIB
 
 

@@ -36,7 +36,7 @@ static const size_t kMaxPhaseRecs = 1 << 16;
 // phases of mlstm_b200_profile_phase_name.  Off by default; the header-only NVTX loads the tools library on first use.
 static std::atomic<int> g_nvtx_on{0};
 static const char* const kPhaseNames[PH_COUNT] = {"gates", "recurrent_fw", "parallel_fw", "recurrent_bw",
-                                                   "parallel_bw", "gate_grads", "step"};
+                                                   "parallel_bw", "gate_grads", "step", "layer_norm", "short_conv", "ssm_scan"};
 
 PhaseScope::PhaseScope(int phase, cudaStream_t s) : slot(-1), st(s), nvtx(false) {
   if (g_nvtx_on.load(std::memory_order_relaxed) != 0 && phase >= 0 && phase < PH_COUNT) {

@@ -122,7 +122,7 @@ int launch_pdl(bool overlap, void (*kern)(KArgs...), unsigned grid, unsigned thr
 
 // Optional per-phase device timing (mlstm_b200_profile_*): when enabled, a pair of CUDA events
 // brackets each phase on the launching stream.
-enum Phase { PH_GATES = 0, PH_REC_FW, PH_PAR_FW, PH_REC_BW, PH_PAR_BW, PH_GATE_GRADS, PH_STEP, PH_COUNT };
+enum Phase { PH_GATES = 0, PH_REC_FW, PH_PAR_FW, PH_REC_BW, PH_PAR_BW, PH_GATE_GRADS, PH_STEP, PH_NORM, PH_CONV, PH_SCAN, PH_COUNT };
 struct PhaseScope {
   PhaseScope(int phase, cudaStream_t st);
   ~PhaseScope();

@@ -8,66 +8,12 @@
 // no interpreter lock.  Signatures, defaults, return conventions and exception types are those of the Python wrappers
 // (chunkwise.py, recurrent.py), which hand over to this module; the operands' sizes and memory are checked before anything
 // touches the device.
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/autocast_mode.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Dtype.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include <array>
-#include <cstdlib>
-#include <cstring>
-
-#include "calls.h"
+#include "host.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace mlstm_host;
 
-int dtype_code(at::ScalarType t) {   // -1: not a kernel element type
-  switch (t) {
-    case at::kFloat: return MLSTM_F32;
-    case at::kBFloat16: return MLSTM_BF16;
-    case at::kHalf: return MLSTM_F16;
-    default: return -1;
-  }
-}
-at::ScalarType code_dtype(int code) {
-  return code == MLSTM_F32 ? at::kFloat : code == MLSTM_BF16 ? at::kBFloat16 : at::kHalf;
-}
-
-const char* const kNeedsCuda = "mlstm_kernels_b200 kernels run on CUDA tensors only (there is no CPU fallback)";
-
-Tensor empty(at::IntArrayRef size, at::ScalarType dt, const at::Device& dev) {
-  return Tensor(at::detail::empty_cuda(size, dt, dev, std::nullopt));
-}
-Tensor conform(const Tensor& t, at::ScalarType dt) {
-  if (t.scalar_type() != dt) return t.to(dt).contiguous();
-  return t.is_contiguous() ? t : t.contiguous();
-}
-Tensor f32c(const Tensor& t) { return t.defined() ? conform(t, at::kFloat) : t; }
-const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-const float* fptr(const Tensor& t) { return static_cast<const float*>(ptr(t)); }
-float* fout(const Tensor& t) { return t.defined() ? static_cast<float*>(t.mutable_data_ptr()) : nullptr; }
-void* current_stream(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
-
-void check(int rc, const char* what) {
-  if (rc == MLSTM_OK) return;
-  std::string msg = std::string(what) + ": " + mlstm_b200_error_string(rc);
-  if (rc == MLSTM_ERR_CUDA) TORCH_CHECK(false, msg, ": ", mlstm_b200_last_cuda_error());
-  C10_THROW_ERROR(ValueError, msg);
-}
-
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-Tensor bytes(size_t n, const at::Device& dev) { return empty({(int64_t)std::max<size_t>(n, 256)}, at::kByte, dev); }
 // `need` bytes, and behind them (from up256(need)) `extra` that only make the call faster: where memory is too short for both,
 // extra becomes 0 and the call does without.  (Asked for last: what a call allocates after it would have to fit beside the extra.)
 Tensor bytes_and(size_t need, size_t& extra, const at::Device& dev) {
@@ -247,46 +193,9 @@ class ChunkwiseFn : public torch::autograd::Function<ChunkwiseFn> {
 // ---- Python glue ----------------------------------------------------------------------------------------
 struct AssertionFailed { std::string what; };
 
-Tensor arg(PyObject* o, const char* name) {
-  if (o == Py_None) return Tensor();
-  if (!THPVariable_Check(o)) throw torch::TypeError(c10::str(name, " must be a tensor, got ", Py_TYPE(o)->tp_name));
-  return THPVariable_Unpack(o);
-}
-Tensor need(PyObject* o, const char* name) {
-  Tensor t = arg(o, name);
-  if (!t.defined()) throw torch::TypeError(c10::str(name, " must be a tensor, got None"));
-  return t;
-}
-at::ScalarType dtype_arg(PyObject* o) {
-  if (!THPDtype_Check(o)) throw torch::TypeError(c10::str("expected a torch.dtype, got ", Py_TYPE(o)->tp_name));
-  return reinterpret_cast<THPDtype*>(o)->scalar_type;
-}
-PyObject* wrap(const Tensor& t) {
-  if (!t.defined()) Py_RETURN_NONE;
-  return THPVariable_Wrap(t);
-}
 PyObject* state_tuple(PyObject* h, const Tensor& c, const Tensor& n, const Tensor& m) {
   return Py_BuildValue("(N(NNN))", h, wrap(c), wrap(n), wrap(m));
 }
-double double_arg(PyObject* o) {
-  const double x = PyFloat_AsDouble(o);
-  if (x == -1.0 && PyErr_Occurred()) throw python_error();
-  return x;
-}
-long long_arg(PyObject* o) {
-  const long x = PyLong_AsLong(o);
-  if (x == -1 && PyErr_Occurred()) throw python_error();
-  return x;
-}
-bool bool_arg(PyObject* o) {
-  const int x = PyObject_IsTrue(o);
-  if (x < 0) throw python_error();
-  return x != 0;
-}
-void nargs_are(Py_ssize_t have, Py_ssize_t want) {
-  if (have != want) throw torch::TypeError(c10::str("expected ", want, " arguments, got ", have));
-}
-
 // chunkwise(q, k, v, i, f, c0, n0, m0, return_last_states, eps, chunk_size, impl, recompute, cast_dtype, variant)
 //   -> (h, c_last, n_last, m_last), the last three None without return_last_states
 PyObject* py_chunkwise(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -481,4 +390,11 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__host(void) {
+  PyObject* m = PyModule_Create(&kModule);
+  if (m != nullptr && PyModule_AddFunctions(m, mlstm_host::kLayerMethods) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

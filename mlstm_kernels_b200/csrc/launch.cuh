@@ -84,4 +84,39 @@ int launch_step_sequence(const void* q, const void* k, const void* v, const void
                          const float* n, const float* m, void* h, float* c_new, float* n_new, float* m_new, int B,
                          int NH, int T, int DHQK, int DHHV, int dtype, int gate_dtype, float eps, cudaStream_t st);
 
+// layer_norm.cu
+size_t layer_norm_bw_bytes(long long rows, int NH, int D);
+int launch_layer_norm_fw(const void* x, const long long* xs, const void* w, const void* b, void* y, float* mean, float* rstd, long long n0,
+                         long long n1, int NH, int D, int dtype, int param_dtype, float eps, cudaStream_t st);
+int launch_layer_norm_bw(const void* x, const long long* xs, const void* w, const float* mean, const float* rstd, const void* dy,
+                         const long long* ys, void* dx, const long long* ds, void* dw, void* db, float* partial, long long n0, long long n1,
+                         int NH, int D, int dtype, int param_dtype, cudaStream_t st);
+
+// short_conv.cu
+size_t short_conv_bw_bytes(int B, int S, int D, int W);
+int launch_short_conv_fw(const void* x, const long long* xs, const void* x0, const void* w, const void* bias, void* y, void* x_last, int B, int S,
+                         int D, int W, bool silu, int dtype, int w_dtype, cudaStream_t st);
+int launch_short_conv_bw(const void* x, const long long* xs, const void* x0, const void* w, const void* bias, const void* dy, const long long* ys,
+                         const void* dlast, void* dx, void* dx0, void* dw, void* db, float* partial, int B, int S, int D, int W, bool silu,
+                         int dtype, int w_dtype, cudaStream_t st);
+int launch_short_conv_step(const void* x, const void* before, const void* w, const void* bias, void* y, void* after, int B, int D, int W, bool silu,
+                           int dtype, int w_dtype, cudaStream_t st);
+
+// ssm_fw.cu, ssm_bw.cu
+struct SsmIn {
+  const void *x, *dt, *z, *b, *c;              // z may be null
+  const float *a, *skip, *dt_bias, *h0;        // skip, dt_bias, h0 may be null
+};
+bool ssm_sizes_ok(int B, int S, int D, int N, int G);
+size_t ssm_ckpt_bytes(int B, int S, int D, int N);
+size_t ssm_fw_bytes(int B, int S, int D, int N, int G);
+size_t ssm_bw_bytes(int B, int S, int D, int N, int G);
+int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* workspace, int B, int S, int D, int N, int G,
+                  bool softplus, int dtype, cudaStream_t st);
+int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, const long long* gs, const float* dh_last, const float* ckpt, void* dx,
+                  void* ddt, void* dz, void* db, void* dc, float* da, float* dskip, float* ddt_bias, float* dh0, void* workspace, int B, int S, int D,
+                  int N, int G, bool softplus, int dtype, cudaStream_t st);
+int launch_ssm_step(const void* x, const void* dt, const void* z, const void* b, const void* c, const float* a, const float* skip, const float* dt_bias,
+                    const float* h, void* y, float* h_new, int B, int D, int N, int G, bool softplus, int dtype, cudaStream_t st);
+
 }  // namespace mlstm
