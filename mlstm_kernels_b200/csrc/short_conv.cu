@@ -82,7 +82,7 @@ conv_fw_kernel(const T* x, const T* x0, const void* w, const void* bias, T* y, T
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) a = fmaf(wr[j][i], win[j][i], a);
         a = fmaf(wr[W - 1][i], v[i], a);
-        o[i] = d.silu ? a * sigmoid_f(a) : a;
+        o[i] = d.silu ? a * logistic_f(a) : a;
 #pragma unroll
         for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
         win[W - 2][i] = v[i];
@@ -160,7 +160,7 @@ conv_bw_kernel(const T* x, const T* x0, const void* w, const void* bias, const T
 #pragma unroll
             for (int j = 0; j < W - 1; ++j) a = fmaf(wr[j][i], win[j][i], a);
             a = fmaf(wr[W - 1][i], v[i], a);
-            const float s = sigmoid_f(a);
+            const float s = logistic_f(a);
             k *= s * fmaf(a, 1.f - s, 1.f);
           }
           if (t < t1) {
@@ -258,7 +258,7 @@ conv_step_kernel(const T* x, const T* before, const void* w, const void* bias, T
     for (int i = 0; i < V; ++i) o[i] = fmaf(wr[j][i], v[i], o[i]);
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = silu ? o[i] * sigmoid_f(o[i]) : o[i];
+  for (int i = 0; i < V; ++i) o[i] = silu ? o[i] * logistic_f(o[i]) : o[i];
   store_pack<T, V>(y + b * D + c, pack<T, V>(o));
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) store_pack<T, V>(after + (b * (W - 1) + j) * D + c, row[j + 1]);

@@ -24,16 +24,6 @@ struct SsmDims {
   long long xb, xt, db, dt, zb, zt, bb, bt, bg, cb, ct, cg, gb, gt;   // x, dt, z, b, c, dy
 };
 
-// 2^x as the hardware has it: off by 2^-22 of the result, results below 2^-126 are zero
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float softplus_f(float x) { return x > 20.f ? x : log1pf(expf(x)); }
-
-constexpr float SSM_LOG2E = 1.4426950408889634f, SSM_LN2 = 0.6931471805599453f;
-
 // Where a thread stands: states 4 sub ... 4 sub + 3 of channel `ch` of the CTA's tile in the recurrence; in the passes over whole
 // tiles, V neighbouring channels from `col` of the tokens row, row + rows, ...
 template <int LN, int V> struct SsmPlace {
@@ -119,7 +109,7 @@ template <int LN, int TB> __device__ __forceinline__ float lane_sums(float (&v)[
 
 template <int LN> __device__ __forceinline__ void ssm_rates(const float* a, const SsmDims& s, int d, int sub, bool on, float (&a2)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a2[i] = on && 4 * sub + i < s.N ? a[(size_t)d * s.N + 4 * sub + i] * SSM_LOG2E : 0.f;
+  for (int i = 0; i < 4; ++i) a2[i] = on && 4 * sub + i < s.N ? a[(size_t)d * s.N + 4 * sub + i] * kLog2e : 0.f;
 }
 
 // host: lanes to a channel

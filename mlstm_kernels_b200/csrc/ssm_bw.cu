@@ -45,7 +45,7 @@ __device__ __forceinline__ void ssm_enter_back(const SsmBw& k, const SsmDims& s,
   }
 }
 
-__device__ __forceinline__ float gate_f(float z) { return z * sigmoid_f(z); }
+__device__ __forceinline__ float gate_f(float z) { return z * logistic_f(z); }
 
 // A segment's own adjoint (nothing entering from behind) as it leaves at its first token, and the sum of its steps.
 template <typename T, int LN, int V>
@@ -267,16 +267,16 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float4 d4 = s_d[q * CH + p.col + e];
-        const float s1 = s_s1[q * P::YS + p.col + e], s2 = s_s2[q * P::YS + p.col + e] * SSM_LN2;
+        const float s1 = s_s1[q * P::YS + p.col + e], s2 = s_s2[q * P::YS + p.col + e] * kLn2;
         const float xv = to_f32(x[i].e[e]);
         ox.e[e] = from_f32<T>(fmaf(d4.x, s1, skip[e] * d4.z));
         float ddt = fmaf(xv, s1, s2);
-        if (s.softplus) ddt *= sigmoid_f(to_f32(dt[i].e[e]) + bias[e]);
+        if (s.softplus) ddt *= logistic_f(to_f32(dt[i].e[e]) + bias[e]);
         ot.e[e] = from_f32<T>(ddt);
         dbias[e] += ddt;
         dskip[e] = fmaf(d4.z, xv, dskip[e]);
         if (gate) {
-          const float zz = to_f32(z[i].e[e]), sg = sigmoid_f(zz);
+          const float zz = to_f32(z[i].e[e]), sg = logistic_f(zz);
           oz.e[e] = from_f32<T>(to_f32(dy[i].e[e]) * fmaf(skip[e], xv, s_yp[q * P::YS + p.col + e]) * sg * fmaf(zz, 1.f - sg, 1.f));
         }
       }

@@ -130,7 +130,7 @@ ssm_fw_kernel(SsmFw k, SsmDims s) {
           float v = fmaf(skip[e], to_f32(x[i].e[e]), s_y[r * P::YS + p.col + e]);
           if (k.in.z != nullptr) {
             const float zz = to_f32(z[i].e[e]);
-            v *= zz * sigmoid_f(zz);
+            v *= zz * logistic_f(zz);
           }
           o.e[e] = from_f32<T>(v);
         }
@@ -193,7 +193,7 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
     for (int i = 0; i < 4; ++i) {
       const bool ok = 4 * sub + i < N;
       const float bv = ok ? to_f32(b[bc + 4 * sub + i]) : 0.f, cv = ok ? to_f32(c[bc + 4 * sub + i]) : 0.f;
-      hv[i] = fmaf(ex2(step * (av[i] * SSM_LOG2E)), hv[i], step * xv * bv);
+      hv[i] = fmaf(ex2(step * (av[i] * kLog2e)), hv[i], step * xv * bv);
       acc = fmaf(cv, hv[i], acc);
     }
     float* op = h_new + row * N + 4 * sub;
@@ -211,7 +211,7 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
     float v = skip != nullptr ? fmaf(skip[d], xv, acc) : acc;
     if (z != nullptr) {
       const float zz = to_f32(z[row]);
-      v *= zz * sigmoid_f(zz);
+      v *= zz * logistic_f(zz);
     }
     y[row] = from_f32<T>(v);
   }

@@ -49,6 +49,55 @@ template <int V> __device__ __forceinline__ void load_any(const void* p, size_t 
 inline bool fits_access(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool stride_fits(long long elements, size_t element_size, size_t bytes) { return (elements * (long long)element_size) % (long long)bytes == 0; }
 
+// ---- exponentials for element-wise work ----------------------------------------------------------------
+// The hardware's 2^x and 1 / x (off by 2^-22 and 2^-23 of the result; results below 2^-126 are zero), eight instructions to an
+// exponential and two more to a logistic function, where expf and a division take thirty.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e), kLn2 = 0.6931471805599453f;
+// e^x up to e^88.  x log2(e) in two parts, the second of which is what rounding the first dropped: 2^(n + r) = 2^n (1 + r ln 2).
+__device__ __forceinline__ float exp_f(float x) {
+  x = min_nan(max_nan(x, -1e4f), 88.f);
+  const float n = x * kLog2e;
+  const float r = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -n));
+  const float e = ex2(n);
+  return fmaf(e * r, kLn2, e);
+}
+__device__ __forceinline__ float logistic_f(float x) { return rcp(1.f + exp_f(-x)); }
+// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|; log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series: the terms
+// left out are below 2^-29 of the sum, and a small e keeps all its digits
+__device__ __forceinline__ float softplus_f(float x) {
+  const float e = exp_f(-fabsf(x));
+  const float s = e * rcp(2.f + e), q = s * s;
+  float p = 1.f / 15.f;
+  p = fmaf(p, q, 1.f / 13.f);
+  p = fmaf(p, q, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  return fmaf(2.f * s, p, max_nan(x, 0.f));
+}
+
 #define MLSTM_DTYPE_SWITCH(code, T, ...)                                            \
   switch (code) {                                                                   \
     case MLSTM_F32: { using T = float; __VA_ARGS__ } break;                         \
