@@ -20,17 +20,6 @@ struct ConvDims {
   bool silu;
 };
 
-template <typename T, int V> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&o)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = to_f32(p.e[i]);
-}
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> pack(const float (&o)[V]) {
-  Pack<T, V> p;
-#pragma unroll
-  for (int i = 0; i < V; ++i) p.e[i] = from_f32<T>(o[i]);
-  return p;
-}
-
 // Token t of the padded sequence: x for t >= 0, x_initial (row t + W - 1) or zeros before.
 template <typename T, int V, int W>
 __device__ __forceinline__ Pack<T, V> conv_token(const T* xb, const T* x0b, long long st, int t, int D) {

@@ -1,17 +1,17 @@
 // What the forward and the backward of the selective state space scan share: sizes, tiles, and the pass over a tile's operands
 // before the recurrence.
 #pragma once
-#include "f32x2.cuh"
 #include "launch.cuh"
 #include "vec.cuh"
 
 namespace mlstm {
 
-// A CTA of 256 threads has SSM_TT tokens of CH = 256 / LN channels at a time: LN neighbouring lanes share a channel, each with four of
-// its states.  (Four states a thread, not all of them: four times the warps for the same sequences, and the sums over the states
-// cost three shuffles for four tokens.)
+// A CTA of 128 threads has SSM_TT tokens of CH = 256 / LN channels at a time: LN neighbouring lanes share two channels, each lane
+// with four states of both.  (Four states a thread, not all of them: as many times the warps for the same sequences, and three
+// shuffles sum four values over the states of sixteen.  Two channels: b and c come from shared memory once for both, which a
+// wave of 128 bytes a clock bounds.)
 constexpr int SSM_TT = 16;
-constexpr int SSM_THREADS = 256;
+constexpr int SSM_THREADS = 128, SSM_WARPS = SSM_THREADS / 32;
 constexpr int SSM_MAX_N = 128;
 
 struct SsmDims {
@@ -24,28 +24,30 @@ struct SsmDims {
   long long xb, xt, db, dt, zb, zt, bb, bt, bg, cb, ct, cg, gb, gt;   // x, dt, z, b, c, dy
 };
 
-// Where a thread stands: states 4 sub ... 4 sub + 3 of channel `ch` of the CTA's tile in the recurrence; in the passes over whole
-// tiles, V neighbouring channels from `col` of the tokens row, row + rows, ...
+// Where a thread stands: states 4 sub ... 4 sub + 3 of the channels `ch` and `ch` + 1 of the CTA's tile in the recurrence; in the
+// passes over whole tiles, V neighbouring channels from `col` of the tokens row, row + ROWS, ...
 template <int LN, int V> struct SsmPlace {
-  static constexpr int CH = SSM_THREADS / LN, NP = 4 * LN, LC = 32 / LN;
+  static constexpr int CH = 2 * SSM_THREADS / LN, NP = 4 * LN, LC = 32 / LN;
   static constexpr int PER_ROW = CH / V, ROWS = SSM_THREADS / PER_ROW;        // threads to a token; tokens at once
   static constexpr int ITEMS = ROWS >= SSM_TT ? 1 : SSM_TT / ROWS;
   static constexpr int BC = (SSM_TT * NP + SSM_THREADS - 1) / SSM_THREADS;    // elements of b (and of c) a thread fetches
-  static constexpr int YS = CH + 32 / (LN < 8 ? LN : 8);                      // row of a (token, channel) array of sums: the lanes' tokens in banks of their own
+  static constexpr int YS = CH + 16;                             // row of a (token, channel) array of sums: two tokens' in different banks
   int sub, chl, ch, warp, tile, g, seg, b, d;
-  bool on;
+  bool on[2];
   int row, col, dcol;
   bool col_on;
-  __device__ __forceinline__ SsmPlace(const SsmDims& s) {
+  // nseg: segments that the launch has, from seg0 on
+  __device__ __forceinline__ SsmPlace(const SsmDims& s, int nseg, int seg0) {
     const int lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
-    sub = lane % LN; chl = lane / LN; ch = warp * LC + chl;
+    sub = lane % LN; chl = lane / LN; ch = 2 * (warp * LC + chl);
     unsigned k = blockIdx.x;
     tile = k % s.tiles; k /= s.tiles;
     g = k % s.G; k /= s.G;
-    seg = k % s.nseg;
-    b = k / s.nseg;
-    on = tile * CH + ch < s.Dg;
+    seg = seg0 + k % nseg;
+    b = k / nseg;
+    on[0] = tile * CH + ch < s.Dg;
+    on[1] = tile * CH + ch + 1 < s.Dg;
     d = g * s.Dg + tile * CH + ch;
     row = threadIdx.x / PER_ROW; col = (threadIdx.x % PER_ROW) * V;
     col_on = tile * CH + col < s.Dg && row < SSM_TT;
@@ -53,22 +55,11 @@ template <int LN, int V> struct SsmPlace {
   }
 };
 
-// The operands of a tile on their way from memory.
-template <typename T, int LN, int V, bool BW, bool WITH_C> struct SsmFetch {
+// b and c of a tile on their way from memory
+template <typename T, int LN, int V, bool WITH_C> struct SsmFetchBC {
   using P = SsmPlace<LN, V>;
-  Pack<T, V> x[P::ITEMS], dt[P::ITEMS], z[P::ITEMS], dy[BW ? P::ITEMS : 1];
   T b[P::BC], c[WITH_C ? P::BC : 1];
-  __device__ __forceinline__ void load(const SsmIn& in, const void* dyp, const SsmDims& s, const P& p, int t0, bool with_z) {
-    const T *xp = static_cast<const T*>(in.x), *tp = static_cast<const T*>(in.dt), *zp = static_cast<const T*>(in.z);
-#pragma unroll
-    for (int i = 0; i < P::ITEMS; ++i) {
-      const int t = t0 + p.row + i * P::ROWS;
-      const bool ok = p.col_on && t < s.S;
-      x[i] = ok ? load_pack<T, V>(xp + p.b * s.xb + t * s.xt + p.dcol) : zero_pack<T, V>();
-      dt[i] = ok ? load_pack<T, V>(tp + p.b * s.db + t * s.dt + p.dcol) : zero_pack<T, V>();
-      if (with_z && in.z != nullptr) z[i] = ok ? load_pack<T, V>(zp + p.b * s.zb + t * s.zt + p.dcol) : zero_pack<T, V>();
-      if (BW) dy[i] = ok ? load_pack<T, V>(static_cast<const T*>(dyp) + p.b * s.gb + t * s.gt + p.dcol) : zero_pack<T, V>();
-    }
+  __device__ __forceinline__ void load(const SsmIn& in, const SsmDims& s, const P& p, int t0) {
     const T *bp = static_cast<const T*>(in.b) + p.b * s.bb + p.g * s.bg, *cp = static_cast<const T*>(in.c) + p.b * s.cb + p.g * s.cg;
 #pragma unroll
     for (int i = 0; i < P::BC; ++i) {
@@ -78,7 +69,7 @@ template <typename T, int LN, int V, bool BW, bool WITH_C> struct SsmFetch {
       if (WITH_C) c[i] = ok ? cp[t * s.ct + n] : from_f32<T>(0.f);
     }
   }
-  __device__ __forceinline__ void put_bc(float* s_b, float* s_c) const {
+  __device__ __forceinline__ void put(float* s_b, float* s_c) const {
 #pragma unroll
     for (int i = 0; i < P::BC; ++i) {
       const int k = threadIdx.x + i * SSM_THREADS;
@@ -90,26 +81,79 @@ template <typename T, int LN, int V, bool BW, bool WITH_C> struct SsmFetch {
   }
 };
 
-// Sums over the LN lanes of a channel of TB values each, one per token: the lane ends with the sum of token sub / (LN / TB).
-template <int LN, int TB> __device__ __forceinline__ float lane_sums(float (&v)[TB], int sub) {
-  constexpr int REP = LN / TB;
+// The step of V channels; zero (nothing moves) where `ok` is false
+template <int V> __device__ __forceinline__ void ssm_step_v(const float (&dt)[V], const float (&bias)[V], bool softplus, bool ok, float (&o)[V]) {
+  float raw[V];
 #pragma unroll
-  for (int half = TB / 2; half >= 1; half >>= 1) {
-    const bool up = (sub & (half * REP)) != 0;
+  for (int i = 0; i < V; ++i) raw[i] = dt[i] + bias[i];
+  if (softplus) softplus_v<V>(raw, o);
 #pragma unroll
-    for (int t = 0; t < half; ++t) {
-      const float mine = up ? v[t + half] : v[t], theirs = up ? v[t] : v[t + half];
-      v[t] = mine + __shfl_xor_sync(0xffffffffu, theirs, half * REP);
-    }
-  }
-#pragma unroll
-  for (int o = REP / 2; o >= 1; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-  return v[0];
+  for (int i = 0; i < V; ++i) o[i] = !ok ? 0.f : softplus ? o[i] : raw[i];
 }
 
-template <int LN> __device__ __forceinline__ void ssm_rates(const float* a, const SsmDims& s, int d, int sub, bool on, float (&a2)[4]) {
+// Sums of four values over the LN lanes of a channel pair, each step halving the values that a lane still carries: a lane ends
+// with LEFT of them, from number `first` on.
+template <int LN> struct LaneSums {
+  static constexpr int LEFT = LN >= 4 ? 1 : 4 / LN;
+  static constexpr int SAME = LN >= 4 ? LN / 4 : 1;      // lanes that end with the same value
+  static __device__ __forceinline__ int run(float (&v)[4], int sub) {
+    int first = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a2[i] = on && 4 * sub + i < s.N ? a[(size_t)d * s.N + 4 * sub + i] * kLog2e : 0.f;
+    for (int bit = LN / 2, n = 4; bit >= 1; bit >>= 1) {
+      if (n > 1) {
+        n >>= 1;
+        const bool up = (sub & bit) != 0;
+#pragma unroll
+        for (int j = 0; j < n; ++j) {
+          const float mine = up ? v[j + n] : v[j], theirs = up ? v[j] : v[j + n];
+          v[j] = mine + __shfl_xor_sync(0xffffffffu, theirs, bit);
+        }
+        first += up ? n : 0;
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);
+      }
+    }
+    return first;
+  }
+};
+
+// Four values of a row of N at `n`, where n may reach past its end
+__device__ __forceinline__ void ssm_load4(const float* row, int N, int n, float (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = n + i < N ? row[n + i] : 0.f;
+}
+// a in powers of two, as pairs of states
+template <int LN, int V> __device__ __forceinline__ void ssm_rates(const float* a, const SsmDims& s, const SsmPlace<LN, V>& p, uint64_t (&a2)[2][2]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.on[c]) ssm_load4(a + (size_t)(p.d + c) * s.N, s.N, 4 * p.sub, v);
+    a2[c][0] = f2(v[0] * kLog2e, v[1] * kLog2e);
+    a2[c][1] = f2(v[2] * kLog2e, v[3] * kLog2e);
+  }
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
+  float a, b;
+  unf2(v, a, b);
+  return f2(ex2(a), ex2(b));
+}
+// From what other segments leave behind, in their order: v = 2^(a sum) v + left.  first ... last - 1, or last - 1 ... first (BACK).
+template <int LN, int V, bool BACK>
+__device__ __forceinline__ void ssm_fold(const float* left, const float* sums, int first, int last, const SsmDims& s, const SsmPlace<LN, V>& p,
+                                         const uint64_t (&a2)[2][2], uint64_t (&v)[2][2]) {
+#pragma unroll 4
+  for (int i = 0; i < last - first; ++i) {
+    const int j = BACK ? last - 1 - i : first + i;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (!p.on[c]) continue;
+      const size_t at = ((size_t)p.b * s.nseg + j) * s.D + p.d + c;
+      const float sum = sums[at];
+      const Pack<uint64_t, 2> l = load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(left + at * (4 * LN) + 4 * p.sub));
+      v[c][0] = fma2(ex2_pair(mul2(f2(sum, sum), a2[c][0])), v[c][0], l.e[0]);
+      v[c][1] = fma2(ex2_pair(mul2(f2(sum, sum), a2[c][1])), v[c][1], l.e[1]);
+    }
+  }
 }
 
 // host: lanes to a channel

@@ -28,193 +28,315 @@ struct SsmBw {
   float *loc_g, *loc_sum;   // (B, nseg, D, NP), (B, nseg, D)
 };
 
-// The adjoint that enters segment p.seg from behind: e_{t+1} g_{t+1} at its last token
+// What comes back into the recurrence from behind the sequence
 template <int LN, int V>
-__device__ __forceinline__ void ssm_enter_back(const SsmBw& k, const SsmDims& s, const SsmPlace<LN, V>& p, const float (&a2)[4], float (&r)[4]) {
-  constexpr int NP = 4 * LN;
+__device__ __forceinline__ void ssm_behind(const float* dh_last, const SsmDims& s, const SsmPlace<LN, V>& p, uint64_t (&r)[2][2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = k.dh_last != nullptr && p.on && 4 * p.sub + i < s.N ? k.dh_last[((size_t)p.b * s.D + p.d) * s.N + 4 * p.sub + i] : 0.f;
-  if (!p.on) return;
-  for (int j = s.nseg - 1; j > p.seg; --j) {
-    const size_t at = ((size_t)p.b * s.nseg + j) * s.D + p.d;
-    const float sum = k.loc_sum[at];
-    const Pack<float, 4> l = load_pack<float, 4>(k.loc_g + at * NP + 4 * p.sub);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = fmaf(ex2(sum * a2[i]), r[i], l.e[i]);
+  for (int c = 0; c < 2; ++c) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (dh_last != nullptr && p.on[c]) ssm_load4(dh_last + ((size_t)p.b * s.D + p.d + c) * s.N, s.N, 4 * p.sub, v);
+    r[c][0] = f2(v[0], v[1]);
+    r[c][1] = f2(v[2], v[3]);
   }
 }
 
-__device__ __forceinline__ float gate_f(float z) { return z * logistic_f(z); }
-
 // A segment's own adjoint (nothing entering from behind) as it leaves at its first token, and the sum of its steps.
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SSM_THREADS, 3)
-ssm_bw_local_kernel(SsmBw k, SsmDims s) {
+__global__ void __launch_bounds__(SSM_THREADS, 5)
+ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
   using P = SsmPlace<LN, V>;
   constexpr int CH = P::CH, NP = P::NP;
-  __shared__ float2 s_d[SSM_TT * CH];                  // (step, dout)
+  __shared__ __align__(16) float2 s_d[SSM_TT * CH];    // (step, dout)
   __shared__ __align__(16) float s_c[SSM_TT * NP];
   pdl_launch_dependents();
   pdl_wait();
-  const P p(s);
-  float a2[4], r[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f, bias[V];
-  ssm_rates<LN>(k.in.a, s, p.d, p.sub, p.on, a2);
+  const P p(s, nseg, 1);
+  uint64_t a2[2][2], r[2][2] = {{0ull, 0ull}, {0ull, 0ull}}, sum = 0ull;
+  float bias[V];
+  ssm_rates<LN, V>(k.in.a, s, p, a2);
 #pragma unroll
   for (int i = 0; i < V; ++i) bias[i] = k.in.dt_bias != nullptr && p.col_on ? k.in.dt_bias[p.dcol + i] : 0.f;
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
+  const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
+  const bool gate = k.in.z != nullptr;
   SsmIn in = k.in;
   in.b = in.c;   // of the two only c is needed
   SsmDims sc = s;
   sc.bb = s.cb; sc.bt = s.ct; sc.bg = s.cg;
-  SsmFetch<T, LN, V, true, false> f;
-  const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
-  f.load(in, k.dy, sc, p, t_last, true);
+  Pack<T, V> ndt[P::ITEMS], nz[P::ITEMS], ndy[P::ITEMS];
+  SsmFetchBC<T, LN, V, false> f;
+  auto fetch = [&](int t0) {
+    const T *tp = static_cast<const T*>(in.dt) + p.b * s.db + p.dcol, *zp = static_cast<const T*>(in.z) + p.b * s.zb + p.dcol;
+    const T* yp = static_cast<const T*>(k.dy) + p.b * s.gb + p.dcol;
+#pragma unroll
+    for (int i = 0; i < P::ITEMS; ++i) {
+      const int t = t0 + p.row + i * P::ROWS;
+      const bool ok = p.col_on && t < s.S;
+      ndt[i] = ok ? load_pack<T, V>(tp + t * s.dt) : zero_pack<T, V>();
+      if (gate) nz[i] = ok ? load_pack<T, V>(zp + t * s.zt) : zero_pack<T, V>();
+      ndy[i] = ok ? load_pack<T, V>(yp + t * s.gt) : zero_pack<T, V>();
+    }
+    f.load(in, sc, p, t0);
+  };
+  fetch(t_last);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
 #pragma unroll
     for (int i = 0; i < P::ITEMS; ++i) {
       const int q = p.row + i * P::ROWS;
       if (q < SSM_TT) {
+        float dt[V], step[V], g[V];
+        unpack(ndt[i], dt);
+        unpack(ndy[i], g);
+        ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
+        if (gate) {
+          float zv[V], sg[V];
+          unpack(nz[i], zv);
+          logistic_v<V>(zv, sg);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float raw = to_f32(f.dt[i].e[e]) + bias[e];
-          const float step = p.col_on && t0 + q < t_end ? (s.softplus ? softplus_f(raw) : raw) : 0.f;
-          const float dy = to_f32(f.dy[i].e[e]);
-          s_d[q * CH + p.col + e] = make_float2(step, in.z != nullptr ? dy * gate_f(to_f32(f.z[i].e[e])) : dy);
+          for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
         }
+        Pack<float2, V> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], g[e]);
+        store_pack<float2, V>(s_d + q * CH + p.col, o);
       }
     }
-    f.put_bc(s_c, nullptr);
+    f.put(s_c, nullptr);
     __syncthreads();
-    if (t0 > t_begin) f.load(in, k.dy, sc, p, t0 - SSM_TT, true);
+    if (t0 > t_begin) fetch(t0 - SSM_TT);
 #pragma unroll 4
     for (int t = SSM_TT - 1; t >= 0; --t) {
-      const float2 q = s_d[t * CH + p.ch];
-      const float4 c = *reinterpret_cast<const float4*>(s_c + t * NP + 4 * p.sub);
-      r[0] = ex2(q.x * a2[0]) * fmaf(q.y, c.x, r[0]);
-      r[1] = ex2(q.x * a2[1]) * fmaf(q.y, c.y, r[1]);
-      r[2] = ex2(q.x * a2[2]) * fmaf(q.y, c.z, r[2]);
-      r[3] = ex2(q.x * a2[3]) * fmaf(q.y, c.w, r[3]);
-      sum += q.x;
+      const float4 q = *reinterpret_cast<const float4*>(s_d + t * CH + p.ch);
+      const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + t * NP + 4 * p.sub);
+      const float qs[2] = {q.x, q.z}, qg[2] = {q.y, q.w};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint64_t step = f2(qs[c], qs[c]), g = f2(qg[c], qg[c]);
+        r[c][0] = mul2(ex2_pair(mul2(step, a2[c][0])), fma2(g, c2.x, r[c][0]));
+        r[c][1] = mul2(ex2_pair(mul2(step, a2[c][1])), fma2(g, c2.y, r[c][1]));
+      }
+      sum = add2(sum, f2(q.x, q.z));
     }
     __syncthreads();
   }
-  if (!p.on) return;
-  const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d;
-  Pack<float, 4> o;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o.e[i] = r[i];
-  store_pack<float, 4>(k.loc_g + at * NP + 4 * p.sub, o);
-  if (p.sub == 0) k.loc_sum[at] = sum;
+  for (int c = 0; c < 2; ++c) {
+    if (!p.on[c]) continue;
+    const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d + c;
+    Pack<uint64_t, 2> o;
+    o.e[0] = r[c][0]; o.e[1] = r[c][1];
+    store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.loc_g + at * NP + 4 * p.sub), o);
+    float s0, s1;
+    unf2(sum, s0, s1);
+    if (p.sub == 0) k.loc_sum[at] = c == 0 ? s0 : s1;
+  }
 }
 
-// Shared memory of the backward, in floats
-template <int LN, int V> struct SsmBwSmem {
+// Shared memory of the backward, in bytes
+template <typename T, int LN, int V> struct SsmBwSmem {
   using P = SsmPlace<LN, V>;
   static constexpr int TF = LN <= 4 ? SSM_TT : 64 / LN;          // tokens whose channel sums wait for the other warps
-  static constexpr int D4 = 0, B = D4 + 4 * SSM_TT * P::CH, C = B + SSM_TT * P::NP, S1 = C + SSM_TT * P::NP, S2 = S1 + SSM_TT * P::YS,
-                       YP = S2 + SSM_TT * P::YS, PART = YP + SSM_TT * P::YS, END = PART + 8 * TF * 2 * P::NP;
-  static constexpr size_t BYTES = END * sizeof(float);
+  static constexpr int RAW = SSM_TT * P::CH;                      // elements of one operand's tile
+  static constexpr size_t Q = 0, G = Q + sizeof(float2) * SSM_TT * P::CH, B = G + sizeof(float) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
+                          SUMS = C + sizeof(float) * SSM_TT * P::NP, PART = SUMS + 3 * sizeof(float) * SSM_TT * P::YS,
+                          X = PART + sizeof(float) * SSM_WARPS * TF * 2 * P::NP, BYTES = X + 2 * 4 * sizeof(T) * RAW;
 };
 
+// V elements to shared memory: they arrive by the next cp_wait(), zeros where `ok` is false
+template <typename T, int V> __device__ __forceinline__ void copy_async(T* dst, const T* src, bool ok) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES >= 4) {
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0) : "memory");
+  } else {
+    store_pack<T, V>(dst, ok ? load_pack<T, V>(src) : zero_pack<T, V>());
+  }
+}
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SSM_THREADS, 2)
+__global__ void __launch_bounds__(SSM_THREADS, 3)
 ssm_bw_kernel(SsmBw k, SsmDims s) {
   using P = SsmPlace<LN, V>;
-  using M = SsmBwSmem<LN, V>;
-  constexpr int CH = P::CH, NP = P::NP, TB = LN < 8 ? LN : 8, REP = LN / TB, TF = M::TF, LC = P::LC;
-  extern __shared__ __align__(16) float sm[];
-  float4* s_d = reinterpret_cast<float4*>(sm + M::D4);           // (step, step x, dout, -)
-  float *s_b = sm + M::B, *s_c = sm + M::C, *s_s1 = sm + M::S1, *s_s2 = sm + M::S2, *s_yp = sm + M::YP, *s_part = sm + M::PART;
+  using M = SsmBwSmem<T, LN, V>;
+  using Sums = LaneSums<LN>;
+  constexpr int CH = P::CH, NP = P::NP, TF = M::TF, LC = P::LC, HALF = SSM_TT / 2;
+  extern __shared__ __align__(16) char sm[];
+  float2* s_q = reinterpret_cast<float2*>(sm + M::Q);            // (step, step x)
+  float *s_g = reinterpret_cast<float*>(sm + M::G), *s_b = reinterpret_cast<float*>(sm + M::B), *s_c = reinterpret_cast<float*>(sm + M::C);
+  float *s_sum = reinterpret_cast<float*>(sm + M::SUMS), *s_part = reinterpret_cast<float*>(sm + M::PART);
+  float* s_yp = s_sum + 2 * SSM_TT * P::YS;                      // s_sum: sum g b, sum a g e h; s_yp: sum c h
+  T* s_raw = reinterpret_cast<T*>(sm + M::X);                    // x, dt, z, dy of two tiles; a thread copies what it reads itself
   pdl_launch_dependents();
   pdl_wait();
-  const P p(s);
+  const P p(s, s.nseg, 0);
   const bool gate = k.in.z != nullptr;
-  float a2[4], r[4], da[4] = {0.f, 0.f, 0.f, 0.f};
-  ssm_rates<LN>(k.in.a, s, p.d, p.sub, p.on, a2);
-  ssm_enter_back<LN, V>(k, s, p, a2, r);
-  float bias[V], skip[V], dskip[V], dbias[V];
+  uint64_t a2[2][2], r[2][2], da[2][2] = {{0ull, 0ull}, {0ull, 0ull}};
+  ssm_rates<LN, V>(k.in.a, s, p, a2);
+  ssm_behind<LN, V>(k.dh_last, s, p, r);
+  ssm_fold<LN, V, true>(k.loc_g, k.loc_sum, p.seg + 1, s.nseg, s, p, a2, r);
+  float dskip[V], dbias[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = k.in.dt_bias != nullptr && p.col_on ? k.in.dt_bias[p.dcol + i] : 0.f;
-    skip[i] = k.in.skip != nullptr && p.col_on ? k.in.skip[p.dcol + i] : 0.f;
-    dskip[i] = dbias[i] = 0.f;
-  }
+  for (int i = 0; i < V; ++i) dskip[i] = dbias[i] = 0.f;
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
-  SsmFetch<T, LN, V, true, true> f;
-  f.load(k.in, k.dy, s, p, t_last, true);
-  float* bc = k.part_bc + ((size_t)(p.g * s.tiles + p.tile) * s.B + p.b) * s.S * (2 * NP);
-  const float* ck = k.ckpt + ((size_t)p.b * s.nt * s.D + (p.on ? p.d : 0)) * NP + 4 * p.sub;
-  Pack<float, 4> h0 = zero_pack<float, 4>();
-  if (p.on) h0 = load_pack<float, 4>(ck + (size_t)(t_last / SSM_TT) * s.D * NP);
-  for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
-    Pack<T, V> x[P::ITEMS], z[P::ITEMS], dy[P::ITEMS], dt[P::ITEMS];
+  auto copy = [&](int t0) {
+    T* dst = s_raw + (t0 / SSM_TT & 1) * 4 * M::RAW;
 #pragma unroll
     for (int i = 0; i < P::ITEMS; ++i) {
-      x[i] = f.x[i]; z[i] = f.z[i]; dy[i] = f.dy[i]; dt[i] = f.dt[i];
-      const int q = p.row + i * P::ROWS;
-      if (q < SSM_TT) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float raw = to_f32(dt[i].e[e]) + bias[e];
-          const float step = p.col_on && t0 + q < t_end ? (s.softplus ? softplus_f(raw) : raw) : 0.f;
-          const float g = to_f32(dy[i].e[e]);
-          s_d[q * CH + p.col + e] = make_float4(step, step * to_f32(x[i].e[e]), gate ? g * gate_f(to_f32(z[i].e[e])) : g, 0.f);
-        }
-      }
+      const int q = p.row + i * P::ROWS, t = t0 + q;
+      const bool ok = p.col_on && t < s.S;
+      const int at = q * CH + p.col;
+      if (q >= SSM_TT) continue;
+      const int tc = ok ? t : 0, cc = ok ? p.dcol : 0;   // (an address that exists, where nothing is read)
+      copy_async<T, V>(dst + at, static_cast<const T*>(k.in.x) + p.b * s.xb + tc * s.xt + cc, ok);
+      copy_async<T, V>(dst + M::RAW + at, static_cast<const T*>(k.in.dt) + p.b * s.db + tc * s.dt + cc, ok);
+      if (gate) copy_async<T, V>(dst + 2 * M::RAW + at, static_cast<const T*>(k.in.z) + p.b * s.zb + tc * s.zt + cc, ok);
+      copy_async<T, V>(dst + 3 * M::RAW + at, static_cast<const T*>(k.dy) + p.b * s.gb + tc * s.gt + cc, ok);
     }
-    f.put_bc(s_b, s_c);
-    __syncthreads();
-    float h[SSM_TT][4];
-    float hb[4] = {h0.e[0], h0.e[1], h0.e[2], h0.e[3]};   // before the tile
-    if (t0 > t_begin) {
-      f.load(k.in, k.dy, s, p, t0 - SSM_TT, true);
-      if (p.on) h0 = load_pack<float, 4>(ck + (size_t)(t0 / SSM_TT - 1) * s.D * NP);
+  };
+  auto param = [&](const float* v, float (&o)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = v != nullptr && p.col_on ? v[p.dcol + i] : 0.f;
+  };
+  SsmFetchBC<T, LN, V, true> f;
+  copy(t_last);
+  f.load(k.in, s, p, t_last);
+  float* bc = k.part_bc + ((size_t)(p.g * s.tiles + p.tile) * s.B + p.b) * s.S * (2 * NP);
+  uint64_t h0[2][2] = {{0ull, 0ull}, {0ull, 0ull}};   // before the tile
+  auto checkpoint = [&](int t0) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (!p.on[c]) continue;
+      const Pack<uint64_t, 2> l =
+          load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub));
+      h0[c][0] = l.e[0]; h0[c][1] = l.e[1];
     }
+  };
+  checkpoint(t_last);
+  for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
+    const T* raw = s_raw + (t0 / SSM_TT & 1) * 4 * M::RAW;
+    cp_wait();
+    {
+      float bias[V];
+      param(k.in.dt_bias, bias);
 #pragma unroll
-    for (int t = 0; t < SSM_TT; t += TB) {
-      float acc[TB];
+      for (int i = 0; i < P::ITEMS; ++i) {
+        const int q = p.row + i * P::ROWS, at = q * CH + p.col;
+        if (q >= SSM_TT) continue;
+        float xv[V], dt[V], step[V];
+        unpack(load_pack<T, V>(raw + at), xv);
+        unpack(load_pack<T, V>(raw + M::RAW + at), dt);
+        ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
+        Pack<float2, V> o;
 #pragma unroll
-      for (int u = 0; u < TB; ++u) {
-        const float4 q = s_d[(t + u) * CH + p.ch];
-        const float4 b = *reinterpret_cast<const float4*>(s_b + (t + u) * NP + 4 * p.sub);
-        const float bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[t + u][i] = fmaf(ex2(q.x * a2[i]), t + u == 0 ? hb[i] : h[t + u == 0 ? 0 : t + u - 1][i], q.y * bv[i]);
+        for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
+        store_pack<float2, V>(s_q + at, o);
+        float g[V];
+        unpack(load_pack<T, V>(raw + 3 * M::RAW + at), g);
         if (gate) {
-          const float4 c = *reinterpret_cast<const float4*>(s_c + (t + u) * NP + 4 * p.sub);
-          acc[u] = fmaf(c.x, h[t + u][0], fmaf(c.y, h[t + u][1], fmaf(c.z, h[t + u][2], c.w * h[t + u][3])));
+          float zv[V], sg[V];
+          unpack(load_pack<T, V>(raw + 2 * M::RAW + at), zv);
+          logistic_v<V>(zv, sg);
+#pragma unroll
+          for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
         }
-      }
-      if (gate) {
-        const float v = lane_sums<LN, TB>(acc, p.sub);
-        if (p.sub % REP == 0) s_yp[(t + p.sub / REP) * P::YS + p.ch] = v;
+        store_pack<float, V>(s_g + at, pack<float, V>(g));
       }
     }
+    f.put(s_b, s_c);
+    __syncthreads();
+    uint64_t hb[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}}, hm[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}};
+    if (t0 > t_begin) {
+      copy(t0 - SSM_TT);
+      f.load(k.in, s, p, t0 - SSM_TT);
+      checkpoint(t0 - SSM_TT);
+    }
+    // one token onwards, for both channels
+    auto onward = [&](int t, const uint64_t (&from)[2][2], uint64_t (&to)[2][2]) {
+      const float4 q = *reinterpret_cast<const float4*>(s_q + t * CH + p.ch);
+      const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + t * NP + 4 * p.sub);
+      const float qs[2] = {q.x, q.z}, qx[2] = {q.y, q.w};
 #pragma unroll
-    for (int tb = SSM_TT - TB; tb >= 0; tb -= TB) {
-      float acc1[TB], acc2[TB];
+      for (int c = 0; c < 2; ++c) {
+        const uint64_t step = f2(qs[c], qs[c]), sx = f2(qx[c], qx[c]);
+        to[c][0] = fma2(ex2_pair(mul2(step, a2[c][0])), from[c][0], mul2(sx, b.x));
+        to[c][1] = fma2(ex2_pair(mul2(step, a2[c][1])), from[c][1], mul2(sx, b.y));
+      }
+    };
+    // The states of eight tokens are kept at a time: first through the tile's first half without keeping any.
+    const bool full = t0 + HALF < t_end;
+    if (full) {
+#pragma unroll 4
+      for (int t = 0; t < HALF; ++t) onward(t, hm, hm);
+    }
+#pragma unroll 1
+    for (int half = full ? HALF : 0; half >= 0; half -= HALF) {
+      uint64_t h[HALF + 1][2][2];
 #pragma unroll
-      for (int u = TB - 1; u >= 0; --u) {
-        const int t = tb + u;
-        const float4 q = s_d[t * CH + p.ch];
-        const float4 b = *reinterpret_cast<const float4*>(s_b + t * NP + 4 * p.sub);
-        const float4 c = *reinterpret_cast<const float4*>(s_c + t * NP + 4 * p.sub);
-        const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
-        float v[8];
-        acc1[u] = acc2[u] = 0.f;
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float g = fmaf(q.z, cv[i], r[i]);
-          acc1[u] = fmaf(g, bv[i], acc1[u]);
-          r[i] = ex2(q.x * a2[i]) * g;
-          const float w = r[i] * (t == 0 ? hb[i] : h[t == 0 ? 0 : t - 1][i]);
-          acc2[u] = fmaf(a2[i], w, acc2[u]);
-          da[i] = fmaf(q.x, w, da[i]);
-          v[i] = q.y * g;
-          v[4 + i] = q.z * h[t][i];
+        for (int i = 0; i < 2; ++i) h[0][c][i] = half ? hm[c][i] : hb[c][i];
+#pragma unroll
+      for (int t = 0; t < HALF; t += 2) {
+        float acc[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          onward(half + t + u, h[t + u], h[t + u + 1]);
+          if (gate) {
+            const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + (half + t + u) * NP + 4 * p.sub);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float lo, hi;
+              unf2(fma2(c2.x, h[t + u + 1][c][0], mul2(c2.y, h[t + u + 1][c][1])), lo, hi);
+              acc[u * 2 + c] = lo + hi;
+            }
+          }
         }
+        if (gate) {
+          const int first = Sums::run(acc, p.sub);
+          if (p.sub % Sums::SAME == 0) {
+#pragma unroll
+            for (int j = 0; j < Sums::LEFT; ++j) s_yp[(half + t + (first + j) / 2) * P::YS + p.ch + (first + j) % 2] = acc[j];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = HALF - 1; u >= 0; --u) {
+        const int t = half + u;
+        const float4 q = *reinterpret_cast<const float4*>(s_q + t * CH + p.ch);
+        const float2 dg = *reinterpret_cast<const float2*>(s_g + t * CH + p.ch);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + t * NP + 4 * p.sub);
+        const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + t * NP + 4 * p.sub);
+        const float qs[2] = {q.x, q.z}, qx[2] = {q.y, q.w}, qg[2] = {dg.x, dg.y};
+        float acc[4], v[8];
+        uint64_t vb[2], vc[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint64_t step = f2(qs[c], qs[c]), sx = f2(qx[c], qx[c]), dout = f2(qg[c], qg[c]);
+          const uint64_t g0 = fma2(dout, c2.x, r[c][0]), g1 = fma2(dout, c2.y, r[c][1]);
+          float lo, hi;
+          unf2(fma2(g0, b.x, mul2(g1, b.y)), lo, hi);
+          acc[c] = lo + hi;
+          r[c][0] = mul2(ex2_pair(mul2(step, a2[c][0])), g0);
+          r[c][1] = mul2(ex2_pair(mul2(step, a2[c][1])), g1);
+          const uint64_t w0 = mul2(r[c][0], h[u][c][0]), w1 = mul2(r[c][1], h[u][c][1]);
+          unf2(fma2(a2[c][0], w0, mul2(a2[c][1], w1)), lo, hi);
+          acc[2 + c] = lo + hi;
+          da[c][0] = fma2(step, w0, da[c][0]);
+          da[c][1] = fma2(step, w1, da[c][1]);
+          vb[0] = c == 0 ? mul2(sx, g0) : fma2(sx, g0, vb[0]);
+          vb[1] = c == 0 ? mul2(sx, g1) : fma2(sx, g1, vb[1]);
+          vc[0] = c == 0 ? mul2(dout, h[u + 1][c][0]) : fma2(dout, h[u + 1][c][0], vc[0]);
+          vc[1] = c == 0 ? mul2(dout, h[u + 1][c][1]) : fma2(dout, h[u + 1][c][1], vc[1]);
+        }
+        const int from = Sums::run(acc, p.sub);
+        if (p.sub % Sums::SAME == 0) {
+#pragma unroll
+          for (int j = 0; j < Sums::LEFT; ++j) s_sum[((from + j) / 2 * SSM_TT + t) * P::YS + p.ch + (from + j) % 2] = acc[j];
+        }
+        unf2(vb[0], v[0], v[1]); unf2(vb[1], v[2], v[3]);
+        unf2(vc[0], v[4], v[5]); unf2(vc[1], v[6], v[7]);
         // over the channels of the warp: each step halves the values that a lane still carries
         int first = 0;
 #pragma unroll
@@ -240,67 +362,83 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
             s_part[((p.warp * TF + t % TF) * 2 + e / 4) * NP + 4 * p.sub + e % 4] = v[j];
           }
         }
-        if (t % TF == 0) {   // TF tokens are there: over the warps
+        if (TF <= HALF ? u % TF == 0 : (u == 0 && half == 0)) {   // TF tokens are there (or all that the tile has): over the warps
           __syncthreads();
           for (int e = threadIdx.x; e < TF * 2 * NP; e += SSM_THREADS) {
             float a = 0.f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) a += s_part[w * TF * 2 * NP + e];
+            for (int w = 0; w < SSM_WARPS; ++w) a += s_part[w * TF * 2 * NP + e];
             const int tt = t0 + t + e / (2 * NP);
             if (tt < t_end) bc[(size_t)tt * (2 * NP) + e % (2 * NP)] = a;
           }
-          if (t > 0) __syncthreads();
+          __syncthreads();
         }
-      }
-      const float v1 = lane_sums<LN, TB>(acc1, p.sub), v2 = lane_sums<LN, TB>(acc2, p.sub);
-      if (p.sub % REP == 0) {
-        s_s1[(tb + p.sub / REP) * P::YS + p.ch] = v1;
-        s_s2[(tb + p.sub / REP) * P::YS + p.ch] = v2;
       }
     }
-    __syncthreads();
+    float bias[V], skip[V];
+    param(k.in.dt_bias, bias);
+    param(k.in.skip, skip);
 #pragma unroll
     for (int i = 0; i < P::ITEMS; ++i) {
-      const int q = p.row + i * P::ROWS, t = t0 + q;
+      const int q = p.row + i * P::ROWS, t = t0 + q, at = q * CH + p.col;
       if (!p.col_on || t >= t_end) continue;
-      Pack<T, V> ox, ot, oz;
+      float xv[V], dt[V], dout[V], s1[V], s2[V], o[V];
+      unpack(load_pack<T, V>(raw + at), xv);
+      unpack(load_pack<T, V>(raw + M::RAW + at), dt);
+      unpack(load_pack<float, V>(s_g + at), dout);
+      unpack(load_pack<float, V>(s_sum + q * P::YS + p.col), s1);
+      unpack(load_pack<float, V>(s_sum + (SSM_TT + q) * P::YS + p.col), s2);
+      const size_t out = ((size_t)p.b * s.S + t) * s.D + p.dcol;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float4 d4 = s_d[q * CH + p.col + e];
-        const float s1 = s_s1[q * P::YS + p.col + e], s2 = s_s2[q * P::YS + p.col + e] * kLn2;
-        const float xv = to_f32(x[i].e[e]);
-        ox.e[e] = from_f32<T>(fmaf(d4.x, s1, skip[e] * d4.z));
-        float ddt = fmaf(xv, s1, s2);
-        if (s.softplus) ddt *= logistic_f(to_f32(dt[i].e[e]) + bias[e]);
-        ot.e[e] = from_f32<T>(ddt);
-        dbias[e] += ddt;
-        dskip[e] = fmaf(d4.z, xv, dskip[e]);
-        if (gate) {
-          const float zz = to_f32(z[i].e[e]), sg = logistic_f(zz);
-          oz.e[e] = from_f32<T>(to_f32(dy[i].e[e]) * fmaf(skip[e], xv, s_yp[q * P::YS + p.col + e]) * sg * fmaf(zz, 1.f - sg, 1.f));
-        }
+        o[e] = fmaf(s_q[at + e].x, s1[e], skip[e] * dout[e]);
+        dskip[e] = fmaf(dout[e], xv[e], dskip[e]);
       }
-      const size_t at = ((size_t)p.b * s.S + t) * s.D + p.dcol;
-      store_pack<T, V>(static_cast<T*>(k.dx) + at, ox);
-      store_pack<T, V>(static_cast<T*>(k.ddt) + at, ot);
-      if (gate) store_pack<T, V>(static_cast<T*>(k.dz) + at, oz);
+      store_pack<T, V>(static_cast<T*>(k.dx) + out, pack<T, V>(o));
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = fmaf(xv[e], s1[e], s2[e] * kLn2);
+      if (s.softplus) {
+        float sg[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) dt[e] += bias[e];
+        logistic_v<V>(dt, sg);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] *= sg[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) dbias[e] += o[e];
+      store_pack<T, V>(static_cast<T*>(k.ddt) + out, pack<T, V>(o));
+      if (gate) {
+        float zv[V], g[V], sg[V], yp[V];
+        unpack(load_pack<T, V>(raw + 2 * M::RAW + at), zv);
+        unpack(load_pack<T, V>(raw + 3 * M::RAW + at), g);
+        unpack(load_pack<float, V>(s_yp + q * P::YS + p.col), yp);
+        logistic_v<V>(zv, sg);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = g[e] * fmaf(skip[e], xv[e], yp[e]) * sg[e] * fmaf(zv[e], 1.f - sg[e], 1.f);
+        store_pack<T, V>(static_cast<T*>(k.dz) + out, pack<T, V>(o));
+      }
     }
     __syncthreads();   // the tile's arrays are free
   }
   const size_t row = (size_t)p.b * s.nseg + p.seg;
-  if (p.on) {
-    Pack<float, 4> o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.e[i] = da[i];
-    store_pack<float, 4>(k.part_a + (row * s.D + p.d) * NP + 4 * p.sub, o);
+  for (int c = 0; c < 2; ++c) {
+    if (!p.on[c]) continue;
+    Pack<uint64_t, 2> o;
+    o.e[0] = da[c][0]; o.e[1] = da[c][1];
+    store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.part_a + (row * s.D + p.d + c) * NP + 4 * p.sub), o);
     if (k.dh0 != nullptr && p.seg == 0) {
+      float v[4];
+      unf2(r[c][0], v[0], v[1]);
+      unf2(r[c][1], v[2], v[3]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (4 * p.sub + i < s.N) k.dh0[((size_t)p.b * s.D + p.d) * s.N + 4 * p.sub + i] = r[i];
+        if (4 * p.sub + i < s.N) k.dh0[((size_t)p.b * s.D + p.d + c) * s.N + 4 * p.sub + i] = v[i];
     }
   }
   // dskip and ddt_bias: over the threads that share a channel
-  float* s_x = sm;
+  float* s_x = reinterpret_cast<float*>(sm);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     if (p.row < SSM_TT) {
@@ -390,11 +528,11 @@ size_t ssm_bw_bytes(int B, int S, int D, int N, int G) { return ssm_bw_layout(ss
 
 template <typename T, int LN, int V>
 static int ssm_bw_t(const SsmBw& k, const SsmDims& s, cudaStream_t st) {
-  const unsigned grid = (unsigned)s.B * s.nseg * s.G * s.tiles;
+  const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
-  if (s.nseg > 1)
-    if (int rc = launch_pdl(overlap, ssm_bw_local_kernel<T, LN, V>, grid, SSM_THREADS, 0, st, k, s)) return rc;
-  constexpr size_t smem = SsmBwSmem<LN, V>::BYTES;
+  if (s.nseg > 1)   // the first segment leaves nothing to another
+    if (int rc = launch_pdl(overlap, ssm_bw_local_kernel<T, LN, V>, per_seg * (s.nseg - 1), SSM_THREADS, 0, st, k, s, s.nseg - 1)) return rc;
+  constexpr size_t smem = SsmBwSmem<T, LN, V>::BYTES;
   auto kern = ssm_bw_kernel<T, LN, V>;
   if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return launch_pdl(overlap, kern, grid, SSM_THREADS, smem, st, k, s);

@@ -21,41 +21,33 @@ struct SsmFw {
   float* loc_sum;      // (B, nseg, D) sums of their steps
 };
 
-// The state before segment p.seg
-template <int LN, int V>
-__device__ __forceinline__ void ssm_enter(const SsmFw& k, const SsmDims& s, const SsmPlace<LN, V>& p, const float (&a2)[4], float (&h)[4]) {
-  constexpr int NP = 4 * LN;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    h[i] = k.in.h0 != nullptr && p.on && 4 * p.sub + i < s.N ? k.in.h0[((size_t)p.b * s.D + p.d) * s.N + 4 * p.sub + i] : 0.f;
-  if (!p.on) return;
-  for (int j = 0; j < p.seg; ++j) {
-    const size_t at = ((size_t)p.b * s.nseg + j) * s.D + p.d;
-    const float sum = k.loc_sum[at];
-    const Pack<float, 4> l = load_pack<float, 4>(k.loc_h + at * NP + 4 * p.sub);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = fmaf(ex2(sum * a2[i]), h[i], l.e[i]);
-  }
-}
-
 // LOCAL: only a segment's own end state and sum of steps
 template <typename T, int LN, int V, bool LOCAL>
-__global__ void __launch_bounds__(SSM_THREADS, 3)
-ssm_fw_kernel(SsmFw k, SsmDims s) {
+__global__ void __launch_bounds__(SSM_THREADS, 5)
+ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   using P = SsmPlace<LN, V>;
-  constexpr int CH = P::CH, NP = P::NP, TB = LN < 8 ? LN : 8;
-  __shared__ float2 s_d[SSM_TT * CH];                          // (step, step x)
+  using Sums = LaneSums<LN>;
+  constexpr int CH = P::CH, NP = P::NP;
+  __shared__ __align__(16) float2 s_d[SSM_TT * CH];            // (step, step x)
   __shared__ __align__(16) float s_b[SSM_TT * NP];
   __shared__ __align__(16) float s_c[LOCAL ? 4 : SSM_TT * NP];
   __shared__ __align__(16) float s_y[LOCAL ? 4 : SSM_TT * P::YS];
   pdl_launch_dependents();
   pdl_wait();
-  const P p(s);
-  float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  ssm_rates<LN>(k.in.a, s, p.d, p.sub, p.on, a2);
-  if (!LOCAL) ssm_enter<LN, V>(k, s, p, a2, h);
-  uint64_t h01 = f2(h[0], h[1]), h23 = f2(h[2], h[3]);
-  const uint64_t a01 = f2(a2[0], a2[1]), a23 = f2(a2[2], a2[3]);
+  const P p(s, nseg, 0);
+  uint64_t a2[2][2], h[2][2] = {{0ull, 0ull}, {0ull, 0ull}};
+  uint64_t sum = 0ull;
+  ssm_rates<LN, V>(k.in.a, s, p, a2);
+  if (!LOCAL) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (k.in.h0 != nullptr && p.on[c]) ssm_load4(k.in.h0 + ((size_t)p.b * s.D + p.d + c) * s.N, s.N, 4 * p.sub, v);
+      h[c][0] = f2(v[0], v[1]);
+      h[c][1] = f2(v[2], v[3]);
+    }
+    ssm_fold<LN, V, false>(k.loc_h, k.loc_sum, 0, p.seg, s, p, a2, h);
+  }
   float bias[V], skip[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -63,106 +55,141 @@ ssm_fw_kernel(SsmFw k, SsmDims s) {
     skip[i] = !LOCAL && k.in.skip != nullptr && p.col_on ? k.in.skip[p.dcol + i] : 0.f;
   }
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
-  SsmFetch<T, LN, V, false, !LOCAL> f;
-  f.load(k.in, nullptr, s, p, t_begin, !LOCAL);
+  const bool gate = !LOCAL && k.in.z != nullptr;
+  Pack<T, V> nx[P::ITEMS], ndt[P::ITEMS], nz[P::ITEMS];
+  SsmFetchBC<T, LN, V, !LOCAL> f;
+  auto fetch = [&](int t0) {
+    const T *xp = static_cast<const T*>(k.in.x) + p.b * s.xb + p.dcol, *tp = static_cast<const T*>(k.in.dt) + p.b * s.db + p.dcol;
+    const T* zp = static_cast<const T*>(k.in.z) + p.b * s.zb + p.dcol;
+#pragma unroll
+    for (int i = 0; i < P::ITEMS; ++i) {
+      const int t = t0 + p.row + i * P::ROWS;
+      const bool ok = p.col_on && t < s.S;
+      nx[i] = ok ? load_pack<T, V>(xp + t * s.xt) : zero_pack<T, V>();
+      ndt[i] = ok ? load_pack<T, V>(tp + t * s.dt) : zero_pack<T, V>();
+      if (gate) nz[i] = ok ? load_pack<T, V>(zp + t * s.zt) : zero_pack<T, V>();
+    }
+    f.load(k.in, s, p, t0);
+  };
+  fetch(t_begin);
   for (int t0 = t_begin; t0 < t_end; t0 += SSM_TT) {
     Pack<T, V> x[P::ITEMS], z[P::ITEMS];
 #pragma unroll
     for (int i = 0; i < P::ITEMS; ++i) {
-      x[i] = f.x[i];
-      z[i] = f.z[i];
+      x[i] = nx[i];
+      z[i] = nz[i];
       const int r = p.row + i * P::ROWS;
       if (r < SSM_TT) {
+        float dt[V], step[V], xv[V];
+        unpack(ndt[i], dt);
+        unpack(x[i], xv);
+        ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + r < t_end, step);
+        Pack<float2, V> o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float raw = to_f32(f.dt[i].e[e]) + bias[e];
-          const float step = p.col_on && t0 + r < t_end ? (s.softplus ? softplus_f(raw) : raw) : 0.f;   // nothing moves past the end
-          s_d[r * CH + p.col + e] = make_float2(step, step * to_f32(x[i].e[e]));
-        }
+        for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
+        store_pack<float2, V>(s_d + r * CH + p.col, o);
       }
     }
-    f.put_bc(s_b, s_c);
+    f.put(s_b, s_c);
     __syncthreads();
-    if (t0 + SSM_TT < t_end) f.load(k.in, nullptr, s, p, t0 + SSM_TT, !LOCAL);
-    if (!LOCAL && k.ckpt != nullptr && p.on) {
-      Pack<float, 4> o;
-      unf2(h01, o.e[0], o.e[1]);
-      unf2(h23, o.e[2], o.e[3]);
-      store_pack<float, 4>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d) * NP + 4 * p.sub, o);
+    if (t0 + SSM_TT < t_end) fetch(t0 + SSM_TT);
+    if (!LOCAL && k.ckpt != nullptr) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (!p.on[c]) continue;
+        Pack<uint64_t, 2> o;
+        o.e[0] = h[c][0]; o.e[1] = h[c][1];
+        store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub), o);
+      }
     }
+#pragma unroll(LOCAL ? 2 : 4)
+    for (int t = 0; t < SSM_TT; t += 2) {
+      float acc[4];
 #pragma unroll
-    for (int t = 0; t < SSM_TT; t += TB) {
-      float acc[TB];
-#pragma unroll
-      for (int u = 0; u < TB; ++u) {
-        const float2 q = s_d[(t + u) * CH + p.ch];
+      for (int u = 0; u < 2; ++u) {
+        const float4 q = *reinterpret_cast<const float4*>(s_d + (t + u) * CH + p.ch);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + (t + u) * NP + 4 * p.sub);
-        const uint64_t step = f2(q.x, q.x), sx = f2(q.y, q.y);
-        float e0, e1, e2, e3;
-        unf2(mul2(step, a01), e0, e1);
-        unf2(mul2(step, a23), e2, e3);
-        h01 = fma2(f2(ex2(e0), ex2(e1)), h01, mul2(sx, b.x));
-        h23 = fma2(f2(ex2(e2), ex2(e3)), h23, mul2(sx, b.y));
+        const float qs[2] = {q.x, q.z}, qx[2] = {q.y, q.w};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint64_t step = f2(qs[c], qs[c]), sx = f2(qx[c], qx[c]);
+          h[c][0] = fma2(ex2_pair(mul2(step, a2[c][0])), h[c][0], mul2(sx, b.x));
+          h[c][1] = fma2(ex2_pair(mul2(step, a2[c][1])), h[c][1], mul2(sx, b.y));
+        }
         if (LOCAL) {
-          sum += q.x;
+          sum = add2(sum, f2(q.x, q.z));
         } else {
-          const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(s_c + (t + u) * NP + 4 * p.sub);
-          float lo, hi;
-          unf2(fma2(c.x, h01, mul2(c.y, h23)), lo, hi);
-          acc[u] = lo + hi;
+          const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + (t + u) * NP + 4 * p.sub);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float lo, hi;
+            unf2(fma2(c2.x, h[c][0], mul2(c2.y, h[c][1])), lo, hi);
+            acc[u * 2 + c] = lo + hi;
+          }
         }
       }
       if (!LOCAL) {
-        const float v = lane_sums<LN, TB>(acc, p.sub);
-        if (p.sub % (LN / TB) == 0) s_y[(t + p.sub / (LN / TB)) * P::YS + p.ch] = v;
+        const int first = Sums::run(acc, p.sub);
+        if (p.sub % Sums::SAME == 0) {
+#pragma unroll
+          for (int j = 0; j < Sums::LEFT; ++j) s_y[(t + (first + j) / 2) * P::YS + p.ch + (first + j) % 2] = acc[j];
+        }
       }
     }
     __syncthreads();
     if (!LOCAL) {
-      T* yp = static_cast<T*>(k.y);
+      T* yp = static_cast<T*>(k.y) + (size_t)p.b * s.S * s.D + p.dcol;
 #pragma unroll
       for (int i = 0; i < P::ITEMS; ++i) {
         const int r = p.row + i * P::ROWS, t = t0 + r;
         if (!p.col_on || t >= t_end) continue;
-        Pack<T, V> o;
+        float xv[V], o[V];
+        unpack(x[i], xv);
+        const Pack<float, V> sums = load_pack<float, V>(s_y + r * P::YS + p.col);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float v = fmaf(skip[e], to_f32(x[i].e[e]), s_y[r * P::YS + p.col + e]);
-          if (k.in.z != nullptr) {
-            const float zz = to_f32(z[i].e[e]);
-            v *= zz * logistic_f(zz);
-          }
-          o.e[e] = from_f32<T>(v);
+        for (int e = 0; e < V; ++e) o[e] = fmaf(skip[e], xv[e], sums.e[e]);
+        if (gate) {
+          float zv[V], sg[V];
+          unpack(z[i], zv);
+          logistic_v<V>(zv, sg);
+#pragma unroll
+          for (int e = 0; e < V; ++e) o[e] *= zv[e] * sg[e];
         }
-        store_pack<T, V>(yp + ((size_t)p.b * s.S + t) * s.D + p.dcol, o);
+        store_pack<T, V>(yp + (size_t)t * s.D, pack<T, V>(o));
       }
     }
   }
-  unf2(h01, h[0], h[1]);
-  unf2(h23, h[2], h[3]);
-  if (!p.on) return;
-  if (LOCAL) {
-    const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d;
-    Pack<float, 4> o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.e[i] = h[i];
-    store_pack<float, 4>(k.loc_h + at * NP + 4 * p.sub, o);
-    if (p.sub == 0) k.loc_sum[at] = sum;
-  } else if (k.h_last != nullptr && p.seg == s.nseg - 1) {
+  for (int c = 0; c < 2; ++c) {
+    if (!p.on[c]) continue;
+    if (LOCAL) {
+      const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d + c;
+      Pack<uint64_t, 2> o;
+      o.e[0] = h[c][0]; o.e[1] = h[c][1];
+      store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.loc_h + at * NP + 4 * p.sub), o);
+      float s0, s1;
+      unf2(sum, s0, s1);
+      if (p.sub == 0) k.loc_sum[at] = c == 0 ? s0 : s1;
+    } else if (k.h_last != nullptr && p.seg == s.nseg - 1) {
+      float v[4];
+      unf2(h[c][0], v[0], v[1]);
+      unf2(h[c][1], v[2], v[3]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * p.sub + i < s.N) k.h_last[((size_t)p.b * s.D + p.d) * s.N + 4 * p.sub + i] = h[i];
+      for (int i = 0; i < 4; ++i)
+        if (4 * p.sub + i < s.N) k.h_last[((size_t)p.b * s.D + p.d + c) * s.N + 4 * p.sub + i] = v[i];
+    }
   }
 }
 
 // One token: bound by the states, in and out once each, 16 bytes a thread (VEC; else element by element).
+constexpr int STEP_THREADS_SSM = 256;
 template <typename T, int LN, bool VEC>
-__global__ void __launch_bounds__(SSM_THREADS)
+__global__ void __launch_bounds__(STEP_THREADS_SSM)
 ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, const float* a, const float* skip, const float* dt_bias,
                 const float* h, T* y, float* h_new, int B, int D, int N, int G, bool softplus) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int CH = SSM_THREADS / LN;
+  constexpr int CH = STEP_THREADS_SSM / LN;
   const int sub = threadIdx.x % LN;
   const size_t row = (size_t)blockIdx.x * CH + threadIdx.x / LN;   // of (B, D)
   const bool on = row < (size_t)B * D;
@@ -187,8 +214,10 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
       }
     }
     xv = to_f32(x[row]);
-    const float raw = to_f32(dt[row]) + (dt_bias != nullptr ? dt_bias[d] : 0.f);
-    step = softplus ? softplus_f(raw) : raw;
+    const float raw[1] = {to_f32(dt[row])}, bias[1] = {dt_bias != nullptr ? dt_bias[d] : 0.f};
+    float st[1];
+    ssm_step_v<1>(raw, bias, softplus, true, st);
+    step = st[0];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool ok = 4 * sub + i < N;
@@ -221,27 +250,25 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
 bool ssm_sizes_ok(int B, int S, int D, int N, int G) {
   if (B <= 0 || S <= 0 || D <= 0 || N <= 0 || N > SSM_MAX_N || G <= 0 || D % G != 0) return false;
   if (S > (1 << 30) || (long long)D * N >= (1ll << 31)) return false;
-  const int ch = SSM_THREADS / ssm_lanes(N), Dg = D / G;
+  const int ch = 2 * SSM_THREADS / ssm_lanes(N), Dg = D / G;
   return (long long)B * G * ceil_div(Dg, ch) * 64 < (1ll << 31);
 }
 
-// Segments: none while the CTAs of whole sequences give every SM work; two cost as much as they gain (each exponential is then
-// taken twice), so at least three.
+// Segments: as many as fit the GPU at once, none where whole sequences fill more than half of it.
 static int ssm_segments(long long ctas, int nt, int per_sm) {
-  const long long room = (long long)per_sm * sm_count();
-  long long n = room / ctas;
+  long long n = (long long)per_sm * sm_count() / ctas;
   if (n > nt / 4) n = nt / 4;      // four tiles each at least
   if (n > 64) n = 64;
-  return n < 3 ? 1 : (int)n;
+  return n < 2 ? 1 : (int)n;
 }
 
 SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* st, bool backward) {
   SsmDims s{};
   s.B = B; s.S = S; s.D = D; s.N = N; s.G = G;
   s.Dg = D / G;
-  s.tiles = ceil_div(s.Dg, SSM_THREADS / ssm_lanes(N));
+  s.tiles = ceil_div(s.Dg, 2 * SSM_THREADS / ssm_lanes(N));
   s.nt = ceil_div(S, SSM_TT);
-  const int n = ssm_segments((long long)B * G * s.tiles, s.nt, backward ? 2 : 3);
+  const int n = ssm_segments((long long)B * G * s.tiles, s.nt, backward ? 3 : 5);
   s.seg = ceil_div(s.nt, n) * SSM_TT;
   s.nseg = ceil_div(S, s.seg);
   s.softplus = softplus;
@@ -277,11 +304,11 @@ template bool ssm_vec<__half>(const SsmIn&, const SsmDims&, const void*, const v
 
 template <typename T, int LN, int V>
 static int ssm_fw_t(const SsmFw& k, const SsmDims& s, cudaStream_t st) {
-  const unsigned grid = (unsigned)s.B * s.nseg * s.G * s.tiles;
+  const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
-  if (s.nseg > 1)
-    if (int rc = launch_pdl(overlap, ssm_fw_kernel<T, LN, V, true>, grid, SSM_THREADS, 0, st, k, s)) return rc;
-  return launch_pdl(overlap, ssm_fw_kernel<T, LN, V, false>, grid, SSM_THREADS, 0, st, k, s);
+  if (s.nseg > 1)   // the last segment leaves nothing to another
+    if (int rc = launch_pdl(overlap, ssm_fw_kernel<T, LN, V, true>, per_seg * (s.nseg - 1), SSM_THREADS, 0, st, k, s, s.nseg - 1)) return rc;
+  return launch_pdl(overlap, ssm_fw_kernel<T, LN, V, false>, grid, SSM_THREADS, 0, st, k, s, s.nseg);
 }
 
 int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* workspace, int B, int S, int D, int N, int G,
@@ -306,11 +333,11 @@ int launch_ssm_step(const void* x, const void* dt, const void* z, const void* b,
   if (!ssm_sizes_ok(B, 1, D, N, G)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_STEP, st);
   const int lanes = ssm_lanes(N);
-  const size_t grid = ((size_t)B * D + SSM_THREADS / lanes - 1) / (SSM_THREADS / lanes);
+  const size_t grid = ((size_t)B * D + STEP_THREADS_SSM / lanes - 1) / (STEP_THREADS_SSM / lanes);
   if (grid >= (1ull << 31)) return MLSTM_ERR_SHAPE;
   const bool vec = N % 4 == 0 && fits_access(a, 16) && fits_access(h, 16) && fits_access(h_new, 16);
 #define RUN(LN, VEC)                                                                                                                              \
-  return launch_pdl(grid <= pdl_max_ctas(), ssm_step_kernel<T, LN, VEC>, (unsigned)grid, SSM_THREADS, 0, st, (const T*)x, (const T*)dt, (const T*)z, \
+  return launch_pdl(grid <= pdl_max_ctas(), ssm_step_kernel<T, LN, VEC>, (unsigned)grid, STEP_THREADS_SSM, 0, st, (const T*)x, (const T*)dt, (const T*)z, \
                     (const T*)b, (const T*)c, a, skip, dt_bias, h, (T*)y, h_new, B, D, N, G, softplus)
   MLSTM_DTYPE_SWITCH(dtype, T, SSM_LANES_SWITCH(lanes, LN, if (vec) RUN(LN, true); RUN(LN, false);))
 #undef RUN

@@ -1,6 +1,7 @@
 // Several neighbouring elements in one access, and parameters whose element type is known at run time only.
 #pragma once
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace mlstm {
 
@@ -82,20 +83,59 @@ __device__ __forceinline__ float exp_f(float x) {
   return fmaf(e * r, kLn2, e);
 }
 __device__ __forceinline__ float logistic_f(float x) { return rcp(1.f + exp_f(-x)); }
-// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|; log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, by its series: the terms
-// left out are below 2^-29 of the sum, and a small e keeps all its digits
-__device__ __forceinline__ float softplus_f(float x) {
-  const float e = exp_f(-fabsf(x));
-  const float s = e * rcp(2.f + e), q = s * s;
-  float p = 1.f / 15.f;
-  p = fmaf(p, q, 1.f / 13.f);
-  p = fmaf(p, q, 1.f / 11.f);
-  p = fmaf(p, q, 1.f / 9.f);
-  p = fmaf(p, q, 1.f / 7.f);
-  p = fmaf(p, q, 1.f / 5.f);
-  p = fmaf(p, q, 1.f / 3.f);
-  p = fmaf(p, q, 1.f);
-  return fmaf(2.f * s, p, max_nan(x, 0.f));
+// The same for pairs of values, in packed instructions where there are any.
+__device__ __forceinline__ uint64_t exp_pair(float x0, float x1) {
+  x0 = min_nan(max_nan(x0, -1e4f), 88.f); x1 = min_nan(max_nan(x1, -1e4f), 88.f);
+  const uint64_t x = f2(x0, x1), m = mul2(x, f2(-kLog2e, -kLog2e));
+  const uint64_t r = fma2(x, f2(kLog2eRest, kLog2eRest), fma2(x, f2(kLog2e, kLog2e), m));
+  float m0, m1;
+  unf2(m, m0, m1);
+  const uint64_t e = f2(ex2(-m0), ex2(-m1));
+  return fma2(mul2(e, r), f2(kLn2, kLn2), e);
+}
+__device__ __forceinline__ uint64_t rcp_pair(uint64_t v) {
+  float a, b;
+  unf2(v, a, b);
+  return f2(rcp(a), rcp(b));
+}
+__device__ __forceinline__ uint64_t logistic_pair(float x0, float x1) { return rcp_pair(add2(f2(1.f, 1.f), exp_pair(-x0, -x1))); }
+// log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|; log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, which keeps all digits of a
+// small e.  artanh(s) / s as a polynomial in s^2, through its values at the Chebyshev points of [0, 1/9]: off by 2^-26.
+__device__ __forceinline__ uint64_t softplus_pair(float x0, float x1) {
+  const uint64_t e = exp_pair(-fabsf(x0), -fabsf(x1));
+  const uint64_t s = mul2(e, rcp_pair(add2(e, f2(2.f, 2.f)))), q = mul2(s, s);
+  uint64_t p = fma2(f2(0.14078890f, 0.14078890f), q, f2(0.13982579f, 0.13982579f));
+  p = fma2(p, q, f2(0.20012298f, 0.20012298f));
+  p = fma2(p, q, f2(0.33333161f, 0.33333161f));
+  p = fma2(p, q, f2(1.f, 1.f));
+  return fma2(add2(s, s), p, f2(max_nan(x0, 0.f), max_nan(x1, 0.f)));
+}
+template <int V> __device__ __forceinline__ void logistic_v(const float (&x)[V], float (&o)[V]) {
+  if constexpr (V == 1) {
+    o[0] = logistic_f(x[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) unf2(logistic_pair(x[i], x[i + 1]), o[i], o[i + 1]);
+  }
+}
+template <int V> __device__ __forceinline__ void softplus_v(const float (&x)[V], float (&o)[V]) {
+  if constexpr (V == 1) {
+    float other;
+    unf2(softplus_pair(x[0], x[0]), o[0], other);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) unf2(softplus_pair(x[i], x[i + 1]), o[i], o[i + 1]);
+  }
+}
+template <typename T, int V> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&o)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = to_f32(p.e[i]);
+}
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> pack(const float (&o)[V]) {
+  Pack<T, V> p;
+#pragma unroll
+  for (int i = 0; i < V; ++i) p.e[i] = from_f32<T>(o[i]);
+  return p;
 }
 
 #define MLSTM_DTYPE_SWITCH(code, T, ...)                                            \
