@@ -20,6 +20,7 @@ struct SsmDims {
   int nseg, seg;          // the sequence in nseg segments of seg tokens (a multiple of SSM_TT), each a CTA of its own
   int nt;                 // tiles of SSM_TT tokens in the sequence
   bool softplus;
+  bool pairs;             // elements of b and c may be fetched two at a time
   // strides in elements (batch, token; and of b and c the group too); the last axis is contiguous
   long long xb, xt, db, dt, zb, zt, bb, bt, bg, cb, ct, cg, gb, gt;   // x, dt, z, b, c, dy
 };
@@ -30,7 +31,7 @@ template <int LN, int V> struct SsmPlace {
   static constexpr int CH = 2 * SSM_THREADS / LN, NP = 4 * LN, LC = 32 / LN;
   static constexpr int PER_ROW = CH / V, ROWS = SSM_THREADS / PER_ROW;        // threads to a token; tokens at once
   static constexpr int ITEMS = ROWS >= SSM_TT ? 1 : SSM_TT / ROWS;
-  static constexpr int BC = (SSM_TT * NP + SSM_THREADS - 1) / SSM_THREADS;    // elements of b (and of c) a thread fetches
+  static constexpr int BC = (SSM_TT * NP / 2 + SSM_THREADS - 1) / SSM_THREADS;   // pairs of b's (and of c's) elements to a thread
   static constexpr int YS = CH + 16;                             // row of a (token, channel) array of sums: two tokens' in different banks
   int sub, chl, ch, warp, tile, g, seg, b, d;
   bool on[2];
@@ -55,29 +56,74 @@ template <int LN, int V> struct SsmPlace {
   }
 };
 
-// b and c of a tile on their way from memory
-template <typename T, int LN, int V, bool WITH_C> struct SsmFetchBC {
+// V elements to shared memory: they arrive by a later cp_wait(), zeros where `ok` is false (the address must exist even so).
+// Accesses below four bytes, which cannot be asynchronous, are made at once.
+template <typename T, int V> __device__ __forceinline__ void copy_async(T* dst, const T* src, bool ok) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES >= 4) {
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0) : "memory");
+  } else {
+    store_pack<T, V>(dst, ok ? load_pack<T, V>(src) : zero_pack<T, V>());
+  }
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The operands of STAGES tiles on their way from memory: ARRS arrays of (token, channel), BCS of (token, state).  Each thread
+// copies just what it reads itself, so that its own wait is all that it takes.
+template <typename T, int LN, int V, int ARRS, int BCS> struct SsmRing {
   using P = SsmPlace<LN, V>;
-  T b[P::BC], c[WITH_C ? P::BC : 1];
-  __device__ __forceinline__ void load(const SsmIn& in, const SsmDims& s, const P& p, int t0) {
-    const T *bp = static_cast<const T*>(in.b) + p.b * s.bb + p.g * s.bg, *cp = static_cast<const T*>(in.c) + p.b * s.cb + p.g * s.cg;
+  static constexpr int RAW = SSM_TT * P::CH, BCN = SSM_TT * P::NP, STAGE = ARRS * RAW + BCS * BCN;
+  static constexpr int STAGES = sizeof(T) * P::CH >= 256 ? 2 : 4;   // as many as leave shared memory for the CTAs that registers allow
+  static constexpr size_t BYTES = sizeof(T) * STAGE * STAGES;
+  T* base;
+  __device__ __forceinline__ T* at(int tile) const { return base + (unsigned)tile % STAGES * STAGE; }
+  // array `i` of the tile of tokens t0 ...: src is the sequence's first element of channel p.dcol
+  __device__ __forceinline__ void copy(const SsmDims& s, const P& p, int t0, int i, const void* from, long long bstride, long long tstride) const {
+    T* dst = at(t0 / SSM_TT) + i * RAW;
+    const T* src = static_cast<const T*>(from) + p.b * bstride;
 #pragma unroll
-    for (int i = 0; i < P::BC; ++i) {
-      const int k = threadIdx.x + i * SSM_THREADS, n = k % P::NP, t = t0 + k / P::NP;
-      const bool ok = n < s.N && t < s.S && k < SSM_TT * P::NP;
-      b[i] = ok ? bp[t * s.bt + n] : from_f32<T>(0.f);
-      if (WITH_C) c[i] = ok ? cp[t * s.ct + n] : from_f32<T>(0.f);
+    for (int j = 0; j < P::ITEMS; ++j) {
+      const int q = p.row + j * P::ROWS;
+      if (q >= SSM_TT) continue;
+      const bool ok = p.col_on && t0 + q < s.S;
+      copy_async<T, V>(dst + q * P::CH + p.col, ok ? src + (t0 + q) * tstride + p.dcol : src, ok);
     }
   }
-  __device__ __forceinline__ void put(float* s_b, float* s_c) const {
+  __device__ __forceinline__ void copy_bc(const SsmDims& s, const P& p, int t0, int i, const void* from, long long bstride, long long tstride,
+                                          long long gstride) const {
+    T* dst = at(t0 / SSM_TT) + ARRS * RAW + i * BCN;
+    const T* src = static_cast<const T*>(from) + p.b * bstride + p.g * gstride;
 #pragma unroll
-    for (int i = 0; i < P::BC; ++i) {
-      const int k = threadIdx.x + i * SSM_THREADS;
-      if (k < SSM_TT * P::NP) {
-        s_b[k] = to_f32(b[i]);
-        if (WITH_C) s_c[k] = to_f32(c[i]);
+    for (int j = 0; j < P::BC; ++j) {
+      const int k = 2 * (threadIdx.x + j * SSM_THREADS), n = k % P::NP, t = t0 + k / P::NP;
+      if (k >= BCN) continue;
+      const bool in = t < s.S, ok0 = in && n < s.N, ok1 = in && n + 1 < s.N;
+      const T* a = ok0 ? src + t * tstride + n : src;
+      if (sizeof(T) == 2 && s.pairs) {
+        copy_async<T, 2>(dst + k, a, ok0);   // (an even number of states)
+      } else {
+        copy_async<T, 1>(dst + k, a, ok0);
+        copy_async<T, 1>(dst + k + 1, ok1 ? a + 1 : src, ok1);
       }
     }
+  }
+  // what copy_bc brought, as f32
+  __device__ __forceinline__ void put(int tile, int i, float* out) const {
+    const T* from = at(tile) + ARRS * RAW + i * BCN;
+#pragma unroll
+    for (int j = 0; j < P::BC; ++j) {
+      const int k = 2 * (threadIdx.x + j * SSM_THREADS);
+      if (k >= BCN) continue;
+      float v[2];
+      unpack(load_pack<T, 2>(from + k), v);
+      *reinterpret_cast<float2*>(out + k) = make_float2(v[0], v[1]);
+    }
+  }
+  // V channels of the thread's j-th token of array i
+  __device__ __forceinline__ void get(int tile, int i, int j, const P& p, float (&o)[V]) const {
+    unpack(load_pack<T, V>(at(tile) + i * RAW + (p.row + j * P::ROWS) * P::CH + p.col), o);
   }
 };
 
@@ -156,7 +202,13 @@ __device__ __forceinline__ void ssm_fold(const float* left, const float* sums, i
   }
 }
 
-// host: lanes to a channel
+// host
+template <typename... KArgs, typename... Args>
+int ssm_launch(void (*kern)(KArgs...), size_t smem, bool overlap, unsigned grid, cudaStream_t st, Args... args) {
+  if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  return launch_pdl(overlap, kern, grid, SSM_THREADS, smem, st, args...);
+}
+// lanes to a channel
 inline int ssm_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
 
 #define SSM_LANES_SWITCH(n, LN, ...)                  \

@@ -40,14 +40,25 @@ __device__ __forceinline__ void ssm_behind(const float* dh_last, const SsmDims& 
   }
 }
 
+// Shared memory of a segment's own adjoint, in bytes
+template <typename T, int LN, int V> struct SsmBwLocalSmem {
+  using P = SsmPlace<LN, V>;
+  using Ring = SsmRing<T, LN, V, 3, 1>;
+  static constexpr size_t D = 0, C = D + sizeof(float2) * SSM_TT * P::CH, X = C + sizeof(float) * SSM_TT * P::NP, BYTES = X + Ring::BYTES;
+};
+
 // A segment's own adjoint (nothing entering from behind) as it leaves at its first token, and the sum of its steps.
 template <typename T, int LN, int V>
 __global__ void __launch_bounds__(SSM_THREADS, 5)
 ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
   using P = SsmPlace<LN, V>;
-  constexpr int CH = P::CH, NP = P::NP;
-  __shared__ __align__(16) float2 s_d[SSM_TT * CH];    // (step, dout)
-  __shared__ __align__(16) float s_c[SSM_TT * NP];
+  using M = SsmBwLocalSmem<T, LN, V>;
+  using Ring = typename M::Ring;
+  constexpr int CH = P::CH, NP = P::NP, AHEAD = Ring::STAGES - 1;
+  extern __shared__ __align__(16) char sm[];
+  float2* s_d = reinterpret_cast<float2*>(sm + M::D);  // (step, dout)
+  float* s_c = reinterpret_cast<float*>(sm + M::C);
+  const Ring ring{reinterpret_cast<T*>(sm + M::X)};    // dt, z, dy; c
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, nseg, 1);
@@ -59,51 +70,43 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
   const bool gate = k.in.z != nullptr;
-  SsmIn in = k.in;
-  in.b = in.c;   // of the two only c is needed
-  SsmDims sc = s;
-  sc.bb = s.cb; sc.bt = s.ct; sc.bg = s.cg;
-  Pack<T, V> ndt[P::ITEMS], nz[P::ITEMS], ndy[P::ITEMS];
-  SsmFetchBC<T, LN, V, false> f;
   auto fetch = [&](int t0) {
-    const T *tp = static_cast<const T*>(in.dt) + p.b * s.db + p.dcol, *zp = static_cast<const T*>(in.z) + p.b * s.zb + p.dcol;
-    const T* yp = static_cast<const T*>(k.dy) + p.b * s.gb + p.dcol;
-#pragma unroll
-    for (int i = 0; i < P::ITEMS; ++i) {
-      const int t = t0 + p.row + i * P::ROWS;
-      const bool ok = p.col_on && t < s.S;
-      ndt[i] = ok ? load_pack<T, V>(tp + t * s.dt) : zero_pack<T, V>();
-      if (gate) nz[i] = ok ? load_pack<T, V>(zp + t * s.zt) : zero_pack<T, V>();
-      ndy[i] = ok ? load_pack<T, V>(yp + t * s.gt) : zero_pack<T, V>();
+    if (t0 >= t_begin) {
+      ring.copy(s, p, t0, 0, k.in.dt, s.db, s.dt);
+      if (gate) ring.copy(s, p, t0, 1, k.in.z, s.zb, s.zt);
+      ring.copy(s, p, t0, 2, k.dy, s.gb, s.gt);
+      ring.copy_bc(s, p, t0, 0, k.in.c, s.cb, s.ct, s.cg);
     }
-    f.load(in, sc, p, t0);
+    cp_commit();
   };
-  fetch(t_last);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
+    const int tile = t0 / SSM_TT;
+    cp_wait<AHEAD - 1>();
 #pragma unroll
     for (int i = 0; i < P::ITEMS; ++i) {
       const int q = p.row + i * P::ROWS;
-      if (q < SSM_TT) {
-        float dt[V], step[V], g[V];
-        unpack(ndt[i], dt);
-        unpack(ndy[i], g);
-        ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
-        if (gate) {
-          float zv[V], sg[V];
-          unpack(nz[i], zv);
-          logistic_v<V>(zv, sg);
+      if (q >= SSM_TT) continue;
+      float dt[V], step[V], g[V];
+      ring.get(tile, 0, i, p, dt);
+      ring.get(tile, 2, i, p, g);
+      ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
+      if (gate) {
+        float zv[V], sg[V];
+        ring.get(tile, 1, i, p, zv);
+        logistic_v<V>(zv, sg);
 #pragma unroll
-          for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
-        }
-        Pack<float2, V> o;
-#pragma unroll
-        for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], g[e]);
-        store_pack<float2, V>(s_d + q * CH + p.col, o);
+        for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
       }
+      Pack<float2, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], g[e]);
+      store_pack<float2, V>(s_d + q * CH + p.col, o);
     }
-    f.put(s_c, nullptr);
+    ring.put(tile, 0, s_c);
     __syncthreads();
-    if (t0 > t_begin) fetch(t0 - SSM_TT);
+    fetch(t0 - AHEAD * SSM_TT);
 #pragma unroll 4
     for (int t = SSM_TT - 1; t >= 0; --t) {
       const float4 q = *reinterpret_cast<const float4*>(s_d + t * CH + p.ch);
@@ -136,37 +139,26 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
 template <typename T, int LN, int V> struct SsmBwSmem {
   using P = SsmPlace<LN, V>;
   static constexpr int TF = LN <= 4 ? SSM_TT : 64 / LN;          // tokens whose channel sums wait for the other warps
-  static constexpr int RAW = SSM_TT * P::CH;                      // elements of one operand's tile
+  using Ring = SsmRing<T, LN, V, 4, 2>;
   static constexpr size_t Q = 0, G = Q + sizeof(float2) * SSM_TT * P::CH, B = G + sizeof(float) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
                           SUMS = C + sizeof(float) * SSM_TT * P::NP, PART = SUMS + 3 * sizeof(float) * SSM_TT * P::YS,
-                          X = PART + sizeof(float) * SSM_WARPS * TF * 2 * P::NP, BYTES = X + 2 * 4 * sizeof(T) * RAW;
+                          X = PART + sizeof(float) * SSM_WARPS * TF * 2 * P::NP, BYTES = X + Ring::BYTES;
 };
-
-// V elements to shared memory: they arrive by the next cp_wait(), zeros where `ok` is false
-template <typename T, int V> __device__ __forceinline__ void copy_async(T* dst, const T* src, bool ok) {
-  constexpr int BYTES = sizeof(T) * V;
-  if constexpr (BYTES >= 4) {
-    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0) : "memory");
-  } else {
-    store_pack<T, V>(dst, ok ? load_pack<T, V>(src) : zero_pack<T, V>());
-  }
-}
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <typename T, int LN, int V>
 __global__ void __launch_bounds__(SSM_THREADS, 3)
 ssm_bw_kernel(SsmBw k, SsmDims s) {
   using P = SsmPlace<LN, V>;
   using M = SsmBwSmem<T, LN, V>;
+  using Ring = typename M::Ring;
   using Sums = LaneSums<LN>;
-  constexpr int CH = P::CH, NP = P::NP, TF = M::TF, LC = P::LC, HALF = SSM_TT / 2;
+  constexpr int CH = P::CH, NP = P::NP, TF = M::TF, LC = P::LC, HALF = SSM_TT / 2, AHEAD = Ring::STAGES - 1;
   extern __shared__ __align__(16) char sm[];
   float2* s_q = reinterpret_cast<float2*>(sm + M::Q);            // (step, step x)
   float *s_g = reinterpret_cast<float*>(sm + M::G), *s_b = reinterpret_cast<float*>(sm + M::B), *s_c = reinterpret_cast<float*>(sm + M::C);
   float *s_sum = reinterpret_cast<float*>(sm + M::SUMS), *s_part = reinterpret_cast<float*>(sm + M::PART);
   float* s_yp = s_sum + 2 * SSM_TT * P::YS;                      // s_sum: sum g b, sum a g e h; s_yp: sum c h
-  T* s_raw = reinterpret_cast<T*>(sm + M::X);                    // x, dt, z, dy of two tiles; a thread copies what it reads itself
+  const Ring ring{reinterpret_cast<T*>(sm + M::X)};              // x, dt, z, dy; b, c
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, s.nseg, 0);
@@ -180,28 +172,23 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
   for (int i = 0; i < V; ++i) dskip[i] = dbias[i] = 0.f;
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
-  auto copy = [&](int t0) {
-    T* dst = s_raw + (t0 / SSM_TT & 1) * 4 * M::RAW;
-#pragma unroll
-    for (int i = 0; i < P::ITEMS; ++i) {
-      const int q = p.row + i * P::ROWS, t = t0 + q;
-      const bool ok = p.col_on && t < s.S;
-      const int at = q * CH + p.col;
-      if (q >= SSM_TT) continue;
-      const int tc = ok ? t : 0, cc = ok ? p.dcol : 0;   // (an address that exists, where nothing is read)
-      copy_async<T, V>(dst + at, static_cast<const T*>(k.in.x) + p.b * s.xb + tc * s.xt + cc, ok);
-      copy_async<T, V>(dst + M::RAW + at, static_cast<const T*>(k.in.dt) + p.b * s.db + tc * s.dt + cc, ok);
-      if (gate) copy_async<T, V>(dst + 2 * M::RAW + at, static_cast<const T*>(k.in.z) + p.b * s.zb + tc * s.zt + cc, ok);
-      copy_async<T, V>(dst + 3 * M::RAW + at, static_cast<const T*>(k.dy) + p.b * s.gb + tc * s.gt + cc, ok);
+  auto fetch = [&](int t0) {
+    if (t0 >= t_begin) {
+      ring.copy(s, p, t0, 0, k.in.x, s.xb, s.xt);
+      ring.copy(s, p, t0, 1, k.in.dt, s.db, s.dt);
+      if (gate) ring.copy(s, p, t0, 2, k.in.z, s.zb, s.zt);
+      ring.copy(s, p, t0, 3, k.dy, s.gb, s.gt);
+      ring.copy_bc(s, p, t0, 0, k.in.b, s.bb, s.bt, s.bg);
+      ring.copy_bc(s, p, t0, 1, k.in.c, s.cb, s.ct, s.cg);
     }
+    cp_commit();
   };
   auto param = [&](const float* v, float (&o)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = v != nullptr && p.col_on ? v[p.dcol + i] : 0.f;
   };
-  SsmFetchBC<T, LN, V, true> f;
-  copy(t_last);
-  f.load(k.in, s, p, t_last);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
   float* bc = k.part_bc + ((size_t)(p.g * s.tiles + p.tile) * s.B + p.b) * s.S * (2 * NP);
   uint64_t h0[2][2] = {{0ull, 0ull}, {0ull, 0ull}};   // before the tile
   auto checkpoint = [&](int t0) {
@@ -215,8 +202,8 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
   };
   checkpoint(t_last);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
-    const T* raw = s_raw + (t0 / SSM_TT & 1) * 4 * M::RAW;
-    cp_wait();
+    const int tile = t0 / SSM_TT;
+    cp_wait<AHEAD - 1>();
     {
       float bias[V];
       param(k.in.dt_bias, bias);
@@ -224,19 +211,18 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
       for (int i = 0; i < P::ITEMS; ++i) {
         const int q = p.row + i * P::ROWS, at = q * CH + p.col;
         if (q >= SSM_TT) continue;
-        float xv[V], dt[V], step[V];
-        unpack(load_pack<T, V>(raw + at), xv);
-        unpack(load_pack<T, V>(raw + M::RAW + at), dt);
+        float xv[V], dt[V], step[V], g[V];
+        ring.get(tile, 0, i, p, xv);
+        ring.get(tile, 1, i, p, dt);
+        ring.get(tile, 3, i, p, g);
         ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
         Pack<float2, V> o;
 #pragma unroll
         for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
         store_pack<float2, V>(s_q + at, o);
-        float g[V];
-        unpack(load_pack<T, V>(raw + 3 * M::RAW + at), g);
         if (gate) {
           float zv[V], sg[V];
-          unpack(load_pack<T, V>(raw + 2 * M::RAW + at), zv);
+          ring.get(tile, 2, i, p, zv);
           logistic_v<V>(zv, sg);
 #pragma unroll
           for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
@@ -244,14 +230,12 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
         store_pack<float, V>(s_g + at, pack<float, V>(g));
       }
     }
-    f.put(s_b, s_c);
+    ring.put(tile, 0, s_b);
+    ring.put(tile, 1, s_c);
     __syncthreads();
     uint64_t hb[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}}, hm[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}};
-    if (t0 > t_begin) {
-      copy(t0 - SSM_TT);
-      f.load(k.in, s, p, t0 - SSM_TT);
-      checkpoint(t0 - SSM_TT);
-    }
+    fetch(t0 - AHEAD * SSM_TT);
+    if (t0 > t_begin) checkpoint(t0 - SSM_TT);
     // one token onwards, for both channels
     auto onward = [&](int t, const uint64_t (&from)[2][2], uint64_t (&to)[2][2]) {
       const float4 q = *reinterpret_cast<const float4*>(s_q + t * CH + p.ch);
@@ -383,8 +367,8 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
       const int q = p.row + i * P::ROWS, t = t0 + q, at = q * CH + p.col;
       if (!p.col_on || t >= t_end) continue;
       float xv[V], dt[V], dout[V], s1[V], s2[V], o[V];
-      unpack(load_pack<T, V>(raw + at), xv);
-      unpack(load_pack<T, V>(raw + M::RAW + at), dt);
+      ring.get(tile, 0, i, p, xv);
+      ring.get(tile, 1, i, p, dt);
       unpack(load_pack<float, V>(s_g + at), dout);
       unpack(load_pack<float, V>(s_sum + q * P::YS + p.col), s1);
       unpack(load_pack<float, V>(s_sum + (SSM_TT + q) * P::YS + p.col), s2);
@@ -410,8 +394,8 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
       store_pack<T, V>(static_cast<T*>(k.ddt) + out, pack<T, V>(o));
       if (gate) {
         float zv[V], g[V], sg[V], yp[V];
-        unpack(load_pack<T, V>(raw + 2 * M::RAW + at), zv);
-        unpack(load_pack<T, V>(raw + 3 * M::RAW + at), g);
+        ring.get(tile, 2, i, p, zv);
+        ring.get(tile, 3, i, p, g);
         unpack(load_pack<float, V>(s_yp + q * P::YS + p.col), yp);
         logistic_v<V>(zv, sg);
 #pragma unroll
@@ -511,6 +495,7 @@ ssm_bw_sums_kernel(SsmSums q, SsmDims s) {
 // ---- launchers ----------------------------------------------------------------------------------------
 SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* strides, bool backward);
 template <typename T> bool ssm_vec(const SsmIn& in, const SsmDims& s, const void* dy, const void* y);
+template <typename T> bool ssm_pairs(const SsmIn& in, const SsmDims& s);
 
 struct SsmBwLayout { size_t bc, a, d, g, sum, end; };
 static SsmBwLayout ssm_bw_layout(const SsmDims& s) {
@@ -531,11 +516,8 @@ static int ssm_bw_t(const SsmBw& k, const SsmDims& s, cudaStream_t st) {
   const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
   if (s.nseg > 1)   // the first segment leaves nothing to another
-    if (int rc = launch_pdl(overlap, ssm_bw_local_kernel<T, LN, V>, per_seg * (s.nseg - 1), SSM_THREADS, 0, st, k, s, s.nseg - 1)) return rc;
-  constexpr size_t smem = SsmBwSmem<T, LN, V>::BYTES;
-  auto kern = ssm_bw_kernel<T, LN, V>;
-  if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  return launch_pdl(overlap, kern, grid, SSM_THREADS, smem, st, k, s);
+    if (int rc = ssm_launch(ssm_bw_local_kernel<T, LN, V>, SsmBwLocalSmem<T, LN, V>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
+  return ssm_launch(ssm_bw_kernel<T, LN, V>, SsmBwSmem<T, LN, V>::BYTES, overlap, grid, st, k, s);
 }
 
 int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, const long long* gs, const float* dh_last, const float* ckpt, void* dx,
@@ -555,6 +537,7 @@ int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, con
   if (grid >= (1ull << 31)) return MLSTM_ERR_SHAPE;
   int rc = MLSTM_ERR_DTYPE;
   MLSTM_DTYPE_SWITCH(dtype, T,
+    s.pairs = ssm_pairs<T>(in, s);
     const bool vec = ssm_vec<T>(in, s, dy, dx) && ssm_vec<T>(in, s, ddt, dz);
     SSM_LANES_SWITCH(lanes, LN, rc = vec ? ssm_bw_t<T, LN, 4>(k, s, st) : ssm_bw_t<T, LN, 1>(k, s, st);)
     if (rc == MLSTM_OK) rc = launch_pdl(grid <= pdl_max_ctas(), ssm_bw_sums_kernel<T>, (unsigned)grid, 256, 0, st, q, s);)

@@ -21,17 +21,28 @@ struct SsmFw {
   float* loc_sum;      // (B, nseg, D) sums of their steps
 };
 
+// Shared memory of the forward, in bytes
+template <typename T, int LN, int V, bool LOCAL> struct SsmFwSmem {
+  using P = SsmPlace<LN, V>;
+  using Ring = SsmRing<T, LN, V, LOCAL ? 2 : 3, LOCAL ? 1 : 2>;
+  static constexpr size_t Q = 0, B = Q + sizeof(float2) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
+                          Y = C + (LOCAL ? 0 : sizeof(float) * SSM_TT * P::NP), X = Y + (LOCAL ? 0 : sizeof(float) * SSM_TT * P::YS),
+                          BYTES = X + Ring::BYTES;
+};
+
 // LOCAL: only a segment's own end state and sum of steps
 template <typename T, int LN, int V, bool LOCAL>
 __global__ void __launch_bounds__(SSM_THREADS, 5)
 ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   using P = SsmPlace<LN, V>;
+  using M = SsmFwSmem<T, LN, V, LOCAL>;
+  using Ring = typename M::Ring;
   using Sums = LaneSums<LN>;
-  constexpr int CH = P::CH, NP = P::NP;
-  __shared__ __align__(16) float2 s_d[SSM_TT * CH];            // (step, step x)
-  __shared__ __align__(16) float s_b[SSM_TT * NP];
-  __shared__ __align__(16) float s_c[LOCAL ? 4 : SSM_TT * NP];
-  __shared__ __align__(16) float s_y[LOCAL ? 4 : SSM_TT * P::YS];
+  constexpr int CH = P::CH, NP = P::NP, AHEAD = Ring::STAGES - 1;
+  extern __shared__ __align__(16) char sm[];
+  float2* s_d = reinterpret_cast<float2*>(sm + M::Q);          // (step, step x)
+  float *s_b = reinterpret_cast<float*>(sm + M::B), *s_c = reinterpret_cast<float*>(sm + M::C), *s_y = reinterpret_cast<float*>(sm + M::Y);
+  const Ring ring{reinterpret_cast<T*>(sm + M::X)};            // x, dt, z; b, c
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, nseg, 0);
@@ -56,43 +67,38 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   }
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const bool gate = !LOCAL && k.in.z != nullptr;
-  Pack<T, V> nx[P::ITEMS], ndt[P::ITEMS], nz[P::ITEMS];
-  SsmFetchBC<T, LN, V, !LOCAL> f;
   auto fetch = [&](int t0) {
-    const T *xp = static_cast<const T*>(k.in.x) + p.b * s.xb + p.dcol, *tp = static_cast<const T*>(k.in.dt) + p.b * s.db + p.dcol;
-    const T* zp = static_cast<const T*>(k.in.z) + p.b * s.zb + p.dcol;
-#pragma unroll
-    for (int i = 0; i < P::ITEMS; ++i) {
-      const int t = t0 + p.row + i * P::ROWS;
-      const bool ok = p.col_on && t < s.S;
-      nx[i] = ok ? load_pack<T, V>(xp + t * s.xt) : zero_pack<T, V>();
-      ndt[i] = ok ? load_pack<T, V>(tp + t * s.dt) : zero_pack<T, V>();
-      if (gate) nz[i] = ok ? load_pack<T, V>(zp + t * s.zt) : zero_pack<T, V>();
+    if (t0 < t_end) {
+      ring.copy(s, p, t0, 0, k.in.x, s.xb, s.xt);
+      ring.copy(s, p, t0, 1, k.in.dt, s.db, s.dt);
+      if (gate) ring.copy(s, p, t0, 2, k.in.z, s.zb, s.zt);
+      ring.copy_bc(s, p, t0, 0, k.in.b, s.bb, s.bt, s.bg);
+      if (!LOCAL) ring.copy_bc(s, p, t0, 1, k.in.c, s.cb, s.ct, s.cg);
     }
-    f.load(k.in, s, p, t0);
+    cp_commit();
   };
-  fetch(t_begin);
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(t_begin + i * SSM_TT);
   for (int t0 = t_begin; t0 < t_end; t0 += SSM_TT) {
-    Pack<T, V> x[P::ITEMS], z[P::ITEMS];
+    const int tile = t0 / SSM_TT;
+    cp_wait<AHEAD - 1>();
 #pragma unroll
     for (int i = 0; i < P::ITEMS; ++i) {
-      x[i] = nx[i];
-      z[i] = nz[i];
       const int r = p.row + i * P::ROWS;
-      if (r < SSM_TT) {
-        float dt[V], step[V], xv[V];
-        unpack(ndt[i], dt);
-        unpack(x[i], xv);
-        ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + r < t_end, step);
-        Pack<float2, V> o;
+      if (r >= SSM_TT) continue;
+      float dt[V], step[V], xv[V];
+      ring.get(tile, 0, i, p, xv);
+      ring.get(tile, 1, i, p, dt);
+      ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + r < t_end, step);
+      Pack<float2, V> o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
-        store_pack<float2, V>(s_d + r * CH + p.col, o);
-      }
+      for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
+      store_pack<float2, V>(s_d + r * CH + p.col, o);
     }
-    f.put(s_b, s_c);
+    ring.put(tile, 0, s_b);
+    if (!LOCAL) ring.put(tile, 1, s_c);
     __syncthreads();
-    if (t0 + SSM_TT < t_end) fetch(t0 + SSM_TT);
+    fetch(t0 + AHEAD * SSM_TT);
     if (!LOCAL && k.ckpt != nullptr) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -144,13 +150,13 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
         const int r = p.row + i * P::ROWS, t = t0 + r;
         if (!p.col_on || t >= t_end) continue;
         float xv[V], o[V];
-        unpack(x[i], xv);
+        ring.get(tile, 0, i, p, xv);
         const Pack<float, V> sums = load_pack<float, V>(s_y + r * P::YS + p.col);
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = fmaf(skip[e], xv[e], sums.e[e]);
         if (gate) {
           float zv[V], sg[V];
-          unpack(z[i], zv);
+          ring.get(tile, 2, i, p, zv);
           logistic_v<V>(zv, sg);
 #pragma unroll
           for (int e = 0; e < V; ++e) o[e] *= zv[e] * sg[e];
@@ -272,6 +278,7 @@ SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long lo
   s.seg = ceil_div(s.nt, n) * SSM_TT;
   s.nseg = ceil_div(S, s.seg);
   s.softplus = softplus;
+  s.pairs = false;
   if (st != nullptr) {
     s.xb = st[0]; s.xt = st[1]; s.db = st[2]; s.dt = st[3]; s.zb = st[4]; s.zt = st[5];
     s.bb = st[6]; s.bt = st[7]; s.bg = st[8]; s.cb = st[9]; s.ct = st[10]; s.cg = st[11];
@@ -298,6 +305,16 @@ template <typename T> bool ssm_vec(const SsmIn& in, const SsmDims& s, const void
     if (!stride_fits(q, sizeof(T), bytes)) return false;
   return true;
 }
+// b and c two elements at a time
+template <typename T> bool ssm_pairs(const SsmIn& in, const SsmDims& s) {
+  if (s.N % 2 != 0 || !fits_access(in.b, 2 * sizeof(T)) || !fits_access(in.c, 2 * sizeof(T))) return false;
+  for (long long q : {s.bb, s.bt, s.bg, s.cb, s.ct, s.cg})
+    if (q % 2 != 0) return false;
+  return true;
+}
+template bool ssm_pairs<float>(const SsmIn&, const SsmDims&);
+template bool ssm_pairs<__nv_bfloat16>(const SsmIn&, const SsmDims&);
+template bool ssm_pairs<__half>(const SsmIn&, const SsmDims&);
 template bool ssm_vec<float>(const SsmIn&, const SsmDims&, const void*, const void*);
 template bool ssm_vec<__nv_bfloat16>(const SsmIn&, const SsmDims&, const void*, const void*);
 template bool ssm_vec<__half>(const SsmIn&, const SsmDims&, const void*, const void*);
@@ -307,15 +324,15 @@ static int ssm_fw_t(const SsmFw& k, const SsmDims& s, cudaStream_t st) {
   const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
   if (s.nseg > 1)   // the last segment leaves nothing to another
-    if (int rc = launch_pdl(overlap, ssm_fw_kernel<T, LN, V, true>, per_seg * (s.nseg - 1), SSM_THREADS, 0, st, k, s, s.nseg - 1)) return rc;
-  return launch_pdl(overlap, ssm_fw_kernel<T, LN, V, false>, grid, SSM_THREADS, 0, st, k, s, s.nseg);
+    if (int rc = ssm_launch(ssm_fw_kernel<T, LN, V, true>, SsmFwSmem<T, LN, V, true>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
+  return ssm_launch(ssm_fw_kernel<T, LN, V, false>, SsmFwSmem<T, LN, V, false>::BYTES, overlap, grid, st, k, s, s.nseg);
 }
 
 int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* workspace, int B, int S, int D, int N, int G,
                   bool softplus, int dtype, cudaStream_t st) {
   if (!ssm_sizes_ok(B, S, D, N, G)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_SCAN, st);
-  const SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, false);
+  SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, false);
   const int lanes = ssm_lanes(N);
   SsmFw k{in, y, h_last, ckpt, nullptr, nullptr};
   if (s.nseg > 1) {
@@ -324,6 +341,7 @@ int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_l
   }
   MLSTM_DTYPE_SWITCH(dtype, T,
     const bool vec = ssm_vec<T>(in, s, nullptr, y);
+    s.pairs = ssm_pairs<T>(in, s);
     SSM_LANES_SWITCH(lanes, LN, return vec ? ssm_fw_t<T, LN, 4>(k, s, st) : ssm_fw_t<T, LN, 1>(k, s, st);))
   return MLSTM_ERR_DTYPE;
 }
