@@ -6,12 +6,10 @@
 
 namespace mlstm {
 
-// A CTA of 128 threads has SSM_TT tokens of CH = 256 / LN channels at a time: LN neighbouring lanes share two channels, each lane
-// with four states of both.  (Four states a thread, not all of them: as many times the warps for the same sequences, and three
-// shuffles sum four values over the states of sixteen.  Two channels: b and c come from shared memory once for both, which a
-// wave of 128 bytes a clock bounds.)
+// A CTA has SSM_TT tokens of CH = 256 / LN channels at a time: LN neighbouring lanes share C channels, each lane with four states of
+// them.  (Four states a thread, not all of them: as many times the warps for the same sequences, and three shuffles sum four values
+// over the states of sixteen.)
 constexpr int SSM_TT = 16;
-constexpr int SSM_THREADS = 128, SSM_WARPS = SSM_THREADS / 32;
 constexpr int SSM_MAX_N = 128;
 
 struct SsmDims {
@@ -25,30 +23,31 @@ struct SsmDims {
   long long xb, xt, db, dt, zb, zt, bb, bt, bg, cb, ct, cg, gb, gt;   // x, dt, z, b, c, dy
 };
 
-// Where a thread stands: states 4 sub ... 4 sub + 3 of the channels `ch` and `ch` + 1 of the CTA's tile in the recurrence; in the
+// Where a thread stands: states 4 sub ... 4 sub + 3 of C channels from `ch` on of the CTA's tile in the recurrence; in the
 // passes over whole tiles, V neighbouring channels from `col` of the tokens row, row + ROWS, ...
-template <int LN, int V> struct SsmPlace {
-  static constexpr int CH = 2 * SSM_THREADS / LN, NP = 4 * LN, LC = 32 / LN;
-  static constexpr int PER_ROW = CH / V, ROWS = SSM_THREADS / PER_ROW;        // threads to a token; tokens at once
+template <int LN, int V, int C_> struct SsmPlace {
+  static constexpr int C = C_, THREADS = 256 / C, WARPS = THREADS / 32;
+  static constexpr int CH = 256 / LN, NP = 4 * LN, LC = 32 / LN;
+  static constexpr int PER_ROW = CH / V, ROWS = THREADS / PER_ROW;        // threads to a token; tokens at once
   static constexpr int ITEMS = ROWS >= SSM_TT ? 1 : SSM_TT / ROWS;
-  static constexpr int BC = (SSM_TT * NP / 2 + SSM_THREADS - 1) / SSM_THREADS;   // pairs of b's (and of c's) elements to a thread
-  static constexpr int YS = CH + 16;                             // row of a (token, channel) array of sums: two tokens' in different banks
+  static constexpr int BC = (SSM_TT * NP / 2 + THREADS - 1) / THREADS;   // pairs of b's (and of c's) elements to a thread
+  static constexpr int YS = CH + 8 * C;                          // row of a (token, channel) array of sums: the tokens of a warp in different banks
   int sub, chl, ch, warp, tile, g, seg, b, d;
-  bool on[2];
+  bool on[C];
   int row, col, dcol;
   bool col_on;
   // nseg: segments that the launch has, from seg0 on
   __device__ __forceinline__ SsmPlace(const SsmDims& s, int nseg, int seg0) {
     const int lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
-    sub = lane % LN; chl = lane / LN; ch = 2 * (warp * LC + chl);
+    sub = lane % LN; chl = lane / LN; ch = C * (warp * LC + chl);
     unsigned k = blockIdx.x;
     tile = k % s.tiles; k /= s.tiles;
     g = k % s.G; k /= s.G;
     seg = seg0 + k % nseg;
     b = k / nseg;
-    on[0] = tile * CH + ch < s.Dg;
-    on[1] = tile * CH + ch + 1 < s.Dg;
+#pragma unroll
+    for (int c = 0; c < C; ++c) on[c] = tile * CH + ch + c < s.Dg;
     d = g * s.Dg + tile * CH + ch;
     row = threadIdx.x / PER_ROW; col = (threadIdx.x % PER_ROW) * V;
     col_on = tile * CH + col < s.Dg && row < SSM_TT;
@@ -72,10 +71,10 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 
 // The operands of STAGES tiles on their way from memory: ARRS arrays of (token, channel), BCS of (token, state).  Each thread
 // copies just what it reads itself, so that its own wait is all that it takes.
-template <typename T, int LN, int V, int ARRS, int BCS> struct SsmRing {
-  using P = SsmPlace<LN, V>;
+template <typename T, typename P, int V, int ARRS, int BCS> struct SsmRing {
   static constexpr int RAW = SSM_TT * P::CH, BCN = SSM_TT * P::NP, STAGE = ARRS * RAW + BCS * BCN;
-  static constexpr int STAGES = sizeof(T) * P::CH >= 256 ? 2 : 4;   // as many as leave shared memory for the CTAs that registers allow
+  // as many as leave shared memory for the CTAs that registers allow; the backward's tiles (four arrays) take long enough for two
+  static constexpr int STAGES = ARRS == 4 || sizeof(T) * P::CH >= 256 ? 2 : 4;
   static constexpr size_t BYTES = sizeof(T) * STAGE * STAGES;
   T* base;
   __device__ __forceinline__ T* at(int tile) const { return base + (unsigned)tile % STAGES * STAGE; }
@@ -97,7 +96,7 @@ template <typename T, int LN, int V, int ARRS, int BCS> struct SsmRing {
     const T* src = static_cast<const T*>(from) + p.b * bstride + p.g * gstride;
 #pragma unroll
     for (int j = 0; j < P::BC; ++j) {
-      const int k = 2 * (threadIdx.x + j * SSM_THREADS), n = k % P::NP, t = t0 + k / P::NP;
+      const int k = 2 * (threadIdx.x + j * P::THREADS), n = k % P::NP, t = t0 + k / P::NP;
       if (k >= BCN) continue;
       const bool in = t < s.S, ok0 = in && n < s.N, ok1 = in && n + 1 < s.N;
       const T* a = ok0 ? src + t * tstride + n : src;
@@ -114,7 +113,7 @@ template <typename T, int LN, int V, int ARRS, int BCS> struct SsmRing {
     const T* from = at(tile) + ARRS * RAW + i * BCN;
 #pragma unroll
     for (int j = 0; j < P::BC; ++j) {
-      const int k = 2 * (threadIdx.x + j * SSM_THREADS);
+      const int k = 2 * (threadIdx.x + j * P::THREADS);
       if (k >= BCN) continue;
       float v[2];
       unpack(load_pack<T, 2>(from + k), v);
@@ -137,7 +136,7 @@ template <int V> __device__ __forceinline__ void ssm_step_v(const float (&dt)[V]
   for (int i = 0; i < V; ++i) o[i] = !ok ? 0.f : softplus ? o[i] : raw[i];
 }
 
-// Sums of four values over the LN lanes of a channel pair, each step halving the values that a lane still carries: a lane ends
+// Sums of four values over the LN lanes that share channels, each step halving the values that a lane still carries: a lane ends
 // with LEFT of them, from number `first` on.
 template <int LN> struct LaneSums {
   static constexpr int LEFT = LN >= 4 ? 1 : 4 / LN;
@@ -169,33 +168,28 @@ __device__ __forceinline__ void ssm_load4(const float* row, int N, int n, float 
   for (int i = 0; i < 4; ++i) o[i] = n + i < N ? row[n + i] : 0.f;
 }
 // a in powers of two, as pairs of states
-template <int LN, int V> __device__ __forceinline__ void ssm_rates(const float* a, const SsmDims& s, const SsmPlace<LN, V>& p, uint64_t (&a2)[2][2]) {
+template <typename P> __device__ __forceinline__ void ssm_rates(const float* a, const SsmDims& s, const P& p, uint64_t (&a2)[P::C][2]) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < P::C; ++c) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (p.on[c]) ssm_load4(a + (size_t)(p.d + c) * s.N, s.N, 4 * p.sub, v);
     a2[c][0] = f2(v[0] * kLog2e, v[1] * kLog2e);
     a2[c][1] = f2(v[2] * kLog2e, v[3] * kLog2e);
   }
 }
-__device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
-  float a, b;
-  unf2(v, a, b);
-  return f2(ex2(a), ex2(b));
-}
 // From what other segments leave behind, in their order: v = 2^(a sum) v + left.  first ... last - 1, or last - 1 ... first (BACK).
-template <int LN, int V, bool BACK>
-__device__ __forceinline__ void ssm_fold(const float* left, const float* sums, int first, int last, const SsmDims& s, const SsmPlace<LN, V>& p,
-                                         const uint64_t (&a2)[2][2], uint64_t (&v)[2][2]) {
+template <bool BACK, typename P>
+__device__ __forceinline__ void ssm_fold(const float* left, const float* sums, int first, int last, const SsmDims& s, const P& p,
+                                         const uint64_t (&a2)[P::C][2], uint64_t (&v)[P::C][2]) {
 #pragma unroll 4
   for (int i = 0; i < last - first; ++i) {
     const int j = BACK ? last - 1 - i : first + i;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < P::C; ++c) {
       if (!p.on[c]) continue;
       const size_t at = ((size_t)p.b * s.nseg + j) * s.D + p.d + c;
       const float sum = sums[at];
-      const Pack<uint64_t, 2> l = load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(left + at * (4 * LN) + 4 * p.sub));
+      const Pack<uint64_t, 2> l = load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(left + at * P::NP + 4 * p.sub));
       v[c][0] = fma2(ex2_pair(mul2(f2(sum, sum), a2[c][0])), v[c][0], l.e[0]);
       v[c][1] = fma2(ex2_pair(mul2(f2(sum, sum), a2[c][1])), v[c][1], l.e[1]);
     }
@@ -204,12 +198,14 @@ __device__ __forceinline__ void ssm_fold(const float* left, const float* sums, i
 
 // host
 template <typename... KArgs, typename... Args>
-int ssm_launch(void (*kern)(KArgs...), size_t smem, bool overlap, unsigned grid, cudaStream_t st, Args... args) {
+int ssm_launch(void (*kern)(KArgs...), unsigned threads, size_t smem, bool overlap, unsigned grid, cudaStream_t st, Args... args) {
   if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  return launch_pdl(overlap, kern, grid, SSM_THREADS, smem, st, args...);
+  return launch_pdl(overlap, kern, grid, threads, smem, st, args...);
 }
 // lanes to a channel
 inline int ssm_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
+
+inline int ssm_tile_channels(int N) { return 256 / ssm_lanes(N); }
 
 #define SSM_LANES_SWITCH(n, LN, ...)                  \
   switch (n) {                                        \

@@ -15,6 +15,8 @@
 
 namespace mlstm {
 
+constexpr int SSM_BW_C = 2, SSM_BW_LOCAL_C = 2;   // channels to a thread
+
 struct SsmBw {
   SsmIn in;
   const void* dy;
@@ -29,10 +31,10 @@ struct SsmBw {
 };
 
 // What comes back into the recurrence from behind the sequence
-template <int LN, int V>
-__device__ __forceinline__ void ssm_behind(const float* dh_last, const SsmDims& s, const SsmPlace<LN, V>& p, uint64_t (&r)[2][2]) {
+template <typename P>
+__device__ __forceinline__ void ssm_behind(const float* dh_last, const SsmDims& s, const P& p, uint64_t (&r)[P::C][2]) {
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < P::C; ++c) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (dh_last != nullptr && p.on[c]) ssm_load4(dh_last + ((size_t)p.b * s.D + p.d + c) * s.N, s.N, 4 * p.sub, v);
     r[c][0] = f2(v[0], v[1]);
@@ -42,17 +44,17 @@ __device__ __forceinline__ void ssm_behind(const float* dh_last, const SsmDims& 
 
 // Shared memory of a segment's own adjoint, in bytes
 template <typename T, int LN, int V> struct SsmBwLocalSmem {
-  using P = SsmPlace<LN, V>;
-  using Ring = SsmRing<T, LN, V, 3, 1>;
+  using P = SsmPlace<LN, V, SSM_BW_LOCAL_C>;
+  using Ring = SsmRing<T, P, V, 3, 1>;
   static constexpr size_t D = 0, C = D + sizeof(float2) * SSM_TT * P::CH, X = C + sizeof(float) * SSM_TT * P::NP, BYTES = X + Ring::BYTES;
 };
 
 // A segment's own adjoint (nothing entering from behind) as it leaves at its first token, and the sum of its steps.
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SSM_THREADS, 5)
+__global__ void __launch_bounds__(SsmBwLocalSmem<T, LN, V>::P::THREADS, 5)
 ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
-  using P = SsmPlace<LN, V>;
   using M = SsmBwLocalSmem<T, LN, V>;
+  using P = typename M::P;
   using Ring = typename M::Ring;
   constexpr int CH = P::CH, NP = P::NP, AHEAD = Ring::STAGES - 1;
   extern __shared__ __align__(16) char sm[];
@@ -62,9 +64,11 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, nseg, 1);
-  uint64_t a2[2][2], r[2][2] = {{0ull, 0ull}, {0ull, 0ull}}, sum = 0ull;
-  float bias[V];
-  ssm_rates<LN, V>(k.in.a, s, p, a2);
+  uint64_t a2[P::C][2], r[P::C][2];
+  float bias[V], sum[P::C];
+#pragma unroll
+  for (int c = 0; c < P::C; ++c) { r[c][0] = r[c][1] = 0ull; sum[c] = 0.f; }
+  ssm_rates(k.in.a, s, p, a2);
 #pragma unroll
   for (int i = 0; i < V; ++i) bias[i] = k.in.dt_bias != nullptr && p.col_on ? k.in.dt_bias[p.dcol + i] : 0.f;
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
@@ -109,47 +113,44 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
     fetch(t0 - AHEAD * SSM_TT);
 #pragma unroll 4
     for (int t = SSM_TT - 1; t >= 0; --t) {
-      const float4 q = *reinterpret_cast<const float4*>(s_d + t * CH + p.ch);
+      const Pack<float2, P::C> q = load_pack<float2, P::C>(s_d + t * CH + p.ch);
       const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + t * NP + 4 * p.sub);
-      const float qs[2] = {q.x, q.z}, qg[2] = {q.y, q.w};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint64_t step = f2(qs[c], qs[c]), g = f2(qg[c], qg[c]);
+      for (int c = 0; c < P::C; ++c) {
+        const uint64_t step = f2(q.e[c].x, q.e[c].x), g = f2(q.e[c].y, q.e[c].y);
         r[c][0] = mul2(ex2_pair(mul2(step, a2[c][0])), fma2(g, c2.x, r[c][0]));
         r[c][1] = mul2(ex2_pair(mul2(step, a2[c][1])), fma2(g, c2.y, r[c][1]));
+        sum[c] += q.e[c].x;
       }
-      sum = add2(sum, f2(q.x, q.z));
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < P::C; ++c) {
     if (!p.on[c]) continue;
     const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d + c;
     Pack<uint64_t, 2> o;
     o.e[0] = r[c][0]; o.e[1] = r[c][1];
     store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.loc_g + at * NP + 4 * p.sub), o);
-    float s0, s1;
-    unf2(sum, s0, s1);
-    if (p.sub == 0) k.loc_sum[at] = c == 0 ? s0 : s1;
+    if (p.sub == 0) k.loc_sum[at] = sum[c];
   }
 }
 
 // Shared memory of the backward, in bytes
 template <typename T, int LN, int V> struct SsmBwSmem {
-  using P = SsmPlace<LN, V>;
-  static constexpr int TF = LN <= 4 ? SSM_TT : 64 / LN;          // tokens whose channel sums wait for the other warps
-  using Ring = SsmRing<T, LN, V, 4, 2>;
+  using P = SsmPlace<LN, V, SSM_BW_C>;
+  static constexpr int TF = LN <= 8 ? SSM_TT / 2 : 64 / LN;          // tokens whose channel sums wait for the other warps
+  using Ring = SsmRing<T, P, V, 4, 2>;
   static constexpr size_t Q = 0, G = Q + sizeof(float2) * SSM_TT * P::CH, B = G + sizeof(float) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
-                          SUMS = C + sizeof(float) * SSM_TT * P::NP, PART = SUMS + 3 * sizeof(float) * SSM_TT * P::YS,
-                          X = PART + sizeof(float) * SSM_WARPS * TF * 2 * P::NP, BYTES = X + Ring::BYTES;
+                          SUMS = C + sizeof(float) * SSM_TT * P::NP, PART = SUMS + sizeof(float) * (3 * SSM_TT * P::YS + 16),
+                          X = PART + sizeof(float) * P::WARPS * TF * 2 * P::NP, BYTES = X + Ring::BYTES;
 };
 
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SSM_THREADS, 3)
+__global__ void __launch_bounds__(SsmBwSmem<T, LN, V>::P::THREADS, 4)
 ssm_bw_kernel(SsmBw k, SsmDims s) {
-  using P = SsmPlace<LN, V>;
   using M = SsmBwSmem<T, LN, V>;
+  using P = typename M::P;
   using Ring = typename M::Ring;
   using Sums = LaneSums<LN>;
   constexpr int CH = P::CH, NP = P::NP, TF = M::TF, LC = P::LC, HALF = SSM_TT / 2, AHEAD = Ring::STAGES - 1;
@@ -157,16 +158,19 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
   float2* s_q = reinterpret_cast<float2*>(sm + M::Q);            // (step, step x)
   float *s_g = reinterpret_cast<float*>(sm + M::G), *s_b = reinterpret_cast<float*>(sm + M::B), *s_c = reinterpret_cast<float*>(sm + M::C);
   float *s_sum = reinterpret_cast<float*>(sm + M::SUMS), *s_part = reinterpret_cast<float*>(sm + M::PART);
-  float* s_yp = s_sum + 2 * SSM_TT * P::YS;                      // s_sum: sum g b, sum a g e h; s_yp: sum c h
+  constexpr int S2 = SSM_TT * P::YS + 16;                        // (the two sums of a warp in different banks)
+  float* s_yp = s_sum + S2 + SSM_TT * P::YS;                     // s_sum: sum g b and, from S2 on, sum a g e h; s_yp: sum c h
   const Ring ring{reinterpret_cast<T*>(sm + M::X)};              // x, dt, z, dy; b, c
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, s.nseg, 0);
   const bool gate = k.in.z != nullptr;
-  uint64_t a2[2][2], r[2][2], da[2][2] = {{0ull, 0ull}, {0ull, 0ull}};
-  ssm_rates<LN, V>(k.in.a, s, p, a2);
-  ssm_behind<LN, V>(k.dh_last, s, p, r);
-  ssm_fold<LN, V, true>(k.loc_g, k.loc_sum, p.seg + 1, s.nseg, s, p, a2, r);
+  uint64_t a2[P::C][2], r[P::C][2], da[P::C][2];
+#pragma unroll
+  for (int c = 0; c < P::C; ++c) da[c][0] = da[c][1] = 0ull;
+  ssm_rates(k.in.a, s, p, a2);
+  ssm_behind(k.dh_last, s, p, r);
+  ssm_fold<true>(k.loc_g, k.loc_sum, p.seg + 1, s.nseg, s, p, a2, r);
   float dskip[V], dbias[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) dskip[i] = dbias[i] = 0.f;
@@ -190,17 +194,15 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
   float* bc = k.part_bc + ((size_t)(p.g * s.tiles + p.tile) * s.B + p.b) * s.S * (2 * NP);
-  uint64_t h0[2][2] = {{0ull, 0ull}, {0ull, 0ull}};   // before the tile
-  auto checkpoint = [&](int t0) {
+  // the state before a tile (fetched when it is needed: the tile's work hides it)
+  auto checkpoint = [&](int t0, uint64_t (&h)[P::C][2]) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      if (!p.on[c]) continue;
-      const Pack<uint64_t, 2> l =
-          load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub));
-      h0[c][0] = l.e[0]; h0[c][1] = l.e[1];
+    for (int c = 0; c < P::C; ++c) {
+      Pack<uint64_t, 2> l = {};
+      if (p.on[c]) l = load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub));
+      h[c][0] = l.e[0]; h[c][1] = l.e[1];
     }
   };
-  checkpoint(t_last);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
     const int tile = t0 / SSM_TT;
     cp_wait<AHEAD - 1>();
@@ -233,47 +235,40 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
     ring.put(tile, 0, s_b);
     ring.put(tile, 1, s_c);
     __syncthreads();
-    uint64_t hb[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}}, hm[2][2] = {{h0[0][0], h0[0][1]}, {h0[1][0], h0[1][1]}};
     fetch(t0 - AHEAD * SSM_TT);
-    if (t0 > t_begin) checkpoint(t0 - SSM_TT);
-    // one token onwards, for both channels
-    auto onward = [&](int t, const uint64_t (&from)[2][2], uint64_t (&to)[2][2]) {
-      const float4 q = *reinterpret_cast<const float4*>(s_q + t * CH + p.ch);
+    // one token onwards
+    auto onward = [&](int t, const uint64_t (&from)[P::C][2], uint64_t (&to)[P::C][2]) {
+      const Pack<float2, P::C> q = load_pack<float2, P::C>(s_q + t * CH + p.ch);
       const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + t * NP + 4 * p.sub);
-      const float qs[2] = {q.x, q.z}, qx[2] = {q.y, q.w};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint64_t step = f2(qs[c], qs[c]), sx = f2(qx[c], qx[c]);
+      for (int c = 0; c < P::C; ++c) {
+        const uint64_t step = f2(q.e[c].x, q.e[c].x), sx = f2(q.e[c].y, q.e[c].y);
         to[c][0] = fma2(ex2_pair(mul2(step, a2[c][0])), from[c][0], mul2(sx, b.x));
         to[c][1] = fma2(ex2_pair(mul2(step, a2[c][1])), from[c][1], mul2(sx, b.y));
       }
     };
-    // The states of eight tokens are kept at a time: first through the tile's first half without keeping any.
+    // The states of eight tokens are kept at a time: for the tile's second half first through the first without keeping any.
     const bool full = t0 + HALF < t_end;
-    if (full) {
-#pragma unroll 4
-      for (int t = 0; t < HALF; ++t) onward(t, hm, hm);
-    }
 #pragma unroll 1
     for (int half = full ? HALF : 0; half >= 0; half -= HALF) {
-      uint64_t h[HALF + 1][2][2];
+      uint64_t h[HALF + 1][P::C][2];
+      checkpoint(t0, h[0]);
+#pragma unroll 4
+      for (int t = 0; t < half; ++t) onward(t, h[0], h[0]);
+      constexpr int UF = 4 / P::C, UB = 2 / P::C;   // tokens whose sums over the states are taken together
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) h[0][c][i] = half ? hm[c][i] : hb[c][i];
-#pragma unroll
-      for (int t = 0; t < HALF; t += 2) {
+      for (int t = 0; t < HALF; t += UF) {
         float acc[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < UF; ++u) {
           onward(half + t + u, h[t + u], h[t + u + 1]);
           if (gate) {
             const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + (half + t + u) * NP + 4 * p.sub);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < P::C; ++c) {
               float lo, hi;
               unf2(fma2(c2.x, h[t + u + 1][c][0], mul2(c2.y, h[t + u + 1][c][1])), lo, hi);
-              acc[u * 2 + c] = lo + hi;
+              acc[u * P::C + c] = lo + hi;
             }
           }
         }
@@ -281,32 +276,33 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
           const int first = Sums::run(acc, p.sub);
           if (p.sub % Sums::SAME == 0) {
 #pragma unroll
-            for (int j = 0; j < Sums::LEFT; ++j) s_yp[(half + t + (first + j) / 2) * P::YS + p.ch + (first + j) % 2] = acc[j];
+            for (int j = 0; j < Sums::LEFT; ++j) s_yp[(half + t + (first + j) / P::C) * P::YS + p.ch + (first + j) % P::C] = acc[j];
           }
         }
       }
+      float acc[4];   // two sums for each of two (token, channel)
 #pragma unroll
       for (int u = HALF - 1; u >= 0; --u) {
         const int t = half + u;
-        const float4 q = *reinterpret_cast<const float4*>(s_q + t * CH + p.ch);
-        const float2 dg = *reinterpret_cast<const float2*>(s_g + t * CH + p.ch);
+        const Pack<float2, P::C> q = load_pack<float2, P::C>(s_q + t * CH + p.ch);
+        const Pack<float, P::C> dg = load_pack<float, P::C>(s_g + t * CH + p.ch);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + t * NP + 4 * p.sub);
         const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + t * NP + 4 * p.sub);
-        const float qs[2] = {q.x, q.z}, qx[2] = {q.y, q.w}, qg[2] = {dg.x, dg.y};
-        float acc[4], v[8];
+        float v[8];
         uint64_t vb[2], vc[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint64_t step = f2(qs[c], qs[c]), sx = f2(qx[c], qx[c]), dout = f2(qg[c], qg[c]);
+        for (int c = 0; c < P::C; ++c) {
+          const uint64_t step = f2(q.e[c].x, q.e[c].x), sx = f2(q.e[c].y, q.e[c].y), dout = f2(dg.e[c], dg.e[c]);
           const uint64_t g0 = fma2(dout, c2.x, r[c][0]), g1 = fma2(dout, c2.y, r[c][1]);
+          const int at = u % UB * P::C + c;
           float lo, hi;
           unf2(fma2(g0, b.x, mul2(g1, b.y)), lo, hi);
-          acc[c] = lo + hi;
+          acc[at] = lo + hi;
           r[c][0] = mul2(ex2_pair(mul2(step, a2[c][0])), g0);
           r[c][1] = mul2(ex2_pair(mul2(step, a2[c][1])), g1);
           const uint64_t w0 = mul2(r[c][0], h[u][c][0]), w1 = mul2(r[c][1], h[u][c][1]);
           unf2(fma2(a2[c][0], w0, mul2(a2[c][1], w1)), lo, hi);
-          acc[2 + c] = lo + hi;
+          acc[2 + at] = lo + hi;
           da[c][0] = fma2(step, w0, da[c][0]);
           da[c][1] = fma2(step, w1, da[c][1]);
           vb[0] = c == 0 ? mul2(sx, g0) : fma2(sx, g0, vb[0]);
@@ -314,10 +310,13 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
           vc[0] = c == 0 ? mul2(dout, h[u + 1][c][0]) : fma2(dout, h[u + 1][c][0], vc[0]);
           vc[1] = c == 0 ? mul2(dout, h[u + 1][c][1]) : fma2(dout, h[u + 1][c][1], vc[1]);
         }
-        const int from = Sums::run(acc, p.sub);
-        if (p.sub % Sums::SAME == 0) {
+        if (u % UB == 0) {
+          const int from = Sums::run(acc, p.sub);
+          if (p.sub % Sums::SAME == 0) {
 #pragma unroll
-          for (int j = 0; j < Sums::LEFT; ++j) s_sum[((from + j) / 2 * SSM_TT + t) * P::YS + p.ch + (from + j) % 2] = acc[j];
+            for (int j = 0; j < Sums::LEFT; ++j)
+              s_sum[(from + j) / 2 * S2 + (t + (from + j) % 2 / P::C) * P::YS + p.ch + (from + j) % P::C] = acc[j];
+          }
         }
         unf2(vb[0], v[0], v[1]); unf2(vb[1], v[2], v[3]);
         unf2(vc[0], v[4], v[5]); unf2(vc[1], v[6], v[7]);
@@ -346,12 +345,12 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
             s_part[((p.warp * TF + t % TF) * 2 + e / 4) * NP + 4 * p.sub + e % 4] = v[j];
           }
         }
-        if (TF <= HALF ? u % TF == 0 : (u == 0 && half == 0)) {   // TF tokens are there (or all that the tile has): over the warps
+        if (u % TF == 0) {   // TF tokens are there: over the warps
           __syncthreads();
-          for (int e = threadIdx.x; e < TF * 2 * NP; e += SSM_THREADS) {
+          for (int e = threadIdx.x; e < TF * 2 * NP; e += P::THREADS) {
             float a = 0.f;
 #pragma unroll
-            for (int w = 0; w < SSM_WARPS; ++w) a += s_part[w * TF * 2 * NP + e];
+            for (int w = 0; w < P::WARPS; ++w) a += s_part[w * TF * 2 * NP + e];
             const int tt = t0 + t + e / (2 * NP);
             if (tt < t_end) bc[(size_t)tt * (2 * NP) + e % (2 * NP)] = a;
           }
@@ -371,11 +370,12 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
       ring.get(tile, 1, i, p, dt);
       unpack(load_pack<float, V>(s_g + at), dout);
       unpack(load_pack<float, V>(s_sum + q * P::YS + p.col), s1);
-      unpack(load_pack<float, V>(s_sum + (SSM_TT + q) * P::YS + p.col), s2);
+      unpack(load_pack<float, V>(s_sum + S2 + q * P::YS + p.col), s2);
+      const Pack<float2, V> step = load_pack<float2, V>(s_q + at);
       const size_t out = ((size_t)p.b * s.S + t) * s.D + p.dcol;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        o[e] = fmaf(s_q[at + e].x, s1[e], skip[e] * dout[e]);
+        o[e] = fmaf(step.e[e].x, s1[e], skip[e] * dout[e]);
         dskip[e] = fmaf(dout[e], xv[e], dskip[e]);
       }
       store_pack<T, V>(static_cast<T*>(k.dx) + out, pack<T, V>(o));
@@ -407,7 +407,7 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
   }
   const size_t row = (size_t)p.b * s.nseg + p.seg;
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < P::C; ++c) {
     if (!p.on[c]) continue;
     Pack<uint64_t, 2> o;
     o.e[0] = da[c][0]; o.e[1] = da[c][1];
@@ -431,7 +431,7 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
     }
     __syncthreads();
     constexpr int N_ROWS = P::ROWS < SSM_TT ? P::ROWS : SSM_TT;
-    for (int c = threadIdx.x; c < CH; c += SSM_THREADS) {
+    for (int c = threadIdx.x; c < CH; c += P::THREADS) {
       float a = 0.f;
 #pragma unroll
       for (int q = 0; q < N_ROWS; ++q) a += s_x[q * CH + c];
@@ -516,8 +516,8 @@ static int ssm_bw_t(const SsmBw& k, const SsmDims& s, cudaStream_t st) {
   const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
   if (s.nseg > 1)   // the first segment leaves nothing to another
-    if (int rc = ssm_launch(ssm_bw_local_kernel<T, LN, V>, SsmBwLocalSmem<T, LN, V>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
-  return ssm_launch(ssm_bw_kernel<T, LN, V>, SsmBwSmem<T, LN, V>::BYTES, overlap, grid, st, k, s);
+    if (int rc = ssm_launch(ssm_bw_local_kernel<T, LN, V>, 256 / SSM_BW_LOCAL_C, SsmBwLocalSmem<T, LN, V>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
+  return ssm_launch(ssm_bw_kernel<T, LN, V>, 256 / SSM_BW_C, SsmBwSmem<T, LN, V>::BYTES, overlap, grid, st, k, s);
 }
 
 int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, const long long* gs, const float* dh_last, const float* ckpt, void* dx,

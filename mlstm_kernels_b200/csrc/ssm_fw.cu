@@ -12,6 +12,9 @@
 
 namespace mlstm {
 
+// Two channels to a thread: b and c come from shared memory once for both, at 128 bytes a clock and SM.
+constexpr int SSM_FW_C = 2;
+
 struct SsmFw {
   SsmIn in;
   void* y;
@@ -23,8 +26,8 @@ struct SsmFw {
 
 // Shared memory of the forward, in bytes
 template <typename T, int LN, int V, bool LOCAL> struct SsmFwSmem {
-  using P = SsmPlace<LN, V>;
-  using Ring = SsmRing<T, LN, V, LOCAL ? 2 : 3, LOCAL ? 1 : 2>;
+  using P = SsmPlace<LN, V, SSM_FW_C>;
+  using Ring = SsmRing<T, P, V, LOCAL ? 2 : 3, LOCAL ? 1 : 2>;
   static constexpr size_t Q = 0, B = Q + sizeof(float2) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
                           Y = C + (LOCAL ? 0 : sizeof(float) * SSM_TT * P::NP), X = Y + (LOCAL ? 0 : sizeof(float) * SSM_TT * P::YS),
                           BYTES = X + Ring::BYTES;
@@ -32,10 +35,10 @@ template <typename T, int LN, int V, bool LOCAL> struct SsmFwSmem {
 
 // LOCAL: only a segment's own end state and sum of steps
 template <typename T, int LN, int V, bool LOCAL>
-__global__ void __launch_bounds__(SSM_THREADS, 5)
+__global__ void __launch_bounds__(SsmFwSmem<T, LN, V, LOCAL>::P::THREADS, 5)
 ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
-  using P = SsmPlace<LN, V>;
   using M = SsmFwSmem<T, LN, V, LOCAL>;
+  using P = typename M::P;
   using Ring = typename M::Ring;
   using Sums = LaneSums<LN>;
   constexpr int CH = P::CH, NP = P::NP, AHEAD = Ring::STAGES - 1;
@@ -46,18 +49,20 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, nseg, 0);
-  uint64_t a2[2][2], h[2][2] = {{0ull, 0ull}, {0ull, 0ull}};
-  uint64_t sum = 0ull;
-  ssm_rates<LN, V>(k.in.a, s, p, a2);
+  uint64_t a2[P::C][2], h[P::C][2];
+  float sum[P::C];
+#pragma unroll
+  for (int c = 0; c < P::C; ++c) { h[c][0] = h[c][1] = 0ull; sum[c] = 0.f; }
+  ssm_rates(k.in.a, s, p, a2);
   if (!LOCAL) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < P::C; ++c) {
       float v[4] = {0.f, 0.f, 0.f, 0.f};
       if (k.in.h0 != nullptr && p.on[c]) ssm_load4(k.in.h0 + ((size_t)p.b * s.D + p.d + c) * s.N, s.N, 4 * p.sub, v);
       h[c][0] = f2(v[0], v[1]);
       h[c][1] = f2(v[2], v[3]);
     }
-    ssm_fold<LN, V, false>(k.loc_h, k.loc_sum, 0, p.seg, s, p, a2, h);
+    ssm_fold<false>(k.loc_h, k.loc_sum, 0, p.seg, s, p, a2, h);
   }
   float bias[V], skip[V];
 #pragma unroll
@@ -101,36 +106,35 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
     fetch(t0 + AHEAD * SSM_TT);
     if (!LOCAL && k.ckpt != nullptr) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < P::C; ++c) {
         if (!p.on[c]) continue;
         Pack<uint64_t, 2> o;
         o.e[0] = h[c][0]; o.e[1] = h[c][1];
         store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub), o);
       }
     }
-#pragma unroll(LOCAL ? 2 : 4)
-    for (int t = 0; t < SSM_TT; t += 2) {
+    constexpr int U = 4 / P::C;   // tokens whose sums over the states are taken together
+#pragma unroll(LOCAL ? 2 : 16)
+    for (int t = 0; t < SSM_TT; t += U) {
       float acc[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float4 q = *reinterpret_cast<const float4*>(s_d + (t + u) * CH + p.ch);
+      for (int u = 0; u < U; ++u) {
+        const Pack<float2, P::C> q = load_pack<float2, P::C>(s_d + (t + u) * CH + p.ch);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + (t + u) * NP + 4 * p.sub);
-        const float qs[2] = {q.x, q.z}, qx[2] = {q.y, q.w};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint64_t step = f2(qs[c], qs[c]), sx = f2(qx[c], qx[c]);
+        for (int c = 0; c < P::C; ++c) {
+          const uint64_t step = f2(q.e[c].x, q.e[c].x), sx = f2(q.e[c].y, q.e[c].y);
           h[c][0] = fma2(ex2_pair(mul2(step, a2[c][0])), h[c][0], mul2(sx, b.x));
           h[c][1] = fma2(ex2_pair(mul2(step, a2[c][1])), h[c][1], mul2(sx, b.y));
+          if (LOCAL) sum[c] += q.e[c].x;
         }
-        if (LOCAL) {
-          sum = add2(sum, f2(q.x, q.z));
-        } else {
+        if (!LOCAL) {
           const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + (t + u) * NP + 4 * p.sub);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < P::C; ++c) {
             float lo, hi;
             unf2(fma2(c2.x, h[c][0], mul2(c2.y, h[c][1])), lo, hi);
-            acc[u * 2 + c] = lo + hi;
+            acc[u * P::C + c] = lo + hi;
           }
         }
       }
@@ -138,7 +142,7 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
         const int first = Sums::run(acc, p.sub);
         if (p.sub % Sums::SAME == 0) {
 #pragma unroll
-          for (int j = 0; j < Sums::LEFT; ++j) s_y[(t + (first + j) / 2) * P::YS + p.ch + (first + j) % 2] = acc[j];
+          for (int j = 0; j < Sums::LEFT; ++j) s_y[(t + (first + j) / P::C) * P::YS + p.ch + (first + j) % P::C] = acc[j];
         }
       }
     }
@@ -166,16 +170,14 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
     }
   }
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+  for (int c = 0; c < P::C; ++c) {
     if (!p.on[c]) continue;
     if (LOCAL) {
       const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d + c;
       Pack<uint64_t, 2> o;
       o.e[0] = h[c][0]; o.e[1] = h[c][1];
       store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.loc_h + at * NP + 4 * p.sub), o);
-      float s0, s1;
-      unf2(sum, s0, s1);
-      if (p.sub == 0) k.loc_sum[at] = c == 0 ? s0 : s1;
+      if (p.sub == 0) k.loc_sum[at] = sum[c];
     } else if (k.h_last != nullptr && p.seg == s.nseg - 1) {
       float v[4];
       unf2(h[c][0], v[0], v[1]);
@@ -256,25 +258,42 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
 bool ssm_sizes_ok(int B, int S, int D, int N, int G) {
   if (B <= 0 || S <= 0 || D <= 0 || N <= 0 || N > SSM_MAX_N || G <= 0 || D % G != 0) return false;
   if (S > (1 << 30) || (long long)D * N >= (1ll << 31)) return false;
-  const int ch = 2 * SSM_THREADS / ssm_lanes(N), Dg = D / G;
+  const int ch = ssm_tile_channels(N), Dg = D / G;
   return (long long)B * G * ceil_div(Dg, ch) * 64 < (1ll << 31);
 }
 
-// Segments: as many as fit the GPU at once, none where whole sequences fill more than half of it.
-static int ssm_segments(long long ctas, int nt, int per_sm) {
-  long long n = (long long)per_sm * sm_count() / ctas;
-  if (n > nt / 4) n = nt / 4;      // four tiles each at least
-  if (n > 64) n = 64;
-  return n < 2 ? 1 : (int)n;
+// The time of a launch of `grid` CTAs, up to `slots` to an SM, for each tile of a CTA: k of them share an SM for k + add, at least
+// `alone`.  More than fit go round; the last round counts half as full as it is not.
+static float ssm_rounds(long long grid, int slots, float add, float alone) {
+  const float per_sm = (float)grid / (float)sm_count(), rounds = per_sm / (float)slots;
+  const float k = rounds > 1.f ? (float)slots : ceilf(per_sm), tile = k + add > alone ? k + add : alone;
+  return rounds > 1.f ? 0.5f * (rounds + ceilf(rounds)) * tile : tile;
+}
+// Segments: the number that should take least, the pass over the segments' own ends (for all but one) among it.  Measured for 128
+// CTAs of 128 tiles (4 x 2048 x 2048 channels, 16 states): forward 327, 222, 212, 206, 205 us with 1, 5, 8, 10, 16 segments,
+// backward 1758, 817, 543, 574, 530 us with 1, 3, 8, 10, 16.  Units of a tile's part of a full SM: 0.8 us forward, 4.1 us backward.
+static int ssm_segments(long long ctas, int nt, bool backward) {
+  int best = 1;
+  float least = 0.f;
+  for (int n = 1; n <= 64 && (n == 1 || n <= nt / 4); ++n) {
+    const int seg = ceil_div(nt, n);
+    if (n > 1 && ceil_div(nt, seg) != n) continue;
+    float t = backward ? ssm_rounds(ctas * n, 4, 0.f, 4.f) : ssm_rounds(ctas * n, 5, 2.5f, 0.f);
+    if (n > 1) t += (backward ? 0.115f : 0.6f) * ssm_rounds(ctas * (n - 1), 5, 2.5f, 0.f);
+    t *= (float)seg + 0.5f;   // (half a tile's time to begin and to end)
+    if (n == 1 || t < least) { best = n; least = t; }
+  }
+  return best;
 }
 
 SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* st, bool backward) {
   SsmDims s{};
   s.B = B; s.S = S; s.D = D; s.N = N; s.G = G;
   s.Dg = D / G;
-  s.tiles = ceil_div(s.Dg, 2 * SSM_THREADS / ssm_lanes(N));
+  s.tiles = ceil_div(s.Dg, ssm_tile_channels(N));
   s.nt = ceil_div(S, SSM_TT);
-  const int n = ssm_segments((long long)B * G * s.tiles, s.nt, backward ? 3 : 5);
+  const long long ctas = (long long)B * G * s.tiles;
+  const int n = ssm_segments(ctas, s.nt, backward);
   s.seg = ceil_div(s.nt, n) * SSM_TT;
   s.nseg = ceil_div(S, s.seg);
   s.softplus = softplus;
@@ -324,8 +343,8 @@ static int ssm_fw_t(const SsmFw& k, const SsmDims& s, cudaStream_t st) {
   const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
   if (s.nseg > 1)   // the last segment leaves nothing to another
-    if (int rc = ssm_launch(ssm_fw_kernel<T, LN, V, true>, SsmFwSmem<T, LN, V, true>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
-  return ssm_launch(ssm_fw_kernel<T, LN, V, false>, SsmFwSmem<T, LN, V, false>::BYTES, overlap, grid, st, k, s, s.nseg);
+    if (int rc = ssm_launch(ssm_fw_kernel<T, LN, V, true>, 256 / SSM_FW_C, SsmFwSmem<T, LN, V, true>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
+  return ssm_launch(ssm_fw_kernel<T, LN, V, false>, 256 / SSM_FW_C, SsmFwSmem<T, LN, V, false>::BYTES, overlap, grid, st, k, s, s.nseg);
 }
 
 int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* workspace, int B, int S, int D, int N, int G,

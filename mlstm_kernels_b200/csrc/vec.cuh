@@ -51,8 +51,9 @@ inline bool fits_access(const void* p, size_t bytes) { return reinterpret_cast<u
 inline bool stride_fits(long long elements, size_t element_size, size_t bytes) { return (elements * (long long)element_size) % (long long)bytes == 0; }
 
 // ---- exponentials for element-wise work ----------------------------------------------------------------
-// The hardware's 2^x and 1 / x (off by 2^-22 and 2^-23 of the result; results below 2^-126 are zero), eight instructions to an
-// exponential and two more to a logistic function, where expf and a division take thirty.
+// The hardware's 2^x and 1 / x, off by 2^-22 and 2^-23 of the result (results below 2^-126 are zero), instead of expf and a
+// division, which take thirty instructions.  What the rounding of x log2(e) does to e^x is left in: 1.5 |x| 2^-24 of the result,
+// which is about what the rounding of x itself did.
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -68,41 +69,26 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one 
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e), kLn2 = 0.6931471805599453f;
-// e^x up to e^88.  x log2(e) in two parts, the second of which is what rounding the first dropped: 2^(n + r) = 2^n (1 + r ln 2).
-__device__ __forceinline__ float exp_f(float x) {
-  x = min_nan(max_nan(x, -1e4f), 88.f);
-  const float n = x * kLog2e;
-  const float r = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -n));
-  const float e = ex2(n);
-  return fmaf(e * r, kLn2, e);
-}
-__device__ __forceinline__ float logistic_f(float x) { return rcp(1.f + exp_f(-x)); }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float logistic_f(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
 // The same for pairs of values, in packed instructions where there are any.
-__device__ __forceinline__ uint64_t exp_pair(float x0, float x1) {
-  x0 = min_nan(max_nan(x0, -1e4f), 88.f); x1 = min_nan(max_nan(x1, -1e4f), 88.f);
-  const uint64_t x = f2(x0, x1), m = mul2(x, f2(-kLog2e, -kLog2e));
-  const uint64_t r = fma2(x, f2(kLog2eRest, kLog2eRest), fma2(x, f2(kLog2e, kLog2e), m));
-  float m0, m1;
-  unf2(m, m0, m1);
-  const uint64_t e = f2(ex2(-m0), ex2(-m1));
-  return fma2(mul2(e, r), f2(kLn2, kLn2), e);
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
+  float a, b;
+  unf2(v, a, b);
+  return f2(ex2(a), ex2(b));
 }
 __device__ __forceinline__ uint64_t rcp_pair(uint64_t v) {
   float a, b;
   unf2(v, a, b);
   return f2(rcp(a), rcp(b));
 }
-__device__ __forceinline__ uint64_t logistic_pair(float x0, float x1) { return rcp_pair(add2(f2(1.f, 1.f), exp_pair(-x0, -x1))); }
+__device__ __forceinline__ uint64_t logistic_pair(float x0, float x1) {
+  return rcp_pair(add2(f2(1.f, 1.f), ex2_pair(mul2(f2(x0, x1), f2(-kLog2e, -kLog2e)))));
+}
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|; log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, which keeps all digits of a
 // small e.  artanh(s) / s as a polynomial in s^2, through its values at the Chebyshev points of [0, 1/9]: off by 2^-26.
 __device__ __forceinline__ uint64_t softplus_pair(float x0, float x1) {
-  const uint64_t e = exp_pair(-fabsf(x0), -fabsf(x1));
+  const uint64_t e = ex2_pair(mul2(f2(fabsf(x0), fabsf(x1)), f2(-kLog2e, -kLog2e)));
   const uint64_t s = mul2(e, rcp_pair(add2(e, f2(2.f, 2.f)))), q = mul2(s, s);
   uint64_t p = fma2(f2(0.14078890f, 0.14078890f), q, f2(0.13982579f, 0.13982579f));
   p = fma2(p, q, f2(0.20012298f, 0.20012298f));

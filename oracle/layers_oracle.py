@@ -2,9 +2,11 @@
 scan, with their gradients written out.
 
 Every function returns {name: (value, error)}: `error` bounds, in units of 2^-24, what f32 arithmetic in any order of the sums may be
-off by, to first order: each rounding of a value adds one unit of the sum of the absolute terms behind it, CUDA's expf, log1pf and
-division a few, and an exponential passes the error of its argument on times itself.  Rounding of a result to its element type comes
-on top (half a step).  The constants are counts of such roundings, rounded up."""
+off by, to first order: each rounding of a value adds one unit of the sum of the absolute terms behind it, an exponential, a
+logarithm and a division a few, and an exponential passes the error of its argument on times itself: e^x as 2^(x log2 e) with both
+the constant and the product rounded is off by 2 |x| units of itself (log2 e is 1.44269504 +- 2^-26, half a unit of 1.44 |x|, and the
+product half a step, at most one unit of it; times ln 2 that is 1.5 |x|) and 4 more (2^x off by 2^-22).  Rounding of a result to its
+element type comes on top (half a step).  The constants are counts of such roundings, rounded up."""
 
 from __future__ import annotations
 
@@ -58,13 +60,15 @@ def short_conv(x, weight, bias=None, x_initial=None, silu=False, dy=None, dlast=
         mag = mag + np.abs(weight[:, j] * v[:, j:j + S])
     u_err = 6 * mag
     s = _sigmoid(u)
-    # sigmoid and its product: 8 units; the derivative of u sigmoid(u) is below 1.1
-    r = {"y": (u * s, 1.1 * u_err + 8 * np.abs(u)) if silu else (u, u_err), "last": (v[:, S:], np.zeros((B, W - 1, D)))}
+    # sigmoid and its product: 8 units, and 2 |u| (1 - s) from the exponential; the derivative of u sigmoid(u) is below 1.1
+    se = 2 * np.abs(u) * (1 - s)
+    r = {"y": (u * s, 1.1 * u_err + (8 + se) * np.abs(u * s)) if silu else (u, u_err), "last": (v[:, S:], np.zeros((B, W - 1, D)))}
     if dy is None:
         return r
     if silu:   # the second derivative of u sigmoid(u) is below 0.6
         f = s * (1 + u * (1 - s))
-        k, k_err = dy * f, np.abs(dy) * (0.6 * u_err + 16 * (s * (1 + np.abs(u) * (1 - s))))
+        # (an error of s also moves 1 - s: by at most as many units of s)
+        k, k_err = dy * f, np.abs(dy) * (0.6 * u_err + (16 + se) * s * (1 + np.abs(u)))
     else:
         k, k_err = dy, np.zeros_like(dy)
     dv, dv_err = np.zeros_like(v), np.zeros_like(v)
@@ -95,9 +99,9 @@ def ssm_scan(x, dt, a, b, c, skip=None, z=None, dt_bias=None, softplus=False, h_
     skip_ = np.zeros(D) if skip is None else skip
     raw = dt + (0 if dt_bias is None else dt_bias)
     step = np.logaddexp(raw, 0) if softplus else raw
-    # the step: 12 units of itself (softplus), and what the rounding of dt + dt_bias does to it: |raw| units, as the derivative of
-    # softplus is at most itself; the argument of an exponential has three more
-    rel = 12 + np.maximum(1, np.abs(raw))
+    # the step: 12 units of itself (softplus), and what the rounding of dt + dt_bias and the exponential's argument do to it: |raw|
+    # and 2 |raw| units, as the derivative of softplus is at most itself; the argument of an exponential has three more
+    rel = 12 + np.maximum(1, 3 * np.abs(raw))
     arg = step[..., None] * a
     dec = np.exp(arg)
     arg_err = np.abs(arg) * (rel[..., None] + 3 + summed)
@@ -115,16 +119,17 @@ def ssm_scan(x, dt, a, b, c, skip=None, z=None, dt_bias=None, softplus=False, h_
     O = (Hs[:, 1:] * np.abs(cd)).sum(-1) + np.abs(skip_ * x)
     o_err = (es[:, 1:] * np.abs(cd)).sum(-1) + 16 * O
     if z is None:
-        s, sz, dsz = np.ones_like(x), np.ones_like(x), np.zeros_like(x)
+        s, sz, dsz, gate_err = np.ones_like(x), np.ones_like(x), np.zeros_like(x), np.zeros_like(x)
     else:
         s = _sigmoid(z)
         sz, dsz = z * s, s * (1 + z * (1 - s))
-    r = {"y": (out * sz, np.abs(sz) * (o_err + 12 * O)), "h_last": (hs[:, S], es[:, S] + Hs[:, S])}
+        gate_err = 12 + 2 * np.abs(z) * (1 - s)   # units of s and of z s
+    r = {"y": (out * sz, np.abs(sz) * (o_err + gate_err * O)), "h_last": (hs[:, S], es[:, S] + Hs[:, S])}
     if dy is None:
         return r
     dout = dy * sz
     Dm = np.abs(dout)
-    d_err = 12 * Dm if z is not None else 0 * Dm
+    d_err = gate_err * Dm
     q = np.zeros((B, D, N)) if dh_last is None else dh_last.astype(np.float64)   # e_{t+1} g_{t+1}
     Q, qe = np.abs(q), np.zeros((B, D, N))
     g, Gm, ge = (np.zeros((B, S, D, N)) for _ in range(3))
@@ -144,9 +149,9 @@ def ssm_scan(x, dt, a, b, c, skip=None, z=None, dt_bias=None, softplus=False, h_
     dr = (T * a).sum(-1) + x * gb
     Dr = (Tm * np.abs(a)).sum(-1) + np.abs(x) * GB
     dr_err = (Te * np.abs(a)).sum(-1) + np.abs(x) * gb_err + 20 * Dr
-    if softplus:   # the logistic function's own error: 6 units, and that of dt + dt_bias times at most a quarter
+    if softplus:   # the logistic function's own error: 6 units, and that of its argument
         sg = _sigmoid(raw)
-        dr, dr_err, Dr = dr * sg, dr_err * sg + Dr * sg * (8 + np.abs(raw)), Dr * sg
+        dr, dr_err, Dr = dr * sg, dr_err * sg + Dr * sg * (8 + 3 * np.abs(raw)), Dr * sg
     r["ddt"] = (dr, dr_err)
     n = S + B + 32
     by = lambda v: v.reshape(B, S, G, D // G, N).sum(3).reshape(b.shape)  # noqa: E731
@@ -159,5 +164,5 @@ def ssm_scan(x, dt, a, b, c, skip=None, z=None, dt_bias=None, softplus=False, h_
     r["dskip"] = ((dout * x).sum((0, 1)), (np.abs(x) * (d_err + n * Dm)).sum((0, 1)))
     r["dh_initial"] = (q, qe)
     if z is not None:
-        r["dz"] = (dy * out * dsz, np.abs(dy) * 1.1 * (o_err + 24 * O))
+        r["dz"] = (dy * out * dsz, np.abs(dy) * (1.1 * (o_err + 8 * O) + (16 + gate_err) * O * s * (1 + np.abs(z))))
     return r
