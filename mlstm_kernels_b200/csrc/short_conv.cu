@@ -6,8 +6,10 @@
 // Tokens before the first are those of x_initial (B, W-1, D), or zeros.  Bound by HBM: x in and y out, in the backward x and dy in
 // and dx out.  A thread walks a run of tokens of a few neighbouring channels with the last W tokens in registers; tokens at the
 // seam of two runs are read by both (W - 1 of a run's length), mostly from L2.
-#include "vec.cuh"
+#include <type_traits>
+
 #include "launch.cuh"
+#include "vec.cuh"
 
 namespace mlstm {
 
@@ -20,6 +22,60 @@ struct ConvDims {
   bool silu;
 };
 
+// V channels as f32: one, or pairs for the packed instructions
+template <int V> struct Chan {
+  using E = uint64_t;
+  static constexpr int N = V / 2;
+  E v[N];
+};
+template <> struct Chan<1> {
+  using E = float;
+  static constexpr int N = 1;
+  E v[1];
+};
+__device__ __forceinline__ float fma_c(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ uint64_t fma_c(uint64_t a, uint64_t b, uint64_t c) { return fma2(a, b, c); }
+__device__ __forceinline__ float mul_c(float a, float b) { return a * b; }
+__device__ __forceinline__ uint64_t mul_c(uint64_t a, uint64_t b) { return mul2(a, b); }
+__device__ __forceinline__ float add_c(float a, float b) { return a + b; }
+__device__ __forceinline__ uint64_t add_c(uint64_t a, uint64_t b) { return add2(a, b); }
+__device__ __forceinline__ void all_c(float& r, float x) { r = x; }
+__device__ __forceinline__ void all_c(uint64_t& r, float x) { r = f2(x, x); }
+__device__ __forceinline__ float logistic_c(float a) { return logistic_f(a); }
+__device__ __forceinline__ uint64_t logistic_c(uint64_t a) {
+  float x, y;
+  unf2(a, x, y);
+  return logistic_pair(x, y);
+}
+template <int V> __device__ __forceinline__ void to_chan(const float (&f)[V], Chan<V>& o) {
+  if constexpr (V == 1) {
+    o.v[0] = f[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) o.v[i] = f2(f[2 * i], f[2 * i + 1]);
+  }
+}
+template <int V> __device__ __forceinline__ void from_chan(const Chan<V>& c, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = c.v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) unf2(c.v[i], f[2 * i], f[2 * i + 1]);
+  }
+}
+template <typename T, int V> __device__ __forceinline__ Chan<V> widen(const Pack<T, V>& p) {
+  float f[V];
+  unpack(p, f);
+  Chan<V> o;
+  to_chan<V>(f, o);
+  return o;
+}
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> narrow(const Chan<V>& c) {
+  float f[V];
+  from_chan<V>(c, f);
+  return pack<T, V>(f);
+}
+
 // Token t of the padded sequence: x for t >= 0, x_initial (row t + W - 1) or zeros before.
 template <typename T, int V, int W>
 __device__ __forceinline__ Pack<T, V> conv_token(const T* xb, const T* x0b, long long st, int t, int D) {
@@ -27,57 +83,98 @@ __device__ __forceinline__ Pack<T, V> conv_token(const T* xb, const T* x0b, long
   return x0b != nullptr ? load_pack<T, V>(x0b + (size_t)(t + W - 1) * D) : zero_pack<T, V>();
 }
 
-template <int V, int W> __device__ __forceinline__ void conv_params(const void* w, const void* bias, int dtype, int c, float (&wr)[W][V], float (&br)[V]) {
+// The taps and the bias of V channels; V > 1 reads the taps, V W neighbours, V at a time.
+template <int V, int W> __device__ __forceinline__ void conv_params(const void* w, const void* bias, int dtype, int c, Chan<V> (&wr)[W], Chan<V>& br) {
+  float f[W][V], all[W * V], b[V];
+  if constexpr (V == 1) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+    for (int j = 0; j < W; ++j) all[j] = load_any(w, (size_t)c * W + j, dtype);
+    b[0] = bias != nullptr ? load_any(bias, c, dtype) : 0.f;
+  } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j) wr[j][i] = load_any(w, (size_t)(c + i) * W + j, dtype);
-    br[i] = bias != nullptr ? load_any(bias, c + i, dtype) : 0.f;
+    for (int j = 0; j < W; ++j) {
+      float four[V];
+      load_any<V>(w, (size_t)c * W + j * V, dtype, four);
+#pragma unroll
+      for (int i = 0; i < V; ++i) all[j * V + i] = four[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = 0.f;
+    if (bias != nullptr) load_any<V>(bias, c, dtype, b);
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) f[j][i] = all[i * W + j];
+#pragma unroll
+  for (int j = 0; j < W; ++j) to_chan<V>(f[j], wr[j]);
+  to_chan<V>(b, br);
 }
 
-// One thread: V channels of one run of one sequence, threads of neighbouring channels next to each other.
+// u of one token from the W - 1 tokens before and itself
+template <int V, int W>
+__device__ __forceinline__ Chan<V> conv_sum(const Chan<V> (&wr)[W], const Chan<V>& br, const Chan<V> (&win)[W - 1], const Chan<V>& x) {
+  Chan<V> a;
+#pragma unroll
+  for (int i = 0; i < Chan<V>::N; ++i) {
+    a.v[i] = br.v[i];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) a.v[i] = fma_c(wr[j].v[i], win[j].v[i], a.v[i]);
+    a.v[i] = fma_c(wr[W - 1].v[i], x.v[i], a.v[i]);
+  }
+  return a;
+}
+template <int V, int W> __device__ __forceinline__ void conv_shift(Chan<V> (&win)[W], const Chan<V>& x) {
+#pragma unroll
+  for (int j = 0; j + 1 < W; ++j) win[j] = win[j + 1];
+  win[W - 1] = x;
+}
+
+constexpr int CONV_U = 4;   // tokens at a time
+
+// One thread: V channels of one run of one sequence, threads of neighbouring channels next to each other; CONV_U tokens are on their
+// way in registers while as many are worked on.  (Copies to shared memory as in the backward cost more instructions than the wait
+// that they save: 32768 x 2048 channels, 71 us against 65.)
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 conv_fw_kernel(const T* x, const T* x0, const void* w, const void* bias, T* y, T* x_last, ConvDims d) {
   pdl_launch_dependents();
   pdl_wait();
   const unsigned nvec = (unsigned)(d.D / V);
   const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= (size_t)nvec * d.runs * d.B) return;
-  const int c = (int)(id % nvec) * V;
   const unsigned rest = (unsigned)(id / nvec);
-  const int run = (int)(rest % (unsigned)d.runs), b = (int)(rest / (unsigned)d.runs);
+  const int c = (int)(id - (size_t)rest * nvec) * V;
+  const int b = (int)(rest / (unsigned)d.runs), run = (int)(rest - (unsigned)b * (unsigned)d.runs);
   const int t0 = run * d.run, t1 = min(d.S, t0 + d.run);
   const T* xb = x + b * d.sb + c;
   const T* x0b = x0 != nullptr ? x0 + (size_t)b * (W - 1) * d.D + c : nullptr;
   T* yb = y + (size_t)b * d.S * d.D + c;
-  float wr[W][V], br[V], win[W - 1][V];
+  Pack<T, V> in[CONV_U], next[CONV_U];
+#pragma unroll
+  for (int u = 0; u < CONV_U; ++u) in[u] = load_pack<T, V>(xb + min(t0 + u, t1 - 1) * d.st);
+  Chan<V> wr[W], br, win[W - 1];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) win[j] = widen(conv_token<T, V, W>(xb, x0b, d.st, t0 - (W - 1) + j, d.D));
   conv_params<V, W>(w, bias, d.w_dtype, c, wr, br);
+  for (int t = t0; t < t1; t += CONV_U) {
+    if (t + CONV_U < t1) {
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) unpack(conv_token<T, V, W>(xb, x0b, d.st, t0 - (W - 1) + j, d.D), win[j]);
-  constexpr int U = 4;   // tokens whose loads are in flight together
-  for (int t = t0; t < t1; t += U) {
-    Pack<T, V> in[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) in[u] = load_pack<T, V>(xb + min(t + u, t1 - 1) * d.st);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[V], o[V];
-      unpack(in[u], v);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float a = br[i];
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) a = fmaf(wr[j][i], win[j][i], a);
-        a = fmaf(wr[W - 1][i], v[i], a);
-        o[i] = d.silu ? a * logistic_f(a) : a;
-#pragma unroll
-        for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-        win[W - 2][i] = v[i];
-      }
-      if (t + u < t1) store_pack<T, V>(yb + (size_t)(t + u) * d.D, pack<T, V>(o));
+      for (int u = 0; u < CONV_U; ++u) next[u] = load_pack<T, V>(xb + min(t + CONV_U + u, t1 - 1) * d.st);
     }
+#pragma unroll
+    for (int u = 0; u < CONV_U; ++u) {
+      const Chan<V> v = widen(in[u]);
+      Chan<V> a = conv_sum<V, W>(wr, br, win, v);
+      if (d.silu) {
+#pragma unroll
+        for (int i = 0; i < Chan<V>::N; ++i) a.v[i] = mul_c(a.v[i], logistic_c(a.v[i]));
+      }
+      conv_shift<V, W - 1>(win, v);
+      if (t + u < t1) store_pack<T, V>(yb + (size_t)(t + u) * d.D, narrow<T, V>(a));
+    }
+#pragma unroll
+    for (int u = 0; u < CONV_U; ++u) in[u] = next[u];
   }
   if (x_last != nullptr && t1 == d.S) {
     T* lb = x_last + (size_t)b * (W - 1) * d.D + c;
@@ -86,32 +183,49 @@ conv_fw_kernel(const T* x, const T* x0, const void* w, const void* bias, T* y, T
   }
 }
 
+// The backward's tokens come into shared memory by asynchronous copies, CONV_U of x and dy at a time and SLOTS times as many ahead;
+// each thread copies just what it reads itself, so that its own wait is all that it takes.  (In registers they did not come early
+// enough: 32768 x 2048 channels, 381 us against 135.)
+template <typename T, int V> struct ConvRing {
+  static constexpr int PIECE = sizeof(T) * V, SLOT = 2 * CONV_U * 256 * PIECE;
+  static constexpr int SLOTS = sizeof(T) * V > 8 ? 3 : 4;   // two CTAs to an SM
+  static constexpr size_t BYTES = (size_t)SLOT * SLOTS;
+  char* base;
+  __device__ __forceinline__ T* at(int slot, int arr, int u) const {
+    return reinterpret_cast<T*>(base + slot * SLOT + ((arr * CONV_U + u) * 256 + threadIdx.x) * PIECE);
+  }
+};
 // CTA: CX threads of V channels each, the other threads runs of tokens; CTA (tile, p) takes the runs p, p + parts, ... of its
 // channels, RY = 256 / CX at a time, so that the sums for dw and dbias stay in registers until the end.
 // partial: (parts, W + 1, D), the last row for dbias; null when neither is wanted.
 template <typename T, int V, int W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 conv_bw_kernel(const T* x, const T* x0, const void* w, const void* bias, const T* dy, const T* dlast, T* dx, T* dx0, float* partial,
                ConvDims d, int cx, int tiles) {
+  using R = ConvRing<T, V>;
+  using C = Chan<V>;
+  extern __shared__ __align__(16) char sm[];
   __shared__ float s_sum[256 * V];
   pdl_launch_dependents();
   pdl_wait();
+  const R ring{sm};
   const int tile = blockIdx.x % tiles, part = blockIdx.x / tiles, parts = gridDim.x / tiles;
   const int lane = threadIdx.x % cx, ry = threadIdx.x / cx, nry = 256 / cx;
   const int c = (tile * cx + lane) * V;
-  const bool on = c < d.D;
-  float wr[W][V], br[V], dw[W][V], db[V];
+  C wr[W], br, dw[W], db;
+  typename C::E zero, one, minus;
+  all_c(zero, 0.f); all_c(one, 1.f); all_c(minus, -1.f);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    db[i] = 0.f;
+  for (int i = 0; i < C::N; ++i) {
+    db.v[i] = zero;
 #pragma unroll
-    for (int j = 0; j < W; ++j) dw[j][i] = 0.f;
+    for (int j = 0; j < W; ++j) dw[j].v[i] = zero;
   }
-  if (on) {
+  if (c < d.D) {
     conv_params<V, W>(w, bias, d.w_dtype, c, wr, br);
     const unsigned items = (unsigned)d.B * (unsigned)d.runs;
     for (unsigned it = (unsigned)part * nry + ry; it < items; it += (unsigned)parts * nry) {
-      const int b = (int)(it / (unsigned)d.runs), run = (int)(it % (unsigned)d.runs);
+      const int b = (int)(it / (unsigned)d.runs), run = (int)(it - (unsigned)b * (unsigned)d.runs);
       const int t0 = run * d.run, t1 = min(d.S, t0 + d.run);
       const T* xb = x + b * d.sb + c;
       const T* x0b = x0 != nullptr ? x0 + (size_t)b * (W - 1) * d.D + c : nullptr;
@@ -119,75 +233,112 @@ conv_bw_kernel(const T* x, const T* x0, const void* w, const void* bias, const T
       const T* lb = dlast != nullptr ? dlast + (size_t)b * (W - 1) * d.D + c : nullptr;
       T* ob = dx + (size_t)b * d.S * d.D + c;
       T* o0b = dx0 != nullptr ? dx0 + (size_t)b * (W - 1) * d.D + c : nullptr;
-      float win[W - 1][V], du[W][V];   // the W - 1 inputs before token t; du of tokens t - W + 1 ... t
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) du[j][i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < W - 1; ++j) unpack(conv_token<T, V, W>(xb, x0b, d.st, t0 - (W - 1) + j, d.D), win[j]);
       // Tokens t0 ... t1 + W - 2: the last W - 1 belong to the next run (or lie behind the sequence, where du = 0), their du is
       // needed for dx here.  Once du of token t is known, dx of token t - W + 1 is; those in front of the run are the run
       // before's, or x_initial's.
-      const int te = t1 + W - 1;
-      for (int t = t0; t < te; ++t) {
-        float v[V], g[V];
-        if (t < d.S) {
-          const Pack<T, V> px = load_pack<T, V>(xb + t * d.st), py = load_pack<T, V>(yb + t * d.yt);
-          unpack(px, v);
-          unpack(py, g);
+      const int te = t1 + W - 1, tr = min(te, d.S);
+      auto fetch = [&](int slot, int t) {
+        const T *px = xb + t * d.st, *py = yb + t * d.yt;
+        if (t + CONV_U <= tr) {
+#pragma unroll
+          for (int u = 0; u < CONV_U; ++u) {
+            copy_async<T, V>(ring.at(slot, 0, u), px + u * d.st, true);
+            copy_async<T, V>(ring.at(slot, 1, u), py + u * d.yt, true);
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] = g[i] = 0.f;
+          for (int u = 0; u < CONV_U; ++u) {
+            const bool ok = t + u < tr;
+            copy_async<T, V>(ring.at(slot, 0, u), ok ? px + u * d.st : xb, ok);
+            copy_async<T, V>(ring.at(slot, 1, u), ok ? py + u * d.yt : yb, ok);
+          }
         }
-        float o[V];
+        cp_commit();
+      };
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float k = g[i];
+      for (int i = 0; i < R::SLOTS; ++i) fetch(i, t0 + i * CONV_U);
+      C win[W - 1], du[W];   // the W - 1 inputs before token t; du of tokens t - W + 1 ... t
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+#pragma unroll
+        for (int i = 0; i < C::N; ++i) du[j].v[i] = zero;
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) win[j] = widen(conv_token<T, V, W>(xb, x0b, d.st, t0 - (W - 1) + j, d.D));
+      int slot = 0;
+      // CONV_U tokens from tb on; INNER: all of them and their outputs are this run's, and none is one of x_last
+      auto some = [&](int tb, auto inner) {
+        constexpr bool INNER = decltype(inner)::value;
+        Pack<T, V> px[CONV_U], py[CONV_U];
+        cp_wait<R::SLOTS - 1>();
+#pragma unroll
+        for (int u = 0; u < CONV_U; ++u) {
+          px[u] = load_pack<T, V>(ring.at(slot, 0, u));
+          py[u] = load_pack<T, V>(ring.at(slot, 1, u));
+        }
+        fetch(slot, tb + R::SLOTS * CONV_U);
+        slot = slot + 1 == R::SLOTS ? 0 : slot + 1;
+        T* out = ob + (long long)(tb - (W - 1)) * d.D;
+#pragma unroll
+        for (int u = 0; u < CONV_U; ++u) {
+          const int t = tb + u;
+          const C v = widen(px[u]);
+          C k = widen(py[u]);
           if (d.silu) {
-            float a = br[i];
+            const C a = conv_sum<V, W>(wr, br, win, v);
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j) a = fmaf(wr[j][i], win[j][i], a);
-            a = fmaf(wr[W - 1][i], v[i], a);
-            const float s = logistic_f(a);
-            k *= s * fmaf(a, 1.f - s, 1.f);
+            for (int i = 0; i < C::N; ++i) {
+              const auto s = logistic_c(a.v[i]);
+              k.v[i] = mul_c(k.v[i], mul_c(s, fma_c(a.v[i], fma_c(s, minus, one), one)));
+            }
           }
-          if (t < t1) {
-            db[i] += k;
+          if (INNER || t < t1) {
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j) dw[j][i] = fmaf(k, win[j][i], dw[j][i]);
-            dw[W - 1][i] = fmaf(k, v[i], dw[W - 1][i]);
+            for (int i = 0; i < C::N; ++i) {
+              db.v[i] = add_c(db.v[i], k.v[i]);
+#pragma unroll
+              for (int j = 0; j < W - 1; ++j) dw[j].v[i] = fma_c(k.v[i], win[j].v[i], dw[j].v[i]);
+              dw[W - 1].v[i] = fma_c(k.v[i], v.v[i], dw[W - 1].v[i]);
+            }
           }
+          conv_shift<V, W>(du, k);
+          conv_shift<V, W - 1>(win, v);
+          C o;   // dx of token t - W + 1
 #pragma unroll
-          for (int j = 0; j < W - 1; ++j) du[j][i] = du[j + 1][i];
-          du[W - 1][i] = k;
-          float a = 0.f;
+          for (int i = 0; i < C::N; ++i) {
+            o.v[i] = mul_c(wr[0].v[i], du[W - 1].v[i]);
 #pragma unroll
-          for (int j = 0; j < W; ++j) a = fmaf(wr[j][i], du[W - 1 - j][i], a);   // dx of token t - W + 1
-          o[i] = a;
+            for (int j = 1; j < W; ++j) o.v[i] = fma_c(wr[j].v[i], du[W - 1 - j].v[i], o.v[i]);
+          }
+          if (INNER) {
+            store_pack<T, V>(out + (size_t)u * d.D, narrow<T, V>(o));
+            continue;
+          }
+          const int to = t - (W - 1);
+          if (t >= te || (to < t0 && (run != 0 || o0b == nullptr))) continue;
+          const int late = to - (d.S - (W - 1));   // row of x_last that this token became
+          if (lb != nullptr && late >= 0) {
+            const C e = widen(load_pack<T, V>(lb + (size_t)late * d.D));
 #pragma unroll
-          for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-          win[W - 2][i] = v[i];
+            for (int i = 0; i < C::N; ++i) o.v[i] = add_c(o.v[i], e.v[i]);
+          }
+          store_pack<T, V>(to >= 0 ? ob + (size_t)to * d.D : o0b + (size_t)(to + W - 1) * d.D, narrow<T, V>(o));
         }
-        const int to = t - (W - 1);
-        const int late = to - (d.S - (W - 1));   // row of x_last that this token became
-        if (lb != nullptr && late >= 0 && (to >= t0 || run == 0)) {
-          float e[V];
-          unpack(load_pack<T, V>(lb + (size_t)late * d.D), e);
-#pragma unroll
-          for (int i = 0; i < V; ++i) o[i] += e[i];
-        }
-        if (to >= t0) store_pack<T, V>(ob + (size_t)to * d.D, pack<T, V>(o));
-        else if (run == 0 && o0b != nullptr) store_pack<T, V>(o0b + (size_t)(to + W - 1) * d.D, pack<T, V>(o));
+      };
+      for (int tb = t0; tb < te; tb += CONV_U) {
+        if (tb > t0 && tb + CONV_U <= t1 && tb + CONV_U <= d.S) some(tb, std::true_type());   // (their outputs end W - 1 tokens before)
+        else some(tb, std::false_type());
       }
+      cp_wait<0>();
     }
   }
   if (partial == nullptr) return;
 #pragma unroll
   for (int j = 0; j <= W; ++j) {   // the CTA's runs together, in their order
+    float f[V];
+    from_chan<V>(j < W ? dw[j < W ? j : 0] : db, f);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < V; ++i) s_sum[(ry * V + i) * cx + lane] = j < W ? dw[j < W ? j : 0][i] : db[i];
+    for (int i = 0; i < V; ++i) s_sum[(ry * V + i) * cx + lane] = f[i];
     __syncthreads();
     for (int k = threadIdx.x; k < cx * V; k += 256) {
       const int i = k / cx, l = k % cx, col = (tile * cx + l) * V + i;
@@ -237,36 +388,41 @@ conv_step_kernel(const T* x, const T* before, const void* w, const void* bias, T
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) row[j] = load_pack<T, V>(before + (b * (W - 1) + j) * D + c);
   row[W - 1] = load_pack<T, V>(x + b * D + c);
-  float wr[W][V], o[V];
-  conv_params<V, W>(w, bias, w_dtype, c, wr, o);
+  Chan<V> wr[W], br, win[W - 1];
+  conv_params<V, W>(w, bias, w_dtype, c, wr, br);
 #pragma unroll
-  for (int j = 0; j < W; ++j) {
-    float v[V];
-    unpack(row[j], v);
+  for (int j = 0; j < W - 1; ++j) win[j] = widen(row[j]);
+  Chan<V> a = conv_sum<V, W>(wr, br, win, widen(row[W - 1]));
+  if (silu) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = fmaf(wr[j][i], v[i], o[i]);
+    for (int i = 0; i < Chan<V>::N; ++i) a.v[i] = mul_c(a.v[i], logistic_c(a.v[i]));
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = silu ? o[i] * logistic_f(o[i]) : o[i];
-  store_pack<T, V>(y + b * D + c, pack<T, V>(o));
+  store_pack<T, V>(y + b * D + c, narrow<T, V>(a));
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) store_pack<T, V>(after + (b * (W - 1) + j) * D + c, row[j + 1]);
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
-constexpr int CONV_BW_V = 4;
+constexpr int CONV_V = 4;   // channels to a thread, where alignment allows
+
+// Tokens to a run: long ones read fewer tokens twice (W - 1 of each run) and fewer parameters, as long as there are runs for three
+// times the threads (`per_sm`) that the GPU has room for.
+static int conv_run(int B, int S, int nvec, int per_sm) {
+  const long long tokens = (long long)B * S * nvec / ((long long)sm_count() * per_sm * 3);
+  return tokens >= 64 ? 64 : tokens <= 8 ? 8 : (int)(tokens / 4 * 4);
+}
 
 struct ConvBwGrid { int run, runs, cx, tiles, parts; };
 static ConvBwGrid conv_bw_grid(int B, int S, int D) {
   ConvBwGrid g;
-  g.run = 32;
+  const int nvec = ceil_div(D, D % CONV_V == 0 ? CONV_V : 1);
+  g.run = conv_run(B, S, nvec, 512);
   g.runs = ceil_div(S, g.run);
-  const int nvec = ceil_div(D, D % CONV_BW_V == 0 ? CONV_BW_V : 1);
   g.cx = 32;
   while (g.cx > 1 && g.cx / 2 >= nvec) g.cx /= 2;
   g.tiles = ceil_div(nvec, g.cx);
   const long long items = (long long)B * g.runs, rounds = (items + 256 / g.cx - 1) / (256 / g.cx);
-  long long parts = ceil_div(2 * sm_count(), g.tiles);
+  long long parts = 2 * sm_count() / g.tiles;   // no more CTAs than run at once: a few over would take as long again
   if (parts > rounds) parts = rounds;
   g.parts = (int)(parts < 1 ? 1 : parts);
   return g;
@@ -281,8 +437,9 @@ static bool conv_sizes_ok(int B, int S, int D, int W) {
   return B > 0 && S > 0 && D > 0 && W >= 2 && W <= 4 && S < (1 << 30) && (long long)B * S < (1ll << 31) && (long long)D * W < (1ll << 31);
 }
 
-template <typename T, int V> static bool conv_vec(int D, const void* const* ptrs, int n, const long long* strides, int m) {
-  if (D % V != 0) return false;
+template <typename T, int V>
+static bool conv_vec(int D, const void* w, const void* bias, const void* const* ptrs, int n, const long long* strides, int m) {
+  if (D % V != 0 || !fits_access(w, 16) || !fits_access(bias, 16)) return false;
   const size_t bytes = sizeof(T) * V < 16 ? sizeof(T) * V : 16;
   for (int i = 0; i < n; ++i)
     if (!fits_access(ptrs[i], bytes)) return false;
@@ -311,13 +468,19 @@ int launch_short_conv_fw(const void* x, const long long* xs, const void* x0, con
                          int D, int W, bool silu, int dtype, int w_dtype, cudaStream_t st) {
   if (!conv_sizes_ok(B, S, D, W)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_CONV, st);
-  ConvDims d{B, S, D, 0, 16, xs[0], xs[1], 0, 0, w_dtype, silu};
-  d.runs = ceil_div(S, d.run);
+  const int run = conv_run(B, S, D % CONV_V == 0 ? D / CONV_V : D, 768);
+  const ConvDims d{B, S, D, ceil_div(S, run), run, xs[0], xs[1], 0, 0, w_dtype, silu};
   const void* ptrs[] = {x, x0, y, x_last};
   MLSTM_DTYPE_SWITCH(dtype, T,
-    if (conv_vec<T, 8>(D, ptrs, 4, xs, 2)) return conv_fw_t<T, 8>(x, x0, w, bias, y, x_last, W, d, st);
+    if (conv_vec<T, CONV_V>(D, w, bias, ptrs, 4, xs, 2)) return conv_fw_t<T, CONV_V>(x, x0, w, bias, y, x_last, W, d, st);
     return conv_fw_t<T, 1>(x, x0, w, bias, y, x_last, W, d, st);)
   return MLSTM_ERR_DTYPE;
+}
+
+template <typename... KArgs, typename... Args>
+static int conv_bw_run(void (*kern)(KArgs...), size_t smem, unsigned grid, cudaStream_t st, Args... args) {
+  if (smem > 40 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  return launch_pdl(grid <= pdl_max_ctas(), kern, grid, 256, smem, st, args...);
 }
 
 template <typename T, int V>
@@ -325,7 +488,7 @@ static int conv_bw_t(const void* x, const void* x0, const void* w, const void* b
                      float* partial, int W, const ConvDims& d, const ConvBwGrid& g, cudaStream_t st) {
   const unsigned grid = (unsigned)(g.parts * ceil_div(ceil_div(d.D, V), g.cx));
 #define RUN(TAPS)                                                                                                                       \
-  return launch_pdl(grid <= pdl_max_ctas(), conv_bw_kernel<T, V, TAPS>, grid, 256, 0, st, (const T*)x, (const T*)x0, w, bias, (const T*)dy, \
+  return conv_bw_run(conv_bw_kernel<T, V, TAPS>, ConvRing<T, V>::BYTES, grid, st, (const T*)x, (const T*)x0, w, bias, (const T*)dy, \
                     (const T*)dlast, (T*)dx, (T*)dx0, partial, d, g.cx, ceil_div(ceil_div(d.D, V), g.cx));
   CONV_TAPS(RUN)
 #undef RUN
@@ -344,7 +507,7 @@ int launch_short_conv_bw(const void* x, const long long* xs, const void* x0, con
   float* p = params ? partial : nullptr;
   int rc = MLSTM_ERR_DTYPE;
   MLSTM_DTYPE_SWITCH(dtype, T,
-    rc = conv_vec<T, CONV_BW_V>(D, ptrs, 6, strides, 4) ? conv_bw_t<T, CONV_BW_V>(x, x0, w, bias, dy, dlast, dx, dx0, p, W, d, g, st)
+    rc = conv_vec<T, CONV_V>(D, w, bias, ptrs, 6, strides, 4) ? conv_bw_t<T, CONV_V>(x, x0, w, bias, dy, dlast, dx, dx0, p, W, d, g, st)
                                                         : conv_bw_t<T, 1>(x, x0, w, bias, dy, dlast, dx, dx0, p, W, d, g, st);)
   if (rc != MLSTM_OK || !params) return rc;
   const unsigned grid = (unsigned)(ceil_div(D, 32) * (W + 1));
@@ -367,7 +530,7 @@ int launch_short_conv_step(const void* x, const void* before, const void* w, con
   PhaseScope ps(PH_CONV, st);
   const void* ptrs[] = {x, before, y, after};
   MLSTM_DTYPE_SWITCH(dtype, T,
-    if (conv_vec<T, 4>(D, ptrs, 4, nullptr, 0)) return conv_step_t<T, 4>(x, before, w, bias, y, after, B, D, W, silu, w_dtype, st);
+    if (conv_vec<T, CONV_V>(D, w, bias, ptrs, 4, nullptr, 0)) return conv_step_t<T, CONV_V>(x, before, w, bias, y, after, B, D, W, silu, w_dtype, st);
     return conv_step_t<T, 1>(x, before, w, bias, y, after, B, D, W, silu, w_dtype, st);)
   return MLSTM_ERR_DTYPE;
 }

@@ -55,20 +55,6 @@ template <int LN, int V, int C_> struct SsmPlace {
   }
 };
 
-// V elements to shared memory: they arrive by a later cp_wait(), zeros where `ok` is false (the address must exist even so).
-// Accesses below four bytes, which cannot be asynchronous, are made at once.
-template <typename T, int V> __device__ __forceinline__ void copy_async(T* dst, const T* src, bool ok) {
-  constexpr int BYTES = sizeof(T) * V;
-  if constexpr (BYTES >= 4) {
-    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0) : "memory");
-  } else {
-    store_pack<T, V>(dst, ok ? load_pack<T, V>(src) : zero_pack<T, V>());
-  }
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // The operands of STAGES tiles on their way from memory: ARRS arrays of (token, channel), BCS of (token, state).  Each thread
 // copies just what it reads itself, so that its own wait is all that it takes.
 template <typename T, typename P, int V, int ARRS, int BCS> struct SsmRing {

@@ -189,68 +189,64 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   }
 }
 
-// One token: bound by the states, in and out once each, 16 bytes a thread (VEC; else element by element).
-constexpr int STEP_THREADS_SSM = 256;
+// One token: bound by the states, in and out once each, 16 bytes a thread (VEC; else element by element).  A CTA has 256 / LN channels
+// of one sequence.  (Two sequences to a thread, which would share what belongs to the channel, took 13 us instead of 11 for 64 x 4096
+// channels of 16 states: fewer warps wait for memory.)
+constexpr int SSM_STEP_THREADS = 256;
 template <typename T, int LN, bool VEC>
-__global__ void __launch_bounds__(STEP_THREADS_SSM)
+__global__ void __launch_bounds__(SSM_STEP_THREADS)
 ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, const float* a, const float* skip, const float* dt_bias,
-                const float* h, T* y, float* h_new, int B, int D, int N, int G, bool softplus) {
+                const float* h, T* y, float* h_new, int tiles, int D, int N, int G, bool softplus) {
+  constexpr int CH = SSM_STEP_THREADS / LN;
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int CH = STEP_THREADS_SSM / LN;
-  const int sub = threadIdx.x % LN;
-  const size_t row = (size_t)blockIdx.x * CH + threadIdx.x / LN;   // of (B, D)
-  const bool on = row < (size_t)B * D;
-  const int d = on ? (int)(row % (unsigned)D) : 0;
-  const size_t bi = on ? row / (unsigned)D : 0;
-  const size_t bc = (bi * G + d / (D / G)) * N;
-  float hv[4], acc = 0.f;
-  float step = 0.f, xv = 0.f;
-  if (on) {
-    const float* hp = h + row * N + 4 * sub;
-    const bool any = 4 * sub < N;
-    float4 q = make_float4(0.f, 0.f, 0.f, 0.f), r = q;
-    if (VEC && any) { q = ld_stream(reinterpret_cast<const float4*>(hp)); r = *reinterpret_cast<const float4*>(a + (size_t)d * N + 4 * sub); }
-    float av[4] = {r.x, r.y, r.z, r.w};
-    hv[0] = q.x; hv[1] = q.y; hv[2] = q.z; hv[3] = q.w;
-    if (!VEC) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool ok = 4 * sub + i < N;
-        hv[i] = ok ? hp[i] : 0.f;
-        av[i] = ok ? a[(size_t)d * N + 4 * sub + i] : 0.f;
-      }
+  const int sub = threadIdx.x % LN, n = 4 * sub;
+  const unsigned bi = blockIdx.x / (unsigned)tiles;
+  const int d = (int)(blockIdx.x - bi * (unsigned)tiles) * CH + threadIdx.x / LN;
+  const bool on = d < D;
+  const int dc = on ? d : 0, g = G == 1 ? 0 : (int)((unsigned)dc / ((unsigned)D / (unsigned)G));
+  const size_t row = (size_t)bi * D + dc, at = row * N + n, bc = ((size_t)bi * G + g) * N + n;
+  float hv[4] = {0.f, 0.f, 0.f, 0.f}, av[4] = {0.f, 0.f, 0.f, 0.f}, bv[4] = {0.f, 0.f, 0.f, 0.f}, cv[4] = {0.f, 0.f, 0.f, 0.f};
+  if (VEC) {
+    if (n < N) {
+      const float4 q = ld_stream(reinterpret_cast<const float4*>(h + at));
+      hv[0] = q.x; hv[1] = q.y; hv[2] = q.z; hv[3] = q.w;
+      unpack(load_pack<float, 4>(a + (size_t)dc * N + n), av);
+      unpack(load_pack<T, 4>(b + bc), bv);
+      unpack(load_pack<T, 4>(c + bc), cv);
     }
-    xv = to_f32(x[row]);
-    const float raw[1] = {to_f32(dt[row])}, bias[1] = {dt_bias != nullptr ? dt_bias[d] : 0.f};
-    float st[1];
-    ssm_step_v<1>(raw, bias, softplus, true, st);
-    step = st[0];
+  } else {
+    ssm_load4(h + row * N, N, n, hv);
+    ssm_load4(a + (size_t)dc * N, N, n, av);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool ok = 4 * sub + i < N;
-      const float bv = ok ? to_f32(b[bc + 4 * sub + i]) : 0.f, cv = ok ? to_f32(c[bc + 4 * sub + i]) : 0.f;
-      hv[i] = fmaf(ex2(step * (av[i] * kLog2e)), hv[i], step * xv * bv);
-      acc = fmaf(cv, hv[i], acc);
+      if (n + i >= N) continue;
+      bv[i] = to_f32(b[bc + i]);
+      cv[i] = to_f32(c[bc + i]);
     }
-    float* op = h_new + row * N + 4 * sub;
-    if (VEC) {
-      if (any) __stcs(reinterpret_cast<float4*>(op), make_float4(hv[0], hv[1], hv[2], hv[3]));
-    } else {
+  }
+  const float raw[1] = {to_f32(dt[row])}, bias[1] = {dt_bias != nullptr ? dt_bias[dc] : 0.f};
+  const float xv = to_f32(x[row]), zv = z != nullptr ? to_f32(z[row]) : 0.f, sk = skip != nullptr ? skip[dc] : 0.f;
+  float st[1], acc = 0.f;
+  ssm_step_v<1>(raw, bias, softplus, true, st);
+  const float sx = st[0] * xv, s2 = st[0] * kLog2e;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * sub + i < N) op[i] = hv[i];
-    }
+  for (int i = 0; i < 4; ++i) {
+    hv[i] = fmaf(ex2(s2 * av[i]), hv[i], sx * bv[i]);
+    acc = fmaf(cv[i], hv[i], acc);
+  }
+  if (VEC) {
+    if (on && n < N) __stcs(reinterpret_cast<float4*>(h_new + at), make_float4(hv[0], hv[1], hv[2], hv[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (on && n + i < N) h_new[at + i] = hv[i];
   }
 #pragma unroll
   for (int o = LN / 2; o >= 1; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
   if (on && sub == 0) {
-    float v = skip != nullptr ? fmaf(skip[d], xv, acc) : acc;
-    if (z != nullptr) {
-      const float zz = to_f32(z[row]);
-      v *= zz * logistic_f(zz);
-    }
-    y[row] = from_f32<T>(v);
+    const float v = fmaf(sk, xv, acc);
+    y[row] = from_f32<T>(z != nullptr ? v * (zv * logistic_f(zv)) : v);
   }
 }
 
@@ -370,12 +366,14 @@ int launch_ssm_step(const void* x, const void* dt, const void* z, const void* b,
   if (!ssm_sizes_ok(B, 1, D, N, G)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_STEP, st);
   const int lanes = ssm_lanes(N);
-  const size_t grid = ((size_t)B * D + STEP_THREADS_SSM / lanes - 1) / (STEP_THREADS_SSM / lanes);
+  const int tiles = ceil_div(D, SSM_STEP_THREADS / lanes);
+  const size_t grid = (size_t)B * tiles;
   if (grid >= (1ull << 31)) return MLSTM_ERR_SHAPE;
-  const bool vec = N % 4 == 0 && fits_access(a, 16) && fits_access(h, 16) && fits_access(h_new, 16);
+  const size_t four = 4 * dtype_size(dtype);
+  const bool vec = N % 4 == 0 && fits_access(a, 16) && fits_access(h, 16) && fits_access(h_new, 16) && fits_access(b, four) && fits_access(c, four);
 #define RUN(LN, VEC)                                                                                                                              \
-  return launch_pdl(grid <= pdl_max_ctas(), ssm_step_kernel<T, LN, VEC>, (unsigned)grid, STEP_THREADS_SSM, 0, st, (const T*)x, (const T*)dt, (const T*)z, \
-                    (const T*)b, (const T*)c, a, skip, dt_bias, h, (T*)y, h_new, B, D, N, G, softplus)
+  return launch_pdl(grid <= pdl_max_ctas(), ssm_step_kernel<T, LN, VEC>, (unsigned)grid, SSM_STEP_THREADS, 0, st, (const T*)x, (const T*)dt,        \
+                    (const T*)z, (const T*)b, (const T*)c, a, skip, dt_bias, h, (T*)y, h_new, tiles, D, N, G, softplus)
   MLSTM_DTYPE_SWITCH(dtype, T, SSM_LANES_SWITCH(lanes, LN, if (vec) RUN(LN, true); RUN(LN, false);))
 #undef RUN
   return MLSTM_ERR_DTYPE;

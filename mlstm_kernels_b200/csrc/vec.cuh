@@ -50,6 +50,21 @@ template <int V> __device__ __forceinline__ void load_any(const void* p, size_t 
 inline bool fits_access(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool stride_fits(long long elements, size_t element_size, size_t bytes) { return (elements * (long long)element_size) % (long long)bytes == 0; }
 
+// ---- asynchronous copies ------------------------------------------------------------------------------
+// V elements to shared memory: they arrive by a later cp_wait(), zeros where `ok` is false (the address must exist even so).
+// Accesses below four bytes, which cannot be asynchronous, are made at once.
+template <typename T, int V> __device__ __forceinline__ void copy_async(T* dst, const T* src, bool ok) {
+  constexpr int BYTES = sizeof(T) * V;
+  if constexpr (BYTES >= 4) {
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0) : "memory");
+  } else {
+    store_pack<T, V>(dst, ok ? load_pack<T, V>(src) : zero_pack<T, V>());
+  }
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // ---- exponentials for element-wise work ----------------------------------------------------------------
 // The hardware's 2^x and 1 / x, off by 2^-22 and 2^-23 of the result (results below 2^-126 are zero), instead of expf and a
 // division, which take thirty instructions.  What the rounding of x log2(e) does to e^x is left in: 1.5 |x| 2^-24 of the result,
@@ -117,10 +132,18 @@ template <typename T, int V> __device__ __forceinline__ void unpack(const Pack<T
 #pragma unroll
   for (int i = 0; i < V; ++i) o[i] = to_f32(p.e[i]);
 }
+// (two 16-bit elements to a conversion)
+__device__ __forceinline__ void from_f32x2(float a, float b, float* o) { o[0] = a; o[1] = b; }
+__device__ __forceinline__ void from_f32x2(float a, float b, __nv_bfloat16* o) { *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ void from_f32x2(float a, float b, __half* o) { *reinterpret_cast<__half2*>(o) = __floats2half2_rn(a, b); }
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> pack(const float (&o)[V]) {
   Pack<T, V> p;
+  if constexpr (V == 1) {
+    p.e[0] = from_f32<T>(o[0]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) p.e[i] = from_f32<T>(o[i]);
+    for (int i = 0; i < V; i += 2) from_f32x2(o[i], o[i + 1], p.e + i);
+  }
   return p;
 }
 
