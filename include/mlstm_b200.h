@@ -358,7 +358,7 @@ int mlstm_b200_short_conv_step(const void* x, const void* state, const void* wei
  *   step_t = softplus(dt_t + dt_bias) with softplus != 0, else dt_t + dt_bias
  *   h_t[n] = exp(step_t a[n]) h_{t-1}[n] + step_t x_t b_t[n];  y_t = (sum_n c_t[n] h_t[n] + skip x_t) z_t sigmoid(z_t)
  *   x, dt, z (B,S,D), b, c (B,S,G,N) dtype, group g for the channels g D/G ... (g+1) D/G - 1; z NULL = no gate
- *   strides[12]: x (B, S), dt (B, S), z (B, S), b (B, S, G), c (B, S, G)
+ *   strides[12]: x (B, S), dt (B, S), z (B, S), b (B, S, G), c (B, S, G); those of S (and dy_strides[1]) below 2^29
  *   a (D,N), skip (D), dt_bias (D), h_initial (B,D,N) f32; skip, dt_bias, h_initial may be NULL (zeros)
  *   y (B,S,D) dtype out; h_last (B,D,N) f32 out or NULL
  *   checkpoints: mlstm_b200_ssm_checkpoint_bytes(), what the backward needs of the forward, or NULL

@@ -401,13 +401,19 @@ struct SsmSizes { int B, S, D, N, G; };
 SsmSizes ssm_sizes(const SsmTensors& t) {
   return {(int)t.x.size(0), (int)t.x.size(1), (int)t.x.size(2), (int)t.a.size(1), t.b.dim() == 4 ? (int)t.b.size(2) : 1};
 }
+// the stride of the token axis; of a single token any number will do
+long long token_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
+Tensor tokens_near(const Tensor& t) {   // the scan takes token strides below 2^29
+  const Tensor d = last_dense(t);
+  return !d.defined() || token_stride(d) < (1ll << 29) ? d : d.clone(at::MemoryFormat::Contiguous);
+}
 SsmTensors ssm_ready(const SsmTensors& t) {   // as the kernels read them
-  return {last_dense(t.x), last_dense(t.dt), f32c(t.a), last_dense(t.b), last_dense(t.c), f32c(t.skip), last_dense(t.z), f32c(t.dt_bias), f32c(t.h0), t.softplus};
+  return {tokens_near(t.x), tokens_near(t.dt), f32c(t.a), tokens_near(t.b), tokens_near(t.c), f32c(t.skip), tokens_near(t.z), f32c(t.dt_bias), f32c(t.h0), t.softplus};
 }
 std::array<long long, 12> ssm_strides(const SsmTensors& t) {
   const bool groups = t.b.dim() == 4;
-  return {t.x.stride(0), t.x.stride(1), t.dt.stride(0), t.dt.stride(1), t.z.defined() ? t.z.stride(0) : 0, t.z.defined() ? t.z.stride(1) : 0,
-          t.b.stride(0), t.b.stride(1), groups ? t.b.stride(2) : 0, t.c.stride(0), t.c.stride(1), groups ? t.c.stride(2) : 0};
+  return {t.x.stride(0), token_stride(t.x), t.dt.stride(0), token_stride(t.dt), t.z.defined() ? t.z.stride(0) : 0, t.z.defined() ? token_stride(t.z) : 0,
+          t.b.stride(0), token_stride(t.b), groups ? t.b.stride(2) : 0, t.c.stride(0), token_stride(t.c), groups ? t.c.stride(2) : 0};
 }
 struct Scanned { Tensor y, h_last, ckpt; };
 Scanned ssm_forward(const SsmTensors& t_, bool want_last, bool keep) {
@@ -453,9 +459,9 @@ ScanGrads ssm_backward(const SsmTensors& t_, const Tensor& ckpt, const Tensor& d
     if (want_h0) { if (dh_last_.defined()) g.dh0.copy_(dh_last_); else g.dh0.zero_(); }
   } else {
     const SsmTensors t = ssm_ready(t_);
-    const Tensor dy = dy_.defined() ? last_dense(to_dtype(dy_, dt)) : zeros(t_.x.sizes(), dt, dev);
+    const Tensor dy = dy_.defined() ? tokens_near(to_dtype(dy_, dt)) : zeros(t_.x.sizes(), dt, dev);
     const Tensor dhl = f32c(dh_last_);
-    const long long gs[2] = {dy.stride(0), dy.stride(1)};
+    const long long gs[2] = {dy.stride(0), token_stride(dy)};
     const size_t need = mlstm_b200_ssm_workspace_bytes(q.B, q.S, q.D, q.N, q.G, 1);
     const Tensor ws = bytes(need, dev);
     const auto st = ssm_strides(t);

@@ -30,18 +30,6 @@ struct SsmBw {
   float *loc_g, *loc_sum;   // (B, nseg, D, NP), (B, nseg, D)
 };
 
-// What comes back into the recurrence from behind the sequence
-template <typename P>
-__device__ __forceinline__ void ssm_behind(const float* dh_last, const SsmDims& s, const P& p, uint64_t (&r)[P::C][2]) {
-#pragma unroll
-  for (int c = 0; c < P::C; ++c) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (dh_last != nullptr && p.on[c]) ssm_load4(dh_last + ((size_t)p.b * s.D + p.d + c) * s.N, s.N, 4 * p.sub, v);
-    r[c][0] = f2(v[0], v[1]);
-    r[c][1] = f2(v[2], v[3]);
-  }
-}
-
 // Shared memory of a segment's own adjoint, in bytes
 template <typename T, int LN, int V> struct SsmBwLocalSmem {
   using P = SsmPlace<LN, V, SSM_BW_LOCAL_C>;
@@ -74,15 +62,18 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
   const bool gate = k.in.z != nullptr;
+  const SsmSource from_dt = ssm_source<T>(k.in.dt, p.b * s.db + p.dcol, s.dt), from_z = ssm_source<T>(k.in.z, p.b * s.zb + p.dcol, s.zt),
+                  from_dy = ssm_source<T>(k.dy, p.b * s.gb + p.dcol, s.gt), from_c = Ring::source_bc(k.in.c, p, s.cb, s.ct, s.cg);
   auto fetch = [&](int t0) {
     if (t0 >= t_begin) {
-      ring.copy(s, p, t0, 0, k.in.dt, s.db, s.dt);
-      if (gate) ring.copy(s, p, t0, 1, k.in.z, s.zb, s.zt);
-      ring.copy(s, p, t0, 2, k.dy, s.gb, s.gt);
-      ring.copy_bc(s, p, t0, 0, k.in.c, s.cb, s.ct, s.cg);
+      ring.copy(s, p, t0, 0, from_dt);
+      if (gate) ring.copy(s, p, t0, 1, from_z);
+      ring.copy(s, p, t0, 2, from_dy);
+      ring.copy_bc(s, p, t0, 0, from_c);
     }
     cp_commit();
   };
+  ring.clear(s, p);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
@@ -95,7 +86,7 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
       float dt[V], step[V], g[V];
       ring.get(tile, 0, i, p, dt);
       ring.get(tile, 2, i, p, g);
-      ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
+      ssm_step_v<V>(dt, bias, s.softplus, t0 + q >= t_end, step);
       if (gate) {
         float zv[V], sg[V];
         ring.get(tile, 1, i, p, zv);
@@ -125,15 +116,11 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
     }
     __syncthreads();
   }
+  const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d;
+  ssm_put_states(k.loc_g, p, at, r);
 #pragma unroll
-  for (int c = 0; c < P::C; ++c) {
-    if (!p.on[c]) continue;
-    const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d + c;
-    Pack<uint64_t, 2> o;
-    o.e[0] = r[c][0]; o.e[1] = r[c][1];
-    store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.loc_g + at * NP + 4 * p.sub), o);
-    if (p.sub == 0) k.loc_sum[at] = sum[c];
-  }
+  for (int c = 0; c < P::C; ++c)
+    if (p.on[c] && p.sub == 0) k.loc_sum[at + c] = sum[c];
 }
 
 // Shared memory of the backward, in bytes
@@ -169,24 +156,25 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
 #pragma unroll
   for (int c = 0; c < P::C; ++c) da[c][0] = da[c][1] = 0ull;
   ssm_rates(k.in.a, s, p, a2);
-  ssm_behind(k.dh_last, s, p, r);
+  ssm_load_states(k.dh_last, s, p, (size_t)p.b * s.D + p.d, r);
   ssm_fold<true>(k.loc_g, k.loc_sum, p.seg + 1, s.nseg, s, p, a2, r);
   float dskip[V], dbias[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) dskip[i] = dbias[i] = 0.f;
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const int t_last = t_begin + (t_end - 1 - t_begin) / SSM_TT * SSM_TT;
-  auto fetch = [&](int t0) {
+  auto fetch = [&](int t0) {   // (the sources anew each time: the loop has no registers left for them)
     if (t0 >= t_begin) {
-      ring.copy(s, p, t0, 0, k.in.x, s.xb, s.xt);
-      ring.copy(s, p, t0, 1, k.in.dt, s.db, s.dt);
-      if (gate) ring.copy(s, p, t0, 2, k.in.z, s.zb, s.zt);
-      ring.copy(s, p, t0, 3, k.dy, s.gb, s.gt);
-      ring.copy_bc(s, p, t0, 0, k.in.b, s.bb, s.bt, s.bg);
-      ring.copy_bc(s, p, t0, 1, k.in.c, s.cb, s.ct, s.cg);
+      ring.copy(s, p, t0, 0, ssm_source<T>(k.in.x, p.b * s.xb + p.dcol, s.xt));
+      ring.copy(s, p, t0, 1, ssm_source<T>(k.in.dt, p.b * s.db + p.dcol, s.dt));
+      if (gate) ring.copy(s, p, t0, 2, ssm_source<T>(k.in.z, p.b * s.zb + p.dcol, s.zt));
+      ring.copy(s, p, t0, 3, ssm_source<T>(k.dy, p.b * s.gb + p.dcol, s.gt));
+      ring.copy_bc(s, p, t0, 0, Ring::source_bc(k.in.b, p, s.bb, s.bt, s.bg));
+      ring.copy_bc(s, p, t0, 1, Ring::source_bc(k.in.c, p, s.cb, s.ct, s.cg));
     }
     cp_commit();
   };
+  ring.clear(s, p);
   auto param = [&](const float* v, float (&o)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = v != nullptr && p.col_on ? v[p.dcol + i] : 0.f;
@@ -194,15 +182,6 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
   float* bc = k.part_bc + ((size_t)(p.g * s.tiles + p.tile) * s.B + p.b) * s.S * (2 * NP);
-  // the state before a tile (fetched when it is needed: the tile's work hides it)
-  auto checkpoint = [&](int t0, uint64_t (&h)[P::C][2]) {
-#pragma unroll
-    for (int c = 0; c < P::C; ++c) {
-      Pack<uint64_t, 2> l = {};
-      if (p.on[c]) l = load_pack<uint64_t, 2>(reinterpret_cast<const uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub));
-      h[c][0] = l.e[0]; h[c][1] = l.e[1];
-    }
-  };
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
     const int tile = t0 / SSM_TT;
     cp_wait<AHEAD - 1>();
@@ -217,7 +196,7 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
         ring.get(tile, 0, i, p, xv);
         ring.get(tile, 1, i, p, dt);
         ring.get(tile, 3, i, p, g);
-        ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + q < t_end, step);
+        ssm_step_v<V>(dt, bias, s.softplus, t0 + q >= t_end, step);
         Pack<float2, V> o;
 #pragma unroll
         for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
@@ -252,7 +231,7 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
 #pragma unroll 1
     for (int half = full ? HALF : 0; half >= 0; half -= HALF) {
       uint64_t h[HALF + 1][P::C][2];
-      checkpoint(t0, h[0]);
+      ssm_get_states(k.ckpt, p, ((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d, h[0]);   // (fetched when it is needed: the tile's work hides it)
 #pragma unroll 4
       for (int t = 0; t < half; ++t) onward(t, h[0], h[0]);
       constexpr int UF = 4 / P::C, UB = 2 / P::C;   // tokens whose sums over the states are taken together
@@ -406,21 +385,8 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
     __syncthreads();   // the tile's arrays are free
   }
   const size_t row = (size_t)p.b * s.nseg + p.seg;
-#pragma unroll
-  for (int c = 0; c < P::C; ++c) {
-    if (!p.on[c]) continue;
-    Pack<uint64_t, 2> o;
-    o.e[0] = da[c][0]; o.e[1] = da[c][1];
-    store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.part_a + (row * s.D + p.d + c) * NP + 4 * p.sub), o);
-    if (k.dh0 != nullptr && p.seg == 0) {
-      float v[4];
-      unf2(r[c][0], v[0], v[1]);
-      unf2(r[c][1], v[2], v[3]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * p.sub + i < s.N) k.dh0[((size_t)p.b * s.D + p.d + c) * s.N + 4 * p.sub + i] = v[i];
-    }
-  }
+  ssm_put_states(k.part_a, p, row * s.D + p.d, da);
+  if (k.dh0 != nullptr && p.seg == 0) ssm_store_states(k.dh0, s, p, (size_t)p.b * s.D + p.d, r);
   // dskip and ddt_bias: over the threads that share a channel
   float* s_x = reinterpret_cast<float*>(sm);
 #pragma unroll
@@ -494,12 +460,13 @@ ssm_bw_sums_kernel(SsmSums q, SsmDims s) {
 
 // ---- launchers ----------------------------------------------------------------------------------------
 SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* strides, bool backward);
+bool ssm_tokens_ok(const long long* strides);
 template <typename T> bool ssm_vec(const SsmIn& in, const SsmDims& s, const void* dy, const void* y);
 template <typename T> bool ssm_pairs(const SsmIn& in, const SsmDims& s);
 
 struct SsmBwLayout { size_t bc, a, d, g, sum, end; };
 static SsmBwLayout ssm_bw_layout(const SsmDims& s) {
-  const size_t np = 4 * ssm_lanes(s.N), rows = (size_t)s.B * s.nseg;
+  const size_t np = ssm_padded(s.N), rows = (size_t)s.B * s.nseg;
   SsmBwLayout l{};
   l.bc = 0;
   l.a = align_up(l.bc + (size_t)s.G * s.tiles * s.B * s.S * 2 * np * sizeof(float), 256);
@@ -523,11 +490,11 @@ static int ssm_bw_t(const SsmBw& k, const SsmDims& s, cudaStream_t st) {
 int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, const long long* gs, const float* dh_last, const float* ckpt, void* dx,
                   void* ddt, void* dz, void* db, void* dc, float* da, float* dskip, float* ddt_bias, float* dh0, void* workspace, int B, int S, int D,
                   int N, int G, bool softplus, int dtype, cudaStream_t st) {
-  if (!ssm_sizes_ok(B, S, D, N, G)) return MLSTM_ERR_SHAPE;
+  if (!ssm_sizes_ok(B, S, D, N, G) || !ssm_tokens_ok(strides) || gs[1] < 0 || gs[1] >= (1ll << 29)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_SCAN, st);
   SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, true);
-  s.gb = gs[0]; s.gt = gs[1];
-  const int lanes = ssm_lanes(N), np = 4 * lanes;
+  s.gb = gs[0]; s.gt = (int)gs[1];
+  const int lanes = ssm_lanes(N), np = ssm_padded(N);
   const SsmBwLayout l = ssm_bw_layout(s);
   char* w = static_cast<char*>(workspace);
   auto at = [&](size_t o) { return reinterpret_cast<float*>(w + o); };

@@ -37,33 +37,25 @@ template <typename T, int LN, int V, bool LOCAL> struct SsmFwSmem {
 template <typename T, int LN, int V, bool LOCAL>
 __global__ void __launch_bounds__(SsmFwSmem<T, LN, V, LOCAL>::P::THREADS, 5)
 ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
-  using M = SsmFwSmem<T, LN, V, LOCAL>;
-  using P = typename M::P;
-  using Ring = typename M::Ring;
+  using Mem = SsmFwSmem<T, LN, V, LOCAL>;
+  using P = typename Mem::P;
+  using Ring = typename Mem::Ring;
   using Sums = LaneSums<LN>;
-  constexpr int CH = P::CH, NP = P::NP, AHEAD = Ring::STAGES - 1;
+  constexpr int CH = P::CH, AHEAD = Ring::STAGES - 1;
   extern __shared__ __align__(16) char sm[];
-  float2* s_d = reinterpret_cast<float2*>(sm + M::Q);          // (step, step x)
-  float *s_b = reinterpret_cast<float*>(sm + M::B), *s_c = reinterpret_cast<float*>(sm + M::C), *s_y = reinterpret_cast<float*>(sm + M::Y);
-  const Ring ring{reinterpret_cast<T*>(sm + M::X)};            // x, dt, z; b, c
+  float2* s_d = reinterpret_cast<float2*>(sm + Mem::Q);          // (step, step x)
+  float *s_b = reinterpret_cast<float*>(sm + Mem::B), *s_c = reinterpret_cast<float*>(sm + Mem::C), *s_y = reinterpret_cast<float*>(sm + Mem::Y);
+  const Ring ring{reinterpret_cast<T*>(sm + Mem::X)};            // x, dt, z; b, c
   pdl_launch_dependents();
   pdl_wait();
   const P p(s, nseg, 0);
-  uint64_t a2[P::C][2], h[P::C][2];
+  uint64_t a2[P::C][P::H], h[P::C][P::H];
   float sum[P::C];
 #pragma unroll
-  for (int c = 0; c < P::C; ++c) { h[c][0] = h[c][1] = 0ull; sum[c] = 0.f; }
+  for (int c = 0; c < P::C; ++c) sum[c] = 0.f;
   ssm_rates(k.in.a, s, p, a2);
-  if (!LOCAL) {
-#pragma unroll
-    for (int c = 0; c < P::C; ++c) {
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (k.in.h0 != nullptr && p.on[c]) ssm_load4(k.in.h0 + ((size_t)p.b * s.D + p.d + c) * s.N, s.N, 4 * p.sub, v);
-      h[c][0] = f2(v[0], v[1]);
-      h[c][1] = f2(v[2], v[3]);
-    }
-    ssm_fold<false>(k.loc_h, k.loc_sum, 0, p.seg, s, p, a2, h);
-  }
+  ssm_load_states(LOCAL ? nullptr : k.in.h0, s, p, (size_t)p.b * s.D + p.d, h);
+  if (!LOCAL) ssm_fold<false>(k.loc_h, k.loc_sum, 0, p.seg, s, p, a2, h);
   float bias[V], skip[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -72,16 +64,20 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   }
   const int t_begin = p.seg * s.seg, t_end = min(s.S, t_begin + s.seg);
   const bool gate = !LOCAL && k.in.z != nullptr;
+  const SsmSource from_x = ssm_source<T>(k.in.x, p.b * s.xb + p.dcol, s.xt), from_dt = ssm_source<T>(k.in.dt, p.b * s.db + p.dcol, s.dt),
+                  from_z = ssm_source<T>(k.in.z, p.b * s.zb + p.dcol, s.zt), from_b = Ring::source_bc(k.in.b, p, s.bb, s.bt, s.bg),
+                  from_c = Ring::source_bc(k.in.c, p, s.cb, s.ct, s.cg);
   auto fetch = [&](int t0) {
     if (t0 < t_end) {
-      ring.copy(s, p, t0, 0, k.in.x, s.xb, s.xt);
-      ring.copy(s, p, t0, 1, k.in.dt, s.db, s.dt);
-      if (gate) ring.copy(s, p, t0, 2, k.in.z, s.zb, s.zt);
-      ring.copy_bc(s, p, t0, 0, k.in.b, s.bb, s.bt, s.bg);
-      if (!LOCAL) ring.copy_bc(s, p, t0, 1, k.in.c, s.cb, s.ct, s.cg);
+      ring.copy(s, p, t0, 0, from_x);
+      ring.copy(s, p, t0, 1, from_dt);
+      if (gate) ring.copy(s, p, t0, 2, from_z);
+      ring.copy_bc(s, p, t0, 0, from_b);
+      if (!LOCAL) ring.copy_bc(s, p, t0, 1, from_c);
     }
     cp_commit();
   };
+  ring.clear(s, p);
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(t_begin + i * SSM_TT);
   for (int t0 = t_begin; t0 < t_end; t0 += SSM_TT) {
@@ -94,7 +90,7 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
       float dt[V], step[V], xv[V];
       ring.get(tile, 0, i, p, xv);
       ring.get(tile, 1, i, p, dt);
-      ssm_step_v<V>(dt, bias, s.softplus, p.col_on && t0 + r < t_end, step);
+      ssm_step_v<V>(dt, bias, s.softplus, t0 + r >= t_end, step);
       Pack<float2, V> o;
 #pragma unroll
       for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
@@ -104,15 +100,7 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
     if (!LOCAL) ring.put(tile, 1, s_c);
     __syncthreads();
     fetch(t0 + AHEAD * SSM_TT);
-    if (!LOCAL && k.ckpt != nullptr) {
-#pragma unroll
-      for (int c = 0; c < P::C; ++c) {
-        if (!p.on[c]) continue;
-        Pack<uint64_t, 2> o;
-        o.e[0] = h[c][0]; o.e[1] = h[c][1];
-        store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.ckpt + (((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d + c) * NP + 4 * p.sub), o);
-      }
-    }
+    if (!LOCAL && k.ckpt != nullptr) ssm_put_states(k.ckpt, p, ((size_t)p.b * s.nt + t0 / SSM_TT) * s.D + p.d, h);
     constexpr int U = 4 / P::C;   // tokens whose sums over the states are taken together
 #pragma unroll(LOCAL ? 2 : 16)
     for (int t = 0; t < SSM_TT; t += U) {
@@ -120,20 +108,23 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const Pack<float2, P::C> q = load_pack<float2, P::C>(s_d + (t + u) * CH + p.ch);
-        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_b + (t + u) * NP + 4 * p.sub);
+        const Pack<uint64_t, P::H> b = ssm_token(s_b, t + u, p);
 #pragma unroll
         for (int c = 0; c < P::C; ++c) {
           const uint64_t step = f2(q.e[c].x, q.e[c].x), sx = f2(q.e[c].y, q.e[c].y);
-          h[c][0] = fma2(ex2_pair(mul2(step, a2[c][0])), h[c][0], mul2(sx, b.x));
-          h[c][1] = fma2(ex2_pair(mul2(step, a2[c][1])), h[c][1], mul2(sx, b.y));
+#pragma unroll
+          for (int i = 0; i < P::H; ++i) h[c][i] = fma2(ex2_pair(mul2(step, a2[c][i])), h[c][i], mul2(sx, b.e[i]));
           if (LOCAL) sum[c] += q.e[c].x;
         }
         if (!LOCAL) {
-          const ulonglong2 c2 = *reinterpret_cast<const ulonglong2*>(s_c + (t + u) * NP + 4 * p.sub);
+          const Pack<uint64_t, P::H> c2 = ssm_token(s_c, t + u, p);
 #pragma unroll
           for (int c = 0; c < P::C; ++c) {
+            uint64_t v = mul2(c2.e[0], h[c][0]);
+#pragma unroll
+            for (int i = 1; i < P::H; ++i) v = fma2(c2.e[i], h[c][i], v);
             float lo, hi;
-            unf2(fma2(c2.x, h[c][0], mul2(c2.y, h[c][1])), lo, hi);
+            unf2(v, lo, hi);
             acc[u * P::C + c] = lo + hi;
           }
         }
@@ -169,23 +160,14 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
       }
     }
   }
+  if (LOCAL) {
+    const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d;
+    ssm_put_states(k.loc_h, p, at, h);
 #pragma unroll
-  for (int c = 0; c < P::C; ++c) {
-    if (!p.on[c]) continue;
-    if (LOCAL) {
-      const size_t at = ((size_t)p.b * s.nseg + p.seg) * s.D + p.d + c;
-      Pack<uint64_t, 2> o;
-      o.e[0] = h[c][0]; o.e[1] = h[c][1];
-      store_pack<uint64_t, 2>(reinterpret_cast<uint64_t*>(k.loc_h + at * NP + 4 * p.sub), o);
-      if (p.sub == 0) k.loc_sum[at] = sum[c];
-    } else if (k.h_last != nullptr && p.seg == s.nseg - 1) {
-      float v[4];
-      unf2(h[c][0], v[0], v[1]);
-      unf2(h[c][1], v[2], v[3]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * p.sub + i < s.N) k.h_last[((size_t)p.b * s.D + p.d + c) * s.N + 4 * p.sub + i] = v[i];
-    }
+    for (int c = 0; c < P::C; ++c)
+      if (p.on[c] && p.sub == 0) k.loc_sum[at + c] = sum[c];
+  } else if (k.h_last != nullptr && p.seg == s.nseg - 1) {
+    ssm_store_states(k.h_last, s, p, (size_t)p.b * s.D + p.d, h);
   }
 }
 
@@ -216,8 +198,8 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
       unpack(load_pack<T, 4>(c + bc), cv);
     }
   } else {
-    ssm_load4(h + row * N, N, n, hv);
-    ssm_load4(a + (size_t)dc * N, N, n, av);
+    ssm_load<4>(h + row * N, N, n, hv);
+    ssm_load<4>(a + (size_t)dc * N, N, n, av);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (n + i >= N) continue;
@@ -228,7 +210,7 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
   const float raw[1] = {to_f32(dt[row])}, bias[1] = {dt_bias != nullptr ? dt_bias[dc] : 0.f};
   const float xv = to_f32(x[row]), zv = z != nullptr ? to_f32(z[row]) : 0.f, sk = skip != nullptr ? skip[dc] : 0.f;
   float st[1], acc = 0.f;
-  ssm_step_v<1>(raw, bias, softplus, true, st);
+  ssm_step_v<1>(raw, bias, softplus, false, st);
   const float sx = st[0] * xv, s2 = st[0] * kLog2e;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -265,6 +247,14 @@ static float ssm_rounds(long long grid, int slots, float add, float alone) {
   const float k = rounds > 1.f ? (float)slots : ceilf(per_sm), tile = k + add > alone ? k + add : alone;
   return rounds > 1.f ? 0.5f * (rounds + ceilf(rounds)) * tile : tile;
 }
+// Token strides are 32-bit numbers of bytes in the kernels.
+bool ssm_tokens_ok(const long long* st) {
+  const long long q[] = {st[1], st[3], st[5], st[7], st[10]};
+  for (const long long t : q)
+    if (t < 0 || t >= (1ll << 29)) return false;
+  return true;
+}
+
 // Segments: the number that should take least, the pass over the segments' own ends (for all but one) among it.  Measured for 128
 // CTAs of 128 tiles (4 x 2048 x 2048 channels, 16 states): forward 327, 222, 212, 206, 205 us with 1, 5, 8, 10, 16 segments,
 // backward 1758, 817, 543, 574, 530 us with 1, 3, 8, 10, 16.  Units of a tile's part of a full SM: 0.8 us forward, 4.1 us backward.
@@ -295,18 +285,18 @@ SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long lo
   s.softplus = softplus;
   s.pairs = false;
   if (st != nullptr) {
-    s.xb = st[0]; s.xt = st[1]; s.db = st[2]; s.dt = st[3]; s.zb = st[4]; s.zt = st[5];
-    s.bb = st[6]; s.bt = st[7]; s.bg = st[8]; s.cb = st[9]; s.ct = st[10]; s.cg = st[11];
+    s.xb = st[0]; s.xt = (int)st[1]; s.db = st[2]; s.dt = (int)st[3]; s.zb = st[4]; s.zt = (int)st[5];
+    s.bb = st[6]; s.bt = (int)st[7]; s.bg = st[8]; s.cb = st[9]; s.ct = (int)st[10]; s.cg = st[11];
   }
   return s;
 }
 
-size_t ssm_ckpt_bytes(int B, int S, int D, int N) { return (size_t)B * ceil_div(S, SSM_TT) * D * 4 * ssm_lanes(N) * sizeof(float); }
+size_t ssm_ckpt_bytes(int B, int S, int D, int N) { return (size_t)B * ceil_div(S, SSM_TT) * D * ssm_padded(N) * sizeof(float); }
 size_t ssm_fw_bytes(int B, int S, int D, int N, int G) {
   const SsmDims s = ssm_dims(B, S, D, N, G, false, nullptr, false);
   if (s.nseg == 1) return 0;
   const size_t rows = (size_t)B * s.nseg * D;
-  return rows * 4 * ssm_lanes(N) * sizeof(float) + rows * sizeof(float);
+  return rows * ssm_padded(N) * sizeof(float) + rows * sizeof(float);
 }
 
 template <typename T> bool ssm_vec(const SsmIn& in, const SsmDims& s, const void* dy, const void* y) {
@@ -323,7 +313,8 @@ template <typename T> bool ssm_vec(const SsmIn& in, const SsmDims& s, const void
 // b and c two elements at a time
 template <typename T> bool ssm_pairs(const SsmIn& in, const SsmDims& s) {
   if (s.N % 2 != 0 || !fits_access(in.b, 2 * sizeof(T)) || !fits_access(in.c, 2 * sizeof(T))) return false;
-  for (long long q : {s.bb, s.bt, s.bg, s.cb, s.ct, s.cg})
+  const long long strides[] = {s.bb, s.bt, s.bg, s.cb, s.ct, s.cg};
+  for (const long long q : strides)
     if (q % 2 != 0) return false;
   return true;
 }
@@ -345,19 +336,18 @@ static int ssm_fw_t(const SsmFw& k, const SsmDims& s, cudaStream_t st) {
 
 int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* workspace, int B, int S, int D, int N, int G,
                   bool softplus, int dtype, cudaStream_t st) {
-  if (!ssm_sizes_ok(B, S, D, N, G)) return MLSTM_ERR_SHAPE;
+  if (!ssm_sizes_ok(B, S, D, N, G) || !ssm_tokens_ok(strides)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_SCAN, st);
   SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, false);
-  const int lanes = ssm_lanes(N);
   SsmFw k{in, y, h_last, ckpt, nullptr, nullptr};
   if (s.nseg > 1) {
     k.loc_h = static_cast<float*>(workspace);
-    k.loc_sum = k.loc_h + (size_t)B * s.nseg * D * 4 * lanes;
+    k.loc_sum = k.loc_h + (size_t)B * s.nseg * D * ssm_padded(N);
   }
   MLSTM_DTYPE_SWITCH(dtype, T,
     const bool vec = ssm_vec<T>(in, s, nullptr, y);
     s.pairs = ssm_pairs<T>(in, s);
-    SSM_LANES_SWITCH(lanes, LN, return vec ? ssm_fw_t<T, LN, 4>(k, s, st) : ssm_fw_t<T, LN, 1>(k, s, st);))
+    SSM_LANES_SWITCH(ssm_lanes(N), LN, return vec ? ssm_fw_t<T, LN, 4>(k, s, st) : ssm_fw_t<T, LN, 1>(k, s, st);))
   return MLSTM_ERR_DTYPE;
 }
 

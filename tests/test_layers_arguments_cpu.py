@@ -136,6 +136,8 @@ def test_c_abi():
     need = lib.mlstm_b200_ssm_workspace_bytes(1, 4096, 64, 16, 1, 0)
     assert need > 0 and fw(64, 16, 1, p, need - 1) == -5 and fw(64, 16, 1, n, 0) == -3 and fw(64, 16, 1, p, need, odd) == -4
     assert fw(64, 129, 1, p, need) == -1 and fw(64, 16, 5, p, need) == -1
+    far = (ctypes.c_longlong * 12)(*([1] * 7 + [1 << 29] + [1] * 4))
+    assert lib.mlstm_b200_ssm_scan_fw(p, p, p, p, p, n, n, n, n, far, p, n, n, p, need, 1, 4096, 64, 16, 1, 1, 1, n) == -1
     need = lib.mlstm_b200_ssm_workspace_bytes(1, 4096, 64, 16, 1, 1)
     bw = lambda dz, ws, size: lib.mlstm_b200_ssm_scan_bw(p, p, p, p, p, n, p, n, st, p, p, st, n, p, p, p, p, p, n, dz, n, n, ws, size, 1, 4096, 64, 16, 1, 1, 1,  # noqa: E731
                                                          n)

@@ -265,6 +265,19 @@ def test_ssm_strides():
     ssm_case(t, True)
 
 
+def test_ssm_token_axis_of_any_stride():
+    """One token, whose stride means nothing; and tokens too far apart for the kernels, which the call gathers first."""
+    rng = np.random.default_rng(4)
+    t = ssm_inputs(3, 2, 1, 24, 16, 0, "f32")
+    t["x"] = make(rng, 2, 24).as_strided((2, 1, 24), (24, 1 << 40, 1)).requires_grad_(True)
+    ssm_case(t, True)
+    t = ssm_inputs(3, 1, 2, 8, 16, 0, "bf16")
+    far = torch.zeros((1 << 29) + 8, dtype=torch.bfloat16, device="cuda")
+    far[:8], far[-8:] = t["x"].detach()[0, 0], t["x"].detach()[0, 1]
+    t["x"] = far.as_strided((1, 2, 8), (1 << 29, 1 << 29, 1)).requires_grad_(True)
+    ssm_case(t, True)
+
+
 def test_ssm_parameters_in_16_bits():
     t = ssm_inputs(5, 2, 20, 32, 16, 0, "bf16")
     for n in ("skip", "dt_bias", "h_initial"):
