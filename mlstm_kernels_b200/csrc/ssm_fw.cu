@@ -171,40 +171,47 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   }
 }
 
-// One token: bound by the states, in and out once each, 16 bytes a thread (VEC; else element by element).  A CTA has 256 / LN channels
-// of one sequence.  (Two sequences to a thread, which would share what belongs to the channel, took 13 us instead of 11 for 64 x 4096
-// channels of 16 states: fewer warps wait for memory.)
-constexpr int SSM_STEP_THREADS = 256;
-template <typename T, int LN, bool VEC>
+// One token: bound by the states, in and out once each, 16 bytes at a time (VEC; else element by element).  LN lanes share a channel,
+// each with J times four of its states, LN apart from one another, so that a warp's accesses are whole sectors; what is done once
+// for a channel (some 150 instructions) is done by few lanes.
+constexpr int SSM_STEP_THREADS = 128;
+template <typename T, int LN, int J, bool VEC>
 __global__ void __launch_bounds__(SSM_STEP_THREADS)
 ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, const float* a, const float* skip, const float* dt_bias,
                 const float* h, T* y, float* h_new, int tiles, int D, int N, int G, bool softplus) {
   constexpr int CH = SSM_STEP_THREADS / LN;
   pdl_launch_dependents();
   pdl_wait();
-  const int sub = threadIdx.x % LN, n = 4 * sub;
+  const int sub = threadIdx.x % LN;
   const unsigned bi = blockIdx.x / (unsigned)tiles;
   const int d = (int)(blockIdx.x - bi * (unsigned)tiles) * CH + threadIdx.x / LN;
   const bool on = d < D;
   const int dc = on ? d : 0, g = G == 1 ? 0 : (int)((unsigned)dc / ((unsigned)D / (unsigned)G));
-  const size_t row = (size_t)bi * D + dc, at = row * N + n, bc = ((size_t)bi * G + g) * N + n;
-  float hv[4] = {0.f, 0.f, 0.f, 0.f}, av[4] = {0.f, 0.f, 0.f, 0.f}, bv[4] = {0.f, 0.f, 0.f, 0.f}, cv[4] = {0.f, 0.f, 0.f, 0.f};
-  if (VEC) {
-    if (n < N) {
-      const float4 q = ld_stream(reinterpret_cast<const float4*>(h + at));
-      hv[0] = q.x; hv[1] = q.y; hv[2] = q.z; hv[3] = q.w;
-      unpack(load_pack<float, 4>(a + (size_t)dc * N + n), av);
-      unpack(load_pack<T, 4>(b + bc), bv);
-      unpack(load_pack<T, 4>(c + bc), cv);
-    }
-  } else {
-    ssm_load<4>(h + row * N, N, n, hv);
-    ssm_load<4>(a + (size_t)dc * N, N, n, av);
+  const size_t row = (size_t)bi * D + dc, bc = ((size_t)bi * G + g) * N;
+  const float *hr = h + row * N, *ar = a + (size_t)dc * N;
+  float hv[J][4], av[J][4], bv[J][4], cv[J][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (n + i >= N) continue;
-      bv[i] = to_f32(b[bc + i]);
-      cv[i] = to_f32(c[bc + i]);
+  for (int j = 0; j < J; ++j) {
+    const int n = 4 * (sub + j * LN);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hv[j][i] = av[j][i] = bv[j][i] = cv[j][i] = 0.f;
+    if (VEC) {
+      if (n < N) {
+        const float4 q = ld_stream(reinterpret_cast<const float4*>(hr + n));
+        hv[j][0] = q.x; hv[j][1] = q.y; hv[j][2] = q.z; hv[j][3] = q.w;
+        unpack(load_pack<float, 4>(ar + n), av[j]);
+        unpack(load_pack<T, 4>(b + bc + n), bv[j]);
+        unpack(load_pack<T, 4>(c + bc + n), cv[j]);
+      }
+    } else {
+      ssm_load<4>(hr, N, n, hv[j]);
+      ssm_load<4>(ar, N, n, av[j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n + i >= N) continue;
+        bv[j][i] = to_f32(b[bc + n + i]);
+        cv[j][i] = to_f32(c[bc + n + i]);
+      }
     }
   }
   const float raw[1] = {to_f32(dt[row])}, bias[1] = {dt_bias != nullptr ? dt_bias[dc] : 0.f};
@@ -212,17 +219,22 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
   float st[1], acc = 0.f;
   ssm_step_v<1>(raw, bias, softplus, false, st);
   const float sx = st[0] * xv, s2 = st[0] * kLog2e;
+  float* out = h_new + row * N;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hv[i] = fmaf(ex2(s2 * av[i]), hv[i], sx * bv[i]);
-    acc = fmaf(cv[i], hv[i], acc);
-  }
-  if (VEC) {
-    if (on && n < N) __stcs(reinterpret_cast<float4*>(h_new + at), make_float4(hv[0], hv[1], hv[2], hv[3]));
-  } else {
+  for (int j = 0; j < J; ++j) {
+    const int n = 4 * (sub + j * LN);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (on && n + i < N) h_new[at + i] = hv[i];
+    for (int i = 0; i < 4; ++i) {
+      hv[j][i] = fmaf(ex2(s2 * av[j][i]), hv[j][i], sx * bv[j][i]);
+      acc = fmaf(cv[j][i], hv[j][i], acc);
+    }
+    if (VEC) {
+      if (on && n < N) __stcs(reinterpret_cast<float4*>(out + n), make_float4(hv[j][0], hv[j][1], hv[j][2], hv[j][3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (on && n + i < N) out[n + i] = hv[j][i];
+    }
   }
 #pragma unroll
   for (int o = LN / 2; o >= 1; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
@@ -255,18 +267,20 @@ bool ssm_tokens_ok(const long long* st) {
   return true;
 }
 
-// Segments: the number that should take least, the pass over the segments' own ends (for all but one) among it.  Measured for 128
-// CTAs of 128 tiles (4 x 2048 x 2048 channels, 16 states): forward 327, 222, 212, 206, 205 us with 1, 5, 8, 10, 16 segments,
-// backward 1758, 817, 543, 574, 530 us with 1, 3, 8, 10, 16.  Units of a tile's part of a full SM: 0.8 us forward, 4.1 us backward.
+// Segments: the number that should take least, the pass over the segments' own ends (for all but one) and its launch among it.
+// Measured for 128 CTAs of 128 tiles (4 x 2048 x 2048 channels, 16 states): forward 293, 208, 198, 193, 192 us with 1, 5, 8, 10, 16
+// segments, backward 1816, 703, 546, 586, 537; for 16 CTAs of 32 tiles (512 x 1024 channels): forward 69, 33, 27, 22, 21 us with 1, 4,
+// 11, 16, 32; for 128 CTAs of 8 tiles: 20 and 24 us with 1 and 4.  Units of a tile's part of a full SM: 0.9 us forward, 4.1 us backward.
 static int ssm_segments(long long ctas, int nt, bool backward) {
   int best = 1;
   float least = 0.f;
-  for (int n = 1; n <= 64 && (n == 1 || n <= nt / 4); ++n) {
+  for (int n = 1; n <= 64 && (n == 1 || n <= nt); ++n) {
     const int seg = ceil_div(nt, n);
     if (n > 1 && ceil_div(nt, seg) != n) continue;
-    float t = backward ? ssm_rounds(ctas * n, 4, 0.f, 4.f) : ssm_rounds(ctas * n, 5, 2.5f, 0.f);
-    if (n > 1) t += (backward ? 0.115f : 0.6f) * ssm_rounds(ctas * (n - 1), 5, 2.5f, 0.f);
-    t *= (float)seg + 0.5f;   // (half a tile's time to begin and to end)
+    float t = backward ? ssm_rounds(ctas * n, 4, 0.f, 4.f) : ssm_rounds(ctas * n, 5, 1.5f, 0.f);
+    if (n > 1) t += (backward ? 0.13f : 0.6f) * ssm_rounds(ctas * (n - 1), 5, 1.5f, 0.f);
+    t *= (float)seg + 0.5f;                      // (half a tile's time to begin and to end)
+    if (n > 1) t += backward ? 0.7f : 3.3f;      // 3 us
     if (n == 1 || t < least) { best = n; least = t; }
   }
   return best;
@@ -355,16 +369,16 @@ int launch_ssm_step(const void* x, const void* dt, const void* z, const void* b,
                     const float* h, void* y, float* h_new, int B, int D, int N, int G, bool softplus, int dtype, cudaStream_t st) {
   if (!ssm_sizes_ok(B, 1, D, N, G)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_STEP, st);
-  const int lanes = ssm_lanes(N);
-  const int tiles = ceil_div(D, SSM_STEP_THREADS / lanes);
+  const int lanes = N <= 4 ? 1 : N <= 16 ? 2 : N <= 64 ? 4 : 8, tiles = ceil_div(D, SSM_STEP_THREADS / lanes);
   const size_t grid = (size_t)B * tiles;
   if (grid >= (1ull << 31)) return MLSTM_ERR_SHAPE;
   const size_t four = 4 * dtype_size(dtype);
   const bool vec = N % 4 == 0 && fits_access(a, 16) && fits_access(h, 16) && fits_access(h_new, 16) && fits_access(b, four) && fits_access(c, four);
-#define RUN(LN, VEC)                                                                                                                              \
-  return launch_pdl(grid <= pdl_max_ctas(), ssm_step_kernel<T, LN, VEC>, (unsigned)grid, SSM_STEP_THREADS, 0, st, (const T*)x, (const T*)dt,        \
-                    (const T*)z, (const T*)b, (const T*)c, a, skip, dt_bias, h, (T*)y, h_new, tiles, D, N, G, softplus)
-  MLSTM_DTYPE_SWITCH(dtype, T, SSM_LANES_SWITCH(lanes, LN, if (vec) RUN(LN, true); RUN(LN, false);))
+#define RUN(LN, J)                                                                                                                                \
+  return launch_pdl(grid <= 2 * pdl_max_ctas(), vec ? ssm_step_kernel<T, LN, J, true> : ssm_step_kernel<T, LN, J, false>, (unsigned)grid,         \
+                    SSM_STEP_THREADS, 0, st, (const T*)x, (const T*)dt, (const T*)z, (const T*)b, (const T*)c, a, skip, dt_bias, h, (T*)y, h_new, \
+                    tiles, D, N, G, softplus)
+  MLSTM_DTYPE_SWITCH(dtype, T, if (N <= 4) RUN(1, 1); if (N <= 8) RUN(2, 1); if (N <= 16) RUN(2, 2); if (N <= 32) RUN(4, 2); if (N <= 64) RUN(4, 4); RUN(8, 4);)
 #undef RUN
   return MLSTM_ERR_DTYPE;
 }
