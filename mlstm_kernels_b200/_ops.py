@@ -286,8 +286,9 @@ def ssm_scan(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, skip: Optio
 def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial):
     B, S, D = x.shape
     N = a.shape[1]
-    n = _lib.load().mlstm_b200_ssm_checkpoint_bytes(B, S, D, N)
-    return _contig(x), x.new_empty((B, D, N), dtype=_F32), x.new_empty((max(n, 256),), dtype=torch.uint8)
+    # (worked out here, not asked for: S may be a symbol; sixteen tokens to a checkpoint)
+    n = B * ((S + 15) // 16) * D * _lib.load().mlstm_b200_ssm_checkpoint_bytes(1, 1, 1, int(N))
+    return _contig(x), x.new_empty((B, D, N), dtype=_F32), x.new_empty((torch.sym_max(n, 256),), dtype=torch.uint8)
 
 
 @torch.library.custom_op("mlstm_b200::ssm_scan_bw", mutates_args=(), device_types="cuda")

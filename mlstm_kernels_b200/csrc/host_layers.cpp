@@ -82,6 +82,7 @@ void check_norm(const Tensor& x, const Tensor& w, const Tensor& b) {
   check_kernel_dtype(x); check_kernel_dtype(w); check_kernel_dtype(b);
   if (x.dim() < 1) bad_shape(kNorm, "x", x, "(..., D)");
   check_int_sizes(kNorm, x);
+  if (x.size(-1) > 16384) C10_THROW_ERROR(ValueError, c10::str("layer_norm__b200: rows of more than 16384 elements (x of shape ", x.sizes(), ")"));
   for (const Tensor* p : {&w, &b}) {
     if (!p->defined()) continue;
     const bool fits = (p->dim() == 1 && p->size(0) == x.size(-1)) ||

@@ -14,7 +14,8 @@ constexpr int SSM_MAX_N = 128;
 
 struct SsmDims {
   int B, S, D, N, G;
-  int Dg, tiles;          // channels of a group; CTAs that they take
+  int Dg, tiles;          // channels of a group; tiles of channels that they take
+  int per_cta, parts;     // tiles that a CTA of the backward takes one after the other; CTAs to a group then
   int nseg, seg;          // the sequence in nseg segments of seg tokens (a multiple of SSM_TT), each a CTA of its own
   int nt;                 // tiles of SSM_TT tokens in the sequence
   bool softplus;
@@ -37,13 +38,14 @@ template <int LN, int V, int C_> struct SsmPlace {
   bool on[C];
   int row, col, dcol;
   bool col_on;
-  // nseg: segments that the launch has, from seg0 on
-  __device__ __forceinline__ SsmPlace(const SsmDims& s, int nseg, int seg0) {
+  // nseg: segments that the launch has, from seg0 on; the `turn`-th of per_cta tiles
+  __device__ __forceinline__ SsmPlace(const SsmDims& s, int nseg, int seg0, int per_cta = 1, int turn = 0) {
     const int lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
     sub = lane % LN; chl = lane / LN; ch = C * (warp * LC + chl);
     unsigned k = blockIdx.x;
-    tile = k % s.tiles; k /= s.tiles;
+    const int ctas = per_cta == 1 ? s.tiles : s.parts;
+    tile = k % ctas * per_cta + turn; k /= ctas;
     g = k % s.G; k /= s.G;
     seg = seg0 + k % nseg;
     b = k / nseg;

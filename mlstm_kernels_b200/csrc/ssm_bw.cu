@@ -24,7 +24,7 @@ struct SsmBw {
   const float* ckpt;        // (B, nt, D, NP)
   void *dx, *ddt, *dz;      // dz null without z
   float* dh0;               // (B, D, N) or null
-  float* part_bc;           // (G, tiles, B, S, 2, NP)
+  float* part_bc;           // (G, parts, B, S, 2, NP)
   float* part_a;            // (B * nseg, D, NP)
   float* part_d;            // (B * nseg, 2, D): dskip, ddt_bias
   float *loc_g, *loc_sum;   // (B, nseg, D, NP), (B, nseg, D)
@@ -133,24 +133,20 @@ template <typename T, int LN, int V> struct SsmBwSmem {
                           X = PART + sizeof(float) * P::WARPS * TF * 2 * P::NP, BYTES = X + Ring::BYTES;
 };
 
+// One tile of channels of a segment.  first: the sums over its channels begin the CTA's part of db and dc, else they are added.
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SsmBwSmem<T, LN, V>::P::THREADS, 4)
-ssm_bw_kernel(SsmBw k, SsmDims s) {
+__device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, const typename SsmBwSmem<T, LN, V>::P& p, bool first_turn, char* sm) {
   using M = SsmBwSmem<T, LN, V>;
   using P = typename M::P;
   using Ring = typename M::Ring;
   using Sums = LaneSums<LN>;
   constexpr int CH = P::CH, NP = P::NP, TF = M::TF, LC = P::LC, HALF = SSM_TT / 2, AHEAD = Ring::STAGES - 1;
-  extern __shared__ __align__(16) char sm[];
   float2* s_q = reinterpret_cast<float2*>(sm + M::Q);            // (step, step x)
   float *s_g = reinterpret_cast<float*>(sm + M::G), *s_b = reinterpret_cast<float*>(sm + M::B), *s_c = reinterpret_cast<float*>(sm + M::C);
   float *s_sum = reinterpret_cast<float*>(sm + M::SUMS), *s_part = reinterpret_cast<float*>(sm + M::PART);
   constexpr int S2 = SSM_TT * P::YS + 16;                        // (the two sums of a warp in different banks)
   float* s_yp = s_sum + S2 + SSM_TT * P::YS;                     // s_sum: sum g b and, from S2 on, sum a g e h; s_yp: sum c h
   const Ring ring{reinterpret_cast<T*>(sm + M::X)};              // x, dt, z, dy; b, c
-  pdl_launch_dependents();
-  pdl_wait();
-  const P p(s, s.nseg, 0);
   const bool gate = k.in.z != nullptr;
   uint64_t a2[P::C][2], r[P::C][2], da[P::C][2];
 #pragma unroll
@@ -181,7 +177,7 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
   };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
-  float* bc = k.part_bc + ((size_t)(p.g * s.tiles + p.tile) * s.B + p.b) * s.S * (2 * NP);
+  float* bc = k.part_bc + ((size_t)(p.g * s.parts + p.tile / s.per_cta) * s.B + p.b) * s.S * (2 * NP);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
     const int tile = t0 / SSM_TT;
     cp_wait<AHEAD - 1>();
@@ -331,7 +327,8 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
 #pragma unroll
             for (int w = 0; w < P::WARPS; ++w) a += s_part[w * TF * 2 * NP + e];
             const int tt = t0 + t + e / (2 * NP);
-            if (tt < t_end) bc[(size_t)tt * (2 * NP) + e % (2 * NP)] = a;
+            float* to = bc + (size_t)tt * (2 * NP) + e % (2 * NP);
+            if (tt < t_end) *to = first_turn ? a : *to + a;
           }
           __syncthreads();
         }
@@ -407,6 +404,20 @@ ssm_bw_kernel(SsmBw k, SsmDims s) {
   }
 }
 
+template <typename T, int LN, int V>
+__global__ void __launch_bounds__(SsmBwSmem<T, LN, V>::P::THREADS, 4)
+ssm_bw_kernel(SsmBw k, SsmDims s) {
+  using P = typename SsmBwSmem<T, LN, V>::P;
+  extern __shared__ __align__(16) char sm[];
+  pdl_launch_dependents();
+  pdl_wait();
+#pragma unroll 1
+  for (int turn = 0; turn < s.per_cta; ++turn) {
+    const P p(s, s.nseg, 0, s.per_cta, turn);
+    if (p.tile < s.tiles) ssm_bw_tile<T, LN, V>(k, s, p, turn == 0, sm);
+  }
+}
+
 // The sums over CTAs, in their order: db and dc over the channel tiles, da, dskip and ddt_bias over sequences and segments.
 struct SsmSums {
   const float *part_bc, *part_a, *part_d;
@@ -430,9 +441,9 @@ ssm_bw_sums_kernel(SsmSums q, SsmDims s) {
     const size_t tok = k % per_tile;
     const int g = (int)(k / per_tile);
     if (n >= s.N) return;
-    const float* src = q.part_bc + ((size_t)g * s.tiles * per_tile + tok) * 2 * q.NP + which * q.NP + n;
+    const float* src = q.part_bc + ((size_t)g * s.parts * per_tile + tok) * 2 * q.NP + which * q.NP + n;
     float a = 0.f;
-    for (int t = 0; t < s.tiles; ++t) a += src[t * per_tile * 2 * q.NP];
+    for (int t = 0; t < s.parts; ++t) a += src[t * per_tile * 2 * q.NP];
     static_cast<T*>(which == 0 ? q.db : q.dc)[(tok * s.G + g) * s.N + n] = from_f32<T>(a);
     return;
   }
@@ -469,7 +480,7 @@ static SsmBwLayout ssm_bw_layout(const SsmDims& s) {
   const size_t np = ssm_padded(s.N), rows = (size_t)s.B * s.nseg;
   SsmBwLayout l{};
   l.bc = 0;
-  l.a = align_up(l.bc + (size_t)s.G * s.tiles * s.B * s.S * 2 * np * sizeof(float), 256);
+  l.a = align_up(l.bc + (size_t)s.G * s.parts * s.B * s.S * 2 * np * sizeof(float), 256);
   l.d = align_up(l.a + rows * s.D * np * sizeof(float), 256);
   l.g = align_up(l.d + rows * 2 * s.D * sizeof(float), 256);
   l.sum = align_up(l.g + (s.nseg > 1 ? rows * s.D * np * sizeof(float) : 0), 256);
@@ -480,7 +491,7 @@ size_t ssm_bw_bytes(int B, int S, int D, int N, int G) { return ssm_bw_layout(ss
 
 template <typename T, int LN, int V>
 static int ssm_bw_t(const SsmBw& k, const SsmDims& s, cudaStream_t st) {
-  const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = per_seg * s.nseg;
+  const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = (unsigned)s.B * s.G * s.parts * s.nseg;
   const bool overlap = grid <= pdl_max_ctas();
   if (s.nseg > 1)   // the first segment leaves nothing to another
     if (int rc = ssm_launch(ssm_bw_local_kernel<T, LN, V>, 256 / SSM_BW_LOCAL_C, SsmBwLocalSmem<T, LN, V>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;

@@ -286,14 +286,18 @@ static int ssm_segments(long long ctas, int nt, bool backward) {
   return best;
 }
 
+constexpr int SSM_MAX_PARTS = 64;
 SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* st, bool backward) {
   SsmDims s{};
   s.B = B; s.S = S; s.D = D; s.N = N; s.G = G;
   s.Dg = D / G;
   s.tiles = ceil_div(s.Dg, ssm_tile_channels(N));
   s.nt = ceil_div(S, SSM_TT);
-  const long long ctas = (long long)B * G * s.tiles;
-  const int n = ssm_segments(ctas, s.nt, backward);
+  // Each CTA of the backward writes its channels' sums of db and dc, 2 N values a token: no more than 64 to a token, so that they
+  // take no more room than the other gradients (8192 channels of 16 states: 128 tiles in 64 CTAs).
+  s.per_cta = backward ? ceil_div(s.tiles, SSM_MAX_PARTS) : 1;
+  s.parts = ceil_div(s.tiles, s.per_cta);
+  const int n = ssm_segments((long long)B * G * s.parts, s.nt, backward);
   s.seg = ceil_div(s.nt, n) * SSM_TT;
   s.nseg = ceil_div(S, s.seg);
   s.softplus = softplus;

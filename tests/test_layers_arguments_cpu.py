@@ -97,6 +97,8 @@ def test_other_limits():
         for taps in (0, 1, 5):
             with pytest.raises(ValueError, match="2 to 4 taps"):
                 mk.short_conv__b200(e(B, S, D), e(D, taps))
+        with pytest.raises(ValueError, match="16384"):
+            mk.layer_norm__b200(e(3, 16385))
         with pytest.raises(ValueError, match="N from 1 to 128"):
             mk.ssm_scan__b200(e(B, S, D), e(B, S, D), e(D, 129, dt=F32), e(B, S, 129), e(B, S, 129))
         with pytest.raises(ValueError, match="multiple of G"):
@@ -109,6 +111,16 @@ def test_other_limits():
         a["state_new"] = e(B, D, W - 1).transpose(1, 2)
         with pytest.raises(ValueError, match="contiguous"):
             mk.short_conv_step__b200(**a)
+
+
+@pytest.mark.parametrize("B,S,D,N", [(2, 100, 24, 16), (1, 16, 7, 1), (3, 17, 65, 33), (1, 1, 1, 128)])
+def test_checkpoints_of_the_traced_operator(B, S, D, N):
+    """The traced operator's own count of the checkpoints' bytes is the library's."""
+    with FakeTensorMode():
+        x, bc = e(B, S, D), e(B, S, N)
+        y, h, ck = torch.ops.mlstm_b200.ssm_scan(x, x, e(D, N, dt=F32), bc, bc, None, None, None, True, None)
+    assert y.shape == (B, S, D) and h.shape == (B, D, N) and h.dtype == F32
+    assert ck.numel() == max(256, _lib.load().mlstm_b200_ssm_checkpoint_bytes(B, S, D, N))
 
 
 def test_c_abi():

@@ -250,6 +250,12 @@ def test_ssm_long_sequences_in_segments(B, S, D, N, G, dtype):
     ssm_case(ssm_inputs(S, B, S, D, N, G, dtype), True, summed=S)
 
 
+def test_ssm_many_channels():
+    """More tiles of channels than CTAs that write sums: each CTA takes several, one after the other."""
+    ssm_case(ssm_inputs(12, 1, 20, 70 * 8 - 4, 128, 0, "f32"), True)
+    ssm_case(ssm_inputs(13, 2, 33, 2 * 131 * 8, 100, 2, "bf16"), True)
+
+
 def test_ssm_strides():
     """Operands as parts of wider rows, at offsets that no wide access fits too; a gradient without memory of its own."""
     rng = np.random.default_rng(3)
@@ -432,6 +438,20 @@ def test_compiled_without_graph_break(op):
         assert torch.equal(a, b)
 
 
+def test_compiled_for_any_length():
+    t = ssm_inputs(4, 2, 50, 64, 16, 0, "bf16", grad=False)
+    tok = ("x", "dt", "b", "c", "z")
+    w = make(np.random.default_rng(1), 64, 4)
+
+    def fn(t):
+        u = mk.short_conv__b200(mk.layer_norm__b200(t["x"]), w, activation="silu")
+        return mk.ssm_scan__b200(**{**t, "x": u}, softplus=True)
+    compiled = torch.compile(fn, fullgraph=True, dynamic=True)
+    for S in (50, 33, 41):
+        cut = {n: v[:, :S].contiguous() if n in tok else v for n, v in t.items()}
+        assert torch.equal(fn(cut), compiled(cut))
+
+
 def test_steps_compile():
     rng = np.random.default_rng(1)
     x, s, w = make(rng, 3, 40), make(rng, 3, 3, 40), make(rng, 40, 4)
@@ -443,6 +463,30 @@ def test_steps_compile():
         return y, s, h
     for p, q in zip(step(x, s, h), torch.compile(step, fullgraph=True)(x, s, h)):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("op", ["norm", "conv", "ssm"])
+def test_offsets_past_32_bits(op):
+    """Tensors of more than 2^31 elements: the last sequence comes out as it does alone."""
+    B, S, D = 521, 2048, 2048
+    dt = torch.bfloat16
+    rng = np.random.default_rng(3)
+    x = torch.zeros(B, S, D, dtype=dt, device="cuda")
+    assert x.numel() > 1 << 31
+    x[-1] = make(rng, S, D, dtype=dt)
+    w, par, bc = make(rng, D, 4), make(rng, D), make(rng, B, S, 16, dtype=dt)
+    a = -torch.exp(make(rng, D, 16))
+    fn = {"norm": lambda x, bc: mk.layer_norm__b200(x, par, par), "conv": lambda x, bc: mk.short_conv__b200(x, w, par, activation="silu"),
+          "ssm": lambda x, bc: mk.ssm_scan__b200(x, x, a, bc, bc, par, None, par, True)}[op]
+
+    def run(x, bc):
+        x = x.requires_grad_(True)
+        y = fn(x, bc)
+        g, = torch.autograd.grad(y, x, x.detach())
+        return y[-1].detach().clone(), g[-1].clone()
+    for got, alone in zip(run(x, bc), run(x.detach()[-1:].clone(), bc[-1:])):
+        # the scan may be cut into other segments, which moves f32 values by some units and so a few bf16 ones by a step
+        assert torch.equal(got, alone) if op != "ssm" else (got.float() - alone.float()).abs().max() <= 2.0 ** -7 * alone.float().abs().max()
 
 
 def test_a_layer_of_them_prompt_then_tokens():
