@@ -54,26 +54,39 @@ constexpr int ln_ctas(int nv, int threads, bool backward) {
   return threads >= most ? 1 : most / threads;
 }
 
-// Sums of two values over the TPR threads of a row; every thread gets both.  `turn` alternates the buffers, so that one barrier does.
-template <int TPR> __device__ __forceinline__ float2 row_sum2(float a, float b, int& turn) {
+// Sums of K values over the TPR threads of a row; every thread gets them.  `turn` alternates the buffers, so that one barrier does.
+template <int TPR, int K> __device__ __forceinline__ void row_sums(float (&v)[K], int& turn) {
 #pragma unroll
-  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
-  if (TPR <= 32) return make_float2(a, b);
-  constexpr int WARPS = TPR <= 32 ? 1 : TPR / 32;
-  __shared__ float2 s_sum[2][WARPS];
-  if ((threadIdx.x & 31) == 0) s_sum[turn][threadIdx.x >> 5] = make_float2(a, b);
-  __syncthreads();
-  float2 v = s_sum[turn][threadIdx.x & (WARPS - 1)];
-  turn ^= 1;
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1)
 #pragma unroll
-  for (int o = WARPS / 2; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    for (int i = 0; i < K; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if constexpr (TPR > 32) {
+    constexpr int WARPS = TPR / 32;
+    __shared__ float s_sum[2][K][WARPS];
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < K; ++i) s_sum[turn][i][threadIdx.x >> 5] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      if constexpr (WARPS <= 8) {   // (each thread adds them up: less latency than shuffles)
+        v[i] = s_sum[turn][i][0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) v[i] += s_sum[turn][i][w];
+      } else {
+        v[i] = s_sum[turn][i][threadIdx.x & (WARPS - 1)];
+#pragma unroll
+        for (int o = WARPS / 2; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+      }
+    }
+    turn ^= 1;
   }
-  return v;
+}
+template <int TPR> __device__ __forceinline__ float row_sum(float a, int& turn) {
+  float v[1] = {a};
+  row_sums<TPR, 1>(v, turn);
+  return v[0];
 }
 
 // What a thread has of a row: NQ chunks of 16 bytes, E elements each, with aligned rows (VEC) neighbours, else one lane beside the
@@ -210,7 +223,7 @@ ln_fw_kernel(const T* x, const void* weight, const void* bias, T* y, float* mean
     for (int i = 0; i < NQ; ++i)
 #pragma unroll
       for (int e = 0; e < H; ++e) s = add2(s, v[i][e]);
-    const float mu = row_sum2<TPR>(sum2(s), 0.f, turn).x * inv_n;
+    const float mu = row_sum<TPR>(sum2(s), turn) * inv_n;
     s = 0ull;
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
@@ -227,7 +240,7 @@ ln_fw_kernel(const T* x, const void* weight, const void* bias, T* y, float* mean
           s = fma2(f2(p, q), f2(p, q), s);
         }
       }
-    const float rs = rsqrtf(row_sum2<TPR>(sum2(s), 0.f, turn).x * inv_n + eps);
+    const float rs = rsqrtf(row_sum<TPR>(sum2(s), turn) * inv_n + eps);
     if (r < d.rows) {
       const size_t out = (size_t)r * d.NH + head;
       if (mean != nullptr && t == 0) { mean[out] = mu; rstd[out] = rs; }
@@ -297,8 +310,9 @@ ln_bw_kernel(const T* x, const void* weight, const float* mean, const float* rst
         s1 = add2(s1, u[i][e]);
         s2 = fma2(u[i][e], v[i][e], s2);
       }
-    const float2 c = row_sum2<TPR>(sum2(s1), sum2(s2), turn);
-    const uint64_t c1 = f2(-c.x * inv_n, -c.x * inv_n), c2 = f2(-c.y * inv_n, -c.y * inv_n);
+    float c[2] = {sum2(s1), sum2(s2)};
+    row_sums<TPR, 2>(c, turn);
+    const uint64_t c1 = f2(-c[0] * inv_n, -c[0] * inv_n), c2 = f2(-c[1] * inv_n, -c[1] * inv_n);
     if (now.r < d.rows) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
