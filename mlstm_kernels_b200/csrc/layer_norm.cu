@@ -4,7 +4,7 @@
 //   g = dy w:  dx = rstd (g - mean(g) - xhat mean(g xhat));  dw = sum over rows of dy xhat,  db = sum over rows of dy
 //
 // Bound by HBM: the forward moves x and y, the backward x, dy and dx.  A row stays in the registers of some lanes of a warp (up to
-// 512 elements) or of one CTA, in pieces of 16 bytes, so that the variance is taken about the mean without a second read; sums are
+// 512 elements) or of one CTA, 16 elements a thread (eight took 235 us instead of 158 for the backward of 131072 x 1024), so that the variance is taken about the mean without a second read; sums are
 // f32, and up to four more rows are on their way meanwhile.  Rows may lie apart in memory (x seen as (B, S, NH, DH) where it lies as
 // (B, NH, S, DH)); every CTA stays with one head, whose weight and bias are read once.
 // bf16, 4096 x 8 x 16 heads of 256 read in place: forward 94 us (5.7 TB/s), backward 126 (6.4 TB/s), 252 without the copies ahead;
@@ -14,7 +14,7 @@
 
 namespace mlstm {
 
-constexpr int LN_V = 8;            // elements of a row to a thread, or twice as many
+constexpr int LN_V = 16;           // elements of a row to a thread
 constexpr int LN_MAX_D = 16384;    // 1024 threads, twice eight elements
 
 // The rows of one head: row r at (r / n1) s0 + (r % n1) s1 + head s2.
@@ -49,8 +49,8 @@ template <int TPR> struct LnGroup {
 };
 // CTAs to an SM that the registers are kept for; the grid is that many CTAs to an SM at most, as each goes through rows until there
 // are no more (a few CTAs over would take as long again).
-constexpr int ln_ctas(int nv, int threads, bool backward) {
-  const int most = backward ? (nv == 1 ? 768 : 512) : (nv == 1 ? 1024 : 768);
+constexpr int ln_ctas(int threads, bool backward) {
+  const int most = backward ? 512 : 768;
   return threads >= most ? 1 : most / threads;
 }
 
@@ -92,8 +92,8 @@ template <int TPR> __device__ __forceinline__ float row_sum(float a, int& turn) 
 // What a thread has of a row: NQ chunks of 16 bytes, E elements each, with aligned rows (VEC) neighbours, else one lane beside the
 // other.  ARRS rows at a time (x, or x and dy) come into shared memory by asynchronous copies, SLOTS of them ahead; each thread
 // copies just what it reads itself, so that its own wait is all that it takes.
-template <typename T, int NV, int TPR, bool VEC, int ARRS, int CTAS> struct LnRing {
-  static constexpr int THREADS = LnGroup<TPR>::THREADS, E = 16 / sizeof(T), NQ = NV * LN_V / E, H = E / 2;
+template <typename T, int TPR, bool VEC, int ARRS, int CTAS> struct LnRing {
+  static constexpr int THREADS = LnGroup<TPR>::THREADS, E = 16 / sizeof(T), NQ = LN_V / E, H = E / 2;
   static constexpr int SLOT = ARRS * NQ * THREADS * 16 + (ARRS == 2 ? 2 * THREADS * 4 : 0);
   static constexpr int FIT = (216 * 1024 / CTAS - (ARRS == 2 && TPR <= 32 ? 16 * 1024 : 0)) / SLOT, SLOTS = FIT > 4 ? 4 : FIT < 1 ? 1 : FIT;
   static constexpr size_t BYTES = (size_t)SLOT * SLOTS;
@@ -183,13 +183,13 @@ __device__ __forceinline__ float sum2(uint64_t v) {
   return a + b;
 }
 
-template <typename T, int NV, int TPR, bool VEC> using LnFwRing = LnRing<T, NV, TPR, VEC, 1, ln_ctas(NV, LnGroup<TPR>::THREADS, false)>;
-template <typename T, int NV, int TPR, bool VEC> using LnBwRing = LnRing<T, NV, TPR, VEC, 2, ln_ctas(NV, LnGroup<TPR>::THREADS, true)>;
+template <typename T, int TPR, bool VEC> using LnFwRing = LnRing<T, TPR, VEC, 1, ln_ctas(LnGroup<TPR>::THREADS, false)>;
+template <typename T, int TPR, bool VEC> using LnBwRing = LnRing<T, TPR, VEC, 2, ln_ctas(LnGroup<TPR>::THREADS, true)>;
 
-template <typename T, int NV, int TPR, bool VEC>
-__global__ void __launch_bounds__(LnGroup<TPR>::THREADS, ln_ctas(NV, LnGroup<TPR>::THREADS, false))
+template <typename T, int TPR, bool VEC>
+__global__ void __launch_bounds__(LnGroup<TPR>::THREADS, ln_ctas(LnGroup<TPR>::THREADS, false))
 ln_fw_kernel(const T* x, const void* weight, const void* bias, T* y, float* mean, float* rstd, LnRows xr, LnDims d, float eps) {
-  using R = LnFwRing<T, NV, TPR, VEC>;
+  using R = LnFwRing<T, TPR, VEC>;
   constexpr int ROWS = LnGroup<TPR>::ROWS, NQ = R::NQ, H = R::H;
   extern __shared__ __align__(16) char sm[];
   pdl_launch_dependents();
@@ -255,14 +255,14 @@ ln_fw_kernel(const T* x, const void* weight, const void* bias, T* y, float* mean
 }
 
 // partial: (parts, 2, NH, D), the sums of this CTA's rows for dw and db; null when neither is wanted
-template <typename T, int NV, int TPR, bool VEC>
-__global__ void __launch_bounds__(LnGroup<TPR>::THREADS, ln_ctas(NV, LnGroup<TPR>::THREADS, true))
+template <typename T, int TPR, bool VEC>
+__global__ void __launch_bounds__(LnGroup<TPR>::THREADS, ln_ctas(LnGroup<TPR>::THREADS, true))
 ln_bw_kernel(const T* x, const void* weight, const float* mean, const float* rstd, const T* dy, T* dx, float* partial, LnRows xr,
              LnRows yr, LnRows dr, LnDims d) {
-  using R = LnBwRing<T, NV, TPR, VEC>;
+  using R = LnBwRing<T, TPR, VEC>;
   constexpr int THREADS = R::THREADS, ROWS = LnGroup<TPR>::ROWS, NQ = R::NQ, H = R::H, E = R::E;
   extern __shared__ __align__(16) char sm[];
-  __shared__ float s_part[ROWS > 1 ? ROWS * NV * LN_V * TPR : 1];
+  __shared__ float s_part[ROWS > 1 ? ROWS * LN_V * TPR : 1];
   pdl_launch_dependents();
   pdl_wait();
   const R ring{sm};
@@ -337,12 +337,12 @@ ln_bw_kernel(const T* x, const void* weight, const float* mean, const float* rst
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) s_part[(g * NV * LN_V + i * E + e) * TPR + t] = f[i][e];
+        for (int e = 0; e < E; ++e) s_part[(g * LN_V + i * E + e) * TPR + t] = f[i][e];
       __syncthreads();
-      for (int k = threadIdx.x; k < NV * LN_V * TPR; k += THREADS) {
+      for (int k = threadIdx.x; k < LN_V * TPR; k += THREADS) {
         float a = 0.f;
 #pragma unroll
-        for (int q = 0; q < ROWS; ++q) a += s_part[q * NV * LN_V * TPR + k];
+        for (int q = 0; q < ROWS; ++q) a += s_part[q * LN_V * TPR + k];
         const int ie = k / TPR, c = R::col(k % TPR, ie / E, ie % E);
         if (c < d.D) out[c] = a;
       }
@@ -383,12 +383,14 @@ ln_param_kernel(const float* partial, int parts, size_t cols, void* dw, void* db
 
 // ---- launchers ----------------------------------------------------------------------------------------
 static int ln_threads(int D) {   // to a row
-  return D <= 64 ? 8 : D <= 256 ? 16 : D <= 512 ? 32 : D <= 1024 ? 128 : D <= 4096 ? 256 : D <= 8192 ? 512 : 1024;
+  int t = 4;
+  while (t * LN_V < D) t *= 2;
+  return t;
 }
 // CTAs per head: as many as the GPU has room for at once, no more than there are rows for.
 static int ln_parts(long long rows, int NH, int D, bool backward) {
-  const int tpr = ln_threads(D), threads = tpr <= 32 ? 256 : tpr, nv = D <= tpr * LN_V ? 1 : 2;
-  const long long per_cta = threads / tpr, room = (long long)sm_count() * ln_ctas(nv, threads, backward);
+  const int tpr = ln_threads(D), threads = tpr <= 32 ? 256 : tpr;
+  const long long per_cta = threads / tpr, room = (long long)sm_count() * ln_ctas(threads, backward);
   // (in the backward every CTA writes two rows of partial sums: four rows of input at least)
   const long long most = (rows + per_cta * (backward ? 4 : 1) - 1) / (per_cta * (backward ? 4 : 1));
   long long parts = room / NH;
@@ -407,16 +409,16 @@ template <typename T> static bool ln_vec(const void* const* ptrs, int n, const L
   return true;
 }
 
-#define LN_FORMS(RUN)                                                            \
-  if (D <= 64) RUN(1, 8)                                                         \
-  if (D <= 128) RUN(1, 16)                                                       \
-  if (D <= 256) RUN(2, 16)                                                       \
-  if (D <= 512) RUN(2, 32)                                                       \
-  if (D <= 1024) RUN(1, 128)                                                     \
-  if (D <= 2048) RUN(1, 256)                                                     \
-  if (D <= 4096) RUN(2, 256)                                                     \
-  if (D <= 8192) RUN(2, 512)                                                     \
-  RUN(2, 1024)
+#define LN_FORMS(RUN)      \
+  if (D <= 64) RUN(4)      \
+  if (D <= 128) RUN(8)     \
+  if (D <= 256) RUN(16)    \
+  if (D <= 512) RUN(32)    \
+  if (D <= 1024) RUN(64)   \
+  if (D <= 2048) RUN(128)  \
+  if (D <= 4096) RUN(256)  \
+  if (D <= 8192) RUN(512)  \
+  RUN(1024)
 
 template <typename... KArgs, typename... Args>
 static int ln_run(void (*kern)(KArgs...), size_t smem, unsigned threads, unsigned grid, cudaStream_t st, Args... args) {
@@ -430,9 +432,9 @@ static int ln_fw_t(const T* x, const LnRows& xr, const void* w, const void* b, T
   const bool vec = ln_vec<T>(ptrs, 4, &xr, 1, d.D);
   const unsigned grid = (unsigned)d.parts * (unsigned)d.NH;
   const int D = d.D;
-#define RUN(NV, TPR)                                                                                                                          \
-  return vec ? ln_run(ln_fw_kernel<T, NV, TPR, true>, LnFwRing<T, NV, TPR, true>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, b, y, mean, rstd, xr, d, eps) \
-             : ln_run(ln_fw_kernel<T, NV, TPR, false>, LnFwRing<T, NV, TPR, false>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, b, y, mean, rstd, xr, d, eps);
+#define RUN(TPR)                                                                                                                              \
+  return vec ? ln_run(ln_fw_kernel<T, TPR, true>, LnFwRing<T, TPR, true>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, b, y, mean, rstd, xr, d, eps) \
+             : ln_run(ln_fw_kernel<T, TPR, false>, LnFwRing<T, TPR, false>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, b, y, mean, rstd, xr, d, eps);
   LN_FORMS(RUN)
 #undef RUN
 }
@@ -445,9 +447,9 @@ static int ln_bw_t(const T* x, const LnRows& xr, const void* w, const float* mea
   const bool vec = ln_vec<T>(ptrs, 4, rows, 3, d.D);
   const unsigned grid = (unsigned)d.parts * (unsigned)d.NH;
   const int D = d.D;
-#define RUN(NV, TPR)                                                                                                                          \
-  return vec ? ln_run(ln_bw_kernel<T, NV, TPR, true>, LnBwRing<T, NV, TPR, true>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, mean, rstd, dy, dx, partial, xr, yr, dr, d) \
-             : ln_run(ln_bw_kernel<T, NV, TPR, false>, LnBwRing<T, NV, TPR, false>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, mean, rstd, dy, dx, partial, xr, yr, dr, d);
+#define RUN(TPR)                                                                                                                              \
+  return vec ? ln_run(ln_bw_kernel<T, TPR, true>, LnBwRing<T, TPR, true>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, mean, rstd, dy, dx, partial, xr, yr, dr, d) \
+             : ln_run(ln_bw_kernel<T, TPR, false>, LnBwRing<T, TPR, false>::BYTES, LnGroup<TPR>::THREADS, grid, st, x, w, mean, rstd, dy, dx, partial, xr, yr, dr, d);
   LN_FORMS(RUN)
 #undef RUN
 }
