@@ -88,6 +88,13 @@ def test_layer_norm_strides(how):
         check(g, r[n], n)
 
 
+@pytest.mark.parametrize("shape", [(3, 40), (1, 40), (2, 1, 40), (5, 5)])
+def test_layer_norm_of_heads_alone(shape):
+    """(NH, D) itself, one head, and as many heads as elements."""
+    rng = np.random.default_rng(9)
+    norm_case(make(rng, *shape, grad=True), make(rng, *shape[-2:], grad=True), make(rng, *shape[-2:], grad=True), make(rng, *shape))
+
+
 def test_layer_norm_constant_rows_and_far_means():
     x = torch.full((3, 64), 7.0, device="cuda")
     assert (mk.layer_norm__b200(x) == 0).all()
@@ -271,6 +278,30 @@ def test_ssm_strides():
     ssm_case(t, True)
 
 
+def test_ssm_only_the_last_state_and_only_some_gradients():
+    t = ssm_inputs(14, 2, 45, 40, 16, 2, "bf16")
+    dh = make(np.random.default_rng(2), 2, 40, 16)
+    ref = O.ssm_scan(**{n: f64(v) for n, v in t.items()}, softplus=True, dy=np.zeros((2, 45, 40)), dh_last=f64(dh))
+    _, h = mk.ssm_scan__b200(**t, softplus=True, return_last_states=True)
+    for n, g in zip(t, torch.autograd.grad(h, list(t.values()), dh, allow_unused=True)):
+        check(g, ref["d" + n], "d" + n)
+    for n in ("a", "b", "h_initial"):   # one input alone wants a gradient
+        only = {m: v.detach().requires_grad_(m == n) for m, v in t.items()}
+        _, h = mk.ssm_scan__b200(**only, softplus=True, return_last_states=True)
+        check(torch.autograd.grad(h, only[n], dh)[0], ref["d" + n], "d" + n)
+
+
+def test_ssm_operands_without_memory_of_their_own():
+    """b and c the same for all sequences, x the same for all tokens: strides of zero, and gradients summed by whoever expanded them."""
+    rng = np.random.default_rng(6)
+    B, S, D, N = 3, 40, 24, 16
+    t = ssm_inputs(15, B, S, D, N, 0, "f32", grad=False)
+    t["b"], t["c"] = (make(rng, 1, S, N).expand(B, S, N) for _ in range(2))
+    t["x"] = make(rng, B, 1, D).expand(B, S, D)
+    t = {n: v.requires_grad_(True) for n, v in t.items()}
+    ssm_case(t, True)
+
+
 def test_ssm_token_axis_of_any_stride():
     """One token, whose stride means nothing; and tokens too far apart for the kernels, which the call gathers first."""
     rng = np.random.default_rng(4)
@@ -377,6 +408,31 @@ def test_same_bits_again_on_another_stream_and_from_a_graph(op):
     graph.replay()
     for a, b in zip(run(), captured):
         assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once():
+    """The same inputs on two streams, neither waiting for the other: workspaces are each call's own."""
+    jobs = {op: fn_leaves for op, fn_leaves in calls().items()}
+    dy = torch.ones(2, 300, 64, dtype=torch.bfloat16, device="cuda")
+
+    def run():
+        out = []
+        for fn, leaves in jobs.values():
+            y = fn()
+            out += [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+        return out
+    alone = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for s, g in zip(streams, got):
+            with torch.cuda.stream(s):
+                g[:] = run()
+    torch.cuda.synchronize()
+    for g in got:
+        for a, b in zip(alone, g):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("op", ["norm", "conv", "ssm"])
