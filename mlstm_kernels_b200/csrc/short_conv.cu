@@ -6,8 +6,8 @@
 // Tokens before the first are those of x_initial (B, W-1, D), or zeros.  Bound by HBM: x in and y out, in the backward x and dy in
 // and dx out.  A thread walks a run of tokens of a few neighbouring channels with the last W tokens in registers; tokens at the
 // seam of two runs are read by both (W - 1 of a run's length), mostly from L2.
-// bf16, 32768 x 2048, four taps and SiLU: forward 65 us (4.1 TB/s; schedulers 60 %, special functions 52 % busy: two of them to an
-// element for the logistic function alone), backward 127 (3.2 TB/s; schedulers 53 %).
+// bf16, 32768 x 2048, four taps and SiLU: forward 60 us (4.4 TB/s; schedulers 60 %, special functions 52 % busy: two of them to an
+// element for the logistic function alone), backward 104 (3.9 TB/s; schedulers 60 %).
 #include <type_traits>
 
 #include "launch.cuh"
@@ -136,7 +136,7 @@ constexpr int CONV_U = 4;   // tokens at a time
 
 // One thread: V channels of one run of one sequence, threads of neighbouring channels next to each other; CONV_U tokens are on their
 // way in registers while as many are worked on.  (Copies to shared memory as in the backward cost more instructions than the wait
-// that they save: 32768 x 2048 channels, 71 us against 65.)
+// that they save: 32768 x 2048 channels in runs of 48, 71 us against 65.)
 template <typename T, int V, int W>
 __global__ void __launch_bounds__(256, 3)
 conv_fw_kernel(const T* x, const T* x0, const void* w, const void* bias, T* y, T* x_last, ConvDims d) {
@@ -187,7 +187,7 @@ conv_fw_kernel(const T* x, const T* x0, const void* w, const void* bias, T* y, T
 
 // The backward's tokens come into shared memory by asynchronous copies, CONV_U of x and dy at a time and SLOTS times as many ahead;
 // each thread copies just what it reads itself, so that its own wait is all that it takes.  (In registers they did not come early
-// enough: 32768 x 2048 channels, 381 us against 135.)
+// enough: 32768 x 2048 channels in runs of 64, 381 us against 135.)
 template <typename T, int V> struct ConvRing {
   static constexpr int PIECE = sizeof(T) * V, SLOT = 2 * CONV_U * 256 * PIECE;
   static constexpr int SLOTS = sizeof(T) * V > 8 ? 3 : 4;   // two CTAs to an SM
@@ -267,6 +267,7 @@ conv_bw_kernel(const T* x, const T* x0, const void* w, const void* bias, const T
 #pragma unroll
       for (int j = 0; j < W - 1; ++j) win[j] = widen(conv_token<T, V, W>(xb, x0b, d.st, t0 - (W - 1) + j, d.D));
       int slot = 0;
+      static_assert(CONV_U >= W - 1, "from the second CONV_U tokens of a run on, every output is one of the run");
       // CONV_U tokens from tb on; INNER: all of them and their outputs are this run's, and none is one of x_last
       auto some = [&](int tb, auto inner) {
         constexpr bool INNER = decltype(inner)::value;
@@ -407,26 +408,37 @@ conv_step_kernel(const T* x, const T* before, const void* w, const void* bias, T
 // ---- launchers ----------------------------------------------------------------------------------------
 constexpr int CONV_V = 4;   // channels to a thread, where alignment allows
 
-// Tokens to a run: long ones read fewer tokens twice (W - 1 of each run) and fewer parameters, as long as there are runs for three
-// times the threads (`per_sm`) that the GPU has room for.
-static int conv_run(int B, int S, int nvec, int per_sm) {
-  const long long tokens = (long long)B * S * nvec / ((long long)sm_count() * per_sm * 3);
-  return tokens >= 64 ? 64 : tokens <= 8 ? 8 : (int)(tokens / 4 * 4);
+// Tokens to a run (a multiple of four): `slots` runs are worked on at once, and the number that ends the last of them soonest is
+// taken, each with eight tokens' time to begin and to end (parameters, the tokens read twice).  32768 x 2048 channels backward: 228
+// tokens, one run to a slot, 104 us; 64 tokens, 3.6 to a slot, 130.
+static int conv_run(int B, int S, long long slots) {
+  int best = S;
+  long long least = -1;
+  for (int rounds = 1; rounds <= 64; ++rounds) {
+    long long runs = slots * rounds / B;
+    if (runs < 1) runs = 1;
+    if (runs > ceil_div(S, 8)) runs = ceil_div(S, 8);
+    const int run = ceil_div((int)((S + runs - 1) / runs), 4) * 4;
+    const long long items = (long long)B * ceil_div(S, run), cost = (items + slots - 1) / slots * (run + 8);
+    if (least < 0 || cost < least) { least = cost; best = run; }
+  }
+  return best;
 }
 
 struct ConvBwGrid { int run, runs, cx, tiles, parts; };
 static ConvBwGrid conv_bw_grid(int B, int S, int D) {
   ConvBwGrid g;
   const int nvec = ceil_div(D, D % CONV_V == 0 ? CONV_V : 1);
-  g.run = conv_run(B, S, nvec, 512);
-  g.runs = ceil_div(S, g.run);
   g.cx = 32;
   while (g.cx > 1 && g.cx / 2 >= nvec) g.cx /= 2;
   g.tiles = ceil_div(nvec, g.cx);
-  const long long items = (long long)B * g.runs, rounds = (items + 256 / g.cx - 1) / (256 / g.cx);
   long long parts = 2 * sm_count() / g.tiles;   // no more CTAs than run at once: a few over would take as long again
-  if (parts > rounds) parts = rounds;
-  g.parts = (int)(parts < 1 ? 1 : parts);
+  if (parts < 1) parts = 1;
+  const int rows = 256 / g.cx;
+  g.run = conv_run(B, S, parts * rows);
+  g.runs = ceil_div(S, g.run);
+  const long long needed = ((long long)B * g.runs + rows - 1) / rows;
+  g.parts = (int)(parts < needed ? parts : needed);
   return g;
 }
 // (sized for either access width: the grid depends on it)
@@ -470,7 +482,8 @@ int launch_short_conv_fw(const void* x, const long long* xs, const void* x0, con
                          int D, int W, bool silu, int dtype, int w_dtype, cudaStream_t st) {
   if (!conv_sizes_ok(B, S, D, W)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_CONV, st);
-  const int run = conv_run(B, S, D % CONV_V == 0 ? D / CONV_V : D, 768);
+  const long long room = 768ll * sm_count() / (D % CONV_V == 0 ? D / CONV_V : D);
+  const int run = conv_run(B, S, room < 1 ? 1 : room);
   const ConvDims d{B, S, D, ceil_div(S, run), run, xs[0], xs[1], 0, 0, w_dtype, silu};
   const void* ptrs[] = {x, x0, y, x_last};
   MLSTM_DTYPE_SWITCH(dtype, T,
