@@ -30,7 +30,7 @@ def norm_case(x, w, b, dy, eps=1e-5):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("D", [1, 2, 7, 8, 31, 64, 248, 256, 257, 264, 512, 520, 1000, 1001, 1024, 1032, 2048, 2056, 4096, 4104, 8192, 8200,
+@pytest.mark.parametrize("D", [1, 2, 7, 8, 31, 64, 248, 256, 257, 264, 512, 520, 1000, 1001, 1024, 1032, 1500, 1536, 2048, 2056, 2500, 2900, 3500, 4096, 4104, 8192, 8200,
                                16383, 16384])
 def test_layer_norm_widths(D, dtype):
     rng = np.random.default_rng(D)
