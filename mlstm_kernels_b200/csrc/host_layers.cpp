@@ -40,6 +40,19 @@ void check_int_sizes(const char* op, const Tensor& t) {   // the kernels count s
 void no_second_derivative(const char* op) {
   if (at::GradMode::is_enabled()) C10_THROW_ERROR(NotImplementedError, c10::str("mlstm_kernels_b200 has no second derivative of ", op));
 }
+// A buffer that a step writes (contiguous, as are those that it reads): it may be the state that it replaces, and lies apart from
+// everything else.  Autograd is told of the write, so that a graph that kept the old contents does not take the new ones for them.
+void check_written(const char* op, const char* name, const Tensor& out, const Tensor& state, std::initializer_list<const Tensor*> ins) {
+  const uintptr_t o = reinterpret_cast<uintptr_t>(out.const_data_ptr());
+  auto meets = [&](const Tensor& t) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+    return p < o + out.nbytes() && o < p + t.nbytes();
+  };
+  bool apart = state.const_data_ptr() == out.const_data_ptr() || !meets(state);
+  for (const Tensor* t : ins) apart = apart && !(t->defined() && meets(*t));
+  if (!apart) C10_THROW_ERROR(ValueError, c10::str(op, ": ", name, " overlaps a tensor that the step reads (only the whole old state may be replaced in place)"));
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
 // as a kernel reads it: the last axis contiguous
 Tensor last_dense(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 Tensor zeros(at::IntArrayRef size, at::ScalarType dt, const at::Device& dev) { return empty(size, dt, dev).zero_(); }
@@ -360,7 +373,8 @@ PyObject* py_short_conv_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     x = x.contiguous(); state = state.contiguous(); w = w.contiguous();
     if (b.defined()) b = b.contiguous();
     y = empty(x.sizes(), x.scalar_type(), dev);
-    if (!after.defined()) after = empty(state.sizes(), x.scalar_type(), dev);
+    if (after.defined()) check_written(op, "state_new", after, state, {&x, &w, &b});
+    else after = empty(state.sizes(), x.scalar_type(), dev);
     if (x.numel() > 0)
       check(mlstm_b200_short_conv_step(ptr(x), ptr(state), ptr(w), ptr(b), y.mutable_data_ptr(), after.mutable_data_ptr(), (int)x.size(0), (int)x.size(1),
                                        (int)w.size(1), silu, dtype_code(x.scalar_type()), dtype_code(w.scalar_type()), current_stream(dev)),
@@ -579,7 +593,8 @@ PyObject* py_ssm_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto c = [](const Tensor& p) { return p.defined() ? p.contiguous() : p; };
     t = SsmTensors{c(t.x), c(t.dt), f32c(t.a), c(t.b), c(t.c), f32c(t.skip), c(t.z), f32c(t.dt_bias), f32c(t.h0), t.softplus};
     y = empty(t.x.sizes(), t.x.scalar_type(), dev);
-    if (!h_new.defined()) h_new = empty(t.h0.sizes(), at::kFloat, dev);
+    if (h_new.defined()) check_written(op, "h_new", h_new, t.h0, {&t.x, &t.dt, &t.a, &t.b, &t.c, &t.skip, &t.z, &t.dt_bias});
+    else h_new = empty(t.h0.sizes(), at::kFloat, dev);
     if (t.x.numel() > 0)
       check(mlstm_b200_ssm_step(ptr(t.x), ptr(t.dt), fptr(t.a), ptr(t.b), ptr(t.c), fptr(t.skip), ptr(t.z), fptr(t.dt_bias), fptr(t.h0),
                                 y.mutable_data_ptr(), fout(h_new), (int)t.x.size(0), (int)t.x.size(1), (int)t.a.size(1),

@@ -62,7 +62,7 @@ def short_conv_step__b200(
     weight: torch.Tensor,  # (D, W)
     bias: torch.Tensor = None,  # (D,)
     activation: str = None,
-    state_new: torch.Tensor = None,  # optional buffer for the new state; may be `state` itself
+    state_new: torch.Tensor = None,  # optional buffer for the new state: `state` itself, or apart from all that is read
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """One token of short_conv__b200: returns y (B, D) and the new state; the old state is untouched unless it is state_new."""
     silu = _silu(activation)
@@ -111,7 +111,7 @@ def ssm_step__b200(
     z: torch.Tensor = None,  # (B, D)
     dt_bias: torch.Tensor = None,
     softplus: bool = False,
-    h_new: torch.Tensor = None,  # optional f32 buffer for the new state; may be `h` itself
+    h_new: torch.Tensor = None,  # optional f32 buffer for the new state: `h` itself, or apart from all that is read
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """One token of ssm_scan__b200: returns y (B, D) and the new state in f32; the old state is untouched unless it is h_new."""
     if torch.compiler.is_compiling() and h_new is None:

@@ -181,6 +181,46 @@ def test_short_conv_tokens_one_by_one(B, D, W, dtype):
     assert torch.equal(state, end)
 
 
+def test_a_steps_buffer_lies_apart_from_what_it_reads():
+    """The new state may be written over the whole old one and over nothing else, and autograd knows of the write."""
+    rng = np.random.default_rng(8)
+    B, D, W, N = 3, 16, 4, 8
+    f = lambda *shape: make(rng, *shape, dtype=torch.float32)
+    pool = f(2 * B * (W - 1) * D)
+    state, shifted = (pool[at : at + B * (W - 1) * D].view(B, W - 1, D) for at in (0, D))
+    x, w = f(B, D), f(D, W)
+    conv = lambda **o: mk.short_conv_step__b200(**{**dict(x=x, state=state, weight=w), **o})
+    before = pool.clone()
+    for o in (dict(state_new=shifted), dict(state=shifted, state_new=state), dict(state_new=state, x=pool[D : D + B * D].view(B, D)),
+              dict(state_new=shifted, state=f(B, W - 1, D), weight=pool[: D * W].view(D, W))):
+        with pytest.raises(ValueError, match="state_new overlaps"):
+            conv(**o)
+    hp = f(2 * B * D * N)
+    h, h_shifted = (hp[at : at + B * D * N].view(B, D, N) for at in (0, N))
+    args = dict(x=x, dt=f(B, D), a=f(D, N), b=f(B, N), c=f(B, N), h=h)
+    h_before = hp.clone()
+    for o in (dict(h_new=h_shifted), dict(h=h_shifted, h_new=h), dict(h_new=h, x=hp[: B * D].view(B, D)), dict(h_new=h, a=hp[D : D + D * N].view(D, N))):
+        with pytest.raises(ValueError, match="h_new overlaps"):
+            mk.ssm_step__b200(**{**args, **o})
+    assert torch.equal(pool, before) and torch.equal(hp, h_before)
+    # the rest of a pool, and an inference tensor, are as good as any
+    y, new = conv()
+    assert torch.equal(conv(state_new=pool[B * (W - 1) * D :].view(B, W - 1, D))[1], new) and torch.equal(state, before[: state.numel()].view_as(state))
+    with torch.inference_mode():
+        assert torch.equal(conv(state_new=torch.empty_like(state))[1], new)
+    # a graph that kept the old state
+    wl = w.clone().requires_grad_()
+    out = mk.short_conv__b200(f(B, 5, D), wl, x_initial=state)
+    conv(state_new=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    hl = h.clone().requires_grad_()
+    out = (hl * h).sum()
+    mk.ssm_step__b200(**args, h_new=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
 # ---- selective state space scan -------------------------------------------------------------------------------------
 def ssm_inputs(seed, B, S, D, N, G, dtype, gate=True, init=True, softplus=True, skip=True, grad=True):
     rng = np.random.default_rng(seed)
