@@ -260,6 +260,9 @@ template <typename P> __device__ __forceinline__ void ssm_rates(const float* a, 
     for (int i = 0; i < P::H; ++i) a2[c][i] = mul2(a2[c][i], f2(kLog2e, kLog2e));
 }
 // From what other segments leave behind, in their order: v = 2^(a sum) v + left.  first ... last - 1, or last - 1 ... first (BACK).
+// A segment's decay can be beyond f32 where token by token no product is (a state of zero, or a small one, that grows; a large one
+// that shrinks): it is multiplied on as four equal factors, none above 2^127, so that zero stays zero and a product is out of range
+// only where it is so itself.
 template <bool BACK, typename P>
 __device__ __forceinline__ void ssm_fold(const float* left, const float* sums, int first, int last, const SsmDims& s, const P& p,
                                          const uint64_t (&a2)[P::C][P::H], uint64_t (&v)[P::C][P::H]) {
@@ -271,9 +274,14 @@ __device__ __forceinline__ void ssm_fold(const float* left, const float* sums, i
     ssm_get_states(left, p, at, l);
 #pragma unroll
     for (int c = 0; c < P::C; ++c) {
-      const float sum = p.on[c] ? sums[at + c] : 0.f;
+      const float sum = p.on[c] ? 0.25f * sums[at + c] : 0.f;
 #pragma unroll
-      for (int e = 0; e < P::H; ++e) v[c][e] = fma2(ex2_pair(mul2(f2(sum, sum), a2[c][e])), v[c][e], l[c][e]);
+      for (int e = 0; e < P::H; ++e) {
+        float x, y;
+        unf2(mul2(f2(sum, sum), a2[c][e]), x, y);
+        const uint64_t q = f2(ex2(min_nan(x, 127.f)), ex2(min_nan(y, 127.f)));
+        v[c][e] = fma2(q, mul2(q, mul2(q, mul2(q, v[c][e]))), l[c][e]);
+      }
     }
   }
 }

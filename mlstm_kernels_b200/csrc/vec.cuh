@@ -84,6 +84,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN where one 
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float logistic_f(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
 // The same for pairs of values, in packed instructions where there are any.
