@@ -251,13 +251,18 @@ template <typename P> __device__ __forceinline__ void ssm_put_states(float* to, 
 template <typename P> __device__ __forceinline__ Pack<uint64_t, P::H> ssm_token(const float* s_bc, int t, const P& p) {
   return load_pack<uint64_t, P::H>(reinterpret_cast<const uint64_t*>(s_bc + t * P::NP + P::M * p.sub));
 }
-// a in powers of two
+// a in powers of two, within f32: a step of zero (a tile's tokens behind the last one have that) times a rate leaves the state as it was
 template <typename P> __device__ __forceinline__ void ssm_rates(const float* a, const SsmDims& s, const P& p, uint64_t (&a2)[P::C][P::H]) {
+  constexpr float MOST = 3.402823466e38f;
   ssm_load_states(a, s, p, (size_t)p.d, a2);
 #pragma unroll
   for (int c = 0; c < P::C; ++c)
 #pragma unroll
-    for (int i = 0; i < P::H; ++i) a2[c][i] = mul2(a2[c][i], f2(kLog2e, kLog2e));
+    for (int i = 0; i < P::H; ++i) {
+      float x, y;
+      unf2(mul2(a2[c][i], f2(kLog2e, kLog2e)), x, y);
+      a2[c][i] = f2(min_nan(max_nan(x, -MOST), MOST), min_nan(max_nan(y, -MOST), MOST));
+    }
 }
 // From what other segments leave behind, in their order: v = 2^(a sum) v + left.  first ... last - 1, or last - 1 ... first (BACK).
 // A segment's decay can be beyond f32 where token by token no product is (a state of zero, or a small one, that grows; a large one

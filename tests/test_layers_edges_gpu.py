@@ -70,3 +70,23 @@ def test_a_state_that_shrinks_out_of_a_segment_and_stays():
     dy = torch.zeros_like(t["x"])
     dy[:, 400:] = make(rng, 1, 200, 8)
     scan({n: v.detach().requires_grad_(True) for n, v in t.items()}, False, dy, make(rng, 1, 8, 4, scale=2.0 ** 100))
+
+
+@pytest.mark.parametrize("S", [16, 17, 40, 601])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rates_at_the_end_of_the_range(S, dtype):
+    """States that forget everything at once, by rates near the lowest f32: behind the last token they still are what they were."""
+    rng = np.random.default_rng(S)
+    B, D, N, T = 2, 12, 8, TDT[dtype]
+    m = lambda *s, **k: make(rng, *s, grad=True, **k)  # noqa: E731
+    t = dict(x=m(B, S, D, dtype=T), dt=m(B, S, D, dtype=T), a=-torch.exp(make(rng, D, N)), b=m(B, S, N, dtype=T), c=m(B, S, N, dtype=T), z=m(B, S, D, dtype=T),
+             h_initial=m(B, D, N))
+    t["a"][:, ::3] = -3e38
+    t["a"][2] = torch.finfo(torch.float32).min
+    t["a"].requires_grad_(True)
+    y, h = scan(t, True, make(rng, B, S, D, dtype=T), make(rng, B, D, N))
+    with torch.no_grad():   # the plain -inf: a factor of zero
+        a = t["a"].clone()
+        a[2] = -float("inf")
+        y2, h2 = mk.ssm_scan__b200(**{**t, "a": a}, softplus=True, return_last_states=True)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
