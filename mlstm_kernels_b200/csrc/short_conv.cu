@@ -43,11 +43,11 @@ __device__ __forceinline__ float add_c(float a, float b) { return a + b; }
 __device__ __forceinline__ uint64_t add_c(uint64_t a, uint64_t b) { return add2(a, b); }
 __device__ __forceinline__ void all_c(float& r, float x) { r = x; }
 __device__ __forceinline__ void all_c(uint64_t& r, float x) { r = f2(x, x); }
-__device__ __forceinline__ float logistic_c(float a) { return logistic_f(a); }
-__device__ __forceinline__ uint64_t logistic_c(uint64_t a) {
+template <typename T> __device__ __forceinline__ float logistic_c(float a) { return logistic_f<T>(a); }
+template <typename T> __device__ __forceinline__ uint64_t logistic_c(uint64_t a) {
   float x, y;
   unf2(a, x, y);
-  return logistic_pair(x, y);
+  return logistic_pair<T>(x, y);
 }
 template <int V> __device__ __forceinline__ void to_chan(const float (&f)[V], Chan<V>& o) {
   if constexpr (V == 1) {
@@ -170,7 +170,7 @@ conv_fw_kernel(const T* x, const T* x0, const void* w, const void* bias, T* y, T
       Chan<V> a = conv_sum<V, W>(wr, br, win, v);
       if (d.silu) {
 #pragma unroll
-        for (int i = 0; i < Chan<V>::N; ++i) a.v[i] = mul_c(a.v[i], logistic_c(a.v[i]));
+        for (int i = 0; i < Chan<V>::N; ++i) a.v[i] = mul_c(a.v[i], logistic_c<T>(a.v[i]));
       }
       conv_shift<V, W - 1>(win, v);
       if (t + u < t1) store_pack<T, V>(yb + (size_t)(t + u) * d.D, narrow<T, V>(a));
@@ -290,7 +290,7 @@ conv_bw_kernel(const T* x, const T* x0, const void* w, const void* bias, const T
             const C a = conv_sum<V, W>(wr, br, win, v);
 #pragma unroll
             for (int i = 0; i < C::N; ++i) {
-              const auto s = logistic_c(a.v[i]);
+              const auto s = logistic_c<T>(a.v[i]);
               k.v[i] = mul_c(k.v[i], mul_c(s, fma_c(a.v[i], fma_c(s, minus, one), one)));
             }
           }
@@ -398,7 +398,7 @@ conv_step_kernel(const T* x, const T* before, const void* w, const void* bias, T
   Chan<V> a = conv_sum<V, W>(wr, br, win, widen(row[W - 1]));
   if (silu) {
 #pragma unroll
-    for (int i = 0; i < Chan<V>::N; ++i) a.v[i] = mul_c(a.v[i], logistic_c(a.v[i]));
+    for (int i = 0; i < Chan<V>::N; ++i) a.v[i] = mul_c(a.v[i], logistic_c<T>(a.v[i]));
   }
   store_pack<T, V>(y + b * D + c, narrow<T, V>(a));
 #pragma unroll

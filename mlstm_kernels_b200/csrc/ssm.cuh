@@ -155,14 +155,14 @@ template <typename T, typename P, int V, int ARRS, int BCS> struct SsmRing {
 };
 
 // The step of V channels; zero (nothing moves) where `out` is true
-template <int V> __device__ __forceinline__ void ssm_step_v(const float (&dt)[V], const float (&bias)[V], bool softplus, bool out, float (&o)[V]) {
+template <typename T, int V> __device__ __forceinline__ void ssm_step_v(const float (&dt)[V], const float (&bias)[V], bool softplus, bool out, float (&o)[V]) {
 #pragma unroll
   for (int i = 0; i < V; ++i) o[i] = dt[i] + bias[i];
   if (softplus) {
     float raw[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) raw[i] = o[i];
-    softplus_v<V>(raw, o);
+    softplus_v<T, V>(raw, o);
   }
   if (out) {
 #pragma unroll

@@ -89,11 +89,11 @@ ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
       float dt[V], step[V], g[V];
       ring.get(tile, 0, i, p, dt);
       ring.get(tile, 2, i, p, g);
-      ssm_step_v<V>(dt, bias, s.softplus, t0 + q >= t_end, step);
+      ssm_step_v<T, V>(dt, bias, s.softplus, t0 + q >= t_end, step);
       if (gate) {
         float zv[V], sg[V];
         ring.get(tile, 1, i, p, zv);
-        logistic_v<V>(zv, sg);
+        logistic_v<T, V>(zv, sg);
 #pragma unroll
         for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
       }
@@ -195,7 +195,7 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
         ring.get(tile, 0, i, p, xv);
         ring.get(tile, 1, i, p, dt);
         ring.get(tile, 3, i, p, g);
-        ssm_step_v<V>(dt, bias, s.softplus, t0 + q >= t_end, step);
+        ssm_step_v<T, V>(dt, bias, s.softplus, t0 + q >= t_end, step);
         Pack<float2, V> o;
 #pragma unroll
         for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
@@ -203,7 +203,7 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
         if (gate) {
           float zv[V], sg[V];
           ring.get(tile, 2, i, p, zv);
-          logistic_v<V>(zv, sg);
+          logistic_v<T, V>(zv, sg);
 #pragma unroll
           for (int e = 0; e < V; ++e) g[e] *= zv[e] * sg[e];
         }
@@ -364,7 +364,7 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
         float sg[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) dt[e] += bias[e];
-        logistic_v<V>(dt, sg);
+        logistic_v<T, V>(dt, sg);
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] *= sg[e];
       }
@@ -376,7 +376,7 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
         ring.get(tile, 2, i, p, zv);
         ring.get(tile, 3, i, p, g);
         unpack(load_pack<float, V>(s_yp + q * P::YS + p.col), yp);
-        logistic_v<V>(zv, sg);
+        logistic_v<T, V>(zv, sg);
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = g[e] * fmaf(skip[e], xv[e], yp[e]) * sg[e] * fmaf(zv[e], 1.f - sg[e], 1.f);
         store_pack<T, V>(static_cast<T*>(k.dz) + out, pack<T, V>(o));

@@ -92,7 +92,7 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
       float dt[V], step[V], xv[V];
       ring.get(tile, 0, i, p, xv);
       ring.get(tile, 1, i, p, dt);
-      ssm_step_v<V>(dt, bias, s.softplus, t0 + r >= t_end, step);
+      ssm_step_v<T, V>(dt, bias, s.softplus, t0 + r >= t_end, step);
       Pack<float2, V> o;
 #pragma unroll
       for (int e = 0; e < V; ++e) o.e[e] = make_float2(step[e], step[e] * xv[e]);
@@ -154,7 +154,7 @@ ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
         if (gate) {
           float zv[V], sg[V];
           ring.get(tile, 2, i, p, zv);
-          logistic_v<V>(zv, sg);
+          logistic_v<T, V>(zv, sg);
 #pragma unroll
           for (int e = 0; e < V; ++e) o[e] *= zv[e] * sg[e];
         }
@@ -219,7 +219,7 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
   const float raw[1] = {to_f32(dt[row])}, bias[1] = {dt_bias != nullptr ? dt_bias[dc] : 0.f};
   const float xv = to_f32(x[row]), zv = z != nullptr ? to_f32(z[row]) : 0.f, sk = skip != nullptr ? skip[dc] : 0.f;
   float st[1], acc = 0.f;
-  ssm_step_v<1>(raw, bias, softplus, false, st);
+  ssm_step_v<T, 1>(raw, bias, softplus, false, st);
   const float sx = st[0] * xv, s2 = st[0] * kLog2e;
   float* out = h_new + row * N;
 #pragma unroll
@@ -242,7 +242,7 @@ ssm_step_kernel(const T* x, const T* dt, const T* z, const T* b, const T* c, con
   for (int o = LN / 2; o >= 1; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
   if (on && sub == 0) {
     const float v = fmaf(sk, xv, acc);
-    y[row] = from_f32<T>(z != nullptr ? v * (zv * logistic_f(zv)) : v);
+    y[row] = from_f32<T>(z != nullptr ? v * (zv * logistic_f<T>(zv)) : v);
   }
 }
 

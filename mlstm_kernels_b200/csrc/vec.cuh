@@ -67,8 +67,7 @@ template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.as
 
 // ---- exponentials for element-wise work ----------------------------------------------------------------
 // The hardware's 2^x and 1 / x, off by 2^-22 and 2^-23 of the result (results below 2^-126 are zero), instead of expf and a
-// division, which take thirty instructions.  What the rounding of x log2(e) does to e^x is left in: 1.5 |x| 2^-24 of the result,
-// which is about what the rounding of x itself did.
+// division, which take thirty instructions.
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -89,9 +88,7 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-__device__ __forceinline__ float logistic_f(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
-// The same for pairs of values, in packed instructions where there are any.
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e), kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t v) {
   float a, b;
   unf2(v, a, b);
@@ -102,13 +99,32 @@ __device__ __forceinline__ uint64_t rcp_pair(uint64_t v) {
   unf2(v, a, b);
   return f2(rcp(a), rcp(b));
 }
-__device__ __forceinline__ uint64_t logistic_pair(float x0, float x1) {
-  return rcp_pair(add2(f2(1.f, 1.f), ex2_pair(mul2(f2(x0, x1), f2(-kLog2e, -kLog2e)))));
+// e^-x of two values.  FULL: what the rounding of x log2(e) dropped, r, is put back, 2^(n + r) = 2^n (1 + r ln 2): all of f32's digits
+// but the last two.  Without, the result is off by 1.5 |x| 2^-24 of itself (x = 60: 5e-6): for results that are rounded to 16 bits
+// next, and for steps, where a dt in 16 bits is off by 2^-12 |x| and more to begin with (put back there too, a training step of the
+// scan of 4 x 2048 x 2048 x 16 in bf16 takes 748 us instead of 736).
+template <bool FULL> __device__ __forceinline__ uint64_t exp_neg_pair(float x0, float x1) {
+  if constexpr (!FULL) return ex2_pair(mul2(f2(x0, x1), f2(-kLog2e, -kLog2e)));
+  // (beyond +-1e4 as there: zero and infinity; r must stay a number)
+  const uint64_t x = f2(min_nan(max_nan(x0, -1e4f), 1e4f), min_nan(max_nan(x1, -1e4f), 1e4f)), n = mul2(x, f2(-kLog2e, -kLog2e));
+  const uint64_t r = fma2(x, f2(-kLog2eRest, -kLog2eRest), fma2(x, f2(-kLog2e, -kLog2e), mul2(x, f2(kLog2e, kLog2e))));
+  return mul2(ex2_pair(n), fma2(r, f2(kLn2, kLn2), f2(1.f, 1.f)));
+}
+// Element types of inputs and results that keep f32's digits
+template <typename T> constexpr bool kFull = sizeof(T) == 4;
+template <typename T> __device__ __forceinline__ uint64_t logistic_pair(float x0, float x1) {
+  return rcp_pair(add2(f2(1.f, 1.f), exp_neg_pair<kFull<T>>(x0, x1)));
+}
+template <typename T> __device__ __forceinline__ float logistic_f(float x) {
+  if constexpr (!kFull<T>) return rcp(1.f + ex2(-kLog2e * x));
+  float a, b;
+  unf2(logistic_pair<T>(x, x), a, b);
+  return a;
 }
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x|; log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3, which keeps all digits of a
 // small e.  artanh(s) / s as a polynomial in s^2, through its values at the Chebyshev points of [0, 1/9]: off by 2^-26.
-__device__ __forceinline__ uint64_t softplus_pair(float x0, float x1) {
-  const uint64_t e = ex2_pair(mul2(f2(fabsf(x0), fabsf(x1)), f2(-kLog2e, -kLog2e)));
+template <typename T> __device__ __forceinline__ uint64_t softplus_pair(float x0, float x1) {
+  const uint64_t e = exp_neg_pair<kFull<T>>(fabsf(x0), fabsf(x1));
   const uint64_t s = mul2(e, rcp_pair(add2(e, f2(2.f, 2.f)))), q = mul2(s, s);
   uint64_t p = fma2(f2(0.14078890f, 0.14078890f), q, f2(0.13982579f, 0.13982579f));
   p = fma2(p, q, f2(0.20012298f, 0.20012298f));
@@ -116,21 +132,21 @@ __device__ __forceinline__ uint64_t softplus_pair(float x0, float x1) {
   p = fma2(p, q, f2(1.f, 1.f));
   return fma2(add2(s, s), p, f2(max_nan(x0, 0.f), max_nan(x1, 0.f)));
 }
-template <int V> __device__ __forceinline__ void logistic_v(const float (&x)[V], float (&o)[V]) {
+template <typename T, int V> __device__ __forceinline__ void logistic_v(const float (&x)[V], float (&o)[V]) {
   if constexpr (V == 1) {
-    o[0] = logistic_f(x[0]);
+    o[0] = logistic_f<T>(x[0]);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) unf2(logistic_pair(x[i], x[i + 1]), o[i], o[i + 1]);
+    for (int i = 0; i < V; i += 2) unf2(logistic_pair<T>(x[i], x[i + 1]), o[i], o[i + 1]);
   }
 }
-template <int V> __device__ __forceinline__ void softplus_v(const float (&x)[V], float (&o)[V]) {
+template <typename T, int V> __device__ __forceinline__ void softplus_v(const float (&x)[V], float (&o)[V]) {
   if constexpr (V == 1) {
     float other;
-    unf2(softplus_pair(x[0], x[0]), o[0], other);
+    unf2(softplus_pair<T>(x[0], x[0]), o[0], other);
   } else {
 #pragma unroll
-    for (int i = 0; i < V; i += 2) unf2(softplus_pair(x[i], x[i + 1]), o[i], o[i + 1]);
+    for (int i = 0; i < V; i += 2) unf2(softplus_pair<T>(x[i], x[i + 1]), o[i], o[i + 1]);
   }
 }
 template <typename T, int V> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&o)[V]) {

@@ -90,3 +90,81 @@ def test_rates_at_the_end_of_the_range(S, dtype):
         a[2] = -float("inf")
         y2, h2 = mk.ssm_scan__b200(**{**t, "a": a}, softplus=True, return_last_states=True)
     assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
+# Logistic functions of f32 inputs.  In units of 2^-24 of e^x: 2^x off by 2^-22 (4), the exponent's rounding put back (1 for the
+# factor, 1 for the product); of 1 / (1 + e): a sum (1), a reciprocal (2); a product (1): 10.  Twelve leave room for second orders.
+UNITS = 12 * 2.0 ** -24
+
+
+def sigmoid64(v):
+    return 1 / (1 + np.exp(-v))
+
+
+def relative(got, value, tol):
+    g = f64(got)
+    assert (np.abs(g - value) <= tol).all(), (np.abs(g - value) / np.maximum(tol, 1e-300)).max()
+
+
+@pytest.mark.parametrize("D", [64, 63])   # four channels to a thread, and one
+@pytest.mark.parametrize("S", [1, 70])
+def test_silu_of_f32_keeps_its_digits(D, S):
+    """u sigmoid(u) down to u = -80, where an argument rounded to f32 alone would cost 57 units."""
+    rng = np.random.default_rng(S)
+    x = torch.from_numpy(rng.uniform(-80, 20, (3, S, D))).float().cuda().requires_grad_(True)
+    w = torch.zeros(D, 4, device="cuda")
+    w[:, 3] = 1
+    y = mk.short_conv__b200(x, w, activation="silu")
+    u = f64(x)
+    s = sigmoid64(u)
+    relative(y, u * s, np.abs(u * s) * UNITS)
+    g, = torch.autograd.grad(y, x, torch.ones_like(y))
+    # s (1 + u (1 - s)): 1 - s is off by s's units and one of its own, so that the bracket is off by at most twice these of 1 + |u|
+    relative(g, s * (1 + u * (1 - s)), s * (1 + np.abs(u)) * 3 * UNITS)
+    one, _ = mk.short_conv_step__b200(x[:, -1].detach(), torch.zeros(3, 3, D, device="cuda"), w, activation="silu")
+    assert torch.equal(one, y[:, -1])
+    for v, want in ((float("inf"), float("inf")), (-200.0, 0.0), (200.0, 200.0)):
+        assert (mk.short_conv__b200(torch.full((1, 1, D), v, device="cuda"), w[:, 2:], activation="silu") == want).all()
+
+
+@pytest.mark.parametrize("D", [64, 63])
+@pytest.mark.parametrize("S", [1, 70, 600])
+def test_gate_of_f32_keeps_its_digits(D, S):
+    rng = np.random.default_rng(S)
+    z = torch.from_numpy(rng.uniform(-80, 20, (1, S, D))).float().cuda().requires_grad_(True)
+    x = torch.ones(1, S, D, device="cuda").requires_grad_(True)
+    nil, a, skip = torch.zeros(1, S, 4, device="cuda"), torch.zeros(D, 4, device="cuda"), torch.ones(D, device="cuda")
+    y = mk.ssm_scan__b200(x, x.detach(), a, nil, nil, skip, z)
+    v = f64(z)
+    s = sigmoid64(v)
+    relative(y, v * s, np.abs(v * s) * UNITS)
+    gz, gx = torch.autograd.grad(y, (z, x), torch.ones_like(y))
+    relative(gz, s * (1 + v * (1 - s)), s * (1 + np.abs(v)) * 3 * UNITS)
+    relative(gx, v * s, np.abs(v * s) * UNITS)
+    one, _ = mk.ssm_step__b200(x[:, -1].detach(), x[:, -1].detach(), a, nil[:, -1], nil[:, -1], torch.zeros(1, D, 4, device="cuda"), skip, z[:, -1].detach())
+    relative(one, (v * s)[:, -1], np.abs(v * s)[:, -1] * UNITS)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 63])
+def test_steps_keep_their_digits(D, dtype):
+    """softplus down to -80 as the f32 state of one token shows it: e^x (6 units), its half logarithm s = e / (2 + e) (sum 1, reciprocal 2,
+    product 1), the polynomial (2^-26 and four roundings: 5) and its product (1), and step * x and its product with b (2): 18.  A dt of 16 bits, itself off by 2^12 times that, leaves the rounding of
+    the exponent in: 2 |dt| more."""
+    rng = np.random.default_rng(D)
+    T = TDT[dtype]
+    dt = torch.from_numpy(rng.uniform(-80, 20, (40, 1, D))).to(T).cuda().requires_grad_(True)
+    x, one = torch.ones(40, 1, D, dtype=T, device="cuda"), torch.ones(40, 1, 4, dtype=T, device="cuda")
+    a = torch.zeros(D, 4, device="cuda")
+    _, h = mk.ssm_scan__b200(x, dt, a, one, one, softplus=True, return_last_states=True)
+    v = f64(dt)[:, 0, :, None] + np.zeros(4)
+    step = np.logaddexp(v, 0)
+    tol = step * (18 + (0 if dtype == "f32" else 2 * np.abs(v))) * 2.0 ** -24
+    relative(h, step, tol)
+    _, h = mk.ssm_step__b200(x[:, 0], dt[:, 0].detach(), a, one[:, 0], one[:, 0], torch.zeros(40, D, 4, device="cuda"), softplus=True)
+    relative(h, step, tol)
+    if dtype == "f32":   # the derivative, the logistic function: 12 units as above, and four products and sums
+        _, h = mk.ssm_scan__b200(x, dt, a, one, one, softplus=True, return_last_states=True)
+        g, = torch.autograd.grad(h, dt, torch.ones_like(h))
+        s = 4 * sigmoid64(f64(dt))
+        relative(g, s, s * 16 * 2.0 ** -24)
