@@ -11,11 +11,9 @@
 // fp16, 8077 rows of 4096: 24.6 us (5.4 TB/s).
 #include "vec.cuh"
 #include "launch.cuh"
+#include "norm_rows.h"
 
 namespace mlstm {
-
-constexpr int LN_V = 16;           // elements of a row to a thread
-constexpr int LN_MAX_D = 16384;    // 1024 threads, twice eight elements
 
 // The rows of one head: row r at (r / n1) s0 + (r % n1) s1 + head s2.
 struct LnRows {
@@ -382,12 +380,6 @@ ln_param_kernel(const float* partial, int parts, size_t cols, void* dw, void* db
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
-static int ln_threads(int D) {   // to a row
-  int t = 4;
-  while (t < 32 && t * LN_V < D) t *= 2;
-  if (t * LN_V < D) t = ceil_div(D, 32 * LN_V) * 32;
-  return t <= 256 ? t : t <= 512 ? 512 : 1024;
-}
 // CTAs per head: as many as the GPU has room for at once, no more than there are rows for.
 static int ln_parts(long long rows, int NH, int D, bool backward) {
   const int tpr = ln_threads(D), threads = tpr <= 32 ? 256 : tpr;
@@ -402,7 +394,7 @@ static int ln_parts(long long rows, int NH, int D, bool backward) {
 size_t layer_norm_bw_bytes(long long rows, int NH, int D) { return (size_t)ln_parts(rows, NH, D, true) * 2 * NH * D * sizeof(float); }
 
 template <typename T> static bool ln_vec(const void* const* ptrs, int n, const LnRows* rows, int m, int D) {
-  if (D % LN_V != 0) return false;
+  if (!ln_whole_chunks(D, sizeof(T))) return false;
   for (int i = 0; i < n; ++i)
     if (!fits_access(ptrs[i], 16)) return false;
   for (int i = 0; i < m; ++i)
