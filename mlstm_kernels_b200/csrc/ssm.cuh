@@ -17,6 +17,7 @@ struct SsmDims {
   int Dg, tiles;          // channels of a group; tiles of channels that they take
   int per_cta, parts;     // tiles that a CTA of the backward takes one after the other; CTAs to a group then
   int nseg, seg;          // the sequence in nseg segments of seg tokens (a multiple of SSM_TT), each a CTA of its own
+  int rows, row0;         // the backward's launch has `rows` (sequence, segment) at most, from row0 on
   int nt;                 // tiles of SSM_TT tokens in the sequence
   bool softplus;
   bool pairs;             // elements of b and c may be fetched two at a time
@@ -47,6 +48,7 @@ template <int LN, int V, int C_> struct SsmPlace {
     const int ctas = per_cta == 1 ? s.tiles : s.parts;
     tile = k % ctas * per_cta + turn; k /= ctas;
     g = k % s.G; k /= s.G;
+    k += s.row0;
     seg = seg0 + k % nseg;
     b = k / nseg;
 #pragma unroll

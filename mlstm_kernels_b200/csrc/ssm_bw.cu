@@ -27,7 +27,7 @@ struct SsmBw {
   const float* ckpt;        // (B, nt, D, NP)
   void *dx, *ddt, *dz;      // dz null without z
   float* dh0;               // (B, D, N) or null
-  float* part_bc;           // (G, parts, B, S, 2, NP)
+  float* part_bc;           // (G, parts, rows, seg, 2, NP)
   float* part_a;            // (B * nseg, D, NP)
   float* part_d;            // (B * nseg, 2, D): dskip, ddt_bias
   float *loc_g, *loc_sum;   // (B, nseg, D, NP), (B, nseg, D)
@@ -180,7 +180,8 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
   };
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) fetch(t_last - i * SSM_TT);
-  float* bc = k.part_bc + ((size_t)(p.g * s.parts + p.tile / s.per_cta) * s.B + p.b) * s.S * (2 * NP);
+  // (of token t_begin on)
+  float* bc = k.part_bc + ((size_t)(p.g * s.parts + p.tile / s.per_cta) * s.rows + (p.b * s.nseg + p.seg - s.row0)) * s.seg * (2 * NP);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SSM_TT) {
     const int tile = t0 / SSM_TT;
     cp_wait<AHEAD - 1>();
@@ -330,7 +331,7 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
 #pragma unroll
             for (int w = 0; w < P::WARPS; ++w) a += s_part[w * TF * 2 * NP + e];
             const int tt = t0 + t + e / (2 * NP);
-            float* to = bc + (size_t)tt * (2 * NP) + e % (2 * NP);
+            float* to = bc + (size_t)(tt - t_begin) * (2 * NP) + e % (2 * NP);
             if (tt < t_end) *to = first_turn ? a : *to + a;
           }
           __syncthreads();
@@ -427,7 +428,7 @@ struct SsmSums {
   void *db, *dc;                       // (B, S, G, N)
   float *da, *dskip, *ddt_bias;        // dskip, ddt_bias may be null
   int NP;
-  size_t n_bc, n_a;                    // threads of each kind; n_bc: 2 * B * S * G * NP
+  size_t n_bc, n_a, n_d;               // threads of each kind: 2 G rows seg NP of this launch's rows, D NP, 2 D
 };
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -440,13 +441,13 @@ ssm_bw_sums_kernel(SsmSums q, SsmDims s) {
     size_t k = id / q.NP;
     const int which = (int)(k % 2);
     k /= 2;
-    const size_t per_tile = (size_t)s.B * s.S;
-    const size_t tok = k % per_tile;
-    const int g = (int)(k / per_tile);
-    if (n >= s.N) return;
-    const float* src = q.part_bc + ((size_t)g * s.parts * per_tile + tok) * 2 * q.NP + which * q.NP + n;
+    const size_t per_part = (size_t)s.rows * s.seg, at = k % per_part;
+    const int g = (int)(k / per_part), row = s.row0 + (int)(at / s.seg), t = row % s.nseg * s.seg + (int)(at % s.seg);
+    if (n >= s.N || row >= s.B * s.nseg || t >= s.S) return;
+    const size_t tok = (size_t)(row / s.nseg) * s.S + t;
+    const float* src = q.part_bc + ((size_t)g * s.parts * per_part + at) * 2 * q.NP + which * q.NP + n;
     float a = 0.f;
-    for (int t = 0; t < s.parts; ++t) a += src[t * per_tile * 2 * q.NP];
+    for (int i = 0; i < s.parts; ++i) a += src[i * per_part * 2 * q.NP];
     static_cast<T*>(which == 0 ? q.db : q.dc)[(tok * s.G + g) * s.N + n] = from_f32<T>(a);
     return;
   }
@@ -462,7 +463,7 @@ ssm_bw_sums_kernel(SsmSums q, SsmDims s) {
     return;
   }
   id -= q.n_a;
-  if (id >= 2 * (size_t)s.D) return;
+  if (id >= q.n_d) return;
   const int which = id >= (size_t)s.D;
   const size_t d = id - (which ? s.D : 0);
   float* out = which ? q.ddt_bias : q.dskip;
@@ -483,7 +484,7 @@ static SsmBwLayout ssm_bw_layout(const SsmDims& s) {
   const size_t np = ssm_padded(s.N), rows = (size_t)s.B * s.nseg;
   SsmBwLayout l{};
   l.bc = 0;
-  l.a = align_up(l.bc + (size_t)s.G * s.parts * s.B * s.S * 2 * np * sizeof(float), 256);
+  l.a = align_up(l.bc + (size_t)s.G * s.parts * s.rows * s.seg * 2 * np * sizeof(float), 256);
   l.d = align_up(l.a + rows * s.D * np * sizeof(float), 256);
   l.g = align_up(l.d + rows * 2 * s.D * sizeof(float), 256);
   l.sum = align_up(l.g + (s.nseg > 1 ? rows * s.D * np * sizeof(float) : 0), 256);
@@ -493,12 +494,22 @@ static SsmBwLayout ssm_bw_layout(const SsmDims& s) {
 size_t ssm_bw_bytes(int B, int S, int D, int N, int G) { return ssm_bw_layout(ssm_dims(B, S, D, N, G, false, nullptr, true)).end; }
 
 template <typename T, int LN, int V>
-static int ssm_bw_t(const SsmBw& k, const SsmDims& s, cudaStream_t st) {
-  const unsigned per_seg = (unsigned)s.B * s.G * s.tiles, grid = (unsigned)s.B * s.G * s.parts * s.nseg;
-  const bool overlap = grid <= pdl_max_ctas();
-  if (s.nseg > 1)   // the first segment leaves nothing to another
-    if (int rc = ssm_launch(ssm_bw_local_kernel<T, LN, V>, 256 / SSM_BW_LOCAL_C, SsmBwLocalSmem<T, LN, V>::BYTES, overlap, per_seg * (s.nseg - 1), st, k, s, s.nseg - 1)) return rc;
-  return ssm_launch(ssm_bw_kernel<T, LN, V>, 256 / SSM_BW_C, SsmBwSmem<T, LN, V>::BYTES, overlap, grid, st, k, s);
+static int ssm_bw_t(const SsmBw& k, SsmDims s, SsmSums q, cudaStream_t st) {
+  if (s.nseg > 1) {   // the first segment leaves nothing to another
+    const unsigned local = (unsigned)s.B * s.G * s.tiles * (s.nseg - 1);
+    if (int rc = ssm_launch(ssm_bw_local_kernel<T, LN, V>, 256 / SSM_BW_LOCAL_C, SsmBwLocalSmem<T, LN, V>::BYTES, local <= pdl_max_ctas(), local, st, k, s, s.nseg - 1)) return rc;
+  }
+  const int all = s.B * s.nseg;
+  for (; s.row0 < all; s.row0 += s.rows) {
+    const int rows = all - s.row0 < s.rows ? all - s.row0 : s.rows;
+    const unsigned grid = (unsigned)s.G * s.parts * rows;
+    if (int rc = ssm_launch(ssm_bw_kernel<T, LN, V>, 256 / SSM_BW_C, SsmBwSmem<T, LN, V>::BYTES, grid <= pdl_max_ctas(), grid, st, k, s)) return rc;
+    SsmSums sums = q;
+    if (s.row0 + s.rows < all) sums.n_a = sums.n_d = 0;   // these when all of their parts are there
+    const size_t threads = sums.n_bc + sums.n_a + sums.n_d, ctas = (threads + 255) / 256;
+    if (int rc = launch_pdl(ctas <= pdl_max_ctas(), ssm_bw_sums_kernel<T>, (unsigned)ctas, 256, 0, st, sums, s)) return rc;
+  }
+  return MLSTM_OK;
 }
 
 int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, const long long* gs, const float* dh_last, const float* ckpt, void* dx,
@@ -513,16 +524,13 @@ int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, con
   char* w = static_cast<char*>(workspace);
   auto at = [&](size_t o) { return reinterpret_cast<float*>(w + o); };
   const SsmBw k{in, dy, dh_last, ckpt, dx, ddt, dz, dh0, at(l.bc), at(l.a), at(l.d), at(l.g), at(l.sum)};
-  SsmSums q{k.part_bc, k.part_a, k.part_d, db, dc, da, dskip, ddt_bias, np, (size_t)2 * B * S * G * np, (size_t)D * np};
-  const size_t threads = q.n_bc + q.n_a + 2 * (size_t)D, grid = (threads + 255) / 256;
-  if (grid >= (1ull << 31)) return MLSTM_ERR_SHAPE;
-  int rc = MLSTM_ERR_DTYPE;
+  const SsmSums q{k.part_bc, k.part_a, k.part_d, db, dc, da, dskip, ddt_bias, np, (size_t)2 * G * s.rows * s.seg * np, (size_t)D * np, 2 * (size_t)D};
+  if ((q.n_bc + q.n_a + q.n_d + 255) / 256 >= (1ull << 31)) return MLSTM_ERR_SHAPE;
   MLSTM_DTYPE_SWITCH(dtype, T,
     s.pairs = ssm_pairs<T>(in, s);
     const bool vec = ssm_vec<T>(in, s, dy, dx) && ssm_vec<T>(in, s, ddt, dz);
-    SSM_LANES_SWITCH(lanes, LN, rc = vec ? ssm_bw_t<T, LN, 4>(k, s, st) : ssm_bw_t<T, LN, 1>(k, s, st);)
-    if (rc == MLSTM_OK) rc = launch_pdl(grid <= pdl_max_ctas(), ssm_bw_sums_kernel<T>, (unsigned)grid, 256, 0, st, q, s);)
-  return rc;
+    SSM_LANES_SWITCH(lanes, LN, return vec ? ssm_bw_t<T, LN, 4>(k, s, q, st) : ssm_bw_t<T, LN, 1>(k, s, q, st);))
+  return MLSTM_ERR_DTYPE;
 }
 
 }  // namespace mlstm

@@ -10,6 +10,8 @@
 // once, each folding what the ones before it left; twice the exponentials, on as many more SMs.
 // 16384 x 2048 channels of 16 states in bf16, 23 segments: end states 173 us (special functions 81 % busy), scan 230 (70 %; whole, in
 // one segment, it is 2084).
+#include <algorithm>
+
 #include "ssm.cuh"
 
 namespace mlstm {
@@ -269,6 +271,8 @@ bool ssm_tokens_ok(const long long* st) {
   return true;
 }
 
+size_t ssm_ckpt_bytes(int B, int S, int D, int N) { return (size_t)B * ceil_div(S, SSM_TT) * D * ssm_padded(N) * sizeof(float); }
+
 // Segments: the number that should take least, the pass over the segments' own ends (for all but one) and its launch among it.
 // Measured for 128 CTAs of 128 tiles (4 x 2048 x 2048 channels, 16 states): forward 293, 208, 198, 193, 192 us with 1, 5, 8, 10, 16
 // segments, backward 1816, 703, 546, 586, 537; for 16 CTAs of 32 tiles (512 x 1024 channels): forward 69, 33, 27, 22, 21 us with 1, 4,
@@ -289,18 +293,36 @@ static int ssm_segments(long long ctas, int nt, bool backward) {
 }
 
 constexpr int SSM_MAX_PARTS = 64;
+constexpr size_t SSM_PART_BYTES = 64 << 20;
 SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* st, bool backward) {
   SsmDims s{};
   s.B = B; s.S = S; s.D = D; s.N = N; s.G = G;
   s.Dg = D / G;
   s.tiles = ceil_div(s.Dg, ssm_tile_channels(N));
   s.nt = ceil_div(S, SSM_TT);
-  // Each CTA of the backward writes its channels' sums of db and dc, 2 N values a token: no more than 64 to a token, so that they
-  // take no more room than the other gradients (8192 channels of 16 states: 128 tiles in 64 CTAs).
+  // Each CTA of the backward writes its channels' sums of db and dc, 2 NP values a token: no more than 64 CTAs to a group (8192
+  // channels of 16 states: 128 tiles in 64 CTAs).
   s.per_cta = backward ? ceil_div(s.tiles, SSM_MAX_PARTS) : 1;
   s.parts = ceil_div(s.tiles, s.per_cta);
-  const int n = ssm_segments((long long)B * G * s.parts, s.nt, backward);
+  int n = ssm_segments((long long)B * G * s.parts, s.nt, backward);
   s.seg = ceil_div(s.nt, n) * SSM_TT;
+  if (backward) {
+    // With many states or groups these sums are more than all other memory of the call together (128 states in 8 groups of 512
+    // channels: 512 KB a token).  They are given 64 MB (half of L2), or twice what the states take that the forward kept, and the
+    // segments go in as many launches as that takes, each followed by the sums over its CTAs; a segment is short enough to fit.
+    const size_t kept = 2 * ssm_ckpt_bytes(B, S, D, N), room = kept > SSM_PART_BYTES ? kept : SSM_PART_BYTES;
+    const size_t token = (size_t)G * s.parts * 2 * ssm_padded(N) * sizeof(float);
+    while (s.seg > SSM_TT && s.seg * token > room) s.seg = ceil_div(s.seg / SSM_TT, 2) * SSM_TT;
+    s.nseg = ceil_div(S, s.seg);
+    const long long rows = (long long)B * s.nseg, fit = (long long)(room / (s.seg * token)), most = (size_t)B * S * token <= room ? rows : fit < 1 ? 1 : std::min(rows, fit);
+    s.rows = (int)most;
+    if (most < rows) {   // of the numbers just below, the one whose launches leave least of the GPU empty at their ends
+      const long long ctas = (long long)G * s.parts, slots = 4ll * sm_count();
+      auto rounds = [&](long long r) { return (rows + r - 1) / r * ((r * ctas + slots - 1) / slots); };
+      for (long long r = most - 1; r > 0 && 2 * r >= most && r > most - 64; --r)
+        if (rounds(r) < rounds(s.rows)) s.rows = (int)r;
+    }
+  }
   s.nseg = ceil_div(S, s.seg);
   s.softplus = softplus;
   s.pairs = false;
@@ -311,7 +333,6 @@ SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long lo
   return s;
 }
 
-size_t ssm_ckpt_bytes(int B, int S, int D, int N) { return (size_t)B * ceil_div(S, SSM_TT) * D * ssm_padded(N) * sizeof(float); }
 size_t ssm_fw_bytes(int B, int S, int D, int N, int G) {
   const SsmDims s = ssm_dims(B, S, D, N, G, false, nullptr, false);
   if (s.nseg == 1) return 0;

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import mlstm_kernels_b200 as mk
+from mlstm_kernels_b200 import _lib
 from oracle import layers_oracle as O
 from util_layers import TDT, check, f64, make
 
@@ -168,3 +169,38 @@ def test_steps_keep_their_digits(D, dtype):
         g, = torch.autograd.grad(h, dt, torch.ones_like(h))
         s = 4 * sigmoid64(f64(dt))
         relative(g, s, s * 16 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("B,S,D,N,G,dtype", [(3, 700, 512, 128, 1, "bf16"), (2, 500, 1040, 100, 8, "f32"), (5, 333, 512, 128, 4, "bf16")])
+def test_sums_over_channels_in_several_launches(B, S, D, N, G, dtype):
+    """So many states and channels that the sums of db and dc do not find room for all segments at once: as one sequence after the other,
+    and the sums over sequences (da, dskip, ddt_bias) as their sums."""
+    lib = _lib.load()
+    parts = G * -(-(D // G) // 8)   # CTAs' sums to a token, 2 KB each
+    assert parts * B * S * 1024 > max(64 << 20, 2 * lib.mlstm_b200_ssm_checkpoint_bytes(B, S, D, N))
+    rng = np.random.default_rng(S)
+    T = TDT[dtype]
+    m = lambda *s: make(rng, *s, dtype=T)  # noqa: E731
+    t = dict(x=m(B, S, D), dt=m(B, S, D), a=-torch.exp(make(rng, D, N)), b=m(B, S, G, N), c=m(B, S, G, N), skip=make(rng, D), z=m(B, S, D),
+             dt_bias=make(rng, D, shift=-2.0), h_initial=make(rng, B, D, N))
+    dy = m(B, S, D)
+    tok = ("x", "dt", "b", "c", "z", "h_initial")
+
+    def grads(t, dy):
+        t = {n: v.detach().requires_grad_(True) for n, v in t.items()}
+        return dict(zip(t, torch.autograd.grad(mk.ssm_scan__b200(**t, softplus=True), list(t.values()), dy)))
+    whole = grads(t, dy)
+    alone = [grads({n: v[i:i + 1] if n in tok else v for n, v in t.items()}, dy[i:i + 1]) for i in range(B)]
+    for n, g in whole.items():
+        other = torch.cat([a[n] for a in alone]) if n in tok else sum(a[n].double() for a in alone)
+        # other segments: f32 roundings of up to S steps' decays, at most a step of a 16-bit result
+        far = (g.double() - other.double()).norm() / other.double().norm()
+        assert far <= (S * 2.0 ** -24 if g.dtype == torch.float32 else 2.0 ** -9), (n, far.item())
+    # a few channels of one sequence against the oracle
+    i, at = B - 1, slice(0, 12)
+    if G == 1:
+        few = {n: (v[i:i + 1] if n in tok else v) for n, v in t.items()}
+        few = {n: v if n in ("b", "c") else v[at] if n in ("a", "skip", "dt_bias") else v[:, at] if n == "h_initial" else v[..., at] for n, v in few.items()}
+        ref = O.ssm_scan(**{n: f64(v) for n, v in few.items()}, softplus=True, dy=f64(dy[i:i + 1, :, at]), summed=S)
+        check(whole["x"][i:i + 1, :, at], ref["dx"], "dx")
+        check(whole["dt"][i:i + 1, :, at], ref["ddt"], "ddt")
