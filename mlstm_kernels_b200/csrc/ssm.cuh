@@ -2,6 +2,7 @@
 // before the recurrence.
 #pragma once
 #include "launch.cuh"
+#include "scan_segments.h"
 #include "vec.cuh"
 
 namespace mlstm {
@@ -74,7 +75,8 @@ template <typename T> __device__ __forceinline__ SsmSource ssm_source(const void
 // copies just what it reads itself, so that its own wait is all that it takes.
 template <typename T, typename P, int V, int ARRS, int BCS> struct SsmRing {
   static constexpr int RAW = SSM_TT * P::CH, BCN = SSM_TT * P::NP, STAGE = ARRS * RAW + BCS * BCN;
-  // as many as leave shared memory for the CTAs that registers allow; the backward's tiles (four arrays) take long enough for two
+  // two where a token's channels are 256 bytes or more; the backward's tiles (four arrays) take long enough for two.  (How many CTAs an
+  // SM then holds is scan_resident()'s to say: the registers are those of as many, and the number of segments goes by it.)
   static constexpr int STAGES = ARRS == 4 || sizeof(T) * P::CH >= 256 ? 2 : 4;
   static constexpr size_t BYTES = sizeof(T) * STAGE * STAGES;
   T* base;
@@ -303,6 +305,8 @@ int ssm_launch(void (*kern)(KArgs...), unsigned threads, size_t smem, bool overl
 inline int ssm_lanes(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
 inline int ssm_padded(int N) { return 4 * ssm_lanes(N); }
 inline int ssm_tile_channels(int N) { return 256 / ssm_lanes(N); }
+
+ScanSlots ssm_bw_slots(int lanes, int dtype);   // of the backward's kernels
 
 #define SSM_LANES_SWITCH(n, LN, ...)                  \
   switch (n) {                                        \

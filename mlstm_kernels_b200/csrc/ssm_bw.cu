@@ -7,13 +7,16 @@
 //
 // The forward left the state before every tile of 16 tokens; a CTA goes through its tiles from the last to the first, eight tokens at a
 // time: forward with their states kept in registers, then back (for a tile's second half first through its first half without
-// keeping any: 2.5 exponentials a state and token; all sixteen tokens' states do not fit the registers of four CTAs to an SM).  The
+// keeping any: 2.5 exponentials a state and token; all sixteen tokens' states do not fit the registers of four CTAs to an SM).  Shared
+// memory holds fewer than four with up to 8 states (two, one in f32) and, in f32, with 9 to 16 and 65 to 128 (three).  The
 // sums over the channels go through the lanes of a warp (seven shuffles to a token's eight values, of two channels at once), the
 // warps of a CTA and, by ssm_bw_sums_kernel, the CTAs, each in a fixed order.  Few sequences of few channels are cut into segments
 // as in the forward, here from the end: a segment's own adjoint first (bound by the special function units, 80 % busy).
 // 4 x 2048 x 2048 channels of 16 states in bf16, nine segments: own adjoints 93 us, backward 444, sums 20.  The backward issues 30
 // instructions to a state and token: its schedulers are 56 % busy, shared memory 59 %, special functions 44 %, with 3.5 warps to a
 // scheduler; one channel to a thread (twice the warps, 15 % more instructions) and two to four CTAs to an SM took the same time.
+#include <algorithm>
+
 #include "ssm.cuh"
 
 namespace mlstm {
@@ -38,11 +41,12 @@ template <typename T, int LN, int V> struct SsmBwLocalSmem {
   using P = SsmPlace<LN, V, SSM_BW_LOCAL_C>;
   using Ring = SsmRing<T, P, V, 3, 1>;
   static constexpr size_t D = 0, C = D + sizeof(float2) * SSM_TT * P::CH, X = C + sizeof(float) * SSM_TT * P::NP, BYTES = X + Ring::BYTES;
+  static constexpr int RESIDENT = scan_resident(BYTES, 5);
 };
 
 // A segment's own adjoint (nothing entering from behind) as it leaves at its first token, and the sum of its steps.
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SsmBwLocalSmem<T, LN, V>::P::THREADS, 5)
+__global__ void __launch_bounds__(SsmBwLocalSmem<T, LN, V>::P::THREADS, SsmBwLocalSmem<T, LN, V>::RESIDENT)
 ssm_bw_local_kernel(SsmBw k, SsmDims s, int nseg) {
   using M = SsmBwLocalSmem<T, LN, V>;
   using P = typename M::P;
@@ -134,6 +138,7 @@ template <typename T, int LN, int V> struct SsmBwSmem {
   static constexpr size_t Q = 0, G = Q + sizeof(float2) * SSM_TT * P::CH, B = G + sizeof(float) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
                           SUMS = C + sizeof(float) * SSM_TT * P::NP, PART = SUMS + sizeof(float) * (3 * SSM_TT * P::YS + 16),
                           X = PART + sizeof(float) * P::WARPS * TF * 2 * P::NP, BYTES = X + Ring::BYTES;
+  static constexpr int RESIDENT = scan_resident(BYTES, 4);
 };
 
 // One tile of channels of a segment.  first: the sums over its channels begin the CTA's part of db and dc, else they are added.
@@ -409,7 +414,7 @@ __device__ __forceinline__ void ssm_bw_tile(const SsmBw& k, const SsmDims& s, co
 }
 
 template <typename T, int LN, int V>
-__global__ void __launch_bounds__(SsmBwSmem<T, LN, V>::P::THREADS, 4)
+__global__ void __launch_bounds__(SsmBwSmem<T, LN, V>::P::THREADS, SsmBwSmem<T, LN, V>::RESIDENT)
 ssm_bw_kernel(SsmBw k, SsmDims s) {
   using P = typename SsmBwSmem<T, LN, V>::P;
   extern __shared__ __align__(16) char sm[];
@@ -474,7 +479,7 @@ ssm_bw_sums_kernel(SsmSums q, SsmDims s) {
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
-SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* strides, bool backward);
+SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* strides, bool backward, int dtype);
 bool ssm_tokens_ok(const long long* strides);
 template <typename T> bool ssm_vec(const SsmIn& in, const SsmDims& s, const void* dy, const void* y);
 template <typename T> bool ssm_pairs(const SsmIn& in, const SsmDims& s);
@@ -491,7 +496,16 @@ static SsmBwLayout ssm_bw_layout(const SsmDims& s) {
   l.end = align_up(l.sum + (s.nseg > 1 ? rows * s.D * sizeof(float) : 0), 256);
   return l;
 }
-size_t ssm_bw_bytes(int B, int S, int D, int N, int G) { return ssm_bw_layout(ssm_dims(B, S, D, N, G, false, nullptr, true)).end; }
+// (for every element type)
+size_t ssm_bw_bytes(int B, int S, int D, int N, int G) {
+  size_t most = 0;
+  for (const int dtype : {MLSTM_F32, MLSTM_BF16}) most = std::max(most, ssm_bw_layout(ssm_dims(B, S, D, N, G, false, nullptr, true, dtype)).end);
+  return most;
+}
+ScanSlots ssm_bw_slots(int lanes, int dtype) {
+  MLSTM_DTYPE_SWITCH(dtype, T, SSM_LANES_SWITCH(lanes, LN, return (ScanSlots{SsmBwSmem<T, LN, 4>::RESIDENT, SsmBwLocalSmem<T, LN, 4>::RESIDENT});))
+  return ScanSlots{1, 1};
+}
 
 template <typename T, int LN, int V>
 static int ssm_bw_t(const SsmBw& k, SsmDims s, SsmSums q, cudaStream_t st) {
@@ -517,7 +531,7 @@ int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, con
                   int N, int G, bool softplus, int dtype, cudaStream_t st) {
   if (!ssm_sizes_ok(B, S, D, N, G) || !ssm_tokens_ok(strides) || gs[1] < 0 || gs[1] >= (1ll << 29)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_SCAN, st);
-  SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, true);
+  SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, true, dtype);
   s.gb = gs[0]; s.gt = (int)gs[1];
   const int lanes = ssm_lanes(N), np = ssm_padded(N);
   const SsmBwLayout l = ssm_bw_layout(s);

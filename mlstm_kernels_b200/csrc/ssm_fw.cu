@@ -35,11 +35,12 @@ template <typename T, int LN, int V, bool LOCAL> struct SsmFwSmem {
   static constexpr size_t Q = 0, B = Q + sizeof(float2) * SSM_TT * P::CH, C = B + sizeof(float) * SSM_TT * P::NP,
                           Y = C + (LOCAL ? 0 : sizeof(float) * SSM_TT * P::NP), X = Y + (LOCAL ? 0 : sizeof(float) * SSM_TT * P::YS),
                           BYTES = X + Ring::BYTES;
+  static constexpr int RESIDENT = scan_resident(BYTES, 5);
 };
 
 // LOCAL: only a segment's own end state and sum of steps
 template <typename T, int LN, int V, bool LOCAL>
-__global__ void __launch_bounds__(SsmFwSmem<T, LN, V, LOCAL>::P::THREADS, 5)
+__global__ void __launch_bounds__(SsmFwSmem<T, LN, V, LOCAL>::P::THREADS, SsmFwSmem<T, LN, V, LOCAL>::RESIDENT)
 ssm_fw_kernel(SsmFw k, SsmDims s, int nseg) {
   using Mem = SsmFwSmem<T, LN, V, LOCAL>;
   using P = typename Mem::P;
@@ -256,13 +257,6 @@ bool ssm_sizes_ok(int B, int S, int D, int N, int G) {
   return (long long)B * G * ceil_div(Dg, ch) * 64 < (1ll << 31);
 }
 
-// The time of a launch of `grid` CTAs, up to `slots` to an SM, for each tile of a CTA: k of them share an SM for k + add, at least
-// `alone`.  More than fit go round; the last round counts half as full as it is not.
-static float ssm_rounds(long long grid, int slots, float add, float alone) {
-  const float per_sm = (float)grid / (float)sm_count(), rounds = per_sm / (float)slots;
-  const float k = rounds > 1.f ? (float)slots : ceilf(per_sm), tile = k + add > alone ? k + add : alone;
-  return rounds > 1.f ? 0.5f * (rounds + ceilf(rounds)) * tile : tile;
-}
 // Token strides are 32-bit numbers of bytes in the kernels.
 bool ssm_tokens_ok(const long long* st) {
   const long long q[] = {st[1], st[3], st[5], st[7], st[10]};
@@ -273,28 +267,13 @@ bool ssm_tokens_ok(const long long* st) {
 
 size_t ssm_ckpt_bytes(int B, int S, int D, int N) { return (size_t)B * ceil_div(S, SSM_TT) * D * ssm_padded(N) * sizeof(float); }
 
-// Segments: the number that should take least, the pass over the segments' own ends (for all but one) and its launch among it.
-// Measured for 128 CTAs of 128 tiles (4 x 2048 x 2048 channels, 16 states): forward 293, 208, 198, 193, 192 us with 1, 5, 8, 10, 16
-// segments, backward 1816, 703, 546, 586, 537; for 16 CTAs of 32 tiles (512 x 1024 channels): forward 69, 33, 27, 22, 21 us with 1, 4,
-// 11, 16, 32; for 128 CTAs of 8 tiles: 20 and 24 us with 1 and 4.  Units of a tile's part of a full SM: 0.9 us forward, 4.1 us backward.
-static int ssm_segments(long long ctas, int nt, bool backward) {
-  int best = 1;
-  float least = 0.f;
-  for (int n = 1; n <= 64 && (n == 1 || n <= nt); ++n) {
-    const int seg = ceil_div(nt, n);
-    if (n > 1 && ceil_div(nt, seg) != n) continue;
-    float t = backward ? ssm_rounds(ctas * n, 4, 0.f, 4.f) : ssm_rounds(ctas * n, 5, 1.5f, 0.f);
-    if (n > 1) t += (backward ? 0.13f : 0.6f) * ssm_rounds(ctas * (n - 1), 5, 1.5f, 0.f);
-    t *= (float)seg + 0.5f;                      // (half a tile's time to begin and to end)
-    if (n > 1) t += backward ? 0.7f : 3.3f;      // 3 us
-    if (n == 1 || t < least) { best = n; least = t; }
-  }
-  return best;
+static ScanSlots ssm_fw_slots(int lanes, int dtype) {
+  MLSTM_DTYPE_SWITCH(dtype, T, SSM_LANES_SWITCH(lanes, LN, return (ScanSlots{SsmFwSmem<T, LN, 4, false>::RESIDENT, SsmFwSmem<T, LN, 4, true>::RESIDENT});))
+  return ScanSlots{1, 1};
 }
-
 constexpr int SSM_MAX_PARTS = 64;
 constexpr size_t SSM_PART_BYTES = 64 << 20;
-SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* st, bool backward) {
+SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long long* st, bool backward, int dtype) {
   SsmDims s{};
   s.B = B; s.S = S; s.D = D; s.N = N; s.G = G;
   s.Dg = D / G;
@@ -304,7 +283,8 @@ SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long lo
   // channels of 16 states: 128 tiles in 64 CTAs).
   s.per_cta = backward ? ceil_div(s.tiles, SSM_MAX_PARTS) : 1;
   s.parts = ceil_div(s.tiles, s.per_cta);
-  int n = ssm_segments((long long)B * G * s.parts, s.nt, backward);
+  const ScanSlots held = backward ? ssm_bw_slots(ssm_lanes(N), dtype) : ssm_fw_slots(ssm_lanes(N), dtype);
+  const int n = scan_segments((long long)B * G * s.parts, s.per_cta, (long long)B * G * s.tiles, s.nt, ssm_padded(N), backward, held, sm_count());
   s.seg = ceil_div(s.nt, n) * SSM_TT;
   if (backward) {
     // With many states or groups these sums are more than all other memory of the call together (128 states in 8 groups of 512
@@ -317,7 +297,7 @@ SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long lo
     const long long rows = (long long)B * s.nseg, fit = (long long)(room / (s.seg * token)), most = (size_t)B * S * token <= room ? rows : fit < 1 ? 1 : std::min(rows, fit);
     s.rows = (int)most;
     if (most < rows) {   // of the numbers just below, the one whose launches leave least of the GPU empty at their ends
-      const long long ctas = (long long)G * s.parts, slots = 4ll * sm_count();
+      const long long ctas = (long long)G * s.parts, slots = (long long)held.whole * sm_count();
       auto rounds = [&](long long r) { return (rows + r - 1) / r * ((r * ctas + slots - 1) / slots); };
       for (long long r = most - 1; r > 0 && 2 * r >= most && r > most - 64; --r)
         if (rounds(r) < rounds(s.rows)) s.rows = (int)r;
@@ -333,10 +313,11 @@ SsmDims ssm_dims(int B, int S, int D, int N, int G, bool softplus, const long lo
   return s;
 }
 
+// (for every element type)
 size_t ssm_fw_bytes(int B, int S, int D, int N, int G) {
-  const SsmDims s = ssm_dims(B, S, D, N, G, false, nullptr, false);
-  if (s.nseg == 1) return 0;
-  const size_t rows = (size_t)B * s.nseg * D;
+  int nseg = 1;
+  for (const int dtype : {MLSTM_F32, MLSTM_BF16}) nseg = std::max(nseg, ssm_dims(B, S, D, N, G, false, nullptr, false, dtype).nseg);
+  const size_t rows = nseg > 1 ? (size_t)B * nseg * D : 0;
   return rows * ssm_padded(N) * sizeof(float) + rows * sizeof(float);
 }
 
@@ -379,7 +360,7 @@ int launch_ssm_fw(const SsmIn& in, const long long* strides, void* y, float* h_l
                   bool softplus, int dtype, cudaStream_t st) {
   if (!ssm_sizes_ok(B, S, D, N, G) || !ssm_tokens_ok(strides)) return MLSTM_ERR_SHAPE;
   PhaseScope ps(PH_SCAN, st);
-  SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, false);
+  SsmDims s = ssm_dims(B, S, D, N, G, softplus, strides, false, dtype);
   SsmFw k{in, y, h_last, ckpt, nullptr, nullptr};
   if (s.nseg > 1) {
     k.loc_h = static_cast<float*>(workspace);
