@@ -195,14 +195,18 @@ def _(x, weight, bias, eps):
 @torch.library.custom_op("mlstm_b200::layer_norm_bw", mutates_args=(), device_types="cuda")
 def layer_norm_bw(x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor, dy: Tensor, heads: bool,
                   param_dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    """dx lies as torch.empty_like(x) does, which for an x that covers its memory once is where the kernels write it."""
     dx, dw, db = _lib.host().layer_norm_bw(x, weight, mean, rstd, dy, heads, param_dtype, True, True)
-    return dx.contiguous(), dw, db
+    if dx.stride() != x.stride():   # (x in parts of wider rows, or without memory of its own)
+        like = torch.empty_like(x)
+        dx = dx if dx.stride() == like.stride() else like.copy_(dx)
+    return dx, dw, db
 
 
 @layer_norm_bw.register_fake
 def _(x, weight, mean, rstd, dy, heads, param_dtype):
     p = x.new_empty(x.shape[-2:] if heads else x.shape[-1:], dtype=param_dtype)
-    return _contig(x), p, torch.empty_like(p)
+    return torch.empty_like(x), p, torch.empty_like(p)
 
 
 def _norm_setup_context(ctx, inputs, output):
