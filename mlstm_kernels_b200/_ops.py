@@ -281,18 +281,20 @@ def _(x, state, weight, bias, silu):
 
 @torch.library.custom_op("mlstm_b200::ssm_scan", mutates_args=(), device_types="cuda")
 def ssm_scan(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, skip: Optional[Tensor], z: Optional[Tensor],
-             dt_bias: Optional[Tensor], softplus: bool, h_initial: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor]:
-    """(y, h_last, checkpoints)"""
-    return _lib.host().ssm_scan_fw(x, dt, a, b, c, skip, z, dt_bias, h_initial, softplus)
+             dt_bias: Optional[Tensor], softplus: bool, h_initial: Optional[Tensor], keep: bool = True, want_last: bool = True
+             ) -> tuple[Tensor, Tensor, Tensor]:
+    """(y, h_last, checkpoints); without `keep` no checkpoints, and no gradient"""
+    y, last, checkpoints = _lib.host().ssm_scan_fw(x, dt, a, b, c, skip, z, dt_bias, h_initial, softplus, keep, want_last)
+    return y, last if want_last else _empty(x), checkpoints if keep else x.new_empty((0,), dtype=torch.uint8)
 
 
 @ssm_scan.register_fake
-def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial):
+def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, keep=True, want_last=True):
     B, S, D = x.shape
     N = a.shape[1]
     # (worked out here, not asked for: S may be a symbol; sixteen tokens to a checkpoint)
-    n = B * ((S + 15) // 16) * D * _lib.load().mlstm_b200_ssm_checkpoint_bytes(1, 1, 1, int(N))
-    return _contig(x), x.new_empty((B, D, N), dtype=_F32), x.new_empty((torch.sym_max(n, 256),), dtype=torch.uint8)
+    n = torch.sym_max(B * ((S + 15) // 16) * D * _lib.load().mlstm_b200_ssm_checkpoint_bytes(1, 1, 1, int(N)), 256) if keep else 0
+    return (_contig(x), x.new_empty((B, D, N) if want_last else (0,), dtype=_F32), x.new_empty((n,), dtype=torch.uint8))
 
 
 @torch.library.custom_op("mlstm_b200::ssm_scan_bw", mutates_args=(), device_types="cuda")
@@ -311,17 +313,20 @@ def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, checkpoints, dy, dh
 
 
 def _ssm_setup_context(ctx, inputs, output):
-    x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial = inputs
+    x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, keep, want_last = inputs
     ctx.save_for_backward(x, dt, a, b, c, skip, z, dt_bias, h_initial, output[2])
-    ctx.softplus = softplus
+    ctx.cfg = (softplus, keep, want_last)
 
 
 def _ssm_backward(ctx, dy, dh_last, _dck):
     x, dt, a, b, c, skip, z, dt_bias, h_initial, checkpoints = ctx.saved_tensors
-    dx, ddt, da, db, dc, dskip, dz, dbias, dh0 = ssm_scan_bw(x, dt, a, b, c, skip, z, dt_bias, ctx.softplus, h_initial,
-                                                             checkpoints, dy, dh_last)
+    softplus, keep, want_last = ctx.cfg
+    if not keep:
+        raise RuntimeError("mlstm_b200::ssm_scan: no gradient without checkpoints (keep=False)")
+    dx, ddt, da, db, dc, dskip, dz, dbias, dh0 = ssm_scan_bw(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial,
+                                                             checkpoints, dy, dh_last if want_last else None)
     return (dx, ddt, da, db, dc, None if skip is None else dskip, None if z is None else dz, None if dt_bias is None else dbias,
-            None, None if h_initial is None else dh0)
+            None, None if h_initial is None else dh0, None, None)
 
 
 torch.library.register_autograd("mlstm_b200::ssm_scan", _ssm_backward, setup_context=_ssm_setup_context)

@@ -547,15 +547,15 @@ PyObject* py_ssm_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Py_BuildValue("(NN)", wrap(y), wrap(last));
   END_HANDLE_TH_ERRORS
 }
-// ssm_scan_fw(..., ) -> (y, h_last, checkpoints)
+// ssm_scan_fw(..., keep, return_last) -> (y, h_last or None, checkpoints or None)
 PyObject* py_ssm_scan_fw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  nargs_are(n, 10);
+  nargs_are(n, 12);
   const SsmTensors t = ssm_args(a, "h_initial", false);
   check_ssm(kSsm, t, false);
   c10::cuda::OptionalCUDAGuard guard(t.x.device());
   at::AutoDispatchBelowADInplaceOrView below;
-  const Scanned o = ssm_forward(t, true, true);
+  const Scanned o = ssm_forward(t, bool_arg(a[11]), bool_arg(a[10]));
   return Py_BuildValue("(NNN)", wrap(o.y), wrap(o.h_last), wrap(o.ckpt));
   END_HANDLE_TH_ERRORS
 }

@@ -94,7 +94,8 @@ def ssm_scan__b200(
     ssm_step__b200 as its state.  Rows of a padded batch do not touch each other, and outputs in front of the padding do not see it;
     the last state does."""
     if torch.compiler.is_compiling():
-        y, last, _ = _ops.ssm_scan(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial)
+        keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, a, b, c, skip, z, dt_bias, h_initial))
+        y, last, _ = _ops.ssm_scan(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, keep, bool(return_last_states))
     else:
         y, last = _lib.host().ssm_scan(x, dt, a, b, c, skip, z, dt_bias, h_initial, softplus, return_last_states)
     return (y, last) if return_last_states else y

@@ -46,3 +46,54 @@ def test_heads_gradient_in_their_layout():
     assert traced[0].is_contiguous()
     for a, b in zip(eager, traced):
         assert torch.equal(a, b)
+
+
+def scan_args(rng, S=200, D=32, N=16):
+    m = lambda *s: make(rng, *s, dtype=BF16)  # noqa: E731
+    return [m(2, S, D), m(2, S, D), -torch.exp(make(rng, D, N)), m(2, S, N), m(2, S, N)]
+
+
+@pytest.mark.parametrize("keep", [False, True])
+@pytest.mark.parametrize("want_last", [False, True])
+def test_scan_says_what_it_returns(keep, want_last):
+    t = scan_args(np.random.default_rng(3))
+    args = (*t, None, None, None, True, None, keep, want_last)
+    torch.library.opcheck(OPS.ssm_scan, args, test_utils=("test_schema", "test_faketensor"))
+    y, h, ck = OPS.ssm_scan(*args)
+    assert ck.numel() == (_lib.load().mlstm_b200_ssm_checkpoint_bytes(2, 200, 32, 16) if keep else 0)
+    assert h.shape == ((2, 32, 16) if want_last else (0,))
+    ref, last = mk.ssm_scan__b200(*t, softplus=True, return_last_states=True)
+    assert torch.equal(y, ref) and (not want_last or torch.equal(h, last))
+
+
+@pytest.mark.parametrize("want_last", [False, True])
+def test_traced_inference_keeps_nothing(want_last):
+    """No checkpoints, and no last state that nobody asked for: a traced call has no more memory at its peak than an eager one."""
+    rng = np.random.default_rng(4)
+    t = scan_args(rng, S=4096, D=256)
+    fn = lambda *t: mk.ssm_scan__b200(*t, softplus=True, return_last_states=want_last)  # noqa: E731
+    traced = torch.compile(fn, fullgraph=True)
+    checkpoints = _lib.load().mlstm_b200_ssm_checkpoint_bytes(2, 4096, 256, 16)
+    peaks = []
+    for f in (fn, traced):
+        f(*t)
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        out = f(*t)
+        torch.cuda.synchronize()
+        peaks.append(torch.cuda.max_memory_allocated() - start)
+        del out
+    assert abs(peaks[1] - peaks[0]) < checkpoints // 2, (peaks, checkpoints)
+    leaf = [v.detach().requires_grad_(True) for v in t]   # and with a gradient it keeps them
+    dy = make(rng, 2, 4096, 256, dtype=BF16)
+    first = lambda r: r[0] if want_last else r  # noqa: E731
+    for a, b in zip(torch.autograd.grad(first(fn(*leaf)), leaf, dy), torch.autograd.grad(first(traced(*leaf)), leaf, dy)):
+        assert torch.equal(a, b)
+
+
+def test_gradient_of_a_scan_that_kept_nothing_is_refused():
+    t = [v.requires_grad_(True) for v in scan_args(np.random.default_rng(5))]
+    y, _, _ = OPS.ssm_scan(*t, None, None, None, True, None, False, False)
+    with pytest.raises(RuntimeError, match="checkpoints"):
+        y.sum().backward()
