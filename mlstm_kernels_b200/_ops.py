@@ -279,6 +279,16 @@ def _(x, state, weight, bias, silu):
     return _contig(x), _contig(state)
 
 
+@torch.library.custom_op("mlstm_b200::short_conv_step_into", mutates_args=("state_new",), device_types="cuda")
+def short_conv_step_into(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor], silu: bool, state_new: Tensor) -> Tensor:
+    return _lib.host().short_conv_step(x, state, weight, bias, silu, state_new)[0]
+
+
+@short_conv_step_into.register_fake
+def _(x, state, weight, bias, silu, state_new):
+    return _contig(x)
+
+
 @torch.library.custom_op("mlstm_b200::ssm_scan", mutates_args=(), device_types="cuda")
 def ssm_scan(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, skip: Optional[Tensor], z: Optional[Tensor],
              dt_bias: Optional[Tensor], softplus: bool, h_initial: Optional[Tensor], keep: bool = True, want_last: bool = True
@@ -341,3 +351,14 @@ def ssm_step(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, h: Tensor, 
 @ssm_step.register_fake
 def _(x, dt, a, b, c, h, skip, z, dt_bias, softplus):
     return _contig(x), h.new_empty(h.shape, dtype=_F32)
+
+
+@torch.library.custom_op("mlstm_b200::ssm_step_into", mutates_args=("h_new",), device_types="cuda")
+def ssm_step_into(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, h: Tensor, skip: Optional[Tensor], z: Optional[Tensor],
+                  dt_bias: Optional[Tensor], softplus: bool, h_new: Tensor) -> Tensor:
+    return _lib.host().ssm_step(x, dt, a, b, c, skip, z, dt_bias, h, softplus, h_new)[0]
+
+
+@ssm_step_into.register_fake
+def _(x, dt, a, b, c, h, skip, z, dt_bias, softplus, h_new):
+    return _contig(x)

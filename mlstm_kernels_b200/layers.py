@@ -66,8 +66,10 @@ def short_conv_step__b200(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """One token of short_conv__b200: returns y (B, D) and the new state; the old state is untouched unless it is state_new."""
     silu = _silu(activation)
-    if torch.compiler.is_compiling() and state_new is None:
-        return _ops.short_conv_step(x, state, weight, bias, silu)
+    if torch.compiler.is_compiling():
+        if state_new is None:
+            return _ops.short_conv_step(x, state, weight, bias, silu)
+        return _ops.short_conv_step_into(x, state, weight, bias, silu, state_new), state_new
     return _lib.host().short_conv_step(x, state, weight, bias, silu, state_new)
 
 
@@ -115,6 +117,8 @@ def ssm_step__b200(
     h_new: torch.Tensor = None,  # optional f32 buffer for the new state: `h` itself, or apart from all that is read
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """One token of ssm_scan__b200: returns y (B, D) and the new state in f32; the old state is untouched unless it is h_new."""
-    if torch.compiler.is_compiling() and h_new is None:
-        return _ops.ssm_step(x, dt, a, b, c, h, skip, z, dt_bias, softplus)
+    if torch.compiler.is_compiling():
+        if h_new is None:
+            return _ops.ssm_step(x, dt, a, b, c, h, skip, z, dt_bias, softplus)
+        return _ops.ssm_step_into(x, dt, a, b, c, h, skip, z, dt_bias, softplus, h_new), h_new
     return _lib.host().ssm_step(x, dt, a, b, c, skip, z, dt_bias, h, softplus, h_new)

@@ -97,3 +97,45 @@ def test_gradient_of_a_scan_that_kept_nothing_is_refused():
     y, _, _ = OPS.ssm_scan(*t, None, None, None, True, None, False, False)
     with pytest.raises(RuntimeError, match="checkpoints"):
         y.sum().backward()
+
+
+def step_inputs(rng, B=3, D=40, N=16):
+    x, s, w = make(rng, B, D, dtype=BF16), make(rng, B, 3, D, dtype=BF16), make(rng, D, 4)
+    return x, s, w, -torch.exp(make(rng, D, N)), make(rng, B, N, dtype=BF16), make(rng, B, D, N)
+
+
+@pytest.mark.parametrize("where", ["in place", "apart"])
+def test_steps_with_buffers_compile(where):
+    """A decode loop over fixed buffers, without a break of the graph: in place, and from one buffer to another and back."""
+    x, s, w, a, b, h = step_inputs(np.random.default_rng(6))
+
+    def steps(x, s, s2, h, h2):
+        out = []
+        for _ in range(2):
+            u, r = mk.short_conv_step__b200(x, s, w, activation="silu", state_new=s2)
+            y, g = mk.ssm_step__b200(u, x, a, b, b, h, softplus=True, h_new=h2)
+            assert r is s2 and g is h2
+            out.append(y)
+            s, s2, h, h2 = s2, s, h2, h
+        return out
+
+    results = []
+    for f in (steps, torch.compile(steps, fullgraph=True)):
+        st, ht = s.clone(), h.clone()
+        st2, ht2 = (st, ht) if where == "in place" else (torch.empty_like(st), torch.empty_like(ht))
+        out = []
+        for _ in range(3):
+            out += f(x, st, st2, ht, ht2)
+        results.append([*out, st, st2, ht, ht2])
+    for p, q in zip(*results):
+        assert torch.equal(p, q)
+
+
+def test_steps_with_buffers_say_what_they_write():
+    x, s, w, a, b, h = step_inputs(np.random.default_rng(7))
+    test = ("test_schema", "test_faketensor")
+    torch.library.opcheck(OPS.short_conv_step_into, (x, s, w, None, True, torch.empty_like(s)), test_utils=test)
+    torch.library.opcheck(OPS.ssm_step_into, (x, x, a, b, b, h, None, None, None, True, torch.empty_like(h)), test_utils=test)
+    y, new = mk.ssm_step__b200(x, x, a, b, b, h, softplus=True)
+    buf = torch.empty_like(h)
+    assert torch.equal(OPS.ssm_step_into(x, x, a, b, b, h, None, None, None, True, buf), y) and torch.equal(buf, new)
