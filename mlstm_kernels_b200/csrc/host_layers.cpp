@@ -53,6 +53,10 @@ void check_written(const char* op, const char* name, const Tensor& out, const Te
   if (!apart) C10_THROW_ERROR(ValueError, c10::str(op, ": ", name, " overlaps a tensor that the step reads (only the whole old state may be replaced in place)"));
   if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
 }
+// What a backward operator is given beside the forward's inputs
+void check_size(const char* op, const char* name, const Tensor& t, at::IntArrayRef size) {
+  if (t.defined() && t.sizes() != size) C10_THROW_ERROR(ValueError, c10::str(op, ": ", name, " of shape ", t.sizes(), " must be of shape ", size));
+}
 // as a kernel reads it: the last axis contiguous
 Tensor last_dense(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 Tensor zeros(at::IntArrayRef size, at::ScalarType dt, const at::Device& dev) { return empty(size, dt, dev).zero_(); }
@@ -220,9 +224,19 @@ PyObject* py_layer_norm_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor x = need(a[0], "x"), w = arg(a[1], "weight"), mean = need(a[2], "mean"), rstd = need(a[3], "rstd"), dy = need(a[4], "dy");
   check_norm(x, w, Tensor());
   check_tensors(kNorm, {&x, &mean, &rstd, &dy});
+  check_size(kNorm, "dy", dy, x.sizes());
+  for (const Tensor* p : {&mean, &rstd}) {
+    check_size(kNorm, "mean and rstd", *p, {x.size(-1) > 0 ? x.numel() / x.size(-1) : 0});
+    if (p->scalar_type() != at::kFloat || !p->is_contiguous()) C10_THROW_ERROR(ValueError, "layer_norm__b200: mean and rstd must be contiguous f32 tensors");
+  }
+  const bool heads = bool_arg(a[5]);
+  const at::ScalarType pdt = dtype_arg(a[6]);
+  if (heads && x.dim() < 2) bad_shape(kNorm, "x", x, "(..., NH, D)");
+  if (w.defined() && (w.dim() == 2) != heads) bad_shape(kNorm, "weight", w, heads ? "(NH, D)" : "(D,)");
+  if (dtype_code(pdt) < 0 || (w.defined() && w.scalar_type() != pdt)) C10_THROW_ERROR(ValueError, "layer_norm__b200: the weight must have the parameters' dtype, a kernel dtype");
   c10::cuda::OptionalCUDAGuard guard(x.device());
   at::AutoDispatchBelowADInplaceOrView below;
-  const NormGrads g = norm_backward(x, w, mean, rstd, dy, bool_arg(a[5]), dtype_arg(a[6]), bool_arg(a[7]), bool_arg(a[8]));
+  const NormGrads g = norm_backward(x, w, mean, rstd, dy, heads, pdt, bool_arg(a[7]), bool_arg(a[8]));
   return Py_BuildValue("(NNN)", wrap(g.dx), wrap(g.dw), wrap(g.db));
   END_HANDLE_TH_ERRORS
 }
@@ -347,6 +361,8 @@ PyObject* py_short_conv_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor x = need(a[0], "x"), w = need(a[1], "weight"), b = arg(a[2], "bias"), before = arg(a[3], "x_initial"), dy = arg(a[4], "dy"), dl = arg(a[5], "dx_last");
   check_conv(kConv, x, w, b, before, false);
   check_tensors(kConv, {&x, &dy, &dl});
+  check_size(kConv, "dy", dy, x.sizes());
+  check_size(kConv, "dx_last", dl, {x.size(0), w.size(1) - 1, x.size(2)});
   c10::cuda::OptionalCUDAGuard guard(x.device());
   at::AutoDispatchBelowADInplaceOrView below;
   const ConvGrads g = conv_backward(x, w, b, before, dy, dl, bool_arg(a[6]), bool_arg(a[7]), bool_arg(a[8]), bool_arg(a[9]));
@@ -567,6 +583,11 @@ PyObject* py_ssm_scan_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor ckpt = need(a[10], "checkpoints"), dy = arg(a[11], "dy"), dhl = arg(a[12], "dh_last");
   check_ssm(kSsm, t, false);
   check_tensors(kSsm, {&t.x, &ckpt, &dy, &dhl});
+  check_size(kSsm, "dy", dy, t.x.sizes());
+  check_size(kSsm, "dh_last", dhl, {t.x.size(0), t.x.size(2), t.a.size(1)});
+  const SsmSizes q = ssm_sizes(t);
+  if (!ckpt.is_contiguous() || ckpt.nbytes() < mlstm_b200_ssm_checkpoint_bytes(q.B, q.S, q.D, q.N))
+    C10_THROW_ERROR(ValueError, "ssm_scan__b200: checkpoints of another call");
   c10::cuda::OptionalCUDAGuard guard(t.x.device());
   at::AutoDispatchBelowADInplaceOrView below;
   const ScanGrads g = ssm_backward(t, ckpt, dy, dhl, t.skip.defined(), t.dt_bias.defined(), t.h0.defined());
