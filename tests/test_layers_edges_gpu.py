@@ -171,6 +171,19 @@ def test_steps_keep_their_digits(D, dtype):
         relative(g, s, s * 16 * 2.0 ** -24)
 
 
+def test_nothing_in_and_nothing_out():
+    """Batches and sequences of length zero: the shapes, and the state that goes through."""
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    for B, S in ((2, 0), (0, 3), (0, 0)):
+        x, bc, h0 = z(B, S, 8), z(B, S, 16), torch.ones(B, 8, 16, device="cuda")
+        y, h = mk.ssm_scan__b200(x, x, z(8, 16), bc, bc, h_initial=h0, return_last_states=True)
+        assert y.shape == x.shape and h.shape == h0.shape and torch.equal(h, h0)
+        assert h.numel() == 0 or h.data_ptr() != h0.data_ptr()
+        y, last = mk.short_conv__b200(x, z(8, 4), x_initial=torch.ones(B, 3, 8, device="cuda"), return_last_states=True)
+        assert y.shape == x.shape and last.shape == (B, 3, 8) and (last == 1).all()
+        assert mk.layer_norm__b200(x).shape == x.shape
+
+
 @pytest.mark.parametrize("B,S,D,N,G,dtype", [(3, 700, 512, 128, 1, "bf16"), (2, 500, 1040, 100, 8, "f32"), (5, 333, 512, 128, 4, "bf16")])
 def test_sums_over_channels_in_several_launches(B, S, D, N, G, dtype):
     """So many states and channels that the sums of db and dc do not find room for all segments at once: as one sequence after the other,
