@@ -7,8 +7,9 @@
 // 512 elements) or of one CTA, 16 elements a thread (eight took 235 us instead of 158 for the backward of 131072 x 1024), so that the variance is taken about the mean without a second read; sums are
 // f32, and up to four more rows are on their way meanwhile.  Rows may lie apart in memory (x seen as (B, S, NH, DH) where it lies as
 // (B, NH, S, DH)); every CTA stays with one head, whose weight and bias are read once.
-// bf16, 4096 x 8 x 16 heads of 256 read in place: forward 94 us (5.7 TB/s), backward 126 (6.4 TB/s), 252 without the copies ahead;
-// fp16, 8077 rows of 4096: 24.6 us (5.4 TB/s).
+// bf16, 4096 x 8 x 16 heads of 256 read in place: forward 93 us (5.8 TB/s), backward 127 (6.3 TB/s; 252 without the copies ahead) and 5
+// for the sums over CTAs, alone; 230-239 one after the other in a stream.  fp16, 8077 rows of 4096: 25-26 us (5.0-5.3 TB/s).  Above
+// 8192 elements a row takes 1024 threads, whose 64 registers the backward spills (400-530 bytes): 4096 x 16384 bf16 215 us (1.9 TB/s).
 #include "vec.cuh"
 #include "launch.cuh"
 #include "norm_rows.h"
@@ -402,7 +403,6 @@ template <typename T> static bool ln_vec(const void* const* ptrs, int n, const L
   return true;
 }
 
-// (above a warp's lanes in steps of a warp: 32768 x 2304 by 160 threads 51.5 us forward, by 256 78.9)
 #define LN_FORMS(RUN)                                                                                                            \
   switch (ln_threads(D)) {                                                                                                       \
     case 4: RUN(4) case 8: RUN(8) case 16: RUN(16) case 32: RUN(32) case 64: RUN(64) case 96: RUN(96) case 128: RUN(128)         \

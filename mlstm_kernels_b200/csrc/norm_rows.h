@@ -7,7 +7,9 @@ namespace mlstm {
 constexpr int LN_V = 16;           // elements of a row to a thread
 constexpr int LN_MAX_D = 16384;    // 1024 threads, twice eight elements
 
-// Threads to a row: a power of two up to a warp, then as many warps as it takes.
+// Threads to a row: a power of two up to a warp, then as many warps as it takes up to 256 threads.  32768 rows in bf16, forward and
+// backward's pass, against the next power of two: 96 threads (1104 elements) 33.2 and 70.8 us against 41.6 and 84.1; 160 (2304) 51.9 and
+// 107 against 79.0 and 161; 192 (2904) 64.8 and 135 against 80.7 and 166; 224 (3304) 77.0 and 152 against 81.9 and 169.
 inline int ln_threads(int D) {
   int t = 4;
   while (t < 32 && t * LN_V < D) t *= 2;

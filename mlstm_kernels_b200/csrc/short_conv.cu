@@ -6,8 +6,8 @@
 // Tokens before the first are those of x_initial (B, W-1, D), or zeros.  Bound by HBM: x in and y out, in the backward x and dy in
 // and dx out.  A thread walks a run of tokens of a few neighbouring channels with the last W tokens in registers; tokens at the
 // seam of two runs are read by both (W - 1 of a run's length), mostly from L2.
-// bf16, 32768 x 2048, four taps and SiLU: forward 60 us (4.4 TB/s; schedulers 60 %, special functions 52 % busy: two of them to an
-// element for the logistic function alone), backward 104 (3.9 TB/s; schedulers 60 %).
+// bf16, 32768 x 2048, four taps and SiLU: forward 60-62 us (4.4 TB/s; schedulers 57 %, special functions 51 % busy: two of them to an
+// element for the logistic function alone), backward with its sums 105 (3.9 TB/s; schedulers 52 %).
 #include <type_traits>
 
 #include "launch.cuh"

@@ -12,9 +12,10 @@
 // sums over the channels go through the lanes of a warp (seven shuffles to a token's eight values, of two channels at once), the
 // warps of a CTA and, by ssm_bw_sums_kernel, the CTAs, each in a fixed order.  Few sequences of few channels are cut into segments
 // as in the forward, here from the end: a segment's own adjoint first (bound by the special function units, 80 % busy).
-// 4 x 2048 x 2048 channels of 16 states in bf16, nine segments: own adjoints 93 us, backward 444, sums 20.  The backward issues 30
-// instructions to a state and token: its schedulers are 56 % busy, shared memory 59 %, special functions 44 %, with 3.5 warps to a
-// scheduler; one channel to a thread (twice the warps, 15 % more instructions) and two to four CTAs to an SM took the same time.
+// 4 x 2048 x 2048 channels of 16 states in bf16, nine segments: 540 us; alone, with cold caches, own adjoints 93, backward 444, sums 20.
+// The backward issues 30 instructions to a state and token: its schedulers are 56 % busy, shared memory 58 %, special functions 44 %,
+// with 3.5 warps to a scheduler, and its 128 registers spill 228 bytes a thread; one channel to a thread (twice the warps, 15 % more
+// instructions) and two to four CTAs to an SM took the same time.
 #include <algorithm>
 
 #include "ssm.cuh"
