@@ -94,7 +94,7 @@ def ssm_scan__b200(
     x, dt, b, c, z share one dtype, that of y.  With G groups, group g of b and c belongs to the channels g D/G ... (g+1) D/G - 1.
     With return_last_states also the state after the last token, (B, D, N) in f32, which the next call takes as h_initial and
     ssm_step__b200 as its state.  Rows of a padded batch do not touch each other, and outputs in front of the padding do not see it;
-    the last state does."""
+    the last state does.  An infinity in x or dt may leave infinities or NaN in its channel from there on."""
     if torch.compiler.is_compiling():
         keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, a, b, c, skip, z, dt_bias, h_initial))
         y, last, _ = _ops.ssm_scan(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, keep, bool(return_last_states))
