@@ -310,8 +310,8 @@ int mlstm_b200_step_sequence(const void* q, const void* k, const void* v, const 
                              void* stream);
 
 /* ---- the operators around a recurrence -------------------------------------------------------------------------
- * Layer norm, the short causal convolution and the selective state space scan of a recurrent layer.  The reference
- * has no counterparts (its layers take them from other packages).  Unlike above, tensors need only be aligned to
+ * Layer norm, the short causal convolution, the selective state space scan, a gated linear recurrence and dropout of a
+ * recurrent layer.  The reference has no counterparts (its layers take them from other packages).  Unlike above, tensors need only be aligned to
  * their element type, and those that come with strides (host arrays, in elements) may lie anywhere as long as their
  * last axis is contiguous; workspaces and checkpoints are 16-byte aligned.  Sums, statistics and states are f32.
  */
@@ -381,6 +381,44 @@ int mlstm_b200_ssm_scan_bw(const void* x, const void* dt, const float* a, const 
 int mlstm_b200_ssm_step(const void* x, const void* dt, const float* a, const void* b, const void* c, const float* skip,
                         const void* z, const float* dt_bias, const float* h, void* y, float* h_new, int B, int D, int N, int G,
                         int softplus, int dtype, void* stream);
+
+/*
+ * Gated linear recurrence, every channel with a decay of its own at every token:
+ *   a_t = sigmoid(f_t), or exp(rate sigmoid(f_t)) with a rate;  s = 1, 1 - a_t or sqrt(1 - a_t^2) (input_scale 0, 1, 2)
+ *   h_t = a_t h_{t-1} + s sigmoid(i_t) x_t;  y_t = h_t z_t sigmoid(z_t)
+ *   x, f, i, z (B,S,D) dtype at strides[8]: x (B, S), f (B, S), i (B, S), z (B, S); i, z NULL = no such gate
+ *   rate (D), h_initial (B,D) f32, each may be NULL (zeros for h_initial); with input_scale 2 the rate is below zero
+ *   y (B,S,D) dtype out; h_last (B,D) f32 out or NULL
+ *   checkpoints: mlstm_b200_gated_checkpoint_bytes(), what the backward needs of the forward, or NULL
+ * Backward: dy at dy_strides[2], dh_last (B,D) f32 or NULL; dx, df, di, dz (B,S,D) contiguous, dtype, out (di, dz NULL without i, z);
+ * drate (D), dh_initial (B,D) f32 out, each may be NULL; workspace: mlstm_b200_gated_bw_workspace_bytes(), for drate.
+ * Step: one token, x, f, i, z, y (B,D) contiguous, h, h_new (B,D) f32; h_new may be h.
+ */
+size_t mlstm_b200_gated_checkpoint_bytes(int B, int S, int D);
+size_t mlstm_b200_gated_bw_workspace_bytes(int B, int S, int D);
+int mlstm_b200_gated_scan_fw(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h_initial,
+                             const long long* strides, void* y, float* h_last, void* checkpoints, int B, int S, int D,
+                             int input_scale, int dtype, void* stream);
+int mlstm_b200_gated_scan_bw(const void* x, const void* f, const void* i, const void* z, const float* rate,
+                             const long long* strides, const void* checkpoints, const void* dy, const long long* dy_strides,
+                             const float* dh_last, void* dx, void* df, void* di, void* dz, float* drate, float* dh_initial,
+                             void* workspace, size_t workspace_bytes, int B, int S, int D, int input_scale, int dtype,
+                             void* stream);
+int mlstm_b200_gated_step(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h,
+                          void* y, float* h_new, int B, int D, int input_scale, int dtype, void* stream);
+
+/*
+ * Dropout by a counter-based generator, added to a residual: y = residual + (kept ? x / (1 - p) : 0).
+ *   Element n of x (its index in the order of the sizes) is kept where word n mod 4 of Philox4x32 with 7 rounds, counter
+ *   (n div 4, offset), key seed, is p 2^32 or more: the mask is the same in every call with the same seed and offset, and is
+ *   never stored.  The backward is the call on dy, without residual.
+ *   x, residual, y of sizes[4], each at strides[3] of its own (of the first three axes; the last is contiguous)
+ *   x dtype; residual (or NULL) and y out_dtype: the same, or one of the two f32
+ *   seed_device: one 64-bit number in device memory that takes the place of `seed`, or NULL
+ */
+int mlstm_b200_dropout(const void* x, const long long* x_strides, const void* residual, const long long* residual_strides,
+                       void* y, const long long* y_strides, const long long* sizes, double p, unsigned long long seed,
+                       const void* seed_device, unsigned long long offset, int dtype, int out_dtype, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -362,3 +362,108 @@ def ssm_step_into(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, h: Ten
 @ssm_step_into.register_fake
 def _(x, dt, a, b, c, h, skip, z, dt_bias, softplus, h_new):
     return _contig(x)
+
+
+@torch.library.custom_op("mlstm_b200::gated_scan", mutates_args=(), device_types="cuda")
+def gated_scan(x: Tensor, f: Tensor, i: Optional[Tensor], z: Optional[Tensor], rate: Optional[Tensor], h_initial: Optional[Tensor],
+               input_scale: int, keep: bool, want_last: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """(y, h_last, checkpoints); without `keep` no checkpoints, and no gradient"""
+    y, last, checkpoints = _lib.host().gated_scan_fw(x, f, i, z, rate, h_initial, input_scale, keep, want_last)
+    return y, last if want_last else _empty(x), checkpoints if keep else x.new_empty((0,), dtype=torch.uint8)
+
+
+@gated_scan.register_fake
+def _(x, f, i, z, rate, h_initial, input_scale, keep, want_last):
+    B, S, D = x.shape
+    # (worked out here, not asked for: S may be a symbol; eight tokens to a checkpoint)
+    n = torch.sym_max(4 * B * ((S + 7) // 8) * D, 256) if keep else 0
+    return (_contig(x), x.new_empty((B, D) if want_last else (0,), dtype=_F32), x.new_empty((n,), dtype=torch.uint8))
+
+
+@torch.library.custom_op("mlstm_b200::gated_scan_bw", mutates_args=(), device_types="cuda")
+def gated_scan_bw(x: Tensor, f: Tensor, i: Optional[Tensor], z: Optional[Tensor], rate: Optional[Tensor], h_initial: Optional[Tensor],
+                  input_scale: int, checkpoints: Tensor, dy: Optional[Tensor], dh_last: Optional[Tensor]
+                  ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    g = _lib.host().gated_scan_bw(x, f, i, z, rate, h_initial, input_scale, checkpoints, dy, dh_last)
+    return tuple(x.new_empty((0,)) if t is None else t for t in g)
+
+
+@gated_scan_bw.register_fake
+def _(x, f, i, z, rate, h_initial, input_scale, checkpoints, dy, dh_last):
+    like = lambda t: x.new_empty((0,)) if t is None else _contig(t)  # noqa: E731
+    return tuple(like(t) for t in (x, f, i, z, rate, h_initial))
+
+
+def _gated_setup_context(ctx, inputs, output):
+    *tensors, input_scale, keep, want_last = inputs
+    ctx.save_for_backward(*tensors, output[2])
+    ctx.cfg = (input_scale, keep, want_last)
+
+
+def _gated_backward(ctx, dy, dh_last, _dck):
+    *tensors, checkpoints = ctx.saved_tensors
+    input_scale, keep, want_last = ctx.cfg
+    if not keep:
+        raise RuntimeError("mlstm_b200::gated_scan: no gradient without checkpoints (keep=False)")
+    grads = gated_scan_bw(*tensors, input_scale, checkpoints, dy, dh_last if want_last else None)
+    return (*(None if t is None else g for t, g in zip(tensors, grads)), None, None, None)
+
+
+torch.library.register_autograd("mlstm_b200::gated_scan", _gated_backward, setup_context=_gated_setup_context)
+
+
+@torch.library.custom_op("mlstm_b200::gated_step", mutates_args=(), device_types="cuda")
+def gated_step(x: Tensor, f: Tensor, i: Optional[Tensor], z: Optional[Tensor], rate: Optional[Tensor], h: Tensor, input_scale: int
+               ) -> tuple[Tensor, Tensor]:
+    return _lib.host().gated_step(x, f, i, z, rate, h, input_scale, None)
+
+
+@gated_step.register_fake
+def _(x, f, i, z, rate, h, input_scale):
+    return _contig(x), h.new_empty(h.shape, dtype=_F32)
+
+
+@torch.library.custom_op("mlstm_b200::gated_step_into", mutates_args=("h_new",), device_types="cuda")
+def gated_step_into(x: Tensor, f: Tensor, i: Optional[Tensor], z: Optional[Tensor], rate: Optional[Tensor], h: Tensor, input_scale: int,
+                    h_new: Tensor) -> Tensor:
+    return _lib.host().gated_step(x, f, i, z, rate, h, input_scale, h_new)[0]
+
+
+@gated_step_into.register_fake
+def _(x, f, i, z, rate, h, input_scale, h_new):
+    return _contig(x)
+
+
+@torch.library.custom_op("mlstm_b200::dropout", mutates_args=(), device_types="cuda")
+def dropout(x: Tensor, residual: Optional[Tensor], seed: Optional[Tensor], seed_value: int, p: float, offset: int) -> Tensor:
+    return _lib.host().dropout(x, residual, seed, seed_value, p, offset)
+
+
+@dropout.register_fake
+def _(x, residual, seed, seed_value, p, offset):
+    return x.new_empty(x.shape, dtype=x.dtype if residual is None else residual.dtype)
+
+
+@torch.library.custom_op("mlstm_b200::dropout_bw", mutates_args=(), device_types="cuda")
+def dropout_bw(dy: Tensor, seed: Optional[Tensor], seed_value: int, p: float, offset: int, dtype: torch.dtype) -> Tensor:
+    return _lib.host().dropout_bw(dy, seed, seed_value, p, offset, dtype)
+
+
+@dropout_bw.register_fake
+def _(dy, seed, seed_value, p, offset, dtype):
+    return dy.new_empty(dy.shape, dtype=dtype)
+
+
+def _dropout_setup_context(ctx, inputs, output):
+    x, residual, seed, seed_value, p, offset = inputs
+    ctx.save_for_backward(seed)
+    ctx.cfg = (seed_value, p, offset, x.dtype, residual is not None)
+
+
+def _dropout_backward(ctx, dy):
+    seed_value, p, offset, dtype, has_residual = ctx.cfg
+    dx = dropout_bw(dy, ctx.saved_tensors[0], seed_value, p, offset, dtype) if ctx.needs_input_grad[0] else None
+    return dx, dy if has_residual else None, None, None, None, None
+
+
+torch.library.register_autograd("mlstm_b200::dropout", _dropout_backward, setup_context=_dropout_setup_context)

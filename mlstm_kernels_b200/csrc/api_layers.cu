@@ -4,6 +4,7 @@
 namespace mlstm {
 
 static bool kernel_dtype(int t) { return t == MLSTM_F32 || t == MLSTM_BF16 || t == MLSTM_F16; }
+static bool gated_scale_ok(int s) { return s >= 0 && s <= 2; }
 static bool scratch_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace mlstm
@@ -110,6 +111,57 @@ int mlstm_b200_ssm_step(const void* x, const void* dt, const float* a, const voi
   if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;
   if (!x || !dt || !a || !b || !c || !h || !y || !h_new) return MLSTM_ERR_NULL;
   return launch_ssm_step(x, dt, z, b, c, a, skip, dt_bias, h, y, h_new, B, D, N, G, softplus != 0, dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t mlstm_b200_gated_checkpoint_bytes(int B, int S, int D) { return gated_sizes_ok(B, S, D) ? gated_ckpt_bytes(B, S, D) : 0; }
+size_t mlstm_b200_gated_bw_workspace_bytes(int B, int S, int D) { return gated_sizes_ok(B, S, D) ? gated_bw_bytes(B, S, D) : 0; }
+
+int mlstm_b200_gated_scan_fw(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h_initial,
+                             const long long* strides, void* y, float* h_last, void* checkpoints, int B, int S, int D, int input_scale, int dtype,
+                             void* stream) {
+  if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;
+  if (!gated_sizes_ok(B, S, D) || !gated_scale_ok(input_scale)) return MLSTM_ERR_SHAPE;
+  if (!x || !f || !strides || !y) return MLSTM_ERR_NULL;
+  if (!scratch_aligned(checkpoints)) return MLSTM_ERR_ALIGN;
+  return launch_gated_fw(GatedIn{x, f, i, z, rate, h_initial}, strides, y, h_last, static_cast<float*>(checkpoints), B, S, D, input_scale, dtype,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int mlstm_b200_gated_scan_bw(const void* x, const void* f, const void* i, const void* z, const float* rate, const long long* strides,
+                             const void* checkpoints, const void* dy, const long long* dy_strides, const float* dh_last, void* dx, void* df, void* di,
+                             void* dz, float* drate, float* dh_initial, void* workspace, size_t workspace_bytes, int B, int S, int D, int input_scale,
+                             int dtype, void* stream) {
+  if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;
+  if (!gated_sizes_ok(B, S, D) || !gated_scale_ok(input_scale)) return MLSTM_ERR_SHAPE;
+  if (!x || !f || !strides || !checkpoints || !dy || !dy_strides || !dx || !df) return MLSTM_ERR_NULL;
+  if ((i != nullptr) != (di != nullptr) || (z != nullptr) != (dz != nullptr) || (drate != nullptr && (rate == nullptr || workspace == nullptr)))
+    return MLSTM_ERR_NULL;
+  if (!scratch_aligned(workspace) || !scratch_aligned(checkpoints)) return MLSTM_ERR_ALIGN;
+  if (drate != nullptr && workspace_bytes < gated_bw_bytes(B, S, D)) return MLSTM_ERR_WORKSPACE;
+  return launch_gated_bw(GatedIn{x, f, i, z, rate, nullptr}, strides, static_cast<const float*>(checkpoints), dy, dy_strides, dh_last, dx, df, di, dz, drate,
+                         dh_initial, static_cast<float*>(workspace), B, S, D, input_scale, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int mlstm_b200_gated_step(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h, void* y, float* h_new, int B, int D,
+                          int input_scale, int dtype, void* stream) {
+  if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;
+  if (!gated_sizes_ok(B, 1, D) || !gated_scale_ok(input_scale)) return MLSTM_ERR_SHAPE;
+  if (!x || !f || !h || !y || !h_new) return MLSTM_ERR_NULL;
+  return launch_gated_step(GatedIn{x, f, i, z, rate, nullptr}, h, y, h_new, B, D, input_scale, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int mlstm_b200_dropout(const void* x, const long long* x_strides, const void* residual, const long long* residual_strides, void* y,
+                       const long long* y_strides, const long long* sizes, double p, unsigned long long seed, const void* seed_device, unsigned long long offset, int dtype, int out_dtype, void* stream) {
+  if (!kernel_dtype(dtype) || !kernel_dtype(out_dtype) || (dtype != out_dtype && dtype != MLSTM_F32 && out_dtype != MLSTM_F32)) return MLSTM_ERR_DTYPE;
+  if (!x || !x_strides || !y || !y_strides || !sizes || (residual != nullptr && !residual_strides)) return MLSTM_ERR_NULL;
+  if (!(p >= 0.0 && p <= 1.0)) return MLSTM_ERR_SHAPE;
+  long long n = 1;
+  for (int k = 0; k < 4; ++k) {
+    if (sizes[k] <= 0 || sizes[k] > (1ll << 40) / n) return MLSTM_ERR_SHAPE;
+    n *= sizes[k];
+  }
+  return launch_dropout(x, x_strides, residual, residual_strides, y, y_strides, sizes, p, seed, static_cast<const long long*>(seed_device), offset, dtype,
+                        out_dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -392,7 +392,7 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nu
 
 PyMODINIT_FUNC PyInit__host(void) {
   PyObject* m = PyModule_Create(&kModule);
-  if (m != nullptr && PyModule_AddFunctions(m, mlstm_host::kLayerMethods) < 0) {
+  if (m != nullptr && (PyModule_AddFunctions(m, mlstm_host::kLayerMethods) < 0 || PyModule_AddFunctions(m, mlstm_host::kGatedMethods) < 0)) {
     Py_DECREF(m);
     return nullptr;
   }

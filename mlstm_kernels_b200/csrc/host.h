@@ -102,5 +102,7 @@ inline void nargs_are(Py_ssize_t have, Py_ssize_t want) {
 
 // host_layers.cpp: layer norm, short convolution, state space scan
 extern PyMethodDef kLayerMethods[];
+// host_gated.cpp: gated linear recurrence, dropout
+extern PyMethodDef kGatedMethods[];
 
 }  // namespace mlstm_host

@@ -1,66 +1,11 @@
 // The host side of the operators around a recurrence - layer norm, short causal convolution, selective state space scan - in the
 // manner of host.cpp: checks of the arguments, allocations, autograd nodes and launches of a call without a Python frame in
 // between.  Tensors whose last axis is contiguous are read where they are, whatever their other strides.
-#include "host.h"
+#include "host_layers.h"
 
 namespace {
 
 using namespace mlstm_host;
-
-using OptT = std::optional<Tensor>;
-OptT given(const Tensor& t) { return t.defined() ? OptT(t) : std::nullopt; }
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
-}
-
-// All on the device of the first; no forward-mode tangents, which would be dropped without a word.
-void check_tensors(const char* op, std::initializer_list<const Tensor*> ts) {
-  const Tensor& first = **ts.begin();
-  for (const Tensor* t : ts) {
-    if (!t->defined()) continue;
-    TORCH_CHECK(t->is_cuda(), kNeedsCuda);
-    if (t->device() != first.device()) C10_THROW_ERROR(ValueError, c10::str(op, ": tensors on different devices (", first.device(), " and ", t->device(), ")"));
-    if (t->layout() != at::kStrided) C10_THROW_ERROR(ValueError, c10::str(op, ": tensors must be dense"));
-    if (t->_fw_grad(0).defined()) C10_THROW_ERROR(NotImplementedError, c10::str("mlstm_kernels_b200 has no forward-mode derivative of ", op));
-  }
-}
-void check_kernel_dtype(const Tensor& t) {
-  if (t.defined() && dtype_code(t.scalar_type()) < 0) C10_THROW_ERROR(ValueError, c10::str("Unsupported kernel dtype ", t.dtype(), "."));
-}
-[[noreturn]] void bad_shape(const char* op, const char* name, const Tensor& t, const char* want) {
-  C10_THROW_ERROR(ValueError, c10::str(op, ": ", name, " of shape ", t.sizes(), " must be ", want));
-}
-void check_int_sizes(const char* op, const Tensor& t) {   // the kernels count single axes in 32 bits
-  for (const int64_t n : t.sizes())
-    if (n > (1ll << 30)) C10_THROW_ERROR(ValueError, c10::str(op, ": an axis of more than 2^30 elements"));
-}
-void no_second_derivative(const char* op) {
-  if (at::GradMode::is_enabled()) C10_THROW_ERROR(NotImplementedError, c10::str("mlstm_kernels_b200 has no second derivative of ", op));
-}
-// A buffer that a step writes (contiguous, as are those that it reads): it may be the state that it replaces, and lies apart from
-// everything else.  Autograd is told of the write, so that a graph that kept the old contents does not take the new ones for them.
-void check_written(const char* op, const char* name, const Tensor& out, const Tensor& state, std::initializer_list<const Tensor*> ins) {
-  const uintptr_t o = reinterpret_cast<uintptr_t>(out.const_data_ptr());
-  auto meets = [&](const Tensor& t) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-    return p < o + out.nbytes() && o < p + t.nbytes();
-  };
-  bool apart = state.const_data_ptr() == out.const_data_ptr() || !meets(state);
-  for (const Tensor* t : ins) apart = apart && !(t->defined() && meets(*t));
-  if (!apart) C10_THROW_ERROR(ValueError, c10::str(op, ": ", name, " overlaps a tensor that the step reads (only the whole old state may be replaced in place)"));
-  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
-}
-// What a backward operator is given beside the forward's inputs
-void check_size(const char* op, const char* name, const Tensor& t, at::IntArrayRef size) {
-  if (t.defined() && t.sizes() != size) C10_THROW_ERROR(ValueError, c10::str(op, ": ", name, " of shape ", t.sizes(), " must be of shape ", size));
-}
-// as a kernel reads it: the last axis contiguous
-Tensor last_dense(const Tensor& t) { return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-Tensor zeros(at::IntArrayRef size, at::ScalarType dt, const at::Device& dev) { return empty(size, dt, dev).zero_(); }
-Tensor to_dtype(const Tensor& t, at::ScalarType dt) { return !t.defined() || t.scalar_type() == dt ? t : t.to(dt); }
 
 // ---- layer norm ---------------------------------------------------------------------------------------
 // The axes in front of the normalised one (and of the heads) as two, cut in front of axis k; null sizes where the strides do
@@ -431,12 +376,6 @@ void check_ssm(const char* op, const SsmTensors& t, bool one_token) {
 struct SsmSizes { int B, S, D, N, G; };
 SsmSizes ssm_sizes(const SsmTensors& t) {
   return {(int)t.x.size(0), (int)t.x.size(1), (int)t.x.size(2), (int)t.a.size(1), t.b.dim() == 4 ? (int)t.b.size(2) : 1};
-}
-// the stride of the token axis; of a single token any number will do
-long long token_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
-Tensor tokens_near(const Tensor& t) {   // the scan takes token strides below 2^29
-  const Tensor d = last_dense(t);
-  return !d.defined() || token_stride(d) < (1ll << 29) ? d : d.clone(at::MemoryFormat::Contiguous);
 }
 SsmTensors ssm_ready(const SsmTensors& t) {   // as the kernels read them
   return {tokens_near(t.x), tokens_near(t.dt), f32c(t.a), tokens_near(t.b), tokens_near(t.c), f32c(t.skip), tokens_near(t.z), f32c(t.dt_bias), f32c(t.h0), t.softplus};

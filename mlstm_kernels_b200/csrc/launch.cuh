@@ -119,4 +119,22 @@ int launch_ssm_bw(const SsmIn& in, const long long* strides, const void* dy, con
 int launch_ssm_step(const void* x, const void* dt, const void* z, const void* b, const void* c, const float* a, const float* skip, const float* dt_bias,
                     const float* h, void* y, float* h_new, int B, int D, int N, int G, bool softplus, int dtype, cudaStream_t st);
 
+// gated_scan.cu
+struct GatedIn {
+  const void *x, *f, *i, *z;        // i, z may be null
+  const float *rate, *h0;           // may be null
+};
+bool gated_sizes_ok(int B, int S, int D);
+size_t gated_ckpt_bytes(int B, int S, int D);
+size_t gated_bw_bytes(int B, int S, int D);
+int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, int B, int S, int D, int scale, int dtype,
+                    cudaStream_t st);
+int launch_gated_bw(const GatedIn& in, const long long* strides, const float* ckpt, const void* dy, const long long* gs, const float* dh_last, void* dx,
+                    void* df, void* di, void* dz, float* drate, float* dh0, float* parts, int B, int S, int D, int scale, int dtype, cudaStream_t st);
+int launch_gated_step(const GatedIn& in, const float* h, void* y, float* h_new, int B, int D, int scale, int dtype, cudaStream_t st);
+
+// dropout.cu
+int launch_dropout(const void* x, const long long* xs, const void* residual, const long long* rs, void* y, const long long* ys, const long long* sizes, double p,
+                   unsigned long long seed, const long long* seed_device, unsigned long long offset, int dtype, int out_dtype, cudaStream_t st);
+
 }  // namespace mlstm
