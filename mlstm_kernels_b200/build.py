@@ -22,7 +22,8 @@ OBJ = os.path.join(PKG, "build")
 LIB = os.path.join(PKG, "libmlstm_b200.so")
 HOST = os.path.join(PKG, "_host.so")
 SOURCES = ["api.cu", "gates.cu", "step.cu", "chunkwise_simt.cu", "chunkwise_sm100.cu", "chunkwise_bw_sm100.cu", "noalloc.cu",
-           "api_layers.cu", "layer_norm.cu", "short_conv.cu", "ssm_fw.cu", "ssm_bw.cu", "gated_scan.cu", "dropout.cu"]
+           "api_layers.cu", "layer_norm.cu", "short_conv.cu", "ssm_fw.cu", "ssm_bw.cu", "gated_scan.cu", "gated_scan_f32.cu",
+           "gated_scan_bf16.cu", "gated_scan_f16.cu", "dropout.cu"]
 HOST_SOURCES = ["host.cpp", "host_layers.cpp", "host_gated.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -17,6 +17,15 @@
 
 namespace mlstm {
 
+constexpr int GATED_CK = 8;   // tokens to a thread, and to a state that the forward keeps for the backward
+struct GatedDims {
+  int B, S, D, nc;      // nc: kept states of a sequence
+  int scale;
+  int blocks;           // CTAs next to each other that take the channels
+  int K, warps;         // CTAs to a cluster, warps to a CTA
+  long long xb, xt, fb, ft, ib, it, zb, zt, gb, gt;   // strides in elements (batch, token) of x, f, i, z, dy
+};
+
 constexpr int GATED_PLAIN = 0, GATED_CONVEX = 1, GATED_VARIANCE = 2;
 
 __device__ __forceinline__ float rsq(float x) {
@@ -43,7 +52,8 @@ template <typename T> __device__ __forceinline__ void logistic_both(uint64_t v, 
 
 // of two values of f: a, 1 - a; and with a rate sigmoid(f) and 1 - sigmoid(f)
 struct Decay { uint64_t a, rest, sf, cf; };
-template <typename T, bool RATE> __device__ __forceinline__ Decay decay_pair(uint64_t f, uint64_t rate) {
+// (FAR = false: the rate is known to be in (-1/2, 0], and no exponential is needed)
+template <typename T, bool RATE, bool FAR = true> __device__ __forceinline__ Decay decay_pair(uint64_t f, uint64_t rate) {
   Decay d;
   logistic_both<T>(f, d.sf, d.cf);
   if constexpr (!RATE) {
@@ -59,6 +69,11 @@ template <typename T, bool RATE> __device__ __forceinline__ Decay decay_pair(uin
     p = fma2(p, rho, dup2(-4.9999982e-1f));
     p = fma2(p, rho, dup2(1.f));
     const uint64_t small = mul2(p, rho);
+    if constexpr (!FAR) {
+      d.rest = small;
+      d.a = fma2(p, neg2(rho), dup2(1.f));
+      return d;
+    }
     float r0, r1, s0, s1, e0, e1;
     unf2(rho, r0, r1);
     unf2(small, s0, s1);

@@ -1,17 +1,10 @@
-// Gated linear recurrence (formulas: gated.cuh): forward, backward, and the step for one token.
-// One thread to a channel of a sequence, token after token; the backward takes GATED_CK tokens at a time, last ones first, and
-// recomputes their states from the one before them, which the forward has kept.
-#include "gated.cuh"
+// Gated linear recurrence: how sequences are divided among CTAs, the calls of the kernels (gated_tiles.cuh), and the step for one
+// token.
+#include <algorithm>
+
+#include "gated_tiles.cuh"
 
 namespace mlstm {
-
-constexpr int GATED_CK = 8;
-
-struct GatedDims {
-  int B, S, D, nc;   // nc: kept states
-  int scale;
-  long long xb, xt, fb, ft, ib, it, zb, zt, gb, gt;   // strides in elements (batch, token) of x, f, i, z, dy
-};
 
 // one token of one channel
 template <typename T, bool RATE> struct GatedToken {
@@ -41,90 +34,17 @@ template <typename T, bool RATE> struct GatedToken {
   }
 };
 
-template <typename T, bool RATE>
-__global__ void gated_fw(const T* x, const T* f, const T* i, const T* z, const float* rate, const float* h0, T* y, float* h_last, float* ckpt, GatedDims q) {
-  const long long n = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= (long long)q.B * q.D) return;
-  const int b = (int)(n / q.D), d = (int)(n % q.D);
-  const float r = RATE ? rate[d] : 0.f;
-  float h = h0 != nullptr ? h0[n] : 0.f;
-  for (int t = 0; t < q.S; ++t) {
-    if (ckpt != nullptr && t % GATED_CK == 0) ckpt[((long long)b * q.nc + t / GATED_CK) * q.D + d] = h;
-    const GatedToken<T, RATE> k(x + b * q.xb + t * q.xt + d, f + b * q.fb + t * q.ft + d, i != nullptr ? i + b * q.ib + t * q.it + d : nullptr, r, q.scale);
-    h = k.a * h + k.s * k.g * k.x;
-    float out = h;
-    if (z != nullptr) {
-      const float zz = to_f32(z[b * q.zb + t * q.zt + d]);
-      out *= zz * logistic_f<T>(zz);
-    }
-    y[((long long)b * q.S + t) * q.D + d] = from_f32<T>(out);
-  }
-  if (h_last != nullptr) h_last[n] = h;
-}
-
-template <typename T, bool RATE>
-__global__ void gated_bw(const T* x, const T* f, const T* i, const T* z, const float* rate, const float* ckpt, const T* dy, const float* dh_last, T* dx,
-                         T* df, T* di, T* dz, float* drate, float* dh0, GatedDims q) {
-  const long long n = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= (long long)q.B * q.D) return;
-  const int b = (int)(n / q.D), d = (int)(n % q.D);
-  const float r = RATE ? rate[d] : 0.f;
-  float c = dh_last != nullptr ? dh_last[n] : 0.f, dr = 0.f;   // c: a_{t+1} G_{t+1}
-  auto token = [&](int t) {
-    return GatedToken<T, RATE>(x + b * q.xb + t * q.xt + d, f + b * q.fb + t * q.ft + d, i != nullptr ? i + b * q.ib + t * q.it + d : nullptr, r, q.scale);
-  };
-  for (int k0 = q.nc - 1; k0 >= 0; --k0) {
-    float before[GATED_CK + 1];
-    before[0] = ckpt[((long long)b * q.nc + k0) * q.D + d];
-#pragma unroll
-    for (int j = 0; j < GATED_CK; ++j) {
-      const int t = k0 * GATED_CK + j;
-      if (t < q.S) {
-        const GatedToken<T, RATE> k = token(t);
-        before[j + 1] = k.a * before[j] + k.s * k.g * k.x;
-      }
-    }
-#pragma unroll
-    for (int j = GATED_CK - 1; j >= 0; --j) {
-      const int t = k0 * GATED_CK + j;
-      if (t >= q.S) continue;
-      const long long at = ((long long)b * q.S + t) * q.D + d;
-      const GatedToken<T, RATE> k = token(t);
-      float up = to_f32(dy[b * q.gb + t * q.gt + d]);
-      if (z != nullptr) {
-        const float zz = to_f32(z[b * q.zb + t * q.zt + d]);
-        uint64_t sp, cp;
-        logistic_both<T>(f2(zz, zz), sp, cp);
-        float s, cs, o;
-        unf2(sp, s, o);
-        unf2(cp, cs, o);
-        dz[at] = from_f32<T>(up * before[j + 1] * (s * (1.f + zz * cs)));
-        up *= zz * s;
-      }
-      const float G = up + c, gx = k.g * k.x;
-      const float w = before[j] - (q.scale == GATED_PLAIN ? 0.f : q.scale == GATED_CONVEX ? gx : k.a * gx * k.rs);
-      c = k.a * G;
-      dx[at] = from_f32<T>(G * k.s * k.g);
-      if (di != nullptr) di[at] = from_f32<T>(G * k.s * gx * k.cg);
-      if constexpr (RATE) {
-        const float base = c * w * k.sf;   // of the rate
-        df[at] = from_f32<T>(base * r * k.cf);
-        dr += base;
-      } else {
-        df[at] = from_f32<T>(c * w * k.rest);
-      }
-    }
-  }
-  if (dh0 != nullptr) dh0[n] = c;
-  if (RATE && drate != nullptr) drate[n] = dr;
-}
-
+// drate: the sums of n rows of D, 32 channels to a CTA of 32 warps
 __global__ void gated_rate_sum(const float* parts, float* drate, int n, int D) {
-  const int d = blockIdx.x * blockDim.x + threadIdx.x;
-  if (d >= D) return;
+  __shared__ float sums[32][33];
+  const int d = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
-  for (int k = 0; k < n; ++k) s += parts[(long long)k * D + d];
-  drate[d] = s;
+  if (d < D)
+    for (int k = threadIdx.y; k < n; k += 32) s += parts[(long long)k * D + d];
+  sums[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = warp_sum(sums[threadIdx.x][threadIdx.y]);   // warp y: channel y's sums
+  if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < D) drate[blockIdx.x * 32 + threadIdx.y] = s;
 }
 
 template <typename T, bool RATE>
@@ -142,47 +62,84 @@ __global__ void gated_one(const T* x, const T* f, const T* i, const T* z, const 
   y[k] = from_f32<T>(out);
 }
 
-bool gated_sizes_ok(int B, int S, int D) { return B > 0 && S > 0 && D > 0 && (long long)B * D <= (1ll << 40); }
-size_t gated_ckpt_bytes(int B, int S, int D) { return (size_t)B * ceil_div(S, GATED_CK) * D * sizeof(float); }
-size_t gated_bw_bytes(int B, int S, int D) { return (size_t)B * D * sizeof(float); }
+// ---- how a sequence is divided ------------------------------------------------------------------------
+static GatedDims gated_dims(int B, int S, int D, int scale, int V, bool back) {
+  GatedDims q{};
+  q.B = B, q.S = S, q.D = D, q.scale = scale;
+  q.nc = ceil_div(S, GATED_CK);
+  q.blocks = ceil_div(D, 32 * V);
+  q.warps = std::min(8, q.nc);
+  q.K = 1;
+  const long long want = (long long)(back ? 2 : 3) * sm_count();
+  while (q.K < 16 && (long long)B * q.blocks * q.K < want && 2 * q.K * q.warps <= ceil_div(S, GATED_CK)) q.K *= 2;
+  return q;
+}
 
-static GatedDims gated_dims(const long long* st, int B, int S, int D, int scale) {
-  return GatedDims{B, S, D, ceil_div(S, GATED_CK), scale, st[0], st[1], st[2], st[3], st[4], st[5], st[6], st[7], 0, 0};
+bool gated_sizes_ok(int B, int S, int D) {
+  return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && (long long)B * ceil_div(D, 32) * 16 <= 0x7fffffffll;
+}
+size_t gated_ckpt_bytes(int B, int S, int D) { return (size_t)B * ceil_div(S, GATED_CK) * D * sizeof(float); }
+size_t gated_bw_bytes(int B, int S, int D) {   // partial sums of the rate's gradient
+  return (size_t)B * std::max(gated_dims(B, S, D, 0, 1, true).K, gated_dims(B, S, D, 0, 2, true).K) * D * sizeof(float);
+}
+
+int gated_run_f32(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
+int gated_run_bf16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
+int gated_run_f16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
+
+struct GatedVoid {   // as GatedPtrs, of any type
+  const void *x, *f, *i, *z, *dy;
+  const float *rate, *h0, *ckpt_in, *dh_last;
+  void *y, *dx, *df, *di, *dz;
+  float *h_last, *ckpt, *dh0, *rate_parts;
+};
+// Two channels to a lane where every pair of them lies on its own size
+static bool gated_pairs(const GatedVoid& p, const long long* st, const long long* gs, int D, size_t el) {
+  if (D % 2 != 0) return false;
+  for (const void* a : {p.x, p.f, p.i, p.z, p.dy, (const void*)p.y, (const void*)p.dx, (const void*)p.df, (const void*)p.di, (const void*)p.dz})
+    if (!fits_access(a, 2 * el)) return false;
+  for (const float* a : {p.rate, p.h0, p.ckpt_in, p.dh_last, (const float*)p.h_last, (const float*)p.ckpt, (const float*)p.dh0, (const float*)p.rate_parts})
+    if (!fits_access(a, 8)) return false;
+  const void* const ins[4] = {p.x, p.f, p.i, p.z};
+  for (int k = 0; k < 8; ++k)
+    if (ins[k / 2] != nullptr && st[k] % 2 != 0) return false;
+  return gs == nullptr || (gs[0] % 2 == 0 && gs[1] % 2 == 0);
+}
+static int gated_call(bool back, const GatedVoid& p, const long long* st, const long long* gs, int B, int S, int D, int scale, int dtype, float* drate,
+                      cudaStream_t stream) {
+  PhaseScope ps(PH_GATED, stream);
+  const int V = gated_pairs(p, st, gs, D, dtype_size(dtype)) ? 2 : 1;
+  GatedDims q = gated_dims(B, S, D, scale, V, back);
+  long long* const to[8] = {&q.xb, &q.xt, &q.fb, &q.ft, &q.ib, &q.it, &q.zb, &q.zt};
+  for (int k = 0; k < 8; ++k) *to[k] = st[k];
+  if (gs != nullptr) q.gb = gs[0], q.gt = gs[1];
+  auto go = [&](auto* t, auto run) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    const GatedPtrs<T> v{(const T*)p.x, (const T*)p.f, (const T*)p.i, (const T*)p.z, (const T*)p.dy, p.rate, p.h0, p.ckpt_in, p.dh_last, (T*)p.y, (T*)p.dx,
+                         (T*)p.df, (T*)p.di, (T*)p.dz, p.h_last, p.ckpt, p.dh0, p.rate_parts};
+    return run(back, V, &v, q, stream);
+  };
+  int rc = MLSTM_OK;
+  if (dtype == MLSTM_F32) rc = go((float*)nullptr, gated_run_f32);
+  else if (dtype == MLSTM_BF16) rc = go((__nv_bfloat16*)nullptr, gated_run_bf16);
+  else rc = go((__half*)nullptr, gated_run_f16);
+  if (rc == MLSTM_OK && drate != nullptr) {
+    gated_rate_sum<<<ceil_div(D, 32), dim3(32, 32), 0, stream>>>(p.rate_parts, drate, B * q.K, D);
+    MLSTM_LAUNCH_CHECK();
+  }
+  return rc;
 }
 
 int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, int B, int S, int D, int scale, int dtype,
                     cudaStream_t st) {
-  PhaseScope ps(PH_GATED, st);
-  const GatedDims q = gated_dims(strides, B, S, D, scale);
-  const unsigned grid = (unsigned)(((long long)B * D + 127) / 128);
-  auto go = [&](auto* t, auto rate) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    gated_fw<T, decltype(rate)::value><<<grid, 128, 0, st>>>((const T*)in.x, (const T*)in.f, (const T*)in.i, (const T*)in.z, in.rate, in.h0, (T*)y, h_last,
-                                                               ckpt, q);
-  };
-  MLSTM_DTYPE_SWITCH(dtype, T, if (in.rate != nullptr) go((T*)nullptr, std::true_type{}); else go((T*)nullptr, std::false_type{});)
-  MLSTM_LAUNCH_CHECK();
-  return MLSTM_OK;
+  GatedVoid p{in.x, in.f, in.i, in.z, nullptr, in.rate, in.h0, nullptr, nullptr, y, nullptr, nullptr, nullptr, nullptr, h_last, ckpt, nullptr, nullptr};
+  return gated_call(false, p, strides, nullptr, B, S, D, scale, dtype, nullptr, st);
 }
 
 int launch_gated_bw(const GatedIn& in, const long long* strides, const float* ckpt, const void* dy, const long long* gs, const float* dh_last, void* dx,
                     void* df, void* di, void* dz, float* drate, float* dh0, float* parts, int B, int S, int D, int scale, int dtype, cudaStream_t st) {
-  PhaseScope ps(PH_GATED, st);
-  GatedDims q = gated_dims(strides, B, S, D, scale);
-  q.gb = gs[0], q.gt = gs[1];
-  const unsigned grid = (unsigned)(((long long)B * D + 127) / 128);
-  auto go = [&](auto* t, auto rate) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    gated_bw<T, decltype(rate)::value><<<grid, 128, 0, st>>>((const T*)in.x, (const T*)in.f, (const T*)in.i, (const T*)in.z, in.rate, ckpt, (const T*)dy,
-                                                               dh_last, (T*)dx, (T*)df, (T*)di, (T*)dz, drate != nullptr ? parts : nullptr, dh0, q);
-  };
-  MLSTM_DTYPE_SWITCH(dtype, T, if (in.rate != nullptr) go((T*)nullptr, std::true_type{}); else go((T*)nullptr, std::false_type{});)
-  MLSTM_LAUNCH_CHECK();
-  if (drate != nullptr) {
-    gated_rate_sum<<<ceil_div(D, 128), 128, 0, st>>>(parts, drate, B, D);
-    MLSTM_LAUNCH_CHECK();
-  }
-  return MLSTM_OK;
+  GatedVoid p{in.x, in.f, in.i, in.z, dy, in.rate, nullptr, ckpt, dh_last, nullptr, dx, df, di, dz, nullptr, nullptr, dh0, drate != nullptr ? parts : nullptr};
+  return gated_call(true, p, strides, gs, B, S, D, scale, dtype, drate, st);
 }
 
 int launch_gated_step(const GatedIn& in, const float* h, void* y, float* h_new, int B, int D, int scale, int dtype, cudaStream_t st) {

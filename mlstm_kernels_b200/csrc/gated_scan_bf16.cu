@@ -1,0 +1,8 @@
+// The gated linear recurrence of bf16 tensors.
+#include "gated_tiles.cuh"
+
+namespace mlstm {
+int gated_run_bf16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st) {
+  return gated_run<__nv_bfloat16>(back, V, *static_cast<const GatedPtrs<__nv_bfloat16>*>(ptrs), q, st);
+}
+}  // namespace mlstm

@@ -1,0 +1,8 @@
+// The gated linear recurrence of f16 tensors.
+#include "gated_tiles.cuh"
+
+namespace mlstm {
+int gated_run_f16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st) {
+  return gated_run<__half>(back, V, *static_cast<const GatedPtrs<__half>*>(ptrs), q, st);
+}
+}  // namespace mlstm

@@ -1,0 +1,8 @@
+// The gated linear recurrence of f32 tensors.
+#include "gated_tiles.cuh"
+
+namespace mlstm {
+int gated_run_f32(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st) {
+  return gated_run<float>(back, V, *static_cast<const GatedPtrs<float>*>(ptrs), q, st);
+}
+}  // namespace mlstm
