@@ -25,19 +25,109 @@ struct DropoutKey {
 };
 
 struct Words { unsigned w[4]; };
-__device__ __forceinline__ Words philox7(unsigned long long n, unsigned long long offset, unsigned k0, unsigned k1) {
-  unsigned c0 = (unsigned)n, c1 = (unsigned)(n >> 32), c2 = (unsigned)offset, c3 = (unsigned)(offset >> 32);
+__device__ __forceinline__ void mul_wide(unsigned a, unsigned b, unsigned& hi, unsigned& lo) {
+  unsigned long long r;
+  asm("mul.wide.u32 %0, %1, %2;" : "=l"(r) : "r"(a), "r"(b));
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(r));
+}
+__device__ __forceinline__ Words philox7(unsigned n_lo, unsigned n_hi, unsigned long long offset, unsigned k0, unsigned k1) {
+  unsigned c0 = n_lo, c1 = n_hi, c2 = (unsigned)offset, c3 = (unsigned)(offset >> 32);
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
-    const unsigned long long p0 = (unsigned long long)c0 * 0xD2511F53u, p1 = (unsigned long long)c2 * 0xCD9E8D57u;
-    c0 = (unsigned)(p1 >> 32) ^ c1 ^ k0;
-    c1 = (unsigned)p1;
-    c2 = (unsigned)(p0 >> 32) ^ c3 ^ k1;
-    c3 = (unsigned)p0;
+    unsigned h0, l0, h1, l1;
+    mul_wide(c0, 0xD2511F53u, h0, l0);
+    mul_wide(c2, 0xCD9E8D57u, h1, l1);
+    c0 = h1 ^ c1 ^ k0;
+    c1 = l1;
+    c2 = h0 ^ c3 ^ k1;
+    c3 = l0;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
   return Words{{c0, c1, c2, c3}};
+}
+
+__device__ __forceinline__ unsigned long long seed_of(const DropoutKey& key) {
+  return key.device != nullptr ? (unsigned long long)*key.device : key.seed;
+}
+__device__ __forceinline__ float dropped(float v, unsigned word, const DropoutKey& key) { return word >= key.threshold ? v * key.scale : 0.f; }
+
+// n / d for n < 2^31: the high half of n m, and n itself, shifted (the quotient's multiplier has 33 bits, the highest of them set)
+struct Divide {
+  unsigned d, m, s;
+  __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, m) + n) >> s; }
+};
+static Divide divide_by(long long d) {
+  unsigned s = 0;
+  while ((1ll << s) < d) ++s;
+  return Divide{(unsigned)d, (unsigned)((((1ull << s) - (unsigned long long)d) << 32) / (unsigned long long)d + 1), s};
+}
+
+// V neighbouring elements to an access of 16 bytes (of the wider type), DROP_U accesses to a thread.  FLAT: all tensors lie in the
+// order of their elements; else rows of D, a multiple of V, at strides that are multiples of it.
+constexpr int DROP_THREADS = 256, DROP_U = 4;
+struct DropoutRows {
+  Divide chunks, n2, n1;
+  unsigned xs[3], rs[3], ys[3];   // strides in chunks: all tensors end below 2^31 of them
+};
+template <typename T, typename O, int V, bool FLAT, bool RES>
+__global__ void __launch_bounds__(DROP_THREADS, 4)
+    dropout_wide(const T* __restrict__ x, const O* __restrict__ residual, O* __restrict__ y, long long count, DropoutRows rows, DropoutKey key) {
+  constexpr int CHUNKS = DROP_U * DROP_THREADS;   // of a CTA: a power of two
+  const long long first = (long long)blockIdx.x * CHUNKS, whole = count / V;
+  const unsigned long long quads = (unsigned long long)first * (V / 4), seed = seed_of(key);
+  auto work = [&](auto all) {
+    Pack<T, V> xv[DROP_U];
+    Pack<O, V> rv[DROP_U];
+    O* to[DROP_U];
+#pragma unroll
+    for (int u = 0; u < DROP_U; ++u) {
+      const int c = threadIdx.x + u * DROP_THREADS;
+      if (!decltype(all)::value && first + c >= whole) break;
+      if constexpr (FLAT) {
+        xv[u] = load_pack<T, V>(x + first * V + c * V);
+        if (RES) rv[u] = load_pack<O, V>(residual + first * V + c * V);
+        to[u] = y + first * V + c * V;
+      } else {
+        const unsigned n = (unsigned)first + c, r = rows.chunks(n), d = n - r * rows.chunks.d, r1 = rows.n2(r), i2 = r - r1 * rows.n2.d, i0 = rows.n1(r1),
+                       i1 = r1 - i0 * rows.n1.d;
+        auto at = [&](const unsigned (&s)[3]) { return (long long)(i0 * s[0] + i1 * s[1] + i2 * s[2] + d) * V; };
+        xv[u] = load_pack<T, V>(x + at(rows.xs));
+        if (RES) rv[u] = load_pack<O, V>(residual + at(rows.rs));
+        to[u] = y + at(rows.ys);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < DROP_U; ++u) {
+      const int c = threadIdx.x + u * DROP_THREADS;
+      if (!decltype(all)::value && first + c >= whole) break;
+      Pack<O, V> o;
+#pragma unroll
+      for (int k = 0; k < V; k += 4) {
+        // The CTA's counters begin at a multiple of their number, a power of two: their high half is one for all, and what the rounds
+        // make of it and of the offset alone is worked out once.
+        const Words w = philox7((unsigned)quads + c * (V / 4) + k / 4, (unsigned)(quads >> 32), key.offset, (unsigned)seed, (unsigned)(seed >> 32));
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          float v[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) v[e] = dropped(to_f32(xv[u].e[k + j + e]), w.w[j + e], key) + (RES ? to_f32(rv[u].e[k + j + e]) : 0.f);
+          from_f32x2(v[0], v[1], o.e + k + j);
+        }
+      }
+      store_pack(to[u], o);
+    }
+  };
+  if (first + CHUNKS <= whole) {
+    work(std::true_type{});
+    return;
+  }
+  work(std::false_type{});
+  const long long n = whole * V + threadIdx.x;   // what is left of a chunk
+  if (FLAT && n < count && n / V / CHUNKS == blockIdx.x) {
+    const Words w = philox7((unsigned)(n / 4), (unsigned)(n / 4 >> 32), key.offset, (unsigned)seed, (unsigned)(seed >> 32));
+    y[n] = from_f32<O>(dropped(to_f32(x[n]), w.w[n % 4], key) + (RES ? to_f32(residual[n]) : 0.f));
+  }
 }
 
 // four elements to a thread, each read where it lies
@@ -45,18 +135,60 @@ template <typename T, typename O>
 __global__ void dropout_any(const T* x, const O* residual, O* y, DropoutDims q, DropoutKey key) {
   const long long quad = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (quad * 4 >= q.n) return;
-  const unsigned long long seed = key.device != nullptr ? (unsigned long long)*key.device : key.seed;
-  const Words w = philox7((unsigned long long)quad, key.offset, (unsigned)seed, (unsigned)(seed >> 32));
+  const unsigned long long seed = seed_of(key);
+  const Words w = philox7((unsigned)quad, (unsigned)(quad >> 32), key.offset, (unsigned)seed, (unsigned)(seed >> 32));
+  long long d = q.D, xa = 0, ra = 0, ya = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const long long n = quad * 4 + j;
     if (n >= q.n) break;
-    const long long d = n % q.D, r = n / q.D, i2 = r % q.n2, r1 = r / q.n2, i1 = r1 % q.n1, i0 = r1 / q.n1;
-    const float v = to_f32(x[i0 * q.xs[0] + i1 * q.xs[1] + i2 * q.xs[2] + d]);
-    float o = w.w[j] >= key.threshold && key.some ? v * key.scale : 0.f;
-    if (residual != nullptr) o += to_f32(residual[i0 * q.rs[0] + i1 * q.rs[1] + i2 * q.rs[2] + d]);
-    y[i0 * q.ys[0] + i1 * q.ys[1] + i2 * q.ys[2] + d] = from_f32<O>(o);
+    if (d == q.D) {   // the first, or a new row
+      const long long r = n / q.D, r1 = r / q.n2, i2 = r - r1 * q.n2, i0 = r1 / q.n1, i1 = r1 - i0 * q.n1;
+      d = n - r * q.D;
+      xa = i0 * q.xs[0] + i1 * q.xs[1] + i2 * q.xs[2];
+      ra = i0 * q.rs[0] + i1 * q.rs[1] + i2 * q.rs[2];
+      ya = i0 * q.ys[0] + i1 * q.ys[1] + i2 * q.ys[2];
+    }
+    float o = !key.some ? 0.f : dropped(to_f32(x[xa + d]), w.w[j], key);
+    if (residual != nullptr) o += to_f32(residual[ra + d]);
+    y[ya + d] = from_f32<O>(o);
+    ++d;
   }
+}
+
+template <typename T, typename O>
+static void dropout_run(const T* x, const O* residual, O* y, const DropoutDims& q, const DropoutKey& key, cudaStream_t st) {
+  constexpr int V = sizeof(T) == 4 || sizeof(O) == 4 ? 4 : 8;
+  const bool flat = q.n == q.D;
+  bool wide = key.some && fits_access(x, sizeof(T) * V) && fits_access(y, sizeof(O) * V) && (residual == nullptr || fits_access(residual, sizeof(O) * V));
+  if (!flat) {
+    wide = wide && q.D % V == 0 && q.n / V < (1ll << 31);
+    const long long n[3] = {q.n / (q.n1 * q.n2 * q.D), q.n1, q.n2};
+    for (const long long* s : {q.xs, q.rs, q.ys}) {   // (without a residual its strides are zero)
+      long long end = q.D / V;
+      for (int k = 0; k < 3; ++k) {
+        wide = wide && s[k] % V == 0 && s[k] / V <= (1ll << 31);
+        end += (n[k] - 1) * (s[k] / V);
+      }
+      wide = wide && end < (1ll << 31);
+    }
+  }
+  if (!wide) {
+    dropout_any<T, O><<<(unsigned)((q.n + 1023) / 1024), 256, 0, st>>>(x, residual, y, q, key);
+    return;
+  }
+  const long long chunks = (q.n + V - 1) / V, per = DROP_U * DROP_THREADS;
+  const unsigned grid = (unsigned)((chunks + per - 1) / per);
+  DropoutRows rows{};
+  if (!flat) {
+    rows = DropoutRows{divide_by(q.D / V), divide_by(q.n2), divide_by(q.n1), {}, {}, {}};
+    for (int k = 0; k < 3; ++k) rows.xs[k] = (unsigned)(q.xs[k] / V), rows.rs[k] = (unsigned)(q.rs[k] / V), rows.ys[k] = (unsigned)(q.ys[k] / V);
+  }
+  auto go = [&](auto f, auto r) {
+    dropout_wide<T, O, V, decltype(f)::value, decltype(r)::value><<<grid, DROP_THREADS, 0, st>>>(x, residual, y, q.n, rows, key);
+  };
+  if (flat) residual != nullptr ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+  else residual != nullptr ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 int launch_dropout(const void* x, const long long* xs, const void* residual, const long long* rs, void* y, const long long* ys, const long long* sizes, double p,
@@ -67,13 +199,10 @@ int launch_dropout(const void* x, const long long* xs, const void* residual, con
     for (int k = 0; k < 3; ++k) q.rs[k] = rs[k];
   const double t = nearbyint(p * 4294967296.0);
   const DropoutKey key{seed_device, seed, offset, t < 4294967296.0 ? (unsigned)t : 0u, t < 4294967296.0, t < 4294967296.0 ? (float)(1.0 / (1.0 - p)) : 0.f};
-  const long long quads = (q.n + 3) / 4;
-  if ((quads + 255) / 256 > 0x7fffffffll) return MLSTM_ERR_SHAPE;
-  const unsigned grid = (unsigned)((quads + 255) / 256);
   auto go = [&](auto* t, auto* o) {
     using T = std::remove_pointer_t<decltype(t)>;
     using O = std::remove_pointer_t<decltype(o)>;
-    dropout_any<T, O><<<grid, 256, 0, st>>>((const T*)x, (const O*)residual, (O*)y, q, key);
+    dropout_run<T, O>((const T*)x, (const O*)residual, (O*)y, q, key, st);
   };
   if (out_dtype == MLSTM_F32) {
     MLSTM_DTYPE_SWITCH(dtype, T, go((T*)nullptr, (float*)nullptr);)
