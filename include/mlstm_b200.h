@@ -391,14 +391,15 @@ int mlstm_b200_ssm_step(const void* x, const void* dt, const float* a, const voi
  *   y (B,S,D) dtype out; h_last (B,D) f32 out or NULL
  *   checkpoints: mlstm_b200_gated_checkpoint_bytes(), what the backward needs of the forward, or NULL
  * Backward: dy at dy_strides[2], dh_last (B,D) f32 or NULL; dx, df, di, dz (B,S,D) contiguous, dtype, out (di, dz NULL without i, z);
- * drate (D), dh_initial (B,D) f32 out, each may be NULL; workspace: mlstm_b200_gated_bw_workspace_bytes(), for drate.
+ * drate (D), dh_initial (B,D) f32 out, each may be NULL.
  * Step: one token, x, f, i, z, y (B,D) contiguous, h, h_new (B,D) f32; h_new may be h.
+ * workspace: mlstm_b200_gated_workspace_bytes() for the forward (backward = 0; may be none) and the backward (1).
  */
 size_t mlstm_b200_gated_checkpoint_bytes(int B, int S, int D);
-size_t mlstm_b200_gated_bw_workspace_bytes(int B, int S, int D);
+size_t mlstm_b200_gated_workspace_bytes(int B, int S, int D, int backward);
 int mlstm_b200_gated_scan_fw(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h_initial,
-                             const long long* strides, void* y, float* h_last, void* checkpoints, int B, int S, int D,
-                             int input_scale, int dtype, void* stream);
+                             const long long* strides, void* y, float* h_last, void* checkpoints, void* workspace,
+                             size_t workspace_bytes, int B, int S, int D, int input_scale, int dtype, void* stream);
 int mlstm_b200_gated_scan_bw(const void* x, const void* f, const void* i, const void* z, const float* rate,
                              const long long* strides, const void* checkpoints, const void* dy, const long long* dy_strides,
                              const float* dh_last, void* dx, void* df, void* di, void* dz, float* drate, float* dh_initial,

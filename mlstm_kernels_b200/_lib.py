@@ -72,8 +72,8 @@ SIGNATURES = {
     "mlstm_b200_ssm_scan_bw": (_i, [_vp] * 8 + [_llp, _vp, _vp, _llp] + [_vp] * 11 + [_sz] + [_i] * 7 + [_vp]),
     "mlstm_b200_ssm_step": (_i, [_vp] * 11 + [_i] * 6 + [_vp]),
     "mlstm_b200_gated_checkpoint_bytes": (_sz, [_i] * 3),
-    "mlstm_b200_gated_bw_workspace_bytes": (_sz, [_i] * 3),
-    "mlstm_b200_gated_scan_fw": (_i, [_vp] * 6 + [_llp] + [_vp] * 3 + [_i] * 5 + [_vp]),
+    "mlstm_b200_gated_workspace_bytes": (_sz, [_i] * 4),
+    "mlstm_b200_gated_scan_fw": (_i, [_vp] * 6 + [_llp] + [_vp] * 4 + [_sz] + [_i] * 5 + [_vp]),
     "mlstm_b200_gated_scan_bw": (_i, [_vp] * 5 + [_llp, _vp, _vp, _llp] + [_vp] * 8 + [_sz] + [_i] * 5 + [_vp]),
     "mlstm_b200_gated_step": (_i, [_vp] * 8 + [_i] * 4 + [_vp]),
     "mlstm_b200_dropout": (_i, [_vp, _llp, _vp, _llp, _vp, _llp, _llp, C.c_double, C.c_ulonglong, _vp, C.c_ulonglong, _i, _i, _vp]),

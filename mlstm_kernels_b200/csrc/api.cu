@@ -301,8 +301,10 @@ long long mlstm_b200_launch_count(void) { return g_launches.load(); }
 
 int mlstm_b200_device_status(int reset) {
   int status = 0;
-  const int rc = sm100_device_status(reset, &status);
-  return rc != MLSTM_OK ? rc : status;
+  int rc = sm100_device_status(reset, &status);
+  int gated = 0;
+  if (rc == MLSTM_OK) rc = gated_status(reset, &gated);
+  return rc != MLSTM_OK ? rc : status != 0 ? status : gated;
 }
 
 int mlstm_b200_selftest_wait_expiry(unsigned int limit_polls, int code, void* stream) {

@@ -114,16 +114,19 @@ int mlstm_b200_ssm_step(const void* x, const void* dt, const float* a, const voi
 }
 
 size_t mlstm_b200_gated_checkpoint_bytes(int B, int S, int D) { return gated_sizes_ok(B, S, D) ? gated_ckpt_bytes(B, S, D) : 0; }
-size_t mlstm_b200_gated_bw_workspace_bytes(int B, int S, int D) { return gated_sizes_ok(B, S, D) ? gated_bw_bytes(B, S, D) : 0; }
+size_t mlstm_b200_gated_workspace_bytes(int B, int S, int D, int backward) { return gated_sizes_ok(B, S, D) ? gated_bytes(B, S, D, backward != 0) : 0; }
 
 int mlstm_b200_gated_scan_fw(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h_initial,
-                             const long long* strides, void* y, float* h_last, void* checkpoints, int B, int S, int D, int input_scale, int dtype,
-                             void* stream) {
+                             const long long* strides, void* y, float* h_last, void* checkpoints, void* workspace, size_t workspace_bytes, int B, int S, int D,
+                             int input_scale, int dtype, void* stream) {
   if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;
   if (!gated_sizes_ok(B, S, D) || !gated_scale_ok(input_scale)) return MLSTM_ERR_SHAPE;
   if (!x || !f || !strides || !y) return MLSTM_ERR_NULL;
-  if (!scratch_aligned(checkpoints)) return MLSTM_ERR_ALIGN;
-  return launch_gated_fw(GatedIn{x, f, i, z, rate, h_initial}, strides, y, h_last, static_cast<float*>(checkpoints), B, S, D, input_scale, dtype,
+  const size_t need = gated_bytes(B, S, D, false);
+  if (need > 0 && !workspace) return MLSTM_ERR_NULL;
+  if (!scratch_aligned(checkpoints) || !scratch_aligned(workspace)) return MLSTM_ERR_ALIGN;
+  if (workspace_bytes < need) return MLSTM_ERR_WORKSPACE;
+  return launch_gated_fw(GatedIn{x, f, i, z, rate, h_initial}, strides, y, h_last, static_cast<float*>(checkpoints), workspace, B, S, D, input_scale, dtype,
                          static_cast<cudaStream_t>(stream));
 }
 
@@ -134,12 +137,12 @@ int mlstm_b200_gated_scan_bw(const void* x, const void* f, const void* i, const 
   if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;
   if (!gated_sizes_ok(B, S, D) || !gated_scale_ok(input_scale)) return MLSTM_ERR_SHAPE;
   if (!x || !f || !strides || !checkpoints || !dy || !dy_strides || !dx || !df) return MLSTM_ERR_NULL;
-  if ((i != nullptr) != (di != nullptr) || (z != nullptr) != (dz != nullptr) || (drate != nullptr && (rate == nullptr || workspace == nullptr)))
+  if ((i != nullptr) != (di != nullptr) || (z != nullptr) != (dz != nullptr) || (drate != nullptr && rate == nullptr) || !workspace)
     return MLSTM_ERR_NULL;
   if (!scratch_aligned(workspace) || !scratch_aligned(checkpoints)) return MLSTM_ERR_ALIGN;
-  if (drate != nullptr && workspace_bytes < gated_bw_bytes(B, S, D)) return MLSTM_ERR_WORKSPACE;
+  if (workspace_bytes < gated_bytes(B, S, D, true)) return MLSTM_ERR_WORKSPACE;
   return launch_gated_bw(GatedIn{x, f, i, z, rate, nullptr}, strides, static_cast<const float*>(checkpoints), dy, dy_strides, dh_last, dx, df, di, dz, drate,
-                         dh_initial, static_cast<float*>(workspace), B, S, D, input_scale, dtype, static_cast<cudaStream_t>(stream));
+                         dh_initial, workspace, B, S, D, input_scale, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int mlstm_b200_gated_step(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h, void* y, float* h_new, int B, int D,

@@ -5,6 +5,7 @@
 // w_n, the word of element n of x (in its logical order, whatever its strides), is word n mod 4 of Philox4x32 with seven rounds, the
 // fewest that its authors found to pass every test of BigCrush (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as
 // 1, 2, 3; 2011), under the key `seed`, of the counter (n div 4, offset).  The backward is the same call on dy.
+#include "divide.cuh"
 #include "launch.cuh"
 #include "vec.cuh"
 
@@ -51,17 +52,6 @@ __device__ __forceinline__ unsigned long long seed_of(const DropoutKey& key) {
   return key.device != nullptr ? (unsigned long long)*key.device : key.seed;
 }
 __device__ __forceinline__ float dropped(float v, unsigned word, const DropoutKey& key) { return word >= key.threshold ? v * key.scale : 0.f; }
-
-// n / d for n < 2^31: the high half of n m, and n itself, shifted (the quotient's multiplier has 33 bits, the highest of them set)
-struct Divide {
-  unsigned d, m, s;
-  __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, m) + n) >> s; }
-};
-static Divide divide_by(long long d) {
-  unsigned s = 0;
-  while ((1ll << s) < d) ++s;
-  return Divide{(unsigned)d, (unsigned)((((1ull << s) - (unsigned long long)d) << 32) / (unsigned long long)d + 1), s};
-}
 
 // V neighbouring elements to an access of 16 bytes (of the wider type), DROP_U accesses to a thread.  FLAT: all tensors lie in the
 // order of their elements; else rows of D, a multiple of V, at strides that are multiples of it.

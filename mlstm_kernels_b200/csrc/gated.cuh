@@ -12,18 +12,29 @@
 //
 // as a ds/da = -a or -a^2 / s; no quotient is left that a closed gate (1 - a = 0) would make 0 / 0.
 #pragma once
+#include "divide.cuh"
+#include "gated_units.h"
 #include "launch.cuh"
 #include "vec.cuh"
 
 namespace mlstm {
 
-constexpr int GATED_CK = 8;   // tokens to a thread, and to a state that the forward keeps for the backward
 struct GatedDims {
   int B, S, D, nc;      // nc: kept states of a sequence
   int scale;
-  int blocks;           // CTAs next to each other that take the channels
-  int K, warps;         // CTAs to a cluster, warps to a CTA
+  int warps, nt, group, groups, units;   // (gated_units.h)
+  Divide chains, blocks;
   long long xb, xt, fb, ft, ib, it, zb, zt, gb, gt;   // strides in elements (batch, token) of x, f, i, z, dy
+  // scratch: null where a chain is one unit
+  unsigned *ticket, *gave_up, *state_flag, *agg_flag;
+  void *state, *agg;
+};
+
+template <typename T> struct GatedPtrs {
+  const T *x, *f, *i, *z, *dy;
+  const float *rate, *h0, *ckpt_in, *dh_last;
+  T *y, *dx, *df, *di, *dz;
+  float *h_last, *ckpt, *dh0, *rate_parts;
 };
 
 constexpr int GATED_PLAIN = 0, GATED_CONVEX = 1, GATED_VARIANCE = 2;
@@ -34,7 +45,13 @@ __device__ __forceinline__ float rsq(float x) {
   return r;
 }
 __device__ __forceinline__ uint64_t dup2(float x) { return f2(x, x); }
-__device__ __forceinline__ uint64_t neg2(uint64_t v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ uint64_t minus2(uint64_t a, uint64_t b) { return fma2(b, dup2(-1.f), a); }   // a - b
+
+template <typename T> __device__ __forceinline__ uint64_t logistic_pair2(uint64_t v) {
+  float a, b;
+  unf2(v, a, b);
+  return logistic_pair<T>(a, b);
+}
 
 // s = sigmoid(v) and c = 1 - s of two values, both with all digits: whichever is above 1/2 is one minus the other
 template <typename T> __device__ __forceinline__ void logistic_both(uint64_t v, uint64_t& s, uint64_t& c) {
@@ -42,47 +59,51 @@ template <typename T> __device__ __forceinline__ void logistic_both(uint64_t v, 
   unf2(v, v0, v1);
   const uint64_t e = exp_neg_pair<kFull<T>>(v0, v1), p = rcp_pair(add2(dup2(1.f), e)), q = mul2(e, p);
   // (where e is infinite, q is no number, and is not taken)
-  float p0, p1, q0, q1;
+  float p0, p1, q0, q1, np0, np1, nq0, nq1;
   unf2(p, p0, p1);
   unf2(q, q0, q1);
-  const float less0 = v0 > 0.f ? q0 : p0, less1 = v1 > 0.f ? q1 : p1, more0 = 1.f - less0, more1 = 1.f - less1;
-  s = f2(v0 > 0.f ? more0 : less0, v1 > 0.f ? more1 : less1);
-  c = f2(v0 > 0.f ? less0 : more0, v1 > 0.f ? less1 : more1);
+  unf2(minus2(dup2(1.f), p), np0, np1);
+  unf2(minus2(dup2(1.f), q), nq0, nq1);
+  const bool up0 = v0 > 0.f, up1 = v1 > 0.f;
+  s = f2(up0 ? nq0 : p0, up1 ? nq1 : p1);
+  c = f2(up0 ? q0 : np0, up1 ? q1 : np1);
 }
 
-// of two values of f: a, 1 - a; and with a rate sigmoid(f) and 1 - sigmoid(f)
+// of two values of f: a, 1 - a; and with a rate sigmoid(f) and 1 - sigmoid(f).
+// FAR = false: the rate is known to be in (-1/2, 0], and no exponential is needed; BOTH = false: 1 - sigmoid(f) is not needed.
 struct Decay { uint64_t a, rest, sf, cf; };
-// (FAR = false: the rate is known to be in (-1/2, 0], and no exponential is needed)
-template <typename T, bool RATE, bool FAR = true> __device__ __forceinline__ Decay decay_pair(uint64_t f, uint64_t rate) {
+template <typename T, bool RATE, bool FAR = true, bool BOTH = true> __device__ __forceinline__ Decay decay_pair(uint64_t f, uint64_t rate) {
   Decay d;
-  logistic_both<T>(f, d.sf, d.cf);
   if constexpr (!RATE) {
+    logistic_both<T>(f, d.sf, d.cf);
     d.a = d.sf;
     d.rest = d.cf;
-  } else {
-    // rho = -log a.  Below 1/2: 1 - e^-rho = rho p(rho), p the polynomial through its values at the Chebyshev points of [0, 1/2],
-    // off by 2^-29, in f32 2^-24; else 1 - a has lost one digit at most.
-    const uint64_t rho = neg2(mul2(rate, d.sf));
-    uint64_t p = fma2(dup2(-1.1234042e-3f), rho, dup2(8.1896136e-3f));
-    p = fma2(p, rho, dup2(-4.1630073e-2f));
-    p = fma2(p, rho, dup2(1.6666242e-1f));
-    p = fma2(p, rho, dup2(-4.9999982e-1f));
-    p = fma2(p, rho, dup2(1.f));
-    const uint64_t small = mul2(p, rho);
-    if constexpr (!FAR) {
-      d.rest = small;
-      d.a = fma2(p, neg2(rho), dup2(1.f));
-      return d;
-    }
-    float r0, r1, s0, s1, e0, e1;
-    unf2(rho, r0, r1);
-    unf2(small, s0, s1);
-    unf2(exp_neg_pair<kFull<T>>(r0, r1), e0, e1);
-    const bool n0 = __float_as_uint(r0) < 0x3f000000u, n1 = __float_as_uint(r1) < 0x3f000000u;   // (0 <= rho < 1/2)
-    const float rest0 = n0 ? s0 : 1.f - e0, rest1 = n1 ? s1 : 1.f - e1;
-    d.rest = f2(rest0, rest1);
-    d.a = f2(n0 ? 1.f - s0 : e0, n1 ? 1.f - s1 : e1);
+    return d;
   }
+  if constexpr (BOTH) logistic_both<T>(f, d.sf, d.cf);
+  else d.sf = logistic_pair2<T>(f);
+  // l = log a = -rho.  Where rho is below 1/2: 1 - e^l = rho p(l), p the polynomial through the values of (e^l - 1) / l at the
+  // Chebyshev points of [-1/2, 0], off by 2^-29, in f32 2^-24; else 1 - a has lost one digit at most.
+  const uint64_t l = mul2(rate, d.sf), rho = mul2(l, dup2(-1.f));
+  uint64_t p = fma2(dup2(1.1234042e-3f), l, dup2(8.1896136e-3f));
+  p = fma2(p, l, dup2(4.1630073e-2f));
+  p = fma2(p, l, dup2(1.6666242e-1f));
+  p = fma2(p, l, dup2(4.9999982e-1f));
+  p = fma2(p, l, dup2(1.f));
+  const uint64_t small = mul2(p, rho), large = fma2(p, l, dup2(1.f));
+  if constexpr (!FAR) {
+    d.rest = small;
+    d.a = large;
+    return d;
+  }
+  float r0, r1, s0, s1, l0, l1, e0, e1;
+  unf2(rho, r0, r1);
+  unf2(small, s0, s1);
+  unf2(large, l0, l1);
+  unf2(exp_neg_pair<kFull<T>>(r0, r1), e0, e1);
+  const bool n0 = __float_as_uint(r0) < 0x3f000000u, n1 = __float_as_uint(r1) < 0x3f000000u;   // (0 <= rho < 1/2)
+  d.rest = f2(n0 ? s0 : 1.f - e0, n1 ? s1 : 1.f - e1);
+  d.a = f2(n0 ? l0 : e0, n1 ? l1 : e1);
   return d;
 }
 
@@ -92,12 +113,14 @@ __device__ __forceinline__ uint64_t inv_scale_pair(uint64_t rest2) {
   unf2(add2(rest2, dup2(1.17549435e-38f)), q0, q1);
   return f2(rsq(q0), rsq(q1));
 }
-__device__ __forceinline__ uint64_t rest2_pair(uint64_t a, uint64_t rest) { return fma2(rest, a, rest); }   // 1 - a^2
-
-template <typename T> __device__ __forceinline__ uint64_t logistic_pair2(uint64_t v) {
-  float a, b;
-  unf2(v, a, b);
-  return logistic_pair<T>(a, b);
+// sqrt(1 - a^2) alone
+__device__ __forceinline__ uint64_t scale_pair(uint64_t rest2) {
+  float q0, q1;
+  unf2(rest2, q0, q1);
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(q0));
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(q1));
+  return f2(q0, q1);
 }
+__device__ __forceinline__ uint64_t rest2_pair(uint64_t a, uint64_t rest) { return fma2(rest, a, rest); }   // 1 - a^2
 
 }  // namespace mlstm

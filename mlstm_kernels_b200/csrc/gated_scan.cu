@@ -2,7 +2,7 @@
 // token.
 #include <algorithm>
 
-#include "gated_tiles.cuh"
+#include "gated.cuh"
 
 namespace mlstm {
 
@@ -62,30 +62,35 @@ __global__ void gated_one(const T* x, const T* f, const T* i, const T* z, const 
   y[k] = from_f32<T>(out);
 }
 
-// ---- how a sequence is divided ------------------------------------------------------------------------
-static GatedDims gated_dims(int B, int S, int D, int scale, int V, bool back) {
-  GatedDims q{};
-  q.B = B, q.S = S, q.D = D, q.scale = scale;
-  q.nc = ceil_div(S, GATED_CK);
-  q.blocks = ceil_div(D, 32 * V);
-  q.warps = std::min(8, q.nc);
-  q.K = 1;
-  const long long want = (long long)(back ? 2 : 3) * sm_count();
-  while (q.K < 16 && (long long)B * q.blocks * q.K < want && 2 * q.K * q.warps <= ceil_div(S, GATED_CK)) q.K *= 2;
-  return q;
-}
+// ---- calls --------------------------------------------------------------------------------------------
+static int gated_slots() { return 2 * sm_count(); }   // CTAs that run at once
 
 bool gated_sizes_ok(int B, int S, int D) {
-  return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && (long long)B * ceil_div(D, 32) * 16 <= 0x7fffffffll;
+  return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && D <= (1 << 30) && gated_plan(B, S, D, 1, gated_slots()).units < (1ll << 31);
 }
 size_t gated_ckpt_bytes(int B, int S, int D) { return (size_t)B * ceil_div(S, GATED_CK) * D * sizeof(float); }
-size_t gated_bw_bytes(int B, int S, int D) {   // partial sums of the rate's gradient
-  return (size_t)B * std::max(gated_dims(B, S, D, 0, 1, true).K, gated_dims(B, S, D, 0, 2, true).K) * D * sizeof(float);
+size_t gated_bytes(int B, int S, int D, bool backward) {
+  size_t most = 0;
+  for (const int V : {1, 2, 4}) most = std::max(most, gated_scratch(gated_plan(B, S, D, V, gated_slots()), B, D, backward).bytes);
+  return most;
 }
 
 int gated_run_f32(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
 int gated_run_bf16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
 int gated_run_f16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
+int gated_status_f32(int reset, int* status);
+int gated_status_bf16(int reset, int* status);
+int gated_status_f16(int reset, int* status);
+int gated_status(int reset, int* status) {
+  *status = 0;
+  for (auto* of : {gated_status_f32, gated_status_bf16, gated_status_f16}) {
+    int one = 0;
+    const int rc = of(reset, &one);
+    if (rc != MLSTM_OK) return rc;
+    if (*status == 0) *status = one;
+  }
+  return MLSTM_OK;
+}
 
 struct GatedVoid {   // as GatedPtrs, of any type
   const void *x, *f, *i, *z, *dy;
@@ -93,23 +98,40 @@ struct GatedVoid {   // as GatedPtrs, of any type
   void *y, *dx, *df, *di, *dz;
   float *h_last, *ckpt, *dh0, *rate_parts;
 };
-// Two channels to a lane where every pair of them lies on its own size
-static bool gated_pairs(const GatedVoid& p, const long long* st, const long long* gs, int D, size_t el) {
-  if (D % 2 != 0) return false;
-  for (const void* a : {p.x, p.f, p.i, p.z, p.dy, (const void*)p.y, (const void*)p.dx, (const void*)p.df, (const void*)p.di, (const void*)p.dz})
-    if (!fits_access(a, 2 * el)) return false;
-  for (const float* a : {p.rate, p.h0, p.ckpt_in, p.dh_last, (const float*)p.h_last, (const float*)p.ckpt, (const float*)p.dh0, (const float*)p.rate_parts})
-    if (!fits_access(a, 8)) return false;
+// Rows by 16 bytes where all of them begin on such a boundary
+static bool gated_rows(const GatedVoid& p, const long long* st, const long long* gs, int D, int el) {
+  const int e = 16 / el;
+  if (D % e != 0) return false;
+  for (const void* a : {p.x, p.f, p.i, p.z, p.dy, (const void*)p.y, (const void*)p.dx, (const void*)p.df, (const void*)p.di, (const void*)p.dz,
+                        (const void*)p.rate, (const void*)p.h0, (const void*)p.ckpt_in, (const void*)p.dh_last, (const void*)p.h_last, (const void*)p.ckpt,
+                        (const void*)p.dh0, (const void*)p.rate_parts})
+    if (!fits_access(a, 16)) return false;
   const void* const ins[4] = {p.x, p.f, p.i, p.z};
   for (int k = 0; k < 8; ++k)
-    if (ins[k / 2] != nullptr && st[k] % 2 != 0) return false;
-  return gs == nullptr || (gs[0] % 2 == 0 && gs[1] % 2 == 0);
+    if (ins[k / 2] != nullptr && st[k] % e != 0) return false;
+  return gs == nullptr || (gs[0] % e == 0 && gs[1] % e == 0);
 }
-static int gated_call(bool back, const GatedVoid& p, const long long* st, const long long* gs, int B, int S, int D, int scale, int dtype, float* drate,
+static int gated_call(bool back, GatedVoid p, const long long* st, const long long* gs, void* scratch, int B, int S, int D, int scale, int dtype, float* drate,
                       cudaStream_t stream) {
   PhaseScope ps(PH_GATED, stream);
-  const int V = gated_pairs(p, st, gs, D, dtype_size(dtype)) ? 2 : 1;
-  GatedDims q = gated_dims(B, S, D, scale, V, back);
+  const int el = (int)dtype_size(dtype), V = !gated_rows(p, st, gs, D, el) ? 1 : back ? 2 : 8 / el;
+  const GatedPlan plan = gated_plan(B, S, D, V, gated_slots());
+  const GatedScratch at = gated_scratch(plan, B, D, back);
+  unsigned char* const base = static_cast<unsigned char*>(scratch);
+  GatedDims q{};
+  q.B = B, q.S = S, q.D = D, q.scale = scale, q.nc = ceil_div(S, GATED_CK);
+  q.warps = plan.warps, q.nt = plan.nt, q.group = plan.group, q.groups = plan.groups, q.units = (int)plan.units;
+  q.chains = divide_by(plan.chains), q.blocks = divide_by(plan.blocks);
+  if (plan.nt > 1) {
+    q.ticket = reinterpret_cast<unsigned*>(base);
+    q.gave_up = q.ticket + 32;
+    q.state_flag = q.ticket + 64;
+    q.agg_flag = q.state_flag + plan.chains * plan.groups;
+    q.state = base + at.state;
+    q.agg = base + at.agg;
+    MLSTM_CUDA_CHECK(cudaMemsetAsync(base, 0, at.zeroed, stream));
+  }
+  if (drate != nullptr) p.rate_parts = reinterpret_cast<float*>(base + at.rate);
   long long* const to[8] = {&q.xb, &q.xt, &q.fb, &q.ft, &q.ib, &q.it, &q.zb, &q.zt};
   for (int k = 0; k < 8; ++k) *to[k] = st[k];
   if (gs != nullptr) q.gb = gs[0], q.gt = gs[1];
@@ -124,22 +146,22 @@ static int gated_call(bool back, const GatedVoid& p, const long long* st, const 
   else if (dtype == MLSTM_BF16) rc = go((__nv_bfloat16*)nullptr, gated_run_bf16);
   else rc = go((__half*)nullptr, gated_run_f16);
   if (rc == MLSTM_OK && drate != nullptr) {
-    gated_rate_sum<<<ceil_div(D, 32), dim3(32, 32), 0, stream>>>(p.rate_parts, drate, B * q.K, D);
+    gated_rate_sum<<<ceil_div(D, 32), dim3(32, 32), 0, stream>>>(p.rate_parts, drate, B * q.nt, D);
     MLSTM_LAUNCH_CHECK();
   }
   return rc;
 }
 
-int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, int B, int S, int D, int scale, int dtype,
-                    cudaStream_t st) {
+int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* scratch, int B, int S, int D, int scale,
+                    int dtype, cudaStream_t st) {
   GatedVoid p{in.x, in.f, in.i, in.z, nullptr, in.rate, in.h0, nullptr, nullptr, y, nullptr, nullptr, nullptr, nullptr, h_last, ckpt, nullptr, nullptr};
-  return gated_call(false, p, strides, nullptr, B, S, D, scale, dtype, nullptr, st);
+  return gated_call(false, p, strides, nullptr, scratch, B, S, D, scale, dtype, nullptr, st);
 }
 
 int launch_gated_bw(const GatedIn& in, const long long* strides, const float* ckpt, const void* dy, const long long* gs, const float* dh_last, void* dx,
-                    void* df, void* di, void* dz, float* drate, float* dh0, float* parts, int B, int S, int D, int scale, int dtype, cudaStream_t st) {
-  GatedVoid p{in.x, in.f, in.i, in.z, dy, in.rate, nullptr, ckpt, dh_last, nullptr, dx, df, di, dz, nullptr, nullptr, dh0, drate != nullptr ? parts : nullptr};
-  return gated_call(true, p, strides, gs, B, S, D, scale, dtype, drate, st);
+                    void* df, void* di, void* dz, float* drate, float* dh0, void* scratch, int B, int S, int D, int scale, int dtype, cudaStream_t st) {
+  GatedVoid p{in.x, in.f, in.i, in.z, dy, in.rate, nullptr, ckpt, dh_last, nullptr, dx, df, di, dz, nullptr, nullptr, dh0, nullptr};
+  return gated_call(true, p, strides, gs, scratch, B, S, D, scale, dtype, drate, st);
 }
 
 int launch_gated_step(const GatedIn& in, const float* h, void* y, float* h_new, int B, int D, int scale, int dtype, cudaStream_t st) {

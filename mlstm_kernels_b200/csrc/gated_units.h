@@ -1,0 +1,51 @@
+// How a gated linear recurrence is cut into units of work (plain numbers: also for the host compiler).
+#pragma once
+#include <algorithm>
+#include <cstddef>
+
+namespace mlstm {
+
+constexpr int GATED_CK = 8;      // tokens to a thread, and to a state that the forward keeps for the backward
+constexpr int GATED_WARPS = 8;   // most warps of a CTA
+constexpr int GATED_GROUP = 16;  // most units of a group
+
+// A unit is `warps` * GATED_CK tokens of 32 V channels of one sequence (a chain).  Units are numbered by time, the chains of one
+// time after one another, and taken in that order.  `group` units of a chain that follow one another take the state in front of their
+// group and join what stands between by themselves.
+struct GatedPlan {
+  int V, blocks, warps, nt, group, groups;   // channels to a lane, units beside each other in D, warps of a CTA, units and groups of a chain
+  long long chains, units;
+};
+inline GatedPlan gated_plan(int B, int S, int D, int V, int slots) {
+  GatedPlan p{};
+  const int runs = (S + GATED_CK - 1) / GATED_CK;
+  p.V = V;
+  p.blocks = (D + 32 * V - 1) / (32 * V);
+  p.nt = (runs + GATED_WARPS - 1) / GATED_WARPS;
+  p.warps = (runs + p.nt - 1) / p.nt;
+  p.chains = (long long)B * p.blocks;
+  p.units = p.chains * p.nt;
+  // As long as a unit's predecessors in its chain are under way beside it, groups are what keeps them from waiting for one another.
+  const long long beside = (slots + p.chains - 1) / p.chains;
+  p.group = 1;
+  while (p.group < GATED_GROUP && p.group < beside * 2 && p.group < p.nt) p.group *= 2;
+  p.groups = (p.nt + p.group - 1) / p.group;
+  return p;
+}
+
+// Scratch: counters and flags that a call zeroes first (none where a chain is one unit), states in front of groups, runs of units,
+// sums of the rate's gradient (backward).  Offsets in bytes.
+struct GatedScratch { size_t zeroed, state, agg, rate, bytes; };
+inline size_t gated_up(size_t n) { return (n + 255) / 256 * 256; }
+inline GatedScratch gated_scratch(const GatedPlan& p, int B, int D, bool backward) {
+  GatedScratch s{};
+  const size_t pairs = 32 * (size_t)((p.V + 1) / 2);   // pairs of channels of a unit
+  if (p.nt > 1) s.zeroed = gated_up(256 + 4 * ((size_t)p.chains * p.groups + (p.group > 1 ? (size_t)p.units : 0)));
+  s.state = s.zeroed;
+  s.agg = s.state + (p.nt > 1 ? gated_up(8 * pairs * (size_t)p.chains * p.groups) : 0);
+  s.rate = s.agg + (p.group > 1 ? gated_up(16 * pairs * (size_t)p.units) : 0);
+  s.bytes = s.rate + (backward ? gated_up(4 * (size_t)B * p.nt * D) : 0);
+  return s;
+}
+
+}  // namespace mlstm

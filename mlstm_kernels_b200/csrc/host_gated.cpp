@@ -48,9 +48,11 @@ Gated gated_forward(const GatedTensors& t_, bool want_last, bool keep) {
   }
   const GatedTensors t = gated_ready(t_);
   if (keep) o.ckpt = bytes(mlstm_b200_gated_checkpoint_bytes(B, S, D), dev);
+  const size_t need = mlstm_b200_gated_workspace_bytes(B, S, D, 0);
+  const Tensor ws = need > 0 ? bytes(need, dev) : Tensor();
   const auto st = gated_strides(t);
   check(mlstm_b200_gated_scan_fw(ptr(t.x), ptr(t.f), ptr(t.i), ptr(t.z), fptr(t.rate), fptr(t.h0), st.data(), o.y.mutable_data_ptr(), fout(o.h_last),
-                                 fout(o.ckpt), B, S, D, t.scale, dtype_code(t.x.scalar_type()), current_stream(dev)),
+                                 fout(o.ckpt), fout(ws), need, B, S, D, t.scale, dtype_code(t.x.scalar_type()), current_stream(dev)),
         "mlstm_b200_gated_scan_fw");
   return o;
 }
@@ -74,8 +76,8 @@ GatedGrads gated_backward(const GatedTensors& t_, const Tensor& ckpt, const Tens
     const Tensor dy = dy_.defined() ? last_dense(to_dtype(dy_, dt)) : zeros(t_.x.sizes(), dt, dev);
     const Tensor dhl = f32c(dh_last_);
     const long long gs[2] = {dy.stride(0), token_stride(dy)};
-    const size_t need = want_rate ? mlstm_b200_gated_bw_workspace_bytes(B, S, D) : 0;
-    const Tensor ws = need > 0 ? bytes(need, dev) : Tensor();
+    const size_t need = mlstm_b200_gated_workspace_bytes(B, S, D, 1);
+    const Tensor ws = bytes(need, dev);
     const auto st = gated_strides(t);
     auto out = [](const Tensor& p) { return p.defined() ? p.mutable_data_ptr() : nullptr; };
     check(mlstm_b200_gated_scan_bw(ptr(t.x), ptr(t.f), ptr(t.i), ptr(t.z), fptr(t.rate), st.data(), fptr(ckpt), ptr(dy), gs, fptr(dhl), out(g.dx),

@@ -126,11 +126,12 @@ struct GatedIn {
 };
 bool gated_sizes_ok(int B, int S, int D);
 size_t gated_ckpt_bytes(int B, int S, int D);
-size_t gated_bw_bytes(int B, int S, int D);
-int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, int B, int S, int D, int scale, int dtype,
-                    cudaStream_t st);
+size_t gated_bytes(int B, int S, int D, bool backward);
+int gated_status(int reset, int* status);   // of its bounded waits
+int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* scratch, int B, int S, int D, int scale,
+                    int dtype, cudaStream_t st);
 int launch_gated_bw(const GatedIn& in, const long long* strides, const float* ckpt, const void* dy, const long long* gs, const float* dh_last, void* dx,
-                    void* df, void* di, void* dz, float* drate, float* dh0, float* parts, int B, int S, int D, int scale, int dtype, cudaStream_t st);
+                    void* df, void* di, void* dz, float* drate, float* dh0, void* scratch, int B, int S, int D, int scale, int dtype, cudaStream_t st);
 int launch_gated_step(const GatedIn& in, const float* h, void* y, float* h_new, int B, int D, int scale, int dtype, cudaStream_t st);
 
 // dropout.cu

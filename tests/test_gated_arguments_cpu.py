@@ -152,16 +152,18 @@ def test_c_abi():
     p = ctypes.c_void_p(1 << 20)   # never read: every call below is refused first
     odd = ctypes.c_void_p((1 << 20) + 4)
     n = None
-    assert lib.mlstm_b200_gated_checkpoint_bytes(0, 1, 8) == lib.mlstm_b200_gated_bw_workspace_bytes(1, 0, 8) == 0
-    fw = lambda S, scale, dt, f=p, ck=n: lib.mlstm_b200_gated_scan_fw(p, f, n, n, n, n, st, p, n, ck, 1, S, 8, scale, dt, n)  # noqa: E731
-    assert fw(0, 0, 1) == -1 and fw(5, 3, 1) == -1 and fw(5, -1, 1) == -1 and fw(5, 0, 7) == -2 and fw(5, 0, 1, n) == -3 and fw(5, 0, 1, p, odd) == -4
-    need = lib.mlstm_b200_gated_bw_workspace_bytes(2, 100, 8)
+    assert lib.mlstm_b200_gated_checkpoint_bytes(0, 1, 8) == lib.mlstm_b200_gated_workspace_bytes(1, 0, 8, 1) == 0
+    need = lib.mlstm_b200_gated_workspace_bytes(1, 500, 8, 0)
+    fw = lambda S=500, scale=0, dt=1, f=p, ck=n, ws=p, size=need: lib.mlstm_b200_gated_scan_fw(p, f, n, n, n, n, st, p, n, ck, ws, size, 1, S, 8, scale, dt, n)  # noqa: E731
+    assert need > 0 and lib.mlstm_b200_gated_workspace_bytes(1, 64, 8, 0) == 0   # one unit of work: nothing to hand on
+    assert fw(0) == -1 and fw(scale=3) == -1 and fw(scale=-1) == -1 and fw(dt=7) == -2 and fw(f=n) == -3 and fw(ck=odd) == -4
+    assert fw(ws=n) == -3 and fw(ws=odd) == -4 and fw(size=need - 1) == -5
+    need = lib.mlstm_b200_gated_workspace_bytes(2, 100, 8, 1)
 
-    def bw(i=n, z=n, rate=n, ck=p, di=n, dz=n, drate=n, ws=n, size=0, dt=1):
+    def bw(i=n, z=n, rate=n, ck=p, di=n, dz=n, drate=n, ws=p, size=need, dt=1):
         return lib.mlstm_b200_gated_scan_bw(p, p, i, z, rate, st, ck, p, st, n, p, p, di, dz, drate, n, ws, size, 2, 100, 8, 1, dt, n)
     assert bw(i=p) == -3 and bw(z=p) == -3 and bw(di=p) == -3 and bw(dz=p) == -3 and bw(ck=n) == -3 and bw(dt=9) == -2 and bw(ck=odd) == -4
-    assert need > 0 and bw(rate=p, drate=p, ws=p, size=need - 1) == -5 and bw(rate=p, drate=p) == -3 and bw(drate=p, ws=p, size=need) == -3
-    assert bw(rate=p, drate=p, ws=odd, size=need) == -4
+    assert need > 0 and bw(size=need - 1) == -5 and bw(ws=n) == -3 and bw(drate=p) == -3 and bw(ws=odd) == -4
     assert lib.mlstm_b200_gated_step(p, p, n, n, n, n, p, p, 1, 8, 0, 1, n) == -3 and lib.mlstm_b200_gated_step(p, p, n, n, n, p, p, p, 0, 8, 0, 1, n) == -1
 
     def drop(n4=(1, 1, 1, 8), prob=0.1, x=p, dt=1, odt=1, res=n, rst=n):
