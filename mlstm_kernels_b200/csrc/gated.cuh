@@ -26,8 +26,9 @@ struct GatedDims {
   Divide chains, blocks;
   long long xb, xt, fb, ft, ib, it, zb, zt, gb, gt;   // strides in elements (batch, token) of x, f, i, z, dy
   // scratch: null where a chain is one unit
-  unsigned *ticket, *gave_up, *state_flag, *agg_flag;
-  void *state, *agg;
+  unsigned *ticket, *gave_up;
+  uint2* state;
+  uint4* agg;
 };
 
 template <typename T> struct GatedPtrs {
@@ -69,6 +70,16 @@ template <typename T> __device__ __forceinline__ void logistic_both(uint64_t v, 
   c = f2(up0 ? q0 : np0, up1 ? q1 : np1);
 }
 
+// The same where it is a gate: s by itself, c = e s, which keeps its digits wherever s is more than zero.  (Exponents end at 127, so
+// that e stays a number; 1 / 2^127 is zero already, and what c is multiplied by then too.)
+template <typename T> __device__ __forceinline__ void logistic_gate(uint64_t v, uint64_t& s, uint64_t& c) {
+  float v0, v1;
+  unf2(v, v0, v1);
+  const uint64_t e = exp_neg_pair<kFull<T>>(max_nan(v0, -88.0296919f), max_nan(v1, -88.0296919f));
+  s = rcp_pair(add2(dup2(1.f), e));
+  c = mul2(e, s);
+}
+
 // of two values of f: a, 1 - a; and with a rate sigmoid(f) and 1 - sigmoid(f).
 // FAR = false: the rate is known to be in (-1/2, 0], and no exponential is needed; BOTH = false: 1 - sigmoid(f) is not needed.
 struct Decay { uint64_t a, rest, sf, cf; };
@@ -80,7 +91,7 @@ template <typename T, bool RATE, bool FAR = true, bool BOTH = true> __device__ _
     d.rest = d.cf;
     return d;
   }
-  if constexpr (BOTH) logistic_both<T>(f, d.sf, d.cf);
+  if constexpr (BOTH) logistic_gate<T>(f, d.sf, d.cf);
   else d.sf = logistic_pair2<T>(f);
   // l = log a = -rho.  Where rho is below 1/2: 1 - e^l = rho p(l), p the polynomial through the values of (e^l - 1) / l at the
   // Chebyshev points of [-1/2, 0], off by 2^-29, in f32 2^-24; else 1 - a has lost one digit at most.
@@ -112,14 +123,6 @@ __device__ __forceinline__ uint64_t inv_scale_pair(uint64_t rest2) {
   float q0, q1;
   unf2(add2(rest2, dup2(1.17549435e-38f)), q0, q1);
   return f2(rsq(q0), rsq(q1));
-}
-// sqrt(1 - a^2) alone
-__device__ __forceinline__ uint64_t scale_pair(uint64_t rest2) {
-  float q0, q1;
-  unf2(rest2, q0, q1);
-  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(q0));
-  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(q1));
-  return f2(q0, q1);
 }
 __device__ __forceinline__ uint64_t rest2_pair(uint64_t a, uint64_t rest) { return fma2(rest, a, rest); }   // 1 - a^2
 

@@ -63,7 +63,7 @@ __global__ void gated_one(const T* x, const T* f, const T* i, const T* z, const 
 }
 
 // ---- calls --------------------------------------------------------------------------------------------
-static int gated_slots() { return 2 * sm_count(); }   // CTAs that run at once
+static int gated_slots() { return 3 * sm_count(); }   // CTAs that run at once
 
 bool gated_sizes_ok(int B, int S, int D) {
   return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && D <= (1 << 30) && gated_plan(B, S, D, 1, gated_slots()).units < (1ll << 31);
@@ -71,7 +71,7 @@ bool gated_sizes_ok(int B, int S, int D) {
 size_t gated_ckpt_bytes(int B, int S, int D) { return (size_t)B * ceil_div(S, GATED_CK) * D * sizeof(float); }
 size_t gated_bytes(int B, int S, int D, bool backward) {
   size_t most = 0;
-  for (const int V : {1, 2, 4}) most = std::max(most, gated_scratch(gated_plan(B, S, D, V, gated_slots()), B, D, backward).bytes);
+  for (const int V : {1, 2}) most = std::max(most, gated_scratch(gated_plan(B, S, D, V, gated_slots()), B, D, backward).bytes);
   return most;
 }
 
@@ -114,7 +114,7 @@ static bool gated_rows(const GatedVoid& p, const long long* st, const long long*
 static int gated_call(bool back, GatedVoid p, const long long* st, const long long* gs, void* scratch, int B, int S, int D, int scale, int dtype, float* drate,
                       cudaStream_t stream) {
   PhaseScope ps(PH_GATED, stream);
-  const int el = (int)dtype_size(dtype), V = !gated_rows(p, st, gs, D, el) ? 1 : back ? 2 : 8 / el;
+  const int el = (int)dtype_size(dtype), V = !gated_rows(p, st, gs, D, el) ? 1 : 2;
   const GatedPlan plan = gated_plan(B, S, D, V, gated_slots());
   const GatedScratch at = gated_scratch(plan, B, D, back);
   unsigned char* const base = static_cast<unsigned char*>(scratch);
@@ -125,11 +125,9 @@ static int gated_call(bool back, GatedVoid p, const long long* st, const long lo
   if (plan.nt > 1) {
     q.ticket = reinterpret_cast<unsigned*>(base);
     q.gave_up = q.ticket + 32;
-    q.state_flag = q.ticket + 64;
-    q.agg_flag = q.state_flag + plan.chains * plan.groups;
-    q.state = base + at.state;
-    q.agg = base + at.agg;
-    MLSTM_CUDA_CHECK(cudaMemsetAsync(base, 0, at.zeroed, stream));
+    q.state = reinterpret_cast<uint2*>(base + at.state);
+    q.agg = reinterpret_cast<uint4*>(base + at.agg);
+    MLSTM_CUDA_CHECK(cudaMemsetAsync(base, 0, at.rate, stream));
   }
   if (drate != nullptr) p.rate_parts = reinterpret_cast<float*>(base + at.rate);
   long long* const to[8] = {&q.xb, &q.xt, &q.fb, &q.ft, &q.ib, &q.it, &q.zb, &q.zt};

@@ -2,15 +2,16 @@
 //
 // A run of tokens acts on the state before it as h -> A h + H (A the product of its factors, H its own end state), and two runs after
 // one another as A2 A1, A2 H1 + H2.  A thread takes GATED_CK tokens of a few channels in registers, the warps of a CTA take runs that
-// follow one another: a unit (gated_units.h).  One pass over the data: every thread reduces its run to (A, H), these are exchanged in
-// shared memory, the unit's first warp finds the state in front of the unit, every thread that in front of its run, and takes its tokens
-// again out of its registers.
+// follow one another: a unit (gated_units.h).  One pass over the data: every thread reduces its run to (A, H), the CTA's last warp, which
+// takes no tokens, works out the state in front of every run, and every thread takes its tokens again out of its registers.
 //
 // Between units the states go through global memory.  CTAs take units in the order of their numbers, by a counter; what a unit waits
 // for has a lower number, so that a CTA that runs has it or has done it: no unit waits for one that is not under way.  A unit
 // publishes its own (A, H) as soon as it has it; the state in front of a group of units is published by the last unit of the group
-// before.  A unit waits for the state in front of its group and joins the runs from there to itself, always in that order: results
-// do not depend on who ran when.  Waits are bounded (gated_wait).
+// before.  A unit joins the runs of its group in front of it, always in that order, and takes the state in front of the group through
+// them: results do not depend on who ran when.  The last warp looks for these while the others work on their tokens.  Its waits are
+// bounded.  A value in global memory says by itself that it is there: the scratch is zero before, and +0 is
+// published as -0, so that neither fences nor flags stand between two CTAs.
 //
 // The backward is the same in the other direction, on a_t (dyh_t + .): the forward has kept the state in front of every run, so that
 // the states are recomputed without an exchange.
@@ -37,6 +38,10 @@ struct GatedAny {
   __device__ bool z() const { return z_; }
 };
 
+#ifndef FWC
+#define FWC 3
+#define BWC 2
+#endif
 constexpr int GL = GATED_CK;
 
 // ---- joining runs -------------------------------------------------------------------------------------
@@ -48,34 +53,33 @@ __device__ __forceinline__ uint64_t through(Run r, uint64_t h) { return fma2(r.A
 // ---- units --------------------------------------------------------------------------------------------
 // Code of the first wait that ran out since it was last asked for (0: none), read by the host
 static __device__ int g_gated_status = 0;
-constexpr unsigned kGatedWaitLimit = 1u << 24;   // polls: some seconds
+constexpr unsigned kGatedWaitLimit = 1u << 24;   // looks at memory: some seconds
 
-__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+__device__ __forceinline__ uint2 look(const uint2* p) {
+  uint2 v;
+  asm volatile("ld.relaxed.gpu.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
   return v;
 }
-// The lanes of a warp wait for a flag each (null: for none).  After kGatedWaitLimit polls, or once another wait of this launch has
-// run out, they go on without: the results are wrong, the status says so, and every CTA ends.
-__device__ __forceinline__ void gated_wait(const unsigned* flag, unsigned* gave_up) {
-  bool there = flag == nullptr;
-#pragma unroll 1
-  for (unsigned n = 0; n < kGatedWaitLimit; ++n) {
-    there = there || load_acquire(flag) != 0;
-    if (__all_sync(0xffffffffu, there)) return;
-    if ((n & 255) == 255 && __any_sync(0xffffffffu, load_acquire(gave_up) != 0)) return;
-    __nanosleep(20);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    atomicExch(gave_up, 1u);
-    atomicCAS(&g_gated_status, 0, 301);
-  }
+__device__ __forceinline__ uint4 look(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
 }
-__device__ __forceinline__ void gated_publish(unsigned* flag) {   // what the warp has written
-  __threadfence();
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
+__device__ __forceinline__ uint2 published(uint64_t v) {
+  uint2 o = make_uint2((unsigned)v, (unsigned)(v >> 32));
+  o.x = o.x == 0 ? 0x80000000u : o.x;
+  o.y = o.y == 0 ? 0x80000000u : o.y;
+  return o;
 }
+__device__ __forceinline__ void publish(uint2* p, uint64_t v) {
+  const uint2 o = published(v);
+  asm volatile("st.relaxed.gpu.global.v2.u32 [%0], {%1, %2};" ::"l"(p), "r"(o.x), "r"(o.y) : "memory");
+}
+__device__ __forceinline__ void publish(uint4* p, Run r) {
+  const uint2 a = published(r.A), h = published(r.H);
+  asm volatile("st.relaxed.gpu.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(h.x), "r"(h.y) : "memory");
+}
+__device__ __forceinline__ uint64_t word(unsigned lo, unsigned hi) { return (uint64_t)hi << 32 | lo; }
 
 struct Unit { int k, chain, b, block; };   // its place in the chain (BACK: from the end), and the chain's
 __device__ __forceinline__ Unit unit_of(int u, const GatedDims& q) {
@@ -87,77 +91,133 @@ __device__ __forceinline__ Unit unit_of(int u, const GatedDims& q) {
   return o;
 }
 
-template <int P> struct alignas(16) GatedShared {
-  Run part[GATED_WARPS][P][32];          // the warps' runs
-  uint64_t start[P][32];                 // the state in front of the unit
-  uint64_t drate[GATED_WARPS][32];       // (backward) sums of the unit before
-  int unit[2];
+// The state in front of a unit, by a whole warp, a pair of channels to a lane: look() until it is there.
+struct GatedFind {
+  const uint4* agg;      // the runs of the group's units
+  const uint2* state;    // the state in front of the group
+  int pos, n;            // runs in front of the unit, and how many of them have been joined
+  bool have;
+  Run front;
+  uint64_t h;
+  // first: the state in front of the unit's chain
+  __device__ __forceinline__ GatedFind(const GatedDims& q, const Unit& u, uint64_t first) : n(0), front(no_tokens()), h(first) {
+    const int lane = threadIdx.x & 31, group = u.k / q.group;
+    pos = u.k - group * q.group;
+    have = group == 0;
+    agg = q.agg + ((long long)u.chain * q.nt + u.k - pos) * 32 + lane;
+    state = q.state + ((long long)u.chain * q.groups + group) * 32 + lane;
+  }
+  __device__ __forceinline__ bool there() const { return have && n == pos; }
+  __device__ __forceinline__ uint64_t value() const { return through(front, h); }
+  __device__ __forceinline__ void look_again() {
+    constexpr int AT_ONCE = 4;
+    uint4 r[AT_ONCE];
+    uint2 s = make_uint2(0, 0);
+    if (!have) s = look(state);
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (n + k < pos) r[k] = look(agg + (n + k) * 32);
+    if (!have && __all_sync(0xffffffffu, s.x != 0 && s.y != 0)) {
+      have = true;
+      h = word(s.x, s.y);
+    }
+    const int end = min(n + AT_ONCE, pos);
+    bool all = true;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      if (!all || n >= end) continue;
+      all = __all_sync(0xffffffffu, r[k].x != 0 && r[k].y != 0 && r[k].z != 0 && r[k].w != 0);
+      if (all) {
+        front = then(front, Run{word(r[k].x, r[k].y), word(r[k].z, r[k].w)});
+        ++n;
+      }
+    }
+  }
 };
-// The next unit: by the counter, or, where no unit waits for another, every gridDim-th
-__device__ __forceinline__ int take_unit(const GatedDims& q, int turn) {
-  return q.ticket != nullptr ? (int)min(atomicAdd(q.ticket, 1u), 0x7fffffffu) : min((long long)blockIdx.x + (long long)turn * gridDim.x, 0x7fffffffll);
+
+struct alignas(16) GatedShared {
+  Run part[GATED_WARPS][32];             // the warps' runs
+  uint64_t start[GATED_WARPS][32];       // the states in front of them
+  uint64_t drate[GATED_WARPS][32];       // (backward) sums of the unit before
+  int unit[2];                           // units to come
+  int runs;                              // how many warps' runs have been there, in all
+};
+// Two barriers between the warps that take tokens and the one that hands the states on: the runs are there; the states are there.
+__device__ __forceinline__ void barrier_arrive(int id) { asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(blockDim.x) : "memory"); }
+__device__ __forceinline__ void barrier_wait(int id) { asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(blockDim.x) : "memory"); }
+constexpr int RUNS_THERE = 1, STATES_THERE = 2;
+// a warp's run is in place; `runs` lets the last warp see, without waiting, that the barrier has all of them
+__device__ __forceinline__ void run_there(GatedShared& sh) {
+  barrier_arrive(RUNS_THERE);
+  if ((threadIdx.x & 31) == 0) atomicAdd(&sh.runs, 1);
 }
 
-// The first warp, behind the barrier behind which all parts are there: finds the state in front of the unit, for all warps, and gives
-// the units after it what they need.  first: the state in front of the chain; returns the state behind the unit.
-template <bool BACK, int P> __device__ __forceinline__ void gated_unit_start(GatedShared<P>& sh, const GatedDims& q, const Unit& u, const uint64_t (&first)[P],
-                                                                               uint64_t (&end)[P]) {
-  const int lane = threadIdx.x & 31, W = blockDim.x >> 5;
-  Run all[P];
-#pragma unroll
-  for (int k = 0; k < P; ++k) all[k] = sh.part[BACK ? W - 1 : 0][k][lane];
-  for (int n = 1; n < W; ++n)
-#pragma unroll
-    for (int k = 0; k < P; ++k) all[k] = then(all[k], sh.part[BACK ? W - 1 - n : n][k][lane]);
-  uint64_t h[P];
-#pragma unroll
-  for (int k = 0; k < P; ++k) h[k] = first[k];
-  if (q.nt > 1) {
-    const int group = u.k / q.group, pos = u.k - group * q.group;
-    const long long in_chain = (long long)u.chain * q.nt + u.k - pos;   // the group's first unit
-    Run* const agg = static_cast<Run*>(q.agg) + in_chain * (P * 32) + lane;
-    uint64_t* const state = static_cast<uint64_t*>(q.state) + ((long long)u.chain * q.groups + group) * (P * 32) + lane;
-    unsigned* const state_flag = q.state_flag + (long long)u.chain * q.groups + group;
-    const bool last = pos == q.group - 1, more = u.k < q.nt - 1;
-    if (more && !last) {
-#pragma unroll
-      for (int k = 0; k < P; ++k) __stcg(reinterpret_cast<ulonglong2*>(agg + (pos * P + k) * 32), make_ulonglong2(all[k].A, all[k].H));
-      gated_publish(q.agg_flag + in_chain + pos);
-    }
-    gated_wait(lane < pos ? q.agg_flag + in_chain + lane : lane == 31 && group > 0 ? state_flag : nullptr, q.gave_up);
-    if (group > 0) {
-#pragma unroll
-      for (int k = 0; k < P; ++k) h[k] = __ldcg(reinterpret_cast<const unsigned long long*>(state + k * 32));
-    }
-#pragma unroll 4
-    for (int n = 0; n < pos; ++n)
-#pragma unroll
-      for (int k = 0; k < P; ++k) {
-        const ulonglong2 r = __ldcg(reinterpret_cast<const ulonglong2*>(agg + (n * P + k) * 32));
-        h[k] = through(Run{r.x, r.y}, h[k]);
-      }
-#pragma unroll
-    for (int k = 0; k < P; ++k) end[k] = through(all[k], h[k]);
-    if (more && last) {
-#pragma unroll
-      for (int k = 0; k < P; ++k) __stcg(reinterpret_cast<unsigned long long*>(state + (P + k) * 32), (unsigned long long)end[k]);
-      gated_publish(state_flag + 1);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < P; ++k) end[k] = through(all[k], h[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < P; ++k) sh.start[k][lane] = h[k];
+// The next unit: by the counter, or, where no unit waits for another, every gridDim-th
+__device__ __forceinline__ int take_unit(const GatedDims& q, int turn) {
+  return q.ticket != nullptr ? (int)min(atomicAdd(q.ticket, 1u), 0x7fffffffu) : (int)min((long long)blockIdx.x + (long long)turn * gridDim.x, 0x7fffffffll);
 }
-// What the warps in front of this one make of the state in front of the unit
-template <bool BACK, int P> __device__ __forceinline__ void gated_front(const GatedShared<P>& sh, Run (&front)[P]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5;
-#pragma unroll
-  for (int k = 0; k < P; ++k) front[k] = no_tokens();
-  for (int n = 0; n < (BACK ? W - 1 - warp : warp); ++n)
-#pragma unroll
-    for (int k = 0; k < P; ++k) front[k] = then(front[k], sh.part[BACK ? W - 1 - n : n][k][lane]);
+
+// What the CTA's last warp does, from the first unit to the last.  first(u): the state in front of a chain; last(u, h): takes that
+// behind it; sums(u): takes the sums of drate of a unit that is done.
+template <bool BACK, class First, class Last, class Sums>
+__device__ __forceinline__ void gated_hand_on(GatedShared& sh, const GatedDims& q, int now, int next, First first, Last last, Sums sums) {
+  const int lane = threadIdx.x & 31, W = (blockDim.x >> 5) - 1;
+  Unit before{};
+  for (int turn = 0; now < q.units; ++turn) {
+    const Unit u = unit_of(now, q);
+    int after = 0;
+    if (lane == 0) after = take_unit(q, turn + 2);
+    const int pos = u.k % q.group;
+    const bool more = u.k < q.nt - 1, ends = pos == q.group - 1;
+    GatedFind find(q, u, u.k < q.group ? first(u) : 0);
+    bool runs = false;
+    unsigned looks = 0;
+#pragma unroll 1
+    do {
+      if (!runs && (find.there() || __any_sync(0xffffffffu, *static_cast<volatile int*>(&sh.runs) == W * (turn + 1)))) {
+        runs = true;
+        barrier_wait(RUNS_THERE);
+        if (turn > 0) sums(before);
+        if (more && !ends) {   // as early as possible: others wait for it
+          Run all = sh.part[BACK ? W - 1 : 0][lane];
+          for (int n = 1; n < W; ++n) all = then(all, sh.part[BACK ? W - 1 - n : n][lane]);
+          publish(q.agg + ((long long)u.chain * q.nt + u.k) * 32 + lane, all);
+        }
+      }
+      if (!find.there()) {
+        find.look_again();
+        // After kGatedWaitLimit looks, or once another wait of this launch has run out, it goes on without: the results are wrong,
+        // the status says so, and every CTA ends.
+        if (++looks % 256 == 0) {
+          unsigned gone;
+          asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(gone) : "l"(q.gave_up) : "memory");
+          if (looks >= kGatedWaitLimit && lane == 0) {
+            atomicExch(q.gave_up, 1u);
+            atomicCAS(&g_gated_status, 0, 301);
+          }
+          if (__any_sync(0xffffffffu, gone != 0 || looks >= kGatedWaitLimit)) find.have = true, find.n = find.pos;
+        }
+      }
+    } while (!runs || !find.there());
+    uint64_t h = find.value();
+    for (int n = 0; n < W; ++n) {
+      const int w = BACK ? W - 1 - n : n;
+      sh.start[w][lane] = h;
+      h = through(sh.part[w][lane], h);
+    }
+    if (lane == 0) sh.unit[turn & 1] = after;
+    __syncwarp();
+    barrier_arrive(STATES_THERE);
+    if (more && ends) publish(q.state + ((long long)u.chain * q.groups + u.k / q.group + 1) * 32 + lane, h);
+    if (!more) last(u, h);
+    before = u;
+    now = next;
+    next = __shfl_sync(0xffffffffu, after, 0);
+    if (BACK && now >= q.units) {   // the last unit's sums
+      barrier_wait(RUNS_THERE);
+      sums(before);
+    }
+  }
 }
 
 // FAR: the rate may be outside (-1/2, 0]
@@ -178,7 +238,10 @@ template <typename T, bool FAR, class M> __device__ __forceinline__ Run gated_to
   uint64_t u = x;
   if (m.i()) u = mul2(u, logistic_pair2<T>(i));
   if (m.scale() == GATED_CONVEX) u = mul2(u, d.rest);
-  if (m.scale() == GATED_VARIANCE) u = mul2(u, scale_pair(rest2_pair(d.a, d.rest)));
+  if (m.scale() == GATED_VARIANCE) {
+    const uint64_t q2 = rest2_pair(d.a, d.rest);
+    u = mul2(mul2(u, q2), inv_scale_pair(q2));
+  }
   return Run{d.a, u};
 }
 // Backward: its factor, what comes in from above, and what dx and di have per unit of G, df and drate per unit of a G
@@ -192,7 +255,7 @@ __device__ __forceinline__ GatedBack gated_token_bw(const M& m, uint64_t f, uint
   uint64_t gx = x, cg = 0, w = h, u;
   t.dx = dup2(1.f);
   if (m.i()) {
-    logistic_both<T>(i, t.dx, cg);
+    logistic_gate<T>(i, t.dx, cg);
     gx = mul2(t.dx, gx);
   }
   u = gx;
@@ -219,7 +282,7 @@ __device__ __forceinline__ GatedBack gated_token_bw(const M& m, uint64_t f, uint
   t.up = dy;
   if (m.z()) {
     uint64_t s, c;
-    logistic_both<T>(z, s, c);
+    logistic_gate<T>(z, s, c);
     dz = mul2(mul2(dy, h), mul2(s, fma2(z, c, dup2(1.f))));
     t.up = mul2(dy, mul2(z, s));
   }
@@ -227,16 +290,16 @@ __device__ __forceinline__ GatedBack gated_token_bw(const M& m, uint64_t f, uint
 }
 
 // ---- channels in rows of 16 bytes ----------------------------------------------------------------------
-// The operands come by asynchronous copies, a tile ahead: each warp copies its own rows (of its 32 lanes' V channels), so that only it
-// waits for them.  Rows behind the sequence and channels behind the last are zeros.
+// The operands come by asynchronous copies, a tile ahead: each warp copies its own rows of 64 channels, so that only it waits for
+// them.  Rows behind the sequence and channels behind the last are zeros.
 constexpr int GATED_STAGES = 2;
-template <typename T, int V> struct GatedRows {
-  static constexpr int CH = 32 * V, BYTES = CH * (int)sizeof(T), CHUNKS = BYTES / 16, PER = 32 / CHUNKS, E = 16 / (int)sizeof(T);
-  static_assert(CHUNKS <= 32 && GL % PER == 0, "");
-  int row, col;   // of this lane's first chunk, and its channel
+template <typename T> struct GatedRows {
+  static constexpr int CH = 64, CHUNKS = CH * (int)sizeof(T) / 16, PER = 32 / CHUNKS, E = 16 / (int)sizeof(T);   // copies of a row, rows of one instruction
+  static_assert(GL % PER == 0, "");
+  int row, col;   // of this lane's first copy, and its channel
   bool ok;
   __device__ GatedRows(int first, int D) : row((threadIdx.x & 31) / CHUNKS), col(((threadIdx.x & 31) % CHUNKS) * E), ok(first + col < D) {}
-  // x: this sequence, at the warp's first channel; tokens t0 ... t0 + 7 to dst[8][CH]
+  // x: this sequence, at the first channel; tokens t0 ... t0 + 7 to dst[8][CH]
   __device__ __forceinline__ void copy(T* dst, const T* x, long long stride, int t0, int S) const {
     const T* src = x + (ok ? col : 0);
 #pragma unroll
@@ -247,30 +310,41 @@ template <typename T, int V> struct GatedRows {
     }
   }
 };
-template <typename T, int V> __device__ __forceinline__ void get_pairs(const T* p, uint64_t (&o)[V / 2]) {
-  const Pack<T, V> v = load_pack<T, V>(p);
-#pragma unroll
-  for (int k = 0; k < V / 2; ++k) o[k] = f2(to_f32(v.e[2 * k]), to_f32(v.e[2 * k + 1]));
+template <typename T> __device__ __forceinline__ uint64_t get_pair(const T* p) {
+  const Pack<T, 2> v = load_pack<T, 2>(p);
+  return f2(to_f32(v.e[0]), to_f32(v.e[1]));
 }
-template <typename T, int V> __device__ __forceinline__ void put_pairs(T* p, const uint64_t (&v)[V / 2]) {
-  float o[V];
-#pragma unroll
-  for (int k = 0; k < V / 2; ++k) unf2(v[k], o[2 * k], o[2 * k + 1]);
-  store_pack(p, pack<T, V>(o));
+template <typename T> __device__ __forceinline__ void put_pair(T* p, uint64_t v) {
+  float o[2];
+  unf2(v, o[0], o[1]);
+  store_pack(p, pack<T, 2>(o));
 }
 
-template <typename T, int V, class M> __global__ void __launch_bounds__(32 * GATED_WARPS, 2) gated_fw_rows(GatedPtrs<T> p, GatedDims q, M m) {
-  constexpr int P = V / 2, CH = 32 * V, NT = 2 + M::i() + M::z(), ROWS = GL * CH;
+template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), FWC) gated_fw_rows(GatedPtrs<T> p, GatedDims q, M m) {
+  constexpr int CH = 64, NT = 2 + M::i() + M::z(), ROWS = GL * CH;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
-  GatedShared<P>& sh = *reinterpret_cast<GatedShared<P>*>(shared_bytes);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, tile = W * GL;
-  T* const tiles = reinterpret_cast<T*>(shared_bytes + sizeof(GatedShared<P>)) + warp * (GATED_STAGES * NT * ROWS);   // this warp's [stage][tensor][8][CH]
+  GatedShared& sh = *reinterpret_cast<GatedShared*>(shared_bytes);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
+  __syncthreads();
+  int now = sh.unit[0], next = sh.unit[1];
+  __syncthreads();   // (they have been read)
+  if (warp == W) {
+    gated_hand_on<false>(
+        sh, q, now, next, [&](const Unit& u) { return p.h0 != nullptr && u.block * CH + 2 * lane < q.D ? get_pair(p.h0 + (long long)u.b * q.D + u.block * CH + 2 * lane) : 0; },
+        [&](const Unit& u, uint64_t h) {
+          if (p.h_last != nullptr && u.block * CH + 2 * lane < q.D) put_pair(p.h_last + (long long)u.b * q.D + u.block * CH + 2 * lane, h);
+        },
+        [](const Unit&) {});
+    return;
+  }
+  T* const tiles = reinterpret_cast<T*>(shared_bytes + sizeof(GatedShared)) + warp * (GATED_STAGES * NT * ROWS);   // this warp's [stage][tensor][8][CH]
   auto fetch = [&](int unit, int stage) {
     if (unit < q.units) {
       const Unit u = unit_of(unit, q);
       T* const dst = tiles + stage * (NT * ROWS);
       const int t0 = u.k * tile + warp * GL, first = u.block * CH;
-      const GatedRows<T, V> rows(first, q.D);
+      const GatedRows<T> rows(first, q.D);
       rows.copy(dst, p.f + u.b * q.fb + first, q.ft, t0, q.S);
       rows.copy(dst + ROWS, p.x + u.b * q.xb + first, q.xt, t0, q.S);
       if (m.i()) rows.copy(dst + 2 * ROWS, p.i + u.b * q.ib + first, q.it, t0, q.S);
@@ -278,89 +352,52 @@ template <typename T, int V, class M> __global__ void __launch_bounds__(32 * GAT
     }
     cp_commit();
   };
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int s = 0; s < GATED_STAGES; ++s) sh.unit[s] = take_unit(q, s);
-  }
-  __syncthreads();
-  int now = sh.unit[0], next = sh.unit[1];
   fetch(now, 0);
   fetch(next, 1);
-  __syncthreads();   // the numbers have been read
   for (int turn = 0; now < q.units; ++turn) {
     const Unit u = unit_of(now, q);
-    const int t0 = u.k * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * V, stage = turn % GATED_STAGES;
+    const int t0 = u.k * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * 2, stage = turn % GATED_STAGES;
     const bool ok = ch < q.D;
-    const T* const mine_x = tiles + stage * (NT * ROWS) + lane * V;
-    int after = 0;
-    if (threadIdx.x == 0) after = take_unit(q, turn + GATED_STAGES);
-    uint64_t rate[P] = {}, first[P] = {};
-    if (ok && m.rate()) get_pairs<float, V>(p.rate + ch, rate);
-    if (ok && warp == 0 && u.k < q.group && p.h0 != nullptr) get_pairs<float, V>(p.h0 + (long long)u.b * q.D + ch, first);
-    bool far = false;
-    if (m.rate()) {
-#pragma unroll
-      for (int k = 0; k < P; ++k) far = far || far_rate(rate[k]);
-      far = __any_sync(0xffffffffu, far);
-    }
-    Run r[GL][P];
+    const T* const mine_x = tiles + stage * (NT * ROWS) + lane * 2;
+    const uint64_t rate = ok && m.rate() ? get_pair(p.rate + ch) : 0;
+    const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate));
+    Run r[GL];
     cp_wait<GATED_STAGES - 1>();
     __syncwarp();
     auto tokens = [&](auto far_) {
 #pragma unroll
-      for (int j = 0; j < GL; ++j) {
-        uint64_t f[P], x[P], i[P] = {};
-        get_pairs<T, V>(mine_x + j * CH, f);
-        get_pairs<T, V>(mine_x + ROWS + j * CH, x);
-        if (m.i()) get_pairs<T, V>(mine_x + 2 * ROWS + j * CH, i);
-#pragma unroll
-        for (int k = 0; k < P; ++k) r[j][k] = gated_token<T, decltype(far_)::value>(m, f[k], x[k], i[k], rate[k]);
-      }
+      for (int j = 0; j < GL; ++j)
+        r[j] = gated_token<T, decltype(far_)::value>(m, get_pair(mine_x + j * CH), get_pair(mine_x + ROWS + j * CH),
+                                                     m.i() ? get_pair(mine_x + 2 * ROWS + j * CH) : 0, rate);
     };
-    if (m.rate() && far) tokens(std::true_type{});
+    if (far) tokens(std::true_type{});
     else tokens(std::false_type{});
     if (n < GL) {   // tokens behind the last leave the state as it is
 #pragma unroll
       for (int j = 0; j < GL; ++j)
-#pragma unroll
-        for (int k = 0; k < P; ++k)
-          if (j >= n) r[j][k] = no_tokens();
+        if (j >= n) r[j] = no_tokens();
     }
+    Run mine = r[0];
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      Run mine = r[0][k];
-#pragma unroll
-      for (int j = 1; j < GL; ++j) mine = then(mine, r[j][k]);
-      sh.part[warp][k][lane] = mine;
-    }
-    if (threadIdx.x == 0) sh.unit[stage] = after;
-    __syncthreads();
-    after = sh.unit[stage];
-    Run front[P];
-    gated_front<false, P>(sh, front);
-    if (warp == 0) {
-      uint64_t end[P];
-      gated_unit_start<false, P>(sh, q, u, first, end);
-      if (p.h_last != nullptr && u.k == q.nt - 1 && ok) put_pairs<float, V>(p.h_last + (long long)u.b * q.D + ch, end);
-    }
-    if (!m.z()) fetch(after, stage);   // (this warp has read its rows)
-    __syncthreads();
+    for (int j = 1; j < GL; ++j) mine = then(mine, r[j]);
+    sh.part[warp][lane] = mine;
+    run_there(sh);
+    barrier_wait(STATES_THERE);
+    const int after = sh.unit[stage];
+    if (!m.z()) fetch(after, stage);
+    uint64_t h = sh.start[warp][lane];
     if (n > 0) {
-      uint64_t h[P];
-#pragma unroll
-      for (int k = 0; k < P; ++k) h[k] = through(front[k], sh.start[k][lane]);
-      if (p.ckpt != nullptr && ok) put_pairs<float, V>(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
+      if (p.ckpt != nullptr && ok) put_pair(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
       T* py = p.y + ((long long)u.b * q.S + t0) * q.D + ch;
 #pragma unroll
       for (int j = 0; j < GL; ++j) {
-        uint64_t o[P], z[P] = {};
-        if (m.z()) get_pairs<T, V>(mine_x + (NT - 1) * ROWS + j * CH, z);
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-          h[k] = through(r[j][k], h[k]);
-          o[k] = m.z() ? mul2(h[k], mul2(z[k], logistic_pair2<T>(z[k]))) : h[k];
+        h = through(r[j], h);
+        uint64_t o = h;
+        if (m.z()) {
+          const uint64_t z = get_pair(mine_x + (NT - 1) * ROWS + j * CH);
+          o = mul2(h, mul2(z, logistic_pair2<T>(z)));
         }
-        if (ok && j < n) put_pairs<T, V>(py, o);
+        if (ok && j < n) put_pair(py, o);
         py += q.D;
       }
     }
@@ -373,25 +410,37 @@ template <typename T, int V, class M> __global__ void __launch_bounds__(32 * GAT
   }
 }
 
-// Sums of drate over a unit's warps, in order, by its last warp
-__device__ __forceinline__ uint64_t gated_rate_of(const uint64_t (&sums)[GATED_WARPS][32]) {
-  uint64_t s = sums[0][threadIdx.x & 31];
-  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) s = add2(s, sums[w][threadIdx.x & 31]);
-  return s;
-}
-
-template <typename T, class M> __global__ void __launch_bounds__(32 * GATED_WARPS, 2) gated_bw_rows(GatedPtrs<T> p, GatedDims q, M m) {
-  constexpr int V = 2, CH = 32 * V, NT = 3 + M::i() + M::z(), ROWS = GL * CH;
+template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), BWC) gated_bw_rows(GatedPtrs<T> p, GatedDims q, M m) {
+  constexpr int CH = 64, NT = 3 + M::i() + M::z(), ROWS = GL * CH;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
-  GatedShared<1>& sh = *reinterpret_cast<GatedShared<1>*>(shared_bytes);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, tile = W * GL;
-  T* const tiles = reinterpret_cast<T*>(shared_bytes + sizeof(GatedShared<1>)) + warp * (GATED_STAGES * NT * ROWS);
+  GatedShared& sh = *reinterpret_cast<GatedShared*>(shared_bytes);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
+  __syncthreads();
+  int now = sh.unit[0], next = sh.unit[1];
+  __syncthreads();
+  if (warp == W) {
+    gated_hand_on<true>(
+        sh, q, now, next,
+        [&](const Unit& u) { return p.dh_last != nullptr && u.block * CH + 2 * lane < q.D ? get_pair(p.dh_last + (long long)u.b * q.D + u.block * CH + 2 * lane) : 0; },
+        [&](const Unit& u, uint64_t h) {
+          if (p.dh0 != nullptr && u.block * CH + 2 * lane < q.D) put_pair(p.dh0 + (long long)u.b * q.D + u.block * CH + 2 * lane, h);
+        },
+        [&](const Unit& u) {
+          if (!m.rate() || p.rate_parts == nullptr) return;
+          uint64_t s = sh.drate[0][lane];   // over the warps, in order
+          for (int w = 1; w < W; ++w) s = add2(s, sh.drate[w][lane]);
+          if (u.block * CH + 2 * lane < q.D) put_pair(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + u.block * CH + 2 * lane, s);
+        });
+    return;
+  }
+  T* const tiles = reinterpret_cast<T*>(shared_bytes + sizeof(GatedShared)) + warp * (GATED_STAGES * NT * ROWS);
   auto fetch = [&](int unit, int stage) {
     if (unit < q.units) {
       const Unit u = unit_of(unit, q);
       T* const dst = tiles + stage * (NT * ROWS);
       const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, first = u.block * CH;   // the last tokens first
-      const GatedRows<T, V> rows(first, q.D);
+      const GatedRows<T> rows(first, q.D);
       rows.copy(dst, p.f + u.b * q.fb + first, q.ft, t0, q.S);
       rows.copy(dst + ROWS, p.x + u.b * q.xb + first, q.xt, t0, q.S);
       rows.copy(dst + 2 * ROWS, p.dy + u.b * q.gb + first, q.gt, t0, q.S);
@@ -401,51 +450,33 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * GATED_WARP
     cp_commit();
   };
   auto state = [&](int unit) {   // in front of this thread's run
-    uint64_t h[1] = {0};
-    if (unit < q.units) {
-      const Unit u = unit_of(unit, q);
-      const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, ch = u.block * CH + lane * V;
-      if (t0 < q.S && ch < q.D) get_pairs<float, 2>(p.ckpt_in + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
-    }
-    return h[0];
+    if (unit >= q.units) return (uint64_t)0;
+    const Unit u = unit_of(unit, q);
+    const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, ch = u.block * CH + lane * 2;
+    return t0 < q.S && ch < q.D ? get_pair(p.ckpt_in + ((long long)u.b * q.nc + t0 / GL) * q.D + ch) : (uint64_t)0;
   };
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int s = 0; s < GATED_STAGES; ++s) sh.unit[s] = take_unit(q, s);
-  }
-  __syncthreads();
-  int now = sh.unit[0], next = sh.unit[1];
   fetch(now, 0);
   fetch(next, 1);
   uint64_t h_next = state(now);
-  float* rate_to = nullptr;   // where the sums of the unit before go
-  __syncthreads();
   for (int turn = 0; now < q.units; ++turn) {
     const Unit u = unit_of(now, q);
-    const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * V, stage = turn % GATED_STAGES;
+    const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * 2, stage = turn % GATED_STAGES;
     const bool ok = ch < q.D;
-    const T* const mine_x = tiles + stage * (NT * ROWS) + lane * V;
+    const T* const mine_x = tiles + stage * (NT * ROWS) + lane * 2;
     const long long at = ((long long)u.b * q.S + t0) * q.D + ch;
-    int after = 0;
-    if (threadIdx.x == 0) after = take_unit(q, turn + GATED_STAGES);
-    uint64_t rate[1] = {0}, first[1] = {0}, drate = 0, h = h_next;
-    if (ok && m.rate()) get_pairs<float, 2>(p.rate + ch, rate);
-    if (ok && warp == 0 && u.k < q.group && p.dh_last != nullptr) get_pairs<float, 2>(p.dh_last + (long long)u.b * q.D + ch, first);
-    const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate[0]));
+    const uint64_t rate = ok && m.rate() ? get_pair(p.rate + ch) : 0;
+    const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate));
+    uint64_t h = h_next;
     GatedBack k[GL];
     cp_wait<GATED_STAGES - 1>();
     __syncwarp();
     auto tokens = [&](auto far_) {
 #pragma unroll
       for (int j = 0; j < GL; ++j) {
-        auto get = [&](int tensor) {
-          uint64_t v[1];
-          get_pairs<T, 2>(mine_x + tensor * ROWS + j * CH, v);
-          return v[0];
-        };
-        uint64_t dz[1];
-        k[j] = gated_token_bw<T, decltype(far_)::value>(m, get(0), get(1), m.i() ? get(3) : 0, m.z() ? get(NT - 1) : 0, get(2), rate[0], h, dz[0]);
-        if (m.z() && ok && j < n) put_pairs<T, 2>(p.dz + at + (long long)j * q.D, dz);
+        auto get = [&](int tensor) { return get_pair(mine_x + tensor * ROWS + j * CH); };
+        uint64_t dz;
+        k[j] = gated_token_bw<T, decltype(far_)::value>(m, get(0), get(1), m.i() ? get(3) : 0, m.z() ? get(NT - 1) : 0, get(2), rate, h, dz);
+        if (m.z() && ok && j < n) put_pair(p.dz + at + (long long)j * q.D, dz);
       }
     };
     if (far) tokens(std::true_type{});
@@ -458,51 +489,27 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * GATED_WARP
     Run mine = no_tokens();
 #pragma unroll
     for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(k[j].a, mine.A), mul2(k[j].a, add2(k[j].up, mine.H))};
-    sh.part[warp][0][lane] = mine;
-    if (threadIdx.x == 0) sh.unit[stage] = after;
-    __syncthreads();
-    after = sh.unit[stage];
+    sh.part[warp][lane] = mine;
+    run_there(sh);
     h_next = state(next);
-    Run front[1];
-    gated_front<true, 1>(sh, front);
-    if (warp == 0) {
-      uint64_t end[1];
-      gated_unit_start<true, 1>(sh, q, u, first, end);
-      if (p.dh0 != nullptr && u.k == q.nt - 1 && ok) put_pairs<float, 2>(p.dh0 + (long long)u.b * q.D + ch, end);
-    }
-    if (m.rate() && warp == W - 1 && rate_to != nullptr) {
-      const uint64_t o[1] = {gated_rate_of(sh.drate)};
-      put_pairs<float, 2>(rate_to, o);
-    }
+    barrier_wait(STATES_THERE);
+    const int after = sh.unit[stage];
     fetch(after, stage);
-    __syncthreads();
-    if (n > 0) {
-      uint64_t c = through(front[0], sh.start[0][lane]);
+    uint64_t c = sh.start[warp][lane], drate = 0;
 #pragma unroll
-      for (int j = GL - 1; j >= 0; --j) {
-        const uint64_t G = add2(k[j].up, c);
-        c = mul2(k[j].a, G);
-        if (j >= n) continue;
-        if (m.rate()) drate = fma2(c, k[j].drate, drate);
-        const uint64_t dx[1] = {mul2(G, k[j].dx)}, df[1] = {mul2(c, k[j].df)}, di[1] = {mul2(G, k[j].di)};
-        if (ok) put_pairs<T, 2>(p.dx + at + (long long)j * q.D, dx);
-        if (ok) put_pairs<T, 2>(p.df + at + (long long)j * q.D, df);
-        if (m.i() && ok) put_pairs<T, 2>(p.di + at + (long long)j * q.D, di);
-      }
+    for (int j = GL - 1; j >= 0; --j) {
+      const uint64_t G = add2(k[j].up, c);
+      c = mul2(k[j].a, G);
+      if (j >= n) continue;
+      if (m.rate()) drate = fma2(c, k[j].drate, drate);
+      if (ok) put_pair(p.dx + at + (long long)j * q.D, mul2(G, k[j].dx));
+      if (ok) put_pair(p.df + at + (long long)j * q.D, mul2(c, k[j].df));
+      if (m.i() && ok) put_pair(p.di + at + (long long)j * q.D, mul2(G, k[j].di));
     }
-    if (m.rate()) {
-      sh.drate[warp][lane] = drate;
-      rate_to = p.rate_parts != nullptr && ok ? p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + ch : nullptr;
-    }
+    if (m.rate()) sh.drate[warp][lane] = drate;
     now = next;
     next = after;
-  }
-  if (m.rate()) {
-    __syncthreads();
-    if (warp == W - 1 && rate_to != nullptr) {
-      const uint64_t o[1] = {gated_rate_of(sh.drate)};
-      put_pairs<float, 2>(rate_to, o);
-    }
+    if (now >= q.units) barrier_arrive(RUNS_THERE);   // the last unit's sums
   }
 }
 
@@ -514,18 +521,27 @@ template <typename T> __device__ __forceinline__ void put_one(T* p, uint64_t v) 
   *p = from_f32<T>(lo);
 }
 
-template <typename T> __global__ void __launch_bounds__(32 * GATED_WARPS, 2) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
-  __shared__ GatedShared<1> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tile = (blockDim.x >> 5) * GL;
-  for (int turn = 0;; ++turn) {
-    if (threadIdx.x == 0) sh.unit[0] = take_unit(q, turn);
-    __syncthreads();
-    const int unit = sh.unit[0];
-    if (unit >= q.units) return;
-    const Unit u = unit_of(unit, q);
+template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 2) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
+  __shared__ GatedShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
+  __syncthreads();
+  int now = sh.unit[0], next = sh.unit[1];
+  __syncthreads();
+  if (warp == W) {
+    gated_hand_on<false>(
+        sh, q, now, next, [&](const Unit& u) { return p.h0 != nullptr && u.block * 32 + lane < q.D ? one(p.h0 + (long long)u.b * q.D + u.block * 32 + lane) : 0; },
+        [&](const Unit& u, uint64_t h) {
+          if (p.h_last != nullptr && u.block * 32 + lane < q.D) put_one(p.h_last + (long long)u.b * q.D + u.block * 32 + lane, h);
+        },
+        [](const Unit&) {});
+    return;
+  }
+  for (int turn = 0; now < q.units; ++turn) {
+    const Unit u = unit_of(now, q);
     const int t0 = u.k * tile + warp * GL, n = q.S - t0, own = u.block * 32 + lane, ch = min(own, q.D - 1);   // (n: may be none, or more)
     const bool ok = own < q.D;
-    const uint64_t rate = m.rate() ? one(p.rate + ch) : 0, first[1] = {p.h0 != nullptr ? one(p.h0 + (long long)u.b * q.D + ch) : 0};
+    const uint64_t rate = m.rate() ? one(p.rate + ch) : 0;
     Run r[GL], mine = no_tokens();
     T rx[GL], rf[GL], ri[GL];
     const T *px = p.x + u.b * q.xb + t0 * q.xt + ch, *pf = p.f + u.b * q.fb + t0 * q.ft + ch, *pi = m.i() ? p.i + u.b * q.ib + t0 * q.it + ch : nullptr;
@@ -541,19 +557,12 @@ template <typename T> __global__ void __launch_bounds__(32 * GATED_WARPS, 2) gat
       r[j] = j < n ? gated_token<T, true>(m, one(rf + j), one(rx + j), m.i() ? one(ri + j) : 0, rate) : no_tokens();
       mine = then(mine, r[j]);
     }
-    sh.part[warp][0][lane] = mine;
-    __syncthreads();
-    Run front[1];
-    gated_front<false, 1>(sh, front);
-    if (warp == 0) {
-      uint64_t end[1];
-      gated_unit_start<false, 1>(sh, q, u, first, end);
-      if (p.h_last != nullptr && u.k == q.nt - 1 && ok) put_one(p.h_last + (long long)u.b * q.D + ch, end[0]);
-    }
-    __syncthreads();
-    if (n <= 0) continue;
-    uint64_t h = through(front[0], sh.start[0][lane]);
-    if (p.ckpt != nullptr && ok) put_one(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
+    sh.part[warp][lane] = mine;
+    run_there(sh);
+    barrier_wait(STATES_THERE);
+    const int after = sh.unit[turn & 1];
+    uint64_t h = sh.start[warp][lane];
+    if (n > 0 && p.ckpt != nullptr && ok) put_one(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
 #pragma unroll
     for (int j = 0; j < GL; ++j) {
       if (j >= n) break;
@@ -565,23 +574,40 @@ template <typename T> __global__ void __launch_bounds__(32 * GATED_WARPS, 2) gat
       }
       if (ok) put_one(p.y + ((long long)u.b * q.S + t0 + j) * q.D + ch, o);
     }
+    __syncwarp();
+    now = next;
+    next = after;
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(32 * GATED_WARPS) gated_bw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
-  __shared__ GatedShared<1> sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = blockDim.x >> 5, tile = W * GL;
-  for (int turn = 0;; ++turn) {
-    if (threadIdx.x == 0) sh.unit[0] = take_unit(q, turn);
-    __syncthreads();
-    const int unit = sh.unit[0];
-    if (unit >= q.units) return;
-    const Unit u = unit_of(unit, q);
+template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) gated_bw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
+  __shared__ GatedShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
+  __syncthreads();
+  int now = sh.unit[0], next = sh.unit[1];
+  __syncthreads();
+  if (warp == W) {
+    gated_hand_on<true>(
+        sh, q, now, next,
+        [&](const Unit& u) { return p.dh_last != nullptr && u.block * 32 + lane < q.D ? one(p.dh_last + (long long)u.b * q.D + u.block * 32 + lane) : 0; },
+        [&](const Unit& u, uint64_t h) {
+          if (p.dh0 != nullptr && u.block * 32 + lane < q.D) put_one(p.dh0 + (long long)u.b * q.D + u.block * 32 + lane, h);
+        },
+        [&](const Unit& u) {
+          if (p.rate_parts == nullptr) return;
+          uint64_t s = sh.drate[0][lane];
+          for (int w = 1; w < W; ++w) s = add2(s, sh.drate[w][lane]);
+          if (u.block * 32 + lane < q.D) put_one(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + u.block * 32 + lane, s);
+        });
+    return;
+  }
+  for (int turn = 0; now < q.units; ++turn) {
+    const Unit u = unit_of(now, q);
     const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0, own = u.block * 32 + lane, ch = min(own, q.D - 1);
     const bool ok = own < q.D;
-    const uint64_t rate = m.rate() ? one(p.rate + ch) : 0, first[1] = {p.dh_last != nullptr ? one(p.dh_last + (long long)u.b * q.D + ch) : 0};
+    const uint64_t rate = m.rate() ? one(p.rate + ch) : 0;
     const long long at = ((long long)u.b * q.S + t0) * q.D + ch;
-    uint64_t drate = 0;
     GatedBack k[GL];
     T rx[GL], rf[GL], ri[GL], rz[GL], rg[GL];
 #pragma unroll
@@ -605,17 +631,12 @@ template <typename T> __global__ void __launch_bounds__(32 * GATED_WARPS) gated_
     Run mine = no_tokens();
 #pragma unroll
     for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(k[j].a, mine.A), mul2(k[j].a, add2(k[j].up, mine.H))};
-    sh.part[warp][0][lane] = mine;
-    __syncthreads();
-    Run front[1];
-    gated_front<true, 1>(sh, front);
-    if (warp == 0) {
-      uint64_t end[1];
-      gated_unit_start<true, 1>(sh, q, u, first, end);
-      if (p.dh0 != nullptr && u.k == q.nt - 1 && ok) put_one(p.dh0 + (long long)u.b * q.D + ch, end[0]);
-    }
-    __syncthreads();
-    uint64_t c = through(front[0], sh.start[0][lane]);
+    __syncwarp();
+    sh.part[warp][lane] = mine;
+    run_there(sh);
+    barrier_wait(STATES_THERE);
+    const int after = sh.unit[turn & 1];
+    uint64_t c = sh.start[warp][lane], drate = 0;
 #pragma unroll
     for (int j = GL - 1; j >= 0; --j) {
       if (j >= n) continue;
@@ -626,11 +647,11 @@ template <typename T> __global__ void __launch_bounds__(32 * GATED_WARPS) gated_
       if (ok) put_one(p.df + at + (long long)j * q.D, mul2(c, k[j].df));
       if (m.i() && ok) put_one(p.di + at + (long long)j * q.D, mul2(G, k[j].di));
     }
-    if (m.rate() && p.rate_parts != nullptr) {
-      sh.drate[warp][lane] = drate;
-      __syncthreads();
-      if (warp == W - 1 && ok) put_one(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + ch, gated_rate_of(sh.drate));
-    }
+    __syncwarp();
+    if (m.rate()) sh.drate[warp][lane] = drate;
+    now = next;
+    next = after;
+    if (now >= q.units) barrier_arrive(RUNS_THERE);   // the last unit's sums
   }
 }
 
@@ -639,22 +660,20 @@ template <typename T, class M> int gated_launch(void (*kern)(GatedPtrs<T>, Gated
                                                 cudaStream_t st) {
   if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int held = 0;
-  MLSTM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, 32 * q.warps, smem));
+  MLSTM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, 32 * (q.warps + 1), smem));
   const long long grid = std::min((long long)q.units, (long long)std::max(held, 1) * sm_count());
-  kern<<<(unsigned)grid, 32 * q.warps, smem, st>>>(p, q, m);
+  kern<<<(unsigned)grid, 32 * (q.warps + 1), smem, st>>>(p, q, m);
   MLSTM_LAUNCH_CHECK();
   return MLSTM_OK;
 }
 
 template <typename T> int gated_run(bool back, int V, const GatedPtrs<T>& p, const GatedDims& q, cudaStream_t st) {
-  constexpr int FV = 8 / (int)sizeof(T);
   const bool rate = p.rate != nullptr, i = p.i != nullptr, z = p.z != nullptr;
   if (V == 1) return gated_launch<T, GatedAny>(back ? gated_bw_any<T> : gated_fw_any<T>, 0, p, q, GatedAny{rate, i, z, q.scale}, st);
-  const size_t rows = (size_t)q.warps * GATED_STAGES * GL * 32 * sizeof(T) * (2 + back + i + z);
+  const size_t smem = sizeof(GatedShared) + (size_t)q.warps * GATED_STAGES * GL * 64 * sizeof(T) * (2 + back + i + z);
   auto pick = [&](auto r, auto s, auto ii, auto zz) {
     using M = GatedFixed<decltype(r)::value, decltype(s)::value, decltype(ii)::value, decltype(zz)::value>;
-    if (back) return gated_launch<T, M>(gated_bw_rows<T, M>, rows * 2 + sizeof(GatedShared<1>), p, q, M{}, st);
-    return gated_launch<T, M>(gated_fw_rows<T, FV, M>, rows * FV + sizeof(GatedShared<FV / 2>), p, q, M{}, st);
+    return gated_launch<T, M>(back ? gated_bw_rows<T, M> : gated_fw_rows<T, M>, smem, p, q, M{}, st);
   };
   auto with_z = [&](auto r, auto s, auto ii) { return z ? pick(r, s, ii, std::true_type{}) : pick(r, s, ii, std::false_type{}); };
   auto with_i = [&](auto r, auto s) { return i ? with_z(r, s, std::true_type{}) : with_z(r, s, std::false_type{}); };

@@ -6,7 +6,7 @@
 namespace mlstm {
 
 constexpr int GATED_CK = 8;      // tokens to a thread, and to a state that the forward keeps for the backward
-constexpr int GATED_WARPS = 8;   // most warps of a CTA
+constexpr int GATED_WARPS = 7;   // most warps of a CTA that take tokens; one more hands the states on
 constexpr int GATED_GROUP = 16;  // most units of a group
 
 // A unit is `warps` * GATED_CK tokens of 32 V channels of one sequence (a chain).  Units are numbered by time, the chains of one
@@ -33,17 +33,15 @@ inline GatedPlan gated_plan(int B, int S, int D, int V, int slots) {
   return p;
 }
 
-// Scratch: counters and flags that a call zeroes first (none where a chain is one unit), states in front of groups, runs of units,
-// sums of the rate's gradient (backward).  Offsets in bytes.
-struct GatedScratch { size_t zeroed, state, agg, rate, bytes; };
+// Scratch, offsets in bytes: a counter, states in front of groups and runs of units, all of which a call zeroes first (none where a
+// chain is one unit), and sums of the rate's gradient (backward).
+struct GatedScratch { size_t state, agg, rate, bytes; };
 inline size_t gated_up(size_t n) { return (n + 255) / 256 * 256; }
 inline GatedScratch gated_scratch(const GatedPlan& p, int B, int D, bool backward) {
   GatedScratch s{};
-  const size_t pairs = 32 * (size_t)((p.V + 1) / 2);   // pairs of channels of a unit
-  if (p.nt > 1) s.zeroed = gated_up(256 + 4 * ((size_t)p.chains * p.groups + (p.group > 1 ? (size_t)p.units : 0)));
-  s.state = s.zeroed;
-  s.agg = s.state + (p.nt > 1 ? gated_up(8 * pairs * (size_t)p.chains * p.groups) : 0);
-  s.rate = s.agg + (p.group > 1 ? gated_up(16 * pairs * (size_t)p.units) : 0);
+  s.state = p.nt > 1 ? 256 : 0;
+  s.agg = s.state + (p.nt > 1 ? gated_up(32 * 8 * (size_t)p.chains * p.groups) : 0);
+  s.rate = s.agg + (p.group > 1 ? gated_up(32 * 16 * (size_t)p.units) : 0);
   s.bytes = s.rate + (backward ? gated_up(4 * (size_t)B * p.nt * D) : 0);
   return s;
 }

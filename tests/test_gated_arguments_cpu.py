@@ -155,7 +155,7 @@ def test_c_abi():
     assert lib.mlstm_b200_gated_checkpoint_bytes(0, 1, 8) == lib.mlstm_b200_gated_workspace_bytes(1, 0, 8, 1) == 0
     need = lib.mlstm_b200_gated_workspace_bytes(1, 500, 8, 0)
     fw = lambda S=500, scale=0, dt=1, f=p, ck=n, ws=p, size=need: lib.mlstm_b200_gated_scan_fw(p, f, n, n, n, n, st, p, n, ck, ws, size, 1, S, 8, scale, dt, n)  # noqa: E731
-    assert need > 0 and lib.mlstm_b200_gated_workspace_bytes(1, 64, 8, 0) == 0   # one unit of work: nothing to hand on
+    assert need > 0 and lib.mlstm_b200_gated_workspace_bytes(1, 56, 8, 0) == 0   # one unit of work: nothing to hand on
     assert fw(0) == -1 and fw(scale=3) == -1 and fw(scale=-1) == -1 and fw(dt=7) == -2 and fw(f=n) == -3 and fw(ck=odd) == -4
     assert fw(ws=n) == -3 and fw(ws=odd) == -4 and fw(size=need - 1) == -5
     need = lib.mlstm_b200_gated_workspace_bytes(2, 100, 8, 1)
