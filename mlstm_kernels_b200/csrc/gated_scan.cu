@@ -98,18 +98,18 @@ struct GatedVoid {   // as GatedPtrs, of any type
   void *y, *dx, *df, *di, *dz;
   float *h_last, *ckpt, *dh0, *rate_parts;
 };
-// Rows by 16 bytes where all of them begin on such a boundary
+// Rows by 16 bytes where all of them begin on such a boundary, and eight tokens lie within 2^31 bytes
 static bool gated_rows(const GatedVoid& p, const long long* st, const long long* gs, int D, int el) {
   const int e = 16 / el;
-  if (D % e != 0) return false;
+  if (D % e != 0 || D > (1 << 26)) return false;
   for (const void* a : {p.x, p.f, p.i, p.z, p.dy, (const void*)p.y, (const void*)p.dx, (const void*)p.df, (const void*)p.di, (const void*)p.dz,
                         (const void*)p.rate, (const void*)p.h0, (const void*)p.ckpt_in, (const void*)p.dh_last, (const void*)p.h_last, (const void*)p.ckpt,
                         (const void*)p.dh0, (const void*)p.rate_parts})
     if (!fits_access(a, 16)) return false;
   const void* const ins[4] = {p.x, p.f, p.i, p.z};
   for (int k = 0; k < 8; ++k)
-    if (ins[k / 2] != nullptr && st[k] % e != 0) return false;
-  return gs == nullptr || (gs[0] % e == 0 && gs[1] % e == 0);
+    if (ins[k / 2] != nullptr && (st[k] % e != 0 || (k % 2 == 1 && st[k] > (1 << 26)))) return false;
+  return gs == nullptr || (gs[0] % e == 0 && gs[1] % e == 0 && gs[1] <= (1 << 26));
 }
 static int gated_call(bool back, GatedVoid p, const long long* st, const long long* gs, void* scratch, int B, int S, int D, int scale, int dtype, float* drate,
                       cudaStream_t stream) {

@@ -138,7 +138,7 @@ struct GatedFind {
 struct alignas(16) GatedShared {
   Run part[GATED_WARPS][32];             // the warps' runs
   uint64_t start[GATED_WARPS][32];       // the states in front of them
-  uint64_t drate[GATED_WARPS][32];       // (backward) sums of the unit before
+  uint64_t drate[2][GATED_WARPS][32];    // (backward) sums of a unit and the one before
   int unit[2];                           // units to come
   int runs;                              // how many warps' runs have been there, in all
 };
@@ -170,52 +170,54 @@ __device__ __forceinline__ void gated_hand_on(GatedShared& sh, const GatedDims& 
     const int pos = u.k % q.group;
     const bool more = u.k < q.nt - 1, ends = pos == q.group - 1;
     GatedFind find(q, u, u.k < q.group ? first(u) : 0);
-    bool runs = false;
+    auto give_run = [&] {
+      Run all = sh.part[BACK ? W - 1 : 0][lane];
+      for (int n = 1; n < W; ++n) all = then(all, sh.part[BACK ? W - 1 - n : n][lane]);
+      publish(q.agg + ((long long)u.chain * q.nt + u.k) * 32 + lane, all);
+    };
+    bool runs = false, gave = !more || ends;   // its own run is wanted by the units of its group behind it
     unsigned looks = 0;
 #pragma unroll 1
-    do {
-      if (!runs && (find.there() || __any_sync(0xffffffffu, *static_cast<volatile int*>(&sh.runs) == W * (turn + 1)))) {
+    while (!find.there()) {
+      if (!runs && __any_sync(0xffffffffu, *static_cast<volatile int*>(&sh.runs) == W * (turn + 1))) {
         runs = true;
         barrier_wait(RUNS_THERE);
-        if (turn > 0) sums(before);
-        if (more && !ends) {   // as early as possible: others wait for it
-          Run all = sh.part[BACK ? W - 1 : 0][lane];
-          for (int n = 1; n < W; ++n) all = then(all, sh.part[BACK ? W - 1 - n : n][lane]);
-          publish(q.agg + ((long long)u.chain * q.nt + u.k) * 32 + lane, all);
-        }
+        if (!gave) give_run();   // as early as possible, unless the unit can go on itself
+        gave = true;
       }
-      if (!find.there()) {
-        find.look_again();
-        // After kGatedWaitLimit looks, or once another wait of this launch has run out, it goes on without: the results are wrong,
-        // the status says so, and every CTA ends.
-        if (++looks % 256 == 0) {
-          unsigned gone;
-          asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(gone) : "l"(q.gave_up) : "memory");
-          if (looks >= kGatedWaitLimit && lane == 0) {
-            atomicExch(q.gave_up, 1u);
-            atomicCAS(&g_gated_status, 0, 301);
-          }
-          if (__any_sync(0xffffffffu, gone != 0 || looks >= kGatedWaitLimit)) find.have = true, find.n = find.pos;
+      find.look_again();
+      // After kGatedWaitLimit looks, or once another wait of this launch has run out, it goes on without: the results are wrong, the
+      // status says so, and every CTA ends.
+      if (++looks % 256 == 0) {
+        unsigned gone;
+        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(gone) : "l"(q.gave_up) : "memory");
+        if (looks >= kGatedWaitLimit && lane == 0) {
+          atomicExch(q.gave_up, 1u);
+          atomicCAS(&g_gated_status, 0, 301);
         }
+        if (__any_sync(0xffffffffu, gone != 0 || looks >= kGatedWaitLimit)) find.have = true, find.n = find.pos;
       }
-    } while (!runs || !find.there());
+    }
     uint64_t h = find.value();
+    if (!runs) barrier_wait(RUNS_THERE);
     for (int n = 0; n < W; ++n) {
       const int w = BACK ? W - 1 - n : n;
       sh.start[w][lane] = h;
       h = through(sh.part[w][lane], h);
     }
     if (lane == 0) sh.unit[turn & 1] = after;
+    if (!gave) give_run();
     __syncwarp();
     barrier_arrive(STATES_THERE);
     if (more && ends) publish(q.state + ((long long)u.chain * q.groups + u.k / q.group + 1) * 32 + lane, h);
     if (!more) last(u, h);
+    if (BACK && turn > 0) sums(before, (turn - 1) & 1);
     before = u;
     now = next;
     next = __shfl_sync(0xffffffffu, after, 0);
     if (BACK && now >= q.units) {   // the last unit's sums
       barrier_wait(RUNS_THERE);
-      sums(before);
+      sums(before, turn & 1);
     }
   }
 }
@@ -299,17 +301,31 @@ template <typename T> struct GatedRows {
   int row, col;   // of this lane's first copy, and its channel
   bool ok;
   __device__ GatedRows(int first, int D) : row((threadIdx.x & 31) / CHUNKS), col(((threadIdx.x & 31) % CHUNKS) * E), ok(first + col < D) {}
-  // x: this sequence, at the first channel; tokens t0 ... t0 + 7 to dst[8][CH]
-  __device__ __forceinline__ void copy(T* dst, const T* x, long long stride, int t0, int S) const {
-    const T* src = x + (ok ? col : 0);
+  // x: this sequence, at the first channel; tokens t0 ... t0 + 7 to dst[8][CH].  (Eight tokens are less than 2^31 bytes apart.)
+  __device__ __forceinline__ void copy(T* dst, const T* x, long long stride, int t0, int S, bool whole) const {
+    T* const to = dst + row * CH + col;
+    if (whole) {
+      const char* const base = reinterpret_cast<const char*>(x + t0 * stride);
+      const unsigned step = (unsigned)stride * (unsigned)sizeof(T);
+      unsigned at = row * step + col * (unsigned)sizeof(T);
 #pragma unroll
-    for (int k = 0; k < GL; k += PER) {
-      const int t = t0 + k + row;
-      const bool in = ok && t < S;
-      copy_async<T, E>(dst + (k + row) * CH + col, src + (in ? t : 0) * stride, in);
+      for (int k = 0; k < GL; k += PER) {
+        copy_async<T, E>(to + k * CH, reinterpret_cast<const T*>(base + at), true);
+        at += PER * step;
+      }
+    } else {
+      const T* src = x + (ok ? col : 0);
+#pragma unroll
+      for (int k = 0; k < GL; k += PER) {
+        const int t = t0 + k + row;
+        const bool in = ok && t < S;
+        copy_async<T, E>(to + k * CH, src + (in ? t : 0) * stride, in);
+      }
     }
   }
 };
+// a value that is the same in the whole warp, which the compiler then knows
+__device__ __forceinline__ int same(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 template <typename T> __device__ __forceinline__ uint64_t get_pair(const T* p) {
   const Pack<T, 2> v = load_pack<T, 2>(p);
   return f2(to_f32(v.e[0]), to_f32(v.e[1]));
@@ -319,15 +335,16 @@ template <typename T> __device__ __forceinline__ void put_pair(T* p, uint64_t v)
   unf2(v, o[0], o[1]);
   store_pack(p, pack<T, 2>(o));
 }
+template <typename T> __device__ __forceinline__ void put_pair(T* row, unsigned at, uint64_t v) { put_pair(reinterpret_cast<T*>(reinterpret_cast<char*>(row) + at), v); }
 
 template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), FWC) gated_fw_rows(GatedPtrs<T> p, GatedDims q, M m) {
   constexpr int CH = 64, NT = 2 + M::i() + M::z(), ROWS = GL * CH;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   GatedShared& sh = *reinterpret_cast<GatedShared*>(shared_bytes);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
   __syncthreads();
-  int now = sh.unit[0], next = sh.unit[1];
+  int now = same(sh.unit[0]), next = same(sh.unit[1]);
   __syncthreads();   // (they have been read)
   if (warp == W) {
     gated_hand_on<false>(
@@ -335,7 +352,7 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
         [&](const Unit& u, uint64_t h) {
           if (p.h_last != nullptr && u.block * CH + 2 * lane < q.D) put_pair(p.h_last + (long long)u.b * q.D + u.block * CH + 2 * lane, h);
         },
-        [](const Unit&) {});
+        [](const Unit&, int) {});
     return;
   }
   T* const tiles = reinterpret_cast<T*>(shared_bytes + sizeof(GatedShared)) + warp * (GATED_STAGES * NT * ROWS);   // this warp's [stage][tensor][8][CH]
@@ -345,10 +362,11 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
       T* const dst = tiles + stage * (NT * ROWS);
       const int t0 = u.k * tile + warp * GL, first = u.block * CH;
       const GatedRows<T> rows(first, q.D);
-      rows.copy(dst, p.f + u.b * q.fb + first, q.ft, t0, q.S);
-      rows.copy(dst + ROWS, p.x + u.b * q.xb + first, q.xt, t0, q.S);
-      if (m.i()) rows.copy(dst + 2 * ROWS, p.i + u.b * q.ib + first, q.it, t0, q.S);
-      if (m.z()) rows.copy(dst + (NT - 1) * ROWS, p.z + u.b * q.zb + first, q.zt, t0, q.S);
+      const bool whole = t0 + GL <= q.S && first + CH <= q.D;
+      rows.copy(dst, p.f + u.b * q.fb + first, q.ft, t0, q.S, whole);
+      rows.copy(dst + ROWS, p.x + u.b * q.xb + first, q.xt, t0, q.S, whole);
+      if (m.i()) rows.copy(dst + 2 * ROWS, p.i + u.b * q.ib + first, q.it, t0, q.S, whole);
+      if (m.z()) rows.copy(dst + (NT - 1) * ROWS, p.z + u.b * q.zb + first, q.zt, t0, q.S, whole);
     }
     cp_commit();
   };
@@ -383,23 +401,30 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
     sh.part[warp][lane] = mine;
     run_there(sh);
     barrier_wait(STATES_THERE);
-    const int after = sh.unit[stage];
+    const int after = same(sh.unit[stage]);
     if (!m.z()) fetch(after, stage);
     uint64_t h = sh.start[warp][lane];
-    if (n > 0) {
-      if (p.ckpt != nullptr && ok) put_pair(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
-      T* py = p.y + ((long long)u.b * q.S + t0) * q.D + ch;
+    auto finish = [&](auto whole) {
+      T* const y = p.y + ((long long)u.b * q.S + t0) * q.D + u.block * CH;
+      const unsigned step = (unsigned)q.D * (unsigned)sizeof(T);
+      unsigned to = lane * 2 * (unsigned)sizeof(T);
 #pragma unroll
       for (int j = 0; j < GL; ++j) {
+        if (!decltype(whole)::value && j >= n) break;
         h = through(r[j], h);
         uint64_t o = h;
         if (m.z()) {
           const uint64_t z = get_pair(mine_x + (NT - 1) * ROWS + j * CH);
           o = mul2(h, mul2(z, logistic_pair2<T>(z)));
         }
-        if (ok && j < n) put_pair(py, o);
-        py += q.D;
+        put_pair(y, to, o);
+        to += step;
       }
+    };
+    if (ok && n > 0) {
+      if (p.ckpt != nullptr) put_pair(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + u.block * CH, lane * 8, h);
+      if (n >= GL) finish(std::true_type{});
+      else finish(std::false_type{});
     }
     if (m.z()) {
       __syncwarp();
@@ -414,10 +439,10 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
   constexpr int CH = 64, NT = 3 + M::i() + M::z(), ROWS = GL * CH;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   GatedShared& sh = *reinterpret_cast<GatedShared*>(shared_bytes);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
   __syncthreads();
-  int now = sh.unit[0], next = sh.unit[1];
+  int now = same(sh.unit[0]), next = same(sh.unit[1]);
   __syncthreads();
   if (warp == W) {
     gated_hand_on<true>(
@@ -426,10 +451,10 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
         [&](const Unit& u, uint64_t h) {
           if (p.dh0 != nullptr && u.block * CH + 2 * lane < q.D) put_pair(p.dh0 + (long long)u.b * q.D + u.block * CH + 2 * lane, h);
         },
-        [&](const Unit& u) {
+        [&](const Unit& u, int buf) {
           if (!m.rate() || p.rate_parts == nullptr) return;
-          uint64_t s = sh.drate[0][lane];   // over the warps, in order
-          for (int w = 1; w < W; ++w) s = add2(s, sh.drate[w][lane]);
+          uint64_t s = sh.drate[buf][0][lane];   // over the warps, in order
+          for (int w = 1; w < W; ++w) s = add2(s, sh.drate[buf][w][lane]);
           if (u.block * CH + 2 * lane < q.D) put_pair(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + u.block * CH + 2 * lane, s);
         });
     return;
@@ -441,11 +466,12 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
       T* const dst = tiles + stage * (NT * ROWS);
       const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, first = u.block * CH;   // the last tokens first
       const GatedRows<T> rows(first, q.D);
-      rows.copy(dst, p.f + u.b * q.fb + first, q.ft, t0, q.S);
-      rows.copy(dst + ROWS, p.x + u.b * q.xb + first, q.xt, t0, q.S);
-      rows.copy(dst + 2 * ROWS, p.dy + u.b * q.gb + first, q.gt, t0, q.S);
-      if (m.i()) rows.copy(dst + 3 * ROWS, p.i + u.b * q.ib + first, q.it, t0, q.S);
-      if (m.z()) rows.copy(dst + (NT - 1) * ROWS, p.z + u.b * q.zb + first, q.zt, t0, q.S);
+      const bool whole = t0 + GL <= q.S && first + CH <= q.D;
+      rows.copy(dst, p.f + u.b * q.fb + first, q.ft, t0, q.S, whole);
+      rows.copy(dst + ROWS, p.x + u.b * q.xb + first, q.xt, t0, q.S, whole);
+      rows.copy(dst + 2 * ROWS, p.dy + u.b * q.gb + first, q.gt, t0, q.S, whole);
+      if (m.i()) rows.copy(dst + 3 * ROWS, p.i + u.b * q.ib + first, q.it, t0, q.S, whole);
+      if (m.z()) rows.copy(dst + (NT - 1) * ROWS, p.z + u.b * q.zb + first, q.zt, t0, q.S, whole);
     }
     cp_commit();
   };
@@ -463,20 +489,20 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
     const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * 2, stage = turn % GATED_STAGES;
     const bool ok = ch < q.D;
     const T* const mine_x = tiles + stage * (NT * ROWS) + lane * 2;
-    const long long at = ((long long)u.b * q.S + t0) * q.D + ch;
     const uint64_t rate = ok && m.rate() ? get_pair(p.rate + ch) : 0;
     const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate));
     uint64_t h = h_next;
     GatedBack k[GL];
     cp_wait<GATED_STAGES - 1>();
     __syncwarp();
+    T* const dz_row = m.z() ? p.dz + ((long long)u.b * q.S + t0) * q.D + u.block * CH : nullptr;
     auto tokens = [&](auto far_) {
 #pragma unroll
       for (int j = 0; j < GL; ++j) {
         auto get = [&](int tensor) { return get_pair(mine_x + tensor * ROWS + j * CH); };
         uint64_t dz;
         k[j] = gated_token_bw<T, decltype(far_)::value>(m, get(0), get(1), m.i() ? get(3) : 0, m.z() ? get(NT - 1) : 0, get(2), rate, h, dz);
-        if (m.z() && ok && j < n) put_pair(p.dz + at + (long long)j * q.D, dz);
+        if (m.z() && ok && j < n) put_pair(dz_row, lane * 2 * (unsigned)sizeof(T) + j * (unsigned)q.D * (unsigned)sizeof(T), dz);
       }
     };
     if (far) tokens(std::true_type{});
@@ -493,20 +519,30 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
     run_there(sh);
     h_next = state(next);
     barrier_wait(STATES_THERE);
-    const int after = sh.unit[stage];
+    const int after = same(sh.unit[stage]);
     fetch(after, stage);
     uint64_t c = sh.start[warp][lane], drate = 0;
+    auto finish = [&](auto whole) {
+      const long long at = ((long long)u.b * q.S + t0) * q.D + u.block * CH;
+      T *const dx = p.dx + at, *const df = p.df + at, *const di = m.i() ? p.di + at : nullptr;
+      const unsigned step = (unsigned)q.D * (unsigned)sizeof(T);
+      unsigned to = lane * 2 * (unsigned)sizeof(T) + (GL - 1) * step;
 #pragma unroll
-    for (int j = GL - 1; j >= 0; --j) {
-      const uint64_t G = add2(k[j].up, c);
-      c = mul2(k[j].a, G);
-      if (j >= n) continue;
-      if (m.rate()) drate = fma2(c, k[j].drate, drate);
-      if (ok) put_pair(p.dx + at + (long long)j * q.D, mul2(G, k[j].dx));
-      if (ok) put_pair(p.df + at + (long long)j * q.D, mul2(c, k[j].df));
-      if (m.i() && ok) put_pair(p.di + at + (long long)j * q.D, mul2(G, k[j].di));
-    }
-    if (m.rate()) sh.drate[warp][lane] = drate;
+      for (int j = GL - 1; j >= 0; --j) {
+        if (decltype(whole)::value || j < n) {
+          const uint64_t G = add2(k[j].up, c);
+          c = mul2(k[j].a, G);
+          if (m.rate()) drate = fma2(c, k[j].drate, drate);
+          put_pair(dx, to, mul2(G, k[j].dx));
+          put_pair(df, to, mul2(c, k[j].df));
+          if (m.i()) put_pair(di, to, mul2(G, k[j].di));
+        }
+        to -= step;
+      }
+    };
+    if (ok && n >= GL) finish(std::true_type{});
+    else if (ok && n > 0) finish(std::false_type{});
+    if (m.rate()) sh.drate[turn & 1][warp][lane] = drate;
     now = next;
     next = after;
     if (now >= q.units) barrier_arrive(RUNS_THERE);   // the last unit's sums
@@ -523,10 +559,10 @@ template <typename T> __device__ __forceinline__ void put_one(T* p, uint64_t v) 
 
 template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 2) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
   __shared__ GatedShared sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
   __syncthreads();
-  int now = sh.unit[0], next = sh.unit[1];
+  int now = same(sh.unit[0]), next = same(sh.unit[1]);
   __syncthreads();
   if (warp == W) {
     gated_hand_on<false>(
@@ -534,7 +570,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
         [&](const Unit& u, uint64_t h) {
           if (p.h_last != nullptr && u.block * 32 + lane < q.D) put_one(p.h_last + (long long)u.b * q.D + u.block * 32 + lane, h);
         },
-        [](const Unit&) {});
+        [](const Unit&, int) {});
     return;
   }
   for (int turn = 0; now < q.units; ++turn) {
@@ -560,7 +596,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
     sh.part[warp][lane] = mine;
     run_there(sh);
     barrier_wait(STATES_THERE);
-    const int after = sh.unit[turn & 1];
+    const int after = same(sh.unit[turn & 1]);
     uint64_t h = sh.start[warp][lane];
     if (n > 0 && p.ckpt != nullptr && ok) put_one(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
 #pragma unroll
@@ -582,10 +618,10 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
 
 template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) gated_bw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
   __shared__ GatedShared sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = (blockDim.x >> 5) - 1, tile = W * GL;
+  const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
   __syncthreads();
-  int now = sh.unit[0], next = sh.unit[1];
+  int now = same(sh.unit[0]), next = same(sh.unit[1]);
   __syncthreads();
   if (warp == W) {
     gated_hand_on<true>(
@@ -594,10 +630,10 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
         [&](const Unit& u, uint64_t h) {
           if (p.dh0 != nullptr && u.block * 32 + lane < q.D) put_one(p.dh0 + (long long)u.b * q.D + u.block * 32 + lane, h);
         },
-        [&](const Unit& u) {
+        [&](const Unit& u, int buf) {
           if (p.rate_parts == nullptr) return;
-          uint64_t s = sh.drate[0][lane];
-          for (int w = 1; w < W; ++w) s = add2(s, sh.drate[w][lane]);
+          uint64_t s = sh.drate[buf][0][lane];
+          for (int w = 1; w < W; ++w) s = add2(s, sh.drate[buf][w][lane]);
           if (u.block * 32 + lane < q.D) put_one(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + u.block * 32 + lane, s);
         });
     return;
@@ -635,7 +671,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
     sh.part[warp][lane] = mine;
     run_there(sh);
     barrier_wait(STATES_THERE);
-    const int after = sh.unit[turn & 1];
+    const int after = same(sh.unit[turn & 1]);
     uint64_t c = sh.start[warp][lane], drate = 0;
 #pragma unroll
     for (int j = GL - 1; j >= 0; --j) {
@@ -648,7 +684,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
       if (m.i() && ok) put_one(p.di + at + (long long)j * q.D, mul2(G, k[j].di));
     }
     __syncwarp();
-    if (m.rate()) sh.drate[warp][lane] = drate;
+    if (m.rate()) sh.drate[turn & 1][warp][lane] = drate;
     now = next;
     next = after;
     if (now >= q.units) barrier_arrive(RUNS_THERE);   // the last unit's sums
