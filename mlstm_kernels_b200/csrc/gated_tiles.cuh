@@ -246,14 +246,27 @@ template <typename T, bool FAR, class M> __device__ __forceinline__ Run gated_to
   }
   return Run{d.a, u};
 }
-// Backward: its factor, what comes in from above, and what dx and di have per unit of G, df and drate per unit of a G
-struct GatedBack { uint64_t a, up, dx, di, df, drate; };
-// h: the state in front of it, and then behind; dz: the gradient of z
-template <typename T, bool FAR, class M>
-__device__ __forceinline__ GatedBack gated_token_bw(const M& m, uint64_t f, uint64_t x, uint64_t i, uint64_t z, uint64_t dy, uint64_t rate, uint64_t& h, uint64_t& dz) {
-  GatedBack t;
+// Backward, what its run needs: its factor, and what comes in from above; what the gates' gradients need of f and z besides
+struct GatedAbove { uint64_t a, up, rest, sf, cf, dz; };
+template <typename T, bool FAR, class M> __device__ __forceinline__ GatedAbove gated_token_above(const M& m, uint64_t f, uint64_t z, uint64_t dy, uint64_t rate) {
   const Decay d = gated_decay<T, FAR, true>(m, f, rate);
-  t.a = d.a;
+  GatedAbove t{d.a, dy, d.rest, 0, 0, 0};
+  if (m.rate()) t.sf = d.sf, t.cf = d.cf;
+  if (m.z()) {
+    uint64_t s, c;
+    logistic_gate<T>(z, s, c);
+    const uint64_t u = mul2(dy, s);
+    t.up = mul2(u, z);
+    t.dz = mul2(u, fma2(z, c, dup2(1.f)));
+  }
+  return t;
+}
+// Backward, what does not need G: what dx and di have per unit of G, df and drate per unit of a G
+struct GatedBack { uint64_t dx, di, df, drate; };
+// h: the state in front of it, and then behind
+template <typename T, class M>
+__device__ __forceinline__ GatedBack gated_token_bw(const M& m, const GatedAbove& d, uint64_t x, uint64_t i, uint64_t rate, uint64_t& h) {
+  GatedBack t;
   uint64_t gx = x, cg = 0, w = h, u;
   t.dx = dup2(1.f);
   if (m.i()) {
@@ -281,13 +294,6 @@ __device__ __forceinline__ GatedBack gated_token_bw(const M& m, uint64_t f, uint
     t.df = mul2(w, d.rest);
   }
   h = fma2(d.a, h, u);
-  t.up = dy;
-  if (m.z()) {
-    uint64_t s, c;
-    logistic_gate<T>(z, s, c);
-    dz = mul2(mul2(dy, h), mul2(s, fma2(z, c, dup2(1.f))));
-    t.up = mul2(dy, mul2(z, s));
-  }
   return t;
 }
 
@@ -437,6 +443,9 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
 
 template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), BWC) gated_bw_rows(GatedPtrs<T> p, GatedDims q, M m) {
   constexpr int CH = 64, NT = 3 + M::i() + M::z(), ROWS = GL * CH;
+  // The run is given away before the rest of the work on the tokens, which the search for the state in front of the unit goes beside.
+  // (With a rate too much lies between the two for the registers: 240 -> 260 us at 8 x 4096 x 2048.)
+  constexpr bool EARLY = !M::rate();
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   GatedShared& sh = *reinterpret_cast<GatedShared*>(shared_bytes);
   const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
@@ -492,17 +501,21 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
     const uint64_t rate = ok && m.rate() ? get_pair(p.rate + ch) : 0;
     const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate));
     uint64_t h = h_next;
+    GatedAbove d[GL];
     GatedBack k[GL];
     cp_wait<GATED_STAGES - 1>();
     __syncwarp();
     T* const dz_row = m.z() ? p.dz + ((long long)u.b * q.S + t0) * q.D + u.block * CH : nullptr;
+    auto get = [&](int tensor, int j) { return get_pair(mine_x + tensor * ROWS + j * CH); };
+    auto rest = [&](int j) {
+      k[j] = gated_token_bw<T>(m, d[j], get(1, j), m.i() ? get(3, j) : 0, rate, h);
+      if (m.z() && ok && j < n) put_pair(dz_row, lane * 2 * (unsigned)sizeof(T) + j * (unsigned)q.D * (unsigned)sizeof(T), mul2(d[j].dz, h));
+    };
     auto tokens = [&](auto far_) {
 #pragma unroll
       for (int j = 0; j < GL; ++j) {
-        auto get = [&](int tensor) { return get_pair(mine_x + tensor * ROWS + j * CH); };
-        uint64_t dz;
-        k[j] = gated_token_bw<T, decltype(far_)::value>(m, get(0), get(1), m.i() ? get(3) : 0, m.z() ? get(NT - 1) : 0, get(2), rate, h, dz);
-        if (m.z() && ok && j < n) put_pair(dz_row, lane * 2 * (unsigned)sizeof(T) + j * (unsigned)q.D * (unsigned)sizeof(T), dz);
+        d[j] = gated_token_above<T, decltype(far_)::value>(m, get(0, j), m.z() ? get(NT - 1, j) : 0, get(2, j), rate);
+        if (!EARLY) rest(j);
       }
     };
     if (far) tokens(std::true_type{});
@@ -510,13 +523,17 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
     if (n < GL) {
 #pragma unroll
       for (int j = 0; j < GL; ++j)
-        if (j >= n) k[j].a = dup2(1.f), k[j].up = 0;
+        if (j >= n) d[j].a = dup2(1.f), d[j].up = 0;
     }
     Run mine = no_tokens();
 #pragma unroll
-    for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(k[j].a, mine.A), mul2(k[j].a, add2(k[j].up, mine.H))};
+    for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(d[j].a, mine.A), mul2(d[j].a, add2(d[j].up, mine.H))};
     sh.part[warp][lane] = mine;
     run_there(sh);
+    if (EARLY) {
+#pragma unroll
+      for (int j = 0; j < GL; ++j) rest(j);
+    }
     h_next = state(next);
     barrier_wait(STATES_THERE);
     const int after = same(sh.unit[stage]);
@@ -530,8 +547,8 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
 #pragma unroll
       for (int j = GL - 1; j >= 0; --j) {
         if (decltype(whole)::value || j < n) {
-          const uint64_t G = add2(k[j].up, c);
-          c = mul2(k[j].a, G);
+          const uint64_t G = add2(d[j].up, c);
+          c = mul2(d[j].a, G);
           if (m.rate()) drate = fma2(c, k[j].drate, drate);
           put_pair(dx, to, mul2(G, k[j].dx));
           put_pair(df, to, mul2(c, k[j].df));
@@ -644,6 +661,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
     const bool ok = own < q.D;
     const uint64_t rate = m.rate() ? one(p.rate + ch) : 0;
     const long long at = ((long long)u.b * q.S + t0) * q.D + ch;
+    GatedAbove d[GL];
     GatedBack k[GL];
     T rx[GL], rf[GL], ri[GL], rz[GL], rg[GL];
 #pragma unroll
@@ -658,15 +676,15 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
     uint64_t h = n > 0 ? one(p.ckpt_in + ((long long)u.b * q.nc + t0 / GL) * q.D + ch) : 0;
 #pragma unroll
     for (int j = 0; j < GL; ++j) {
-      k[j].a = dup2(1.f), k[j].up = 0;
+      d[j].a = dup2(1.f), d[j].up = 0;
       if (j >= n) continue;
-      uint64_t dz = 0;
-      k[j] = gated_token_bw<T, true>(m, one(rf + j), one(rx + j), m.i() ? one(ri + j) : 0, m.z() ? one(rz + j) : 0, one(rg + j), rate, h, dz);
-      if (m.z() && ok) put_one(p.dz + at + (long long)j * q.D, dz);
+      d[j] = gated_token_above<T, true>(m, one(rf + j), m.z() ? one(rz + j) : 0, one(rg + j), rate);
+      k[j] = gated_token_bw<T>(m, d[j], one(rx + j), m.i() ? one(ri + j) : 0, rate, h);
+      if (m.z() && ok) put_one(p.dz + at + (long long)j * q.D, mul2(d[j].dz, h));
     }
     Run mine = no_tokens();
 #pragma unroll
-    for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(k[j].a, mine.A), mul2(k[j].a, add2(k[j].up, mine.H))};
+    for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(d[j].a, mine.A), mul2(d[j].a, add2(d[j].up, mine.H))};
     __syncwarp();
     sh.part[warp][lane] = mine;
     run_there(sh);
@@ -676,8 +694,8 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
 #pragma unroll
     for (int j = GL - 1; j >= 0; --j) {
       if (j >= n) continue;
-      const uint64_t G = add2(k[j].up, c);
-      c = mul2(k[j].a, G);
+      const uint64_t G = add2(d[j].up, c);
+      c = mul2(d[j].a, G);
       if (m.rate()) drate = fma2(c, k[j].drate, drate);
       if (ok) put_one(p.dx + at + (long long)j * q.D, mul2(G, k[j].dx));
       if (ok) put_one(p.df + at + (long long)j * q.D, mul2(c, k[j].df));
