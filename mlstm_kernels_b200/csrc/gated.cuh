@@ -126,4 +126,45 @@ __device__ __forceinline__ uint64_t inv_scale_pair(uint64_t rest2) {
 }
 __device__ __forceinline__ uint64_t rest2_pair(uint64_t a, uint64_t rest) { return fma2(rest, a, rest); }   // 1 - a^2
 
+// What is there, known when a kernel is called
+struct GatedAny {
+  bool rate_, i_, z_;
+  int scale_;
+  __device__ bool rate() const { return rate_; }
+  __device__ int scale() const { return scale_; }
+  __device__ bool i() const { return i_; }
+  __device__ bool z() const { return z_; }
+};
+
+// ---- runs of tokens ---------------------------------------------------------------------------------
+struct Run { uint64_t A, H; };   // of two channels
+__device__ __forceinline__ Run no_tokens() { return Run{dup2(1.f), 0}; }
+__device__ __forceinline__ Run then(Run first, Run second) { return Run{mul2(second.A, first.A), fma2(second.A, first.H, second.H)}; }
+__device__ __forceinline__ uint64_t through(Run r, uint64_t h) { return fma2(r.A, h, r.H); }
+
+// FAR: the rate may be outside (-1/2, 0]
+template <typename T, bool FAR, bool BOTH, class M> __device__ __forceinline__ Decay gated_decay(const M& m, uint64_t f, uint64_t rate) {
+  if (m.rate()) return decay_pair<T, true, FAR, BOTH>(f, rate);
+  return decay_pair<T, false>(f, rate);
+}
+__device__ __forceinline__ bool far_rate(uint64_t rate) {
+  float r0, r1;
+  unf2(rate, r0, r1);
+  return !(r0 > -0.5f && r0 <= 0.f && r1 > -0.5f && r1 <= 0.f);
+}
+
+// ---- one token of a pair of channels ------------------------------------------------------------------
+// Forward: its factor, and what it adds
+template <typename T, bool FAR, class M> __device__ __forceinline__ Run gated_token(const M& m, uint64_t f, uint64_t x, uint64_t i, uint64_t rate) {
+  const Decay d = gated_decay<T, FAR, false>(m, f, rate);
+  uint64_t u = x;
+  if (m.i()) u = mul2(u, logistic_pair2<T>(i));
+  if (m.scale() == GATED_CONVEX) u = mul2(u, d.rest);
+  if (m.scale() == GATED_VARIANCE) {
+    const uint64_t q2 = rest2_pair(d.a, d.rest);
+    u = mul2(mul2(u, q2), inv_scale_pair(q2));
+  }
+  return Run{d.a, u};
+}
+
 }  // namespace mlstm

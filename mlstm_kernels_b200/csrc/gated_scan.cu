@@ -6,34 +6,6 @@
 
 namespace mlstm {
 
-// one token of one channel
-template <typename T, bool RATE> struct GatedToken {
-  float a, rest, sf, cf, g, cg, x, s, rs;   // sigmoid(i) and one minus it; the input's scale and 1 / sqrt(1 - a^2)
-  __device__ GatedToken(const T* x_, const T* f_, const T* i_, float rate, int scale) {
-    x = to_f32(*x_);
-    const float f = to_f32(*f_);
-    const Decay d = decay_pair<T, RATE>(f2(f, f), f2(rate, rate));
-    float o;
-    unf2(d.a, a, o);
-    unf2(d.rest, rest, o);
-    unf2(d.sf, sf, o);
-    unf2(d.cf, cf, o);
-    g = 1.f, cg = 0.f;
-    if (i_ != nullptr) {
-      const float i = to_f32(*i_);
-      uint64_t gp, cp;
-      logistic_both<T>(f2(i, i), gp, cp);
-      unf2(gp, g, o);
-      unf2(cp, cg, o);
-    }
-    const uint64_t q = rest2_pair(d.a, d.rest), r = inv_scale_pair(q);
-    float qq;
-    unf2(q, qq, o);
-    unf2(r, rs, o);
-    s = scale == GATED_PLAIN ? 1.f : scale == GATED_CONVEX ? rest : qq * rs;
-  }
-};
-
 // drate: the sums of n rows of D, 32 channels to a CTA of 32 warps
 __global__ void gated_rate_sum(const float* parts, float* drate, int n, int D) {
   __shared__ float sums[32][33];
@@ -47,19 +19,36 @@ __global__ void gated_rate_sum(const float* parts, float* drate, int n, int D) {
   if (threadIdx.x == 0 && blockIdx.x * 32 + threadIdx.y < D) drate[blockIdx.x * 32 + threadIdx.y] = s;
 }
 
-template <typename T, bool RATE>
-__global__ void gated_one(const T* x, const T* f, const T* i, const T* z, const float* rate, const float* h, T* y, float* h_new, long long n, int D, int scale) {
-  const long long k = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+// The step: V neighbouring channels to a thread, all from one sequence
+template <typename T, int V>
+__global__ void __launch_bounds__(256) gated_one(const T* x, const T* f, const T* i, const T* z, const float* rate, const float* h, T* y, float* h_new, long long n,
+                                                 Divide row, bool small, GatedAny m) {
+  const long long k = ((long long)blockIdx.x * 256 + threadIdx.x) * V;
   if (k >= n) return;
-  const GatedToken<T, RATE> t(x + k, f + k, i != nullptr ? i + k : nullptr, RATE ? rate[k % D] : 0.f, scale);
-  const float v = t.a * h[k] + t.s * t.g * t.x;
-  h_new[k] = v;
-  float out = v;
-  if (z != nullptr) {
-    const float zz = to_f32(z[k]);
-    out *= zz * logistic_f<T>(zz);
+  const Pack<T, V> px = load_pack<T, V>(x + k), pf = load_pack<T, V>(f + k);
+  const Pack<float, V> ph = load_pack<float, V>(h + k);
+  Pack<T, V> pi, pz;
+  Pack<float, V> pr;
+  if (m.i()) pi = load_pack<T, V>(i + k);
+  if (m.z()) pz = load_pack<T, V>(z + k);
+  if (m.rate()) {
+    const long long first = k / V, d = small ? first - (long long)row((unsigned)first) * row.d : first % row.d;
+    pr = load_pack<float, V>(rate + d * V);
   }
-  y[k] = from_f32<T>(out);
+  float out[V], state[V];
+  auto pair = [](const auto& p, int j) { return f2(to_f32(p.e[j]), to_f32(p.e[V > 1 ? j + 1 : j])); };
+#pragma unroll
+  for (int j = 0; j < V; j += 2) {
+    const Run t = gated_token<T, true>(m, pair(pf, j), pair(px, j), m.i() ? pair(pi, j) : 0, m.rate() ? pair(pr, j) : 0);
+    const uint64_t v = through(t, pair(ph, j));
+    uint64_t o = v;
+    if (m.z()) o = mul2(o, mul2(pair(pz, j), logistic_pair2<T>(pair(pz, j))));
+    float rest;
+    unf2(v, state[j], V > 1 ? state[j + 1] : rest);
+    unf2(o, out[j], V > 1 ? out[j + 1] : rest);
+  }
+  store_pack(h_new + k, pack<float, V>(state));
+  store_pack(y + k, pack<T, V>(out));
 }
 
 // ---- calls --------------------------------------------------------------------------------------------
@@ -165,13 +154,18 @@ int launch_gated_bw(const GatedIn& in, const long long* strides, const float* ck
 int launch_gated_step(const GatedIn& in, const float* h, void* y, float* h_new, int B, int D, int scale, int dtype, cudaStream_t st) {
   PhaseScope ps(PH_GATED, st);
   const long long n = (long long)B * D;
-  const unsigned grid = (unsigned)((n + 127) / 128);
-  auto go = [&](auto* t, auto rate) {
+  const size_t el = dtype_size(dtype);
+  bool four = D % 4 == 0;
+  for (const void* p : {in.x, in.f, in.i, in.z, (const void*)y}) four = four && fits_access(p, 4 * el);
+  for (const float* p : {in.rate, h, (const float*)h_new}) four = four && fits_access(p, 16);
+  auto go = [&](auto* t, auto v) {
     using T = std::remove_pointer_t<decltype(t)>;
-    gated_one<T, decltype(rate)::value><<<grid, 128, 0, st>>>((const T*)in.x, (const T*)in.f, (const T*)in.i, (const T*)in.z, in.rate, h, (T*)y, h_new, n,
-                                                                D, scale);
+    constexpr int V = decltype(v)::value;
+    const long long chunks = n / V;
+    gated_one<T, V><<<(unsigned)((chunks + 255) / 256), 256, 0, st>>>((const T*)in.x, (const T*)in.f, (const T*)in.i, (const T*)in.z, in.rate, h, (T*)y, h_new, n,
+                                                                        divide_by(D / V), chunks < (1ll << 31), GatedAny{in.rate != nullptr, in.i != nullptr, in.z != nullptr, scale});
   };
-  MLSTM_DTYPE_SWITCH(dtype, T, if (in.rate != nullptr) go((T*)nullptr, std::true_type{}); else go((T*)nullptr, std::false_type{});)
+  MLSTM_DTYPE_SWITCH(dtype, T, if (four) go((T*)nullptr, std::integral_constant<int, 4>{}); else go((T*)nullptr, std::integral_constant<int, 1>{});)
   MLSTM_LAUNCH_CHECK();
   return MLSTM_OK;
 }

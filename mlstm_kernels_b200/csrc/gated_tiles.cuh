@@ -29,26 +29,7 @@ template <bool RATE, int SCALE, bool I, bool Z> struct GatedFixed {
   __host__ __device__ static constexpr bool i() { return I; }
   __host__ __device__ static constexpr bool z() { return Z; }
 };
-struct GatedAny {
-  bool rate_, i_, z_;
-  int scale_;
-  __device__ bool rate() const { return rate_; }
-  __device__ int scale() const { return scale_; }
-  __device__ bool i() const { return i_; }
-  __device__ bool z() const { return z_; }
-};
-
-#ifndef FWC
-#define FWC 3
-#define BWC 2
-#endif
 constexpr int GL = GATED_CK;
-
-// ---- joining runs -------------------------------------------------------------------------------------
-struct Run { uint64_t A, H; };   // of two channels
-__device__ __forceinline__ Run no_tokens() { return Run{dup2(1.f), 0}; }
-__device__ __forceinline__ Run then(Run first, Run second) { return Run{mul2(second.A, first.A), fma2(second.A, first.H, second.H)}; }
-__device__ __forceinline__ uint64_t through(Run r, uint64_t h) { return fma2(r.A, h, r.H); }
 
 // ---- units --------------------------------------------------------------------------------------------
 // Code of the first wait that ran out since it was last asked for (0: none), read by the host
@@ -200,11 +181,16 @@ __device__ __forceinline__ void gated_hand_on(GatedShared& sh, const GatedDims& 
     }
     uint64_t h = find.value();
     if (!runs) barrier_wait(RUNS_THERE);
-    for (int n = 0; n < W; ++n) {
-      const int w = BACK ? W - 1 - n : n;
-      sh.start[w][lane] = h;
-      h = through(sh.part[w][lane], h);
-    }
+    Run r[GATED_WARPS];
+#pragma unroll
+    for (int n = 0; n < GATED_WARPS; ++n)
+      if (n < W) r[n] = sh.part[BACK ? W - 1 - n : n][lane];
+#pragma unroll
+    for (int n = 0; n < GATED_WARPS; ++n)
+      if (n < W) {
+        sh.start[BACK ? W - 1 - n : n][lane] = h;
+        h = through(r[n], h);
+      }
     if (lane == 0) sh.unit[turn & 1] = after;
     if (!gave) give_run();
     __syncwarp();
@@ -222,30 +208,7 @@ __device__ __forceinline__ void gated_hand_on(GatedShared& sh, const GatedDims& 
   }
 }
 
-// FAR: the rate may be outside (-1/2, 0]
-template <typename T, bool FAR, bool BOTH, class M> __device__ __forceinline__ Decay gated_decay(const M& m, uint64_t f, uint64_t rate) {
-  if (m.rate()) return decay_pair<T, true, FAR, BOTH>(f, rate);
-  return decay_pair<T, false>(f, rate);
-}
-__device__ __forceinline__ bool far_rate(uint64_t rate) {
-  float r0, r1;
-  unf2(rate, r0, r1);
-  return !(r0 > -0.5f && r0 <= 0.f && r1 > -0.5f && r1 <= 0.f);
-}
-
-// ---- one token of a pair of channels ------------------------------------------------------------------
-// Forward: its factor, and what it adds
-template <typename T, bool FAR, class M> __device__ __forceinline__ Run gated_token(const M& m, uint64_t f, uint64_t x, uint64_t i, uint64_t rate) {
-  const Decay d = gated_decay<T, FAR, false>(m, f, rate);
-  uint64_t u = x;
-  if (m.i()) u = mul2(u, logistic_pair2<T>(i));
-  if (m.scale() == GATED_CONVEX) u = mul2(u, d.rest);
-  if (m.scale() == GATED_VARIANCE) {
-    const uint64_t q2 = rest2_pair(d.a, d.rest);
-    u = mul2(mul2(u, q2), inv_scale_pair(q2));
-  }
-  return Run{d.a, u};
-}
+// ---- one token of a pair of channels, backward ----------------------------------------------------------
 // Backward, what its run needs: its factor, and what comes in from above; what the gates' gradients need of f and z besides
 struct GatedAbove { uint64_t a, up, rest, sf, cf, dz; };
 template <typename T, bool FAR, class M> __device__ __forceinline__ GatedAbove gated_token_above(const M& m, uint64_t f, uint64_t z, uint64_t dy, uint64_t rate) {
@@ -343,7 +306,7 @@ template <typename T> __device__ __forceinline__ void put_pair(T* p, uint64_t v)
 }
 template <typename T> __device__ __forceinline__ void put_pair(T* row, unsigned at, uint64_t v) { put_pair(reinterpret_cast<T*>(reinterpret_cast<char*>(row) + at), v); }
 
-template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), FWC) gated_fw_rows(GatedPtrs<T> p, GatedDims q, M m) {
+template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 3) gated_fw_rows(GatedPtrs<T> p, GatedDims q, M m) {
   constexpr int CH = 64, NT = 2 + M::i() + M::z(), ROWS = GL * CH;
   extern __shared__ __align__(16) unsigned char shared_bytes[];
   GatedShared& sh = *reinterpret_cast<GatedShared*>(shared_bytes);
@@ -378,12 +341,18 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
   };
   fetch(now, 0);
   fetch(next, 1);
+  auto rate_of = [&](int unit) {
+    if (!m.rate() || unit >= q.units) return (uint64_t)0;
+    const int ch = unit_of(unit, q).block * CH + lane * 2;
+    return ch < q.D ? get_pair(p.rate + ch) : (uint64_t)0;
+  };
+  uint64_t rate_next = rate_of(now);
   for (int turn = 0; now < q.units; ++turn) {
     const Unit u = unit_of(now, q);
     const int t0 = u.k * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * 2, stage = turn % GATED_STAGES;
     const bool ok = ch < q.D;
     const T* const mine_x = tiles + stage * (NT * ROWS) + lane * 2;
-    const uint64_t rate = ok && m.rate() ? get_pair(p.rate + ch) : 0;
+    const uint64_t rate = rate_next;
     const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate));
     Run r[GL];
     cp_wait<GATED_STAGES - 1>();
@@ -406,6 +375,7 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
     for (int j = 1; j < GL; ++j) mine = then(mine, r[j]);
     sh.part[warp][lane] = mine;
     run_there(sh);
+    rate_next = rate_of(next);
     barrier_wait(STATES_THERE);
     const int after = same(sh.unit[stage]);
     if (!m.z()) fetch(after, stage);
@@ -441,7 +411,7 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
   }
 }
 
-template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), BWC) gated_bw_rows(GatedPtrs<T> p, GatedDims q, M m) {
+template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 2) gated_bw_rows(GatedPtrs<T> p, GatedDims q, M m) {
   constexpr int CH = 64, NT = 3 + M::i() + M::z(), ROWS = GL * CH;
   // The run is given away before the rest of the work on the tokens, which the search for the state in front of the unit goes beside.
   // (With a rate too much lies between the two for the registers: 240 -> 260 us at 8 x 4096 x 2048.)
@@ -492,13 +462,19 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
   };
   fetch(now, 0);
   fetch(next, 1);
+  auto rate_of = [&](int unit) {
+    if (!m.rate() || unit >= q.units) return (uint64_t)0;
+    const int ch = unit_of(unit, q).block * CH + lane * 2;
+    return ch < q.D ? get_pair(p.rate + ch) : (uint64_t)0;
+  };
+  uint64_t rate_next = rate_of(now);
   uint64_t h_next = state(now);
   for (int turn = 0; now < q.units; ++turn) {
     const Unit u = unit_of(now, q);
     const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0, ch = u.block * CH + lane * 2, stage = turn % GATED_STAGES;
     const bool ok = ch < q.D;
     const T* const mine_x = tiles + stage * (NT * ROWS) + lane * 2;
-    const uint64_t rate = ok && m.rate() ? get_pair(p.rate + ch) : 0;
+    const uint64_t rate = rate_next;
     const bool far = m.rate() && __any_sync(0xffffffffu, far_rate(rate));
     uint64_t h = h_next;
     GatedAbove d[GL];
@@ -535,6 +511,7 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
       for (int j = 0; j < GL; ++j) rest(j);
     }
     h_next = state(next);
+    rate_next = rate_of(next);
     barrier_wait(STATES_THERE);
     const int after = same(sh.unit[stage]);
     fetch(after, stage);
@@ -574,7 +551,7 @@ template <typename T> __device__ __forceinline__ void put_one(T* p, uint64_t v) 
   *p = from_f32<T>(lo);
 }
 
-template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 2) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
+template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 3) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
   __shared__ GatedShared sh;
   const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
