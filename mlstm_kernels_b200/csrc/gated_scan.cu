@@ -55,18 +55,16 @@ __global__ void __launch_bounds__(256) gated_one(const T* x, const T* f, const T
 static int gated_slots() { return 3 * sm_count(); }   // CTAs that run at once
 
 bool gated_sizes_ok(int B, int S, int D) {
-  return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && D <= (1 << 30) && gated_plan(B, S, D, 1, gated_slots()).units < (1ll << 31);
+  return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && D <= (1 << 30) && gated_plan(B, S, D, gated_slots()).units < (1ll << 31);
 }
 size_t gated_ckpt_bytes(int B, int S, int D) { return (size_t)B * ceil_div(S, GATED_CK) * D * sizeof(float); }
 size_t gated_bytes(int B, int S, int D, bool backward) {
-  size_t most = 0;
-  for (const int V : {1, 2}) most = std::max(most, gated_scratch(gated_plan(B, S, D, V, gated_slots()), B, D, backward).bytes);
-  return most;
+  return gated_scratch(gated_plan(B, S, D, gated_slots()), B, D, backward).bytes;
 }
 
-int gated_run_f32(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
-int gated_run_bf16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
-int gated_run_f16(bool back, int V, const void* ptrs, const GatedDims& q, cudaStream_t st);
+int gated_run_f32(bool back, bool rows, const void* ptrs, const GatedDims& q, cudaStream_t st);
+int gated_run_bf16(bool back, bool rows, const void* ptrs, const GatedDims& q, cudaStream_t st);
+int gated_run_f16(bool back, bool rows, const void* ptrs, const GatedDims& q, cudaStream_t st);
 int gated_status_f32(int reset, int* status);
 int gated_status_bf16(int reset, int* status);
 int gated_status_f16(int reset, int* status);
@@ -103,8 +101,8 @@ static bool gated_rows(const GatedVoid& p, const long long* st, const long long*
 static int gated_call(bool back, GatedVoid p, const long long* st, const long long* gs, void* scratch, int B, int S, int D, int scale, int dtype, float* drate,
                       cudaStream_t stream) {
   PhaseScope ps(PH_GATED, stream);
-  const int el = (int)dtype_size(dtype), V = !gated_rows(p, st, gs, D, el) ? 1 : 2;
-  const GatedPlan plan = gated_plan(B, S, D, V, gated_slots());
+  const bool rows = gated_rows(p, st, gs, D, (int)dtype_size(dtype));
+  const GatedPlan plan = gated_plan(B, S, D, gated_slots());
   const GatedScratch at = gated_scratch(plan, B, D, back);
   unsigned char* const base = static_cast<unsigned char*>(scratch);
   GatedDims q{};
@@ -126,7 +124,7 @@ static int gated_call(bool back, GatedVoid p, const long long* st, const long lo
     using T = std::remove_pointer_t<decltype(t)>;
     const GatedPtrs<T> v{(const T*)p.x, (const T*)p.f, (const T*)p.i, (const T*)p.z, (const T*)p.dy, p.rate, p.h0, p.ckpt_in, p.dh_last, (T*)p.y, (T*)p.dx,
                          (T*)p.df, (T*)p.di, (T*)p.dz, p.h_last, p.ckpt, p.dh0, p.rate_parts};
-    return run(back, V, &v, q, stream);
+    return run(back, rows, &v, q, stream);
   };
   int rc = MLSTM_OK;
   if (dtype == MLSTM_F32) rc = go((float*)nullptr, gated_run_f32);

@@ -295,10 +295,8 @@ template <typename T> struct GatedRows {
 };
 // a value that is the same in the whole warp, which the compiler then knows
 __device__ __forceinline__ int same(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-template <typename T> __device__ __forceinline__ uint64_t get_pair(const T* p) {
-  const Pack<T, 2> v = load_pack<T, 2>(p);
-  return f2(to_f32(v.e[0]), to_f32(v.e[1]));
-}
+template <typename T> __device__ __forceinline__ uint64_t pair_of(const Pack<T, 2>& v) { return f2(to_f32(v.e[0]), to_f32(v.e[1])); }
+template <typename T> __device__ __forceinline__ uint64_t get_pair(const T* p) { return pair_of(load_pack<T, 2>(p)); }
 template <typename T> __device__ __forceinline__ void put_pair(T* p, uint64_t v) {
   float o[2];
   unf2(v, o[0], o[1]);
@@ -544,14 +542,29 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
 }
 
 // ---- channels one by one: any width, any alignment -----------------------------------------------------
-template <typename T> __device__ __forceinline__ uint64_t one(const T* p) { return f2(to_f32(*p), 0.f); }
-template <typename T> __device__ __forceinline__ void put_one(T* p, uint64_t v) {
-  float lo, hi;
-  unf2(v, lo, hi);
-  *p = from_f32<T>(lo);
-}
+// A lane's two channels are 32 apart, so that neighbouring lanes have neighbouring channels of any alignment.
+template <typename T> struct GatedApart {
+  int c0, c1;        // where to read: the last channel for those behind it
+  bool ok0, ok1;
+  __device__ __forceinline__ GatedApart(const Unit& u, int D) {
+    const int c = u.block * 64 + (threadIdx.x & 31);
+    c0 = min(c, D - 1), c1 = min(c + 32, D - 1), ok0 = c < D, ok1 = c + 32 < D;
+  }
+  __device__ __forceinline__ Pack<T, 2> load(const T* row) const {
+    Pack<T, 2> v;
+    v.e[0] = row[c0], v.e[1] = row[c1];
+    return v;
+  }
+  template <typename O> __device__ __forceinline__ void put(O* row, uint64_t v) const {
+    float lo, hi;
+    unf2(v, lo, hi);
+    if (ok0) row[c0] = from_f32<O>(lo);
+    if (ok1) row[c1] = from_f32<O>(hi);
+  }
+  __device__ __forceinline__ uint64_t get(const float* row) const { return f2(row[c0], row[c1]); }
+};
 
-template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 3) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
+template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 2) gated_fw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
   __shared__ GatedShared sh;
   const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
@@ -560,31 +573,33 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
   __syncthreads();
   if (warp == W) {
     gated_hand_on<false>(
-        sh, q, now, next, [&](const Unit& u) { return p.h0 != nullptr && u.block * 32 + lane < q.D ? one(p.h0 + (long long)u.b * q.D + u.block * 32 + lane) : 0; },
+        sh, q, now, next, [&](const Unit& u) { return p.h0 != nullptr ? GatedApart<T>(u, q.D).get(p.h0 + (long long)u.b * q.D) : 0; },
         [&](const Unit& u, uint64_t h) {
-          if (p.h_last != nullptr && u.block * 32 + lane < q.D) put_one(p.h_last + (long long)u.b * q.D + u.block * 32 + lane, h);
+          if (p.h_last != nullptr) GatedApart<T>(u, q.D).put(p.h_last + (long long)u.b * q.D, h);
         },
         [](const Unit&, int) {});
     return;
   }
   for (int turn = 0; now < q.units; ++turn) {
     const Unit u = unit_of(now, q);
-    const int t0 = u.k * tile + warp * GL, n = q.S - t0, own = u.block * 32 + lane, ch = min(own, q.D - 1);   // (n: may be none, or more)
-    const bool ok = own < q.D;
-    const uint64_t rate = m.rate() ? one(p.rate + ch) : 0;
+    const GatedApart<T> at(u, q.D);
+    const int t0 = u.k * tile + warp * GL, n = q.S - t0;   // (n: may be none, or more)
+    const uint64_t rate = m.rate() ? at.get(p.rate) : 0;
     Run r[GL], mine = no_tokens();
-    T rx[GL], rf[GL], ri[GL];
-    const T *px = p.x + u.b * q.xb + t0 * q.xt + ch, *pf = p.f + u.b * q.fb + t0 * q.ft + ch, *pi = m.i() ? p.i + u.b * q.ib + t0 * q.it + ch : nullptr;
+    Pack<T, 2> rx[GL], rf[GL], ri[GL], rz[GL];
+    const T *pz = m.z() ? p.z + u.b * q.zb + t0 * q.zt : nullptr;
+    const T *px = p.x + u.b * q.xb + t0 * q.xt, *pf = p.f + u.b * q.fb + t0 * q.ft, *pi = m.i() ? p.i + u.b * q.ib + t0 * q.it : nullptr;
 #pragma unroll
     for (int j = 0; j < GL; ++j) {
       if (j >= n) break;
-      rf[j] = pf[j * q.ft];
-      rx[j] = px[j * q.xt];
-      if (m.i()) ri[j] = pi[j * q.it];
+      rf[j] = at.load(pf + j * q.ft);
+      rx[j] = at.load(px + j * q.xt);
+      if (m.i()) ri[j] = at.load(pi + j * q.it);
+      if (m.z()) rz[j] = at.load(pz + j * q.zt);
     }
 #pragma unroll
     for (int j = 0; j < GL; ++j) {
-      r[j] = j < n ? gated_token<T, true>(m, one(rf + j), one(rx + j), m.i() ? one(ri + j) : 0, rate) : no_tokens();
+      r[j] = j < n ? gated_token<T, true>(m, pair_of(rf[j]), pair_of(rx[j]), m.i() ? pair_of(ri[j]) : 0, rate) : no_tokens();
       mine = then(mine, r[j]);
     }
     sh.part[warp][lane] = mine;
@@ -592,17 +607,17 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
     barrier_wait(STATES_THERE);
     const int after = same(sh.unit[turn & 1]);
     uint64_t h = sh.start[warp][lane];
-    if (n > 0 && p.ckpt != nullptr && ok) put_one(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D + ch, h);
+    if (n > 0 && p.ckpt != nullptr) at.put(p.ckpt + ((long long)u.b * q.nc + t0 / GL) * q.D, h);
 #pragma unroll
     for (int j = 0; j < GL; ++j) {
       if (j >= n) break;
       h = through(r[j], h);
       uint64_t o = h;
       if (m.z()) {
-        const uint64_t z = one(p.z + u.b * q.zb + (t0 + j) * q.zt + ch);
+        const uint64_t z = pair_of(rz[j]);
         o = mul2(o, mul2(z, logistic_pair2<T>(z)));
       }
-      if (ok) put_one(p.y + ((long long)u.b * q.S + t0 + j) * q.D + ch, o);
+      at.put(p.y + ((long long)u.b * q.S + t0 + j) * q.D, o);
     }
     __syncwarp();
     now = next;
@@ -610,7 +625,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
   }
 }
 
-template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) gated_bw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
+template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 2) gated_bw_any(GatedPtrs<T> p, GatedDims q, GatedAny m) {
   __shared__ GatedShared sh;
   const int lane = threadIdx.x & 31, warp = same(threadIdx.x >> 5), W = (blockDim.x >> 5) - 1, tile = W * GL;
   if (threadIdx.x == 0) sh.unit[0] = take_unit(q, 0), sh.unit[1] = take_unit(q, 1), sh.runs = 0;
@@ -619,49 +634,55 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
   __syncthreads();
   if (warp == W) {
     gated_hand_on<true>(
-        sh, q, now, next,
-        [&](const Unit& u) { return p.dh_last != nullptr && u.block * 32 + lane < q.D ? one(p.dh_last + (long long)u.b * q.D + u.block * 32 + lane) : 0; },
+        sh, q, now, next, [&](const Unit& u) { return p.dh_last != nullptr ? GatedApart<T>(u, q.D).get(p.dh_last + (long long)u.b * q.D) : 0; },
         [&](const Unit& u, uint64_t h) {
-          if (p.dh0 != nullptr && u.block * 32 + lane < q.D) put_one(p.dh0 + (long long)u.b * q.D + u.block * 32 + lane, h);
+          if (p.dh0 != nullptr) GatedApart<T>(u, q.D).put(p.dh0 + (long long)u.b * q.D, h);
         },
         [&](const Unit& u, int buf) {
           if (p.rate_parts == nullptr) return;
           uint64_t s = sh.drate[buf][0][lane];
           for (int w = 1; w < W; ++w) s = add2(s, sh.drate[buf][w][lane]);
-          if (u.block * 32 + lane < q.D) put_one(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D + u.block * 32 + lane, s);
+          GatedApart<T>(u, q.D).put(p.rate_parts + ((long long)u.b * q.nt + u.k) * q.D, s);
         });
     return;
   }
   for (int turn = 0; now < q.units; ++turn) {
     const Unit u = unit_of(now, q);
-    const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0, own = u.block * 32 + lane, ch = min(own, q.D - 1);
-    const bool ok = own < q.D;
-    const uint64_t rate = m.rate() ? one(p.rate + ch) : 0;
-    const long long at = ((long long)u.b * q.S + t0) * q.D + ch;
-    GatedAbove d[GL];
+    const GatedApart<T> at(u, q.D);
+    const int t0 = (q.nt - 1 - u.k) * tile + warp * GL, n = q.S - t0;
+    const uint64_t rate = m.rate() ? at.get(p.rate) : 0;
+    const long long row = ((long long)u.b * q.S + t0) * q.D;
+    uint64_t a[GL], up[GL];
     GatedBack k[GL];
-    T rx[GL], rf[GL], ri[GL], rz[GL], rg[GL];
+    uint64_t h = n > 0 ? at.get(p.ckpt_in + ((long long)u.b * q.nc + t0 / GL) * q.D) : 0;
+    constexpr int AT_ONCE = 2;   // tokens: with 4 and 8, 90 and 50 us more at 4 x 4096 x 2049 (registers)
 #pragma unroll
-    for (int j = 0; j < GL; ++j) {
-      if (j >= n) break;
-      rf[j] = p.f[u.b * q.fb + (t0 + j) * q.ft + ch];
-      rx[j] = p.x[u.b * q.xb + (t0 + j) * q.xt + ch];
-      rg[j] = p.dy[u.b * q.gb + (t0 + j) * q.gt + ch];
-      if (m.i()) ri[j] = p.i[u.b * q.ib + (t0 + j) * q.it + ch];
-      if (m.z()) rz[j] = p.z[u.b * q.zb + (t0 + j) * q.zt + ch];
-    }
-    uint64_t h = n > 0 ? one(p.ckpt_in + ((long long)u.b * q.nc + t0 / GL) * q.D + ch) : 0;
+    for (int j0 = 0; j0 < GL; j0 += AT_ONCE) {
+      Pack<T, 2> rx[AT_ONCE], rf[AT_ONCE], ri[AT_ONCE], rz[AT_ONCE], rg[AT_ONCE];
 #pragma unroll
-    for (int j = 0; j < GL; ++j) {
-      d[j].a = dup2(1.f), d[j].up = 0;
-      if (j >= n) continue;
-      d[j] = gated_token_above<T, true>(m, one(rf + j), m.z() ? one(rz + j) : 0, one(rg + j), rate);
-      k[j] = gated_token_bw<T>(m, d[j], one(rx + j), m.i() ? one(ri + j) : 0, rate, h);
-      if (m.z() && ok) put_one(p.dz + at + (long long)j * q.D, mul2(d[j].dz, h));
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int t = t0 + j0 + e;
+        if (j0 + e >= n) break;
+        rf[e] = at.load(p.f + u.b * q.fb + t * q.ft);
+        rx[e] = at.load(p.x + u.b * q.xb + t * q.xt);
+        rg[e] = at.load(p.dy + u.b * q.gb + t * q.gt);
+        if (m.i()) ri[e] = at.load(p.i + u.b * q.ib + t * q.it);
+        if (m.z()) rz[e] = at.load(p.z + u.b * q.zb + t * q.zt);
+      }
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const int j = j0 + e;
+        a[j] = dup2(1.f), up[j] = 0;
+        if (j >= n) continue;
+        const GatedAbove d = gated_token_above<T, true>(m, pair_of(rf[e]), m.z() ? pair_of(rz[e]) : 0, pair_of(rg[e]), rate);
+        a[j] = d.a, up[j] = d.up;
+        k[j] = gated_token_bw<T>(m, d, pair_of(rx[e]), m.i() ? pair_of(ri[e]) : 0, rate, h);
+        if (m.z()) at.put(p.dz + row + (long long)j * q.D, mul2(d.dz, h));
+      }
     }
     Run mine = no_tokens();
 #pragma unroll
-    for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(d[j].a, mine.A), mul2(d[j].a, add2(d[j].up, mine.H))};
+    for (int j = GL - 1; j >= 0; --j) mine = Run{mul2(a[j], mine.A), mul2(a[j], add2(up[j], mine.H))};
     __syncwarp();
     sh.part[warp][lane] = mine;
     run_there(sh);
@@ -671,12 +692,12 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1)) 
 #pragma unroll
     for (int j = GL - 1; j >= 0; --j) {
       if (j >= n) continue;
-      const uint64_t G = add2(d[j].up, c);
-      c = mul2(d[j].a, G);
+      const uint64_t G = add2(up[j], c);
+      c = mul2(a[j], G);
       if (m.rate()) drate = fma2(c, k[j].drate, drate);
-      if (ok) put_one(p.dx + at + (long long)j * q.D, mul2(G, k[j].dx));
-      if (ok) put_one(p.df + at + (long long)j * q.D, mul2(c, k[j].df));
-      if (m.i() && ok) put_one(p.di + at + (long long)j * q.D, mul2(G, k[j].di));
+      at.put(p.dx + row + (long long)j * q.D, mul2(G, k[j].dx));
+      at.put(p.df + row + (long long)j * q.D, mul2(c, k[j].df));
+      if (m.i()) at.put(p.di + row + (long long)j * q.D, mul2(G, k[j].di));
     }
     __syncwarp();
     if (m.rate()) sh.drate[turn & 1][warp][lane] = drate;
@@ -698,9 +719,9 @@ template <typename T, class M> int gated_launch(void (*kern)(GatedPtrs<T>, Gated
   return MLSTM_OK;
 }
 
-template <typename T> int gated_run(bool back, int V, const GatedPtrs<T>& p, const GatedDims& q, cudaStream_t st) {
+template <typename T> int gated_run(bool back, bool rows, const GatedPtrs<T>& p, const GatedDims& q, cudaStream_t st) {
   const bool rate = p.rate != nullptr, i = p.i != nullptr, z = p.z != nullptr;
-  if (V == 1) return gated_launch<T, GatedAny>(back ? gated_bw_any<T> : gated_fw_any<T>, 0, p, q, GatedAny{rate, i, z, q.scale}, st);
+  if (!rows) return gated_launch<T, GatedAny>(back ? gated_bw_any<T> : gated_fw_any<T>, 0, p, q, GatedAny{rate, i, z, q.scale}, st);
   const size_t smem = sizeof(GatedShared) + (size_t)q.warps * GATED_STAGES * GL * 64 * sizeof(T) * (2 + back + i + z);
   auto pick = [&](auto r, auto s, auto ii, auto zz) {
     using M = GatedFixed<decltype(r)::value, decltype(s)::value, decltype(ii)::value, decltype(zz)::value>;

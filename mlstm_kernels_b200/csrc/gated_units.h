@@ -6,21 +6,21 @@
 namespace mlstm {
 
 constexpr int GATED_CK = 8;      // tokens to a thread, and to a state that the forward keeps for the backward
+constexpr int GATED_CHANNELS = 64;   // of a unit
 constexpr int GATED_WARPS = 7;   // most warps of a CTA that take tokens; one more hands the states on
 constexpr int GATED_GROUP = 16;  // most units of a group
 
-// A unit is `warps` * GATED_CK tokens of 32 V channels of one sequence (a chain).  Units are numbered by time, the chains of one
+// A unit is `warps` * GATED_CK tokens of GATED_CHANNELS channels of one sequence (a chain).  Units are numbered by time, the chains of one
 // time after one another, and taken in that order.  `group` units of a chain that follow one another take the state in front of their
 // group and join what stands between by themselves.
 struct GatedPlan {
-  int V, blocks, warps, nt, group, groups;   // channels to a lane, units beside each other in D, warps of a CTA, units and groups of a chain
+  int blocks, warps, nt, group, groups;   // units beside each other in D, warps of a CTA, units and groups of a chain
   long long chains, units;
 };
-inline GatedPlan gated_plan(int B, int S, int D, int V, int slots) {
+inline GatedPlan gated_plan(int B, int S, int D, int slots) {
   GatedPlan p{};
   const int runs = (S + GATED_CK - 1) / GATED_CK;
-  p.V = V;
-  p.blocks = (D + 32 * V - 1) / (32 * V);
+  p.blocks = (D + GATED_CHANNELS - 1) / GATED_CHANNELS;
   p.nt = (runs + GATED_WARPS - 1) / GATED_WARPS;
   p.warps = (runs + p.nt - 1) / p.nt;
   p.chains = (long long)B * p.blocks;

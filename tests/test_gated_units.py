@@ -13,9 +13,9 @@ PROGRAM = r"""
 #include <cstdio>
 #include "gated_units.h"
 int main() {
-  int B, S, D, V, slots, back;
-  while (scanf("%d %d %d %d %d %d", &B, &S, &D, &V, &slots, &back) == 6) {
-    const mlstm::GatedPlan p = mlstm::gated_plan(B, S, D, V, slots);
+  int B, S, D, slots, back;
+  while (scanf("%d %d %d %d %d", &B, &S, &D, &slots, &back) == 5) {
+    const mlstm::GatedPlan p = mlstm::gated_plan(B, S, D, slots);
     const mlstm::GatedScratch s = mlstm::gated_scratch(p, B, D, back != 0);
     printf("%d %d %d %d %d %lld %lld %zu %zu %zu %zu\n", p.blocks, p.warps, p.nt, p.group, p.groups, p.chains, p.units, s.state, s.agg, s.rate, s.bytes);
   }
@@ -39,14 +39,13 @@ def plan(tmp_path_factory):
 
 
 @pytest.mark.parametrize("B,S,D", SIZES)
-@pytest.mark.parametrize("V", [1, 2])
 @pytest.mark.parametrize("slots", [2, 444])
-def test_units_cover_everything_and_scratch_holds_them(plan, B, S, D, V, slots):
+def test_units_cover_everything_and_scratch_holds_them(plan, B, S, D, slots):
     for back in (0, 1):
-        p = plan(B, S, D, V, slots, back)
+        p = plan(B, S, D, slots, back)
         tile = 8 * p["warps"]
         assert 1 <= p["warps"] <= 7 and p["nt"] * tile >= S > (p["nt"] - 1) * tile
-        assert p["blocks"] * 32 * V >= D > (p["blocks"] - 1) * 32 * V
+        assert p["blocks"] * 64 >= D > (p["blocks"] - 1) * 64
         assert p["chains"] == B * p["blocks"] and p["units"] == p["chains"] * p["nt"] < 1 << 31
         assert p["group"] in (1, 2, 4, 8, 16) and p["groups"] * p["group"] >= p["nt"] > (p["groups"] - 1) * p["group"]
         # a pair of channels to a lane: 8 bytes of a state, 16 of a run
