@@ -157,7 +157,7 @@ static void dropout_run(const T* x, const O* residual, O* y, const DropoutDims& 
     for (const long long* s : {q.xs, q.rs, q.ys}) {   // (without a residual its strides are zero)
       long long end = q.D / V;
       for (int k = 0; k < 3; ++k) {
-        wide = wide && s[k] % V == 0 && s[k] / V <= (1ll << 31);
+        wide = wide && s[k] >= 0 && s[k] % V == 0 && s[k] / V <= (1ll << 31);
         end += (n[k] - 1) * (s[k] / V);
       }
       wide = wide && end < (1ll << 31);

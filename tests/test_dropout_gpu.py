@@ -1,11 +1,14 @@
 """Dropout without a stored mask on the GPU: the mask against the generator restated in numpy, element by element, and the values against
 float64; and a residual block of a recurrent layer with it."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import mlstm_kernels_b200 as mk
+from mlstm_kernels_b200 import _lib
 from oracle import gated_oracle as O
 from util_layers import TDT, check, f64, make
 
@@ -81,6 +84,17 @@ def test_strides(how, D):
     if how == "heads":   # the gradient in the heads' own layout
         assert g.transpose(1, 2).is_contiguous()
     case(x, res, dy=torch.ones((), dtype=BF16, device="cuda").expand(x.shape))
+
+
+def test_strides_below_zero_in_the_c_interface():
+    n, D = 300, 64
+    x = make(np.random.default_rng(6), n, D, dtype=BF16)
+    back, y = x.flip(0).contiguous(), torch.empty_like(x)
+    axes = lambda *s: (ctypes.c_longlong * len(s))(*s)  # noqa: E731
+    code = _lib.dtype_code(BF16)
+    assert _lib.load().mlstm_b200_dropout(back.data_ptr() + (n - 1) * D * 2, axes(0, 0, -D), None, None, y.data_ptr(), axes(0, 0, D), axes(1, 1, n, D),
+                                          0.3, SEED, None, OFFSET, code, code, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(y, mk.dropout__b200(x, 0.3, SEED, OFFSET))
 
 
 def test_seed_on_the_device():
