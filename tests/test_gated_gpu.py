@@ -1,5 +1,7 @@
 """The gated linear recurrence on the GPU, against the oracle in float64."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -83,6 +85,43 @@ def test_few_channels_and_many_tokens(B, S, D, dtype):
 @pytest.mark.parametrize("B,S,D", [(700, 3, 64), (300, 20, 70), (33, 40, 513), (1000, 1, 8)])
 def test_many_sequences(B, S, D):
     case(inputs(S, B, S, D, "bf16"), "convex")
+
+
+@pytest.mark.parametrize("B,S,D", [(513, 9, 65), (1100, 60, 33), (270000, 1, 2)])
+def test_sums_of_the_rate_s_gradient_over_many_rows(B, S, D):
+    """One, two and three passes over partial sums."""
+    case(inputs(S, B, S, D, "f32", gates="", init=False), "convex", last=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rate,scale", [(False, "convex"), (False, None), (True, "variance"), (True, "convex")])
+@pytest.mark.parametrize("gates", ["", "z", "iz"])
+@pytest.mark.parametrize("D", [96, 95])
+def test_many_units_with_every_gate(D, gates, rate, scale, dtype):
+    case(inputs(D, 2, 1123, D, dtype, gates, rate), scale)
+
+
+def test_strides_below_zero_in_the_c_interface():
+    """Tokens from the last to the first, by a stride that runs backwards."""
+    B, S, D = 2, 130, 64
+    t = inputs(3, B, S, D, "bf16", gates="", rate=False, init=False, grad=False)
+    dy = make(np.random.default_rng(4), B, S, D, dtype=BF16)
+    back = {n: v.flip(1).contiguous() for n, v in (("x", t["x"]), ("f", t["f"]), ("dy", dy))}
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    end = lambda v: v.data_ptr() + (S - 1) * D * 2  # noqa: E731
+    strides = (ctypes.c_longlong * 8)(*[S * D, -D] * 2)
+    y, ck, *grads = (torch.empty_like(t["x"]), torch.empty(lib.mlstm_b200_gated_checkpoint_bytes(B, S, D), dtype=torch.uint8, device="cuda"),
+                     torch.empty_like(dy), torch.empty_like(dy))
+    ws = torch.empty(lib.mlstm_b200_gated_workspace_bytes(B, S, D, 1), dtype=torch.uint8, device="cuda")
+    fw = lib.mlstm_b200_gated_scan_fw(end(back["x"]), end(back["f"]), None, None, None, None, strides, y.data_ptr(), None, ck.data_ptr(), ws.data_ptr(),
+                                      ws.numel(), B, S, D, 1, _lib.dtype_code(BF16), st)
+    bw = lib.mlstm_b200_gated_scan_bw(end(back["x"]), end(back["f"]), None, None, None, strides, ck.data_ptr(), end(back["dy"]),
+                                      (ctypes.c_longlong * 2)(S * D, -D), None, grads[0].data_ptr(), grads[1].data_ptr(), None, None, None, None,
+                                      ws.data_ptr(), ws.numel(), B, S, D, 1, _lib.dtype_code(BF16), st)
+    assert fw == bw == 0
+    ref = O.gated_scan(x=f64(t["x"]), f=f64(t["f"]), input_scale="convex", dy=f64(dy))
+    for got, n in zip((y, *grads), ("y", "dx", "df")):
+        check(got, ref[n], n)
 
 
 def test_strides():
