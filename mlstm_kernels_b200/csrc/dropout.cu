@@ -55,10 +55,22 @@ __device__ __forceinline__ float dropped(float v, unsigned word, const DropoutKe
 
 // V neighbouring elements to an access of 16 bytes (of the wider type), DROP_U accesses to a thread.  FLAT: all tensors lie in the
 // order of their elements; else rows of D, a multiple of V, at strides that are multiples of it.
+//
+// Memory bounds it, once the generator does not: seven rounds for four elements are 14 wide multiplications and as many three-input
+// exclusive ors.  Two bytes read and two written an element leave little for them (8 x 4096 x 2048 bf16 45 us, 5.9 TB/s); with a bf16
+// residual 61 us (6.6 TB/s), 4 x 8192 x 4096 with an f32 residual 195 (6.9), without one in 16 bits from heads' layout 53 (5.0).
 constexpr int DROP_THREADS = 256, DROP_U = 4;
 struct DropoutRows {
   Divide chunks, n2, n1;
   unsigned xs[3], rs[3], ys[3];   // strides in chunks: all tensors end below 2^31 of them
+};
+struct RowsAt {   // where chunk n lies
+  unsigned i0, i1, i2, d;
+  __device__ __forceinline__ RowsAt(const DropoutRows& rows, unsigned n) {
+    const unsigned r = rows.chunks(n), r1 = rows.n2(r);
+    d = n - r * rows.chunks.d, i2 = r - r1 * rows.n2.d, i0 = rows.n1(r1), i1 = r1 - i0 * rows.n1.d;
+  }
+  __device__ __forceinline__ unsigned operator()(const unsigned (&s)[3]) const { return i0 * s[0] + i1 * s[1] + i2 * s[2] + d; }
 };
 template <typename T, typename O, int V, bool FLAT, bool RES>
 __global__ void __launch_bounds__(DROP_THREADS, 4)
@@ -79,12 +91,10 @@ __global__ void __launch_bounds__(DROP_THREADS, 4)
         if (RES) rv[u] = load_pack<O, V>(residual + first * V + c * V);
         to[u] = y + first * V + c * V;
       } else {
-        const unsigned n = (unsigned)first + c, r = rows.chunks(n), d = n - r * rows.chunks.d, r1 = rows.n2(r), i2 = r - r1 * rows.n2.d, i0 = rows.n1(r1),
-                       i1 = r1 - i0 * rows.n1.d;
-        auto at = [&](const unsigned (&s)[3]) { return (long long)(i0 * s[0] + i1 * s[1] + i2 * s[2] + d) * V; };
-        xv[u] = load_pack<T, V>(x + at(rows.xs));
-        if (RES) rv[u] = load_pack<O, V>(residual + at(rows.rs));
-        to[u] = y + at(rows.ys);
+        const RowsAt at(rows, (unsigned)first + c);
+        xv[u] = load_pack<T, V>(x + (long long)at(rows.xs) * V);
+        if (RES) rv[u] = load_pack<O, V>(residual + (long long)at(rows.rs) * V);
+        to[u] = y + (long long)at(rows.ys) * V;
       }
     }
 #pragma unroll
@@ -120,60 +130,98 @@ __global__ void __launch_bounds__(DROP_THREADS, 4)
   }
 }
 
-// four elements to a thread, each read where it lies
-template <typename T, typename O>
-__global__ void dropout_any(const T* x, const O* residual, O* y, DropoutDims q, DropoutKey key) {
-  const long long quad = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (quad * 4 >= q.n) return;
+// For any alignment, and for p = 1: a warp hands its words round, so that neighbouring lanes have neighbouring elements.  Single elements
+// are bound by instructions: 8 x 4096 x 2048 bf16, one element off the boundary, 93 us (the kernel above 45), with a residual 101 (60), in
+// rows 140.  (Four neighbours to a thread 189 and 211; one or four times 128 elements to a warp 95 and 105.)
+constexpr int DROP_ANY = 2;   // times 128 elements to a warp
+enum class Lie { FLAT, ROWS, FAR };   // as above, the same in 32-bit offsets of elements, in 64-bit ones
+template <typename T, typename O, Lie LIE>
+__global__ void __launch_bounds__(DROP_THREADS)
+    dropout_any(const T* __restrict__ x, const O* __restrict__ residual, O* __restrict__ y, DropoutDims q, DropoutRows rows, DropoutKey key) {
+  constexpr int E = 4 * DROP_ANY;
+  using Where = std::conditional_t<LIE == Lie::ROWS, unsigned, long long>;
+  __shared__ uint4 words[DROP_THREADS];
+  const int lane = threadIdx.x & 31;
+  const long long first = ((long long)blockIdx.x * DROP_THREADS + threadIdx.x - lane) * E;   // of this warp
   const unsigned long long seed = seed_of(key);
-  const Words w = philox7((unsigned)quad, (unsigned)(quad >> 32), key.offset, (unsigned)seed, (unsigned)(seed >> 32));
-  long long d = q.D, xa = 0, ra = 0, ya = 0;
+  const unsigned* const mine = reinterpret_cast<const unsigned*>(words + threadIdx.x - lane) + lane;
+  auto work = [&](auto all) {
+    float v[E], add[E];
+    Where to[E];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const long long n = quad * 4 + j;
-    if (n >= q.n) break;
-    if (d == q.D) {   // the first, or a new row
-      const long long r = n / q.D, r1 = r / q.n2, i2 = r - r1 * q.n2, i0 = r1 / q.n1, i1 = r1 - i0 * q.n1;
-      d = n - r * q.D;
-      xa = i0 * q.xs[0] + i1 * q.xs[1] + i2 * q.xs[2];
-      ra = i0 * q.rs[0] + i1 * q.rs[1] + i2 * q.rs[2];
-      ya = i0 * q.ys[0] + i1 * q.ys[1] + i2 * q.ys[2];
+    for (int j = 0; j < E; ++j) {
+      const long long n = first + 32 * j + lane;
+      if (!decltype(all)::value && n >= q.n) break;
+      Where xa = (Where)n, ra = xa;
+      to[j] = xa;
+      if constexpr (LIE == Lie::ROWS) {
+        const RowsAt at(rows, (unsigned)n);
+        xa = at(rows.xs), ra = at(rows.rs), to[j] = at(rows.ys);
+      }
+      if constexpr (LIE == Lie::FAR) {
+        const long long r = n / q.D, d = n - r * q.D, r1 = r / q.n2, i2 = r - r1 * q.n2, i0 = r1 / q.n1, i1 = r1 - i0 * q.n1;
+        auto at = [&](const long long (&s)[3]) { return i0 * s[0] + i1 * s[1] + i2 * s[2] + d; };
+        xa = at(q.xs), ra = at(q.rs), to[j] = at(q.ys);
+      }
+      v[j] = to_f32(x[xa]);
+      add[j] = residual != nullptr ? to_f32(residual[ra]) : 0.f;
     }
-    float o = !key.some ? 0.f : dropped(to_f32(x[xa + d]), w.w[j], key);
-    if (residual != nullptr) o += to_f32(residual[ra + d]);
-    y[ya + d] = from_f32<O>(o);
-    ++d;
+#pragma unroll
+    for (int u = 0; u < DROP_ANY; ++u) {
+      const long long quad = first / 4 + 32 * u + lane;
+      const Words w = philox7((unsigned)quad, (unsigned)(quad >> 32), key.offset, (unsigned)seed, (unsigned)(seed >> 32));
+      __syncwarp();
+      words[threadIdx.x] = make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]);
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = 4 * u + k;
+        if (!decltype(all)::value && first + 32 * j + lane >= q.n) break;
+        y[to[j]] = from_f32<O>((key.some ? dropped(v[j], mine[32 * k], key) : 0.f) + add[j]);
+      }
+    }
+  };
+  if (first + 32 * E <= q.n) work(std::true_type{});
+  else work(std::false_type{});
+}
+
+// Rows in chunks of V elements; false where strides or widths are not multiples of V, or 32-bit offsets do not reach
+static bool dropout_rows(const DropoutDims& q, int V, DropoutRows& rows) {
+  if (q.D % V != 0 || q.n / V >= (1ll << 31)) return false;
+  rows = DropoutRows{divide_by(q.D / V), divide_by(q.n2), divide_by(q.n1), {}, {}, {}};
+  const long long n[3] = {q.n / (q.n1 * q.n2 * q.D), q.n1, q.n2};
+  struct { const long long* from; unsigned* to; } strides[] = {{q.xs, rows.xs}, {q.rs, rows.rs}, {q.ys, rows.ys}};
+  for (const auto& s : strides) {   // (without a residual its strides are zero)
+    long long end = q.D / V;
+    for (int k = 0; k < 3; ++k) {
+      if (s.from[k] < 0 || s.from[k] % V != 0 || s.from[k] / V > (1ll << 31)) return false;
+      end += (n[k] - 1) * (s.from[k] / V);
+      s.to[k] = (unsigned)(s.from[k] / V);
+    }
+    if (end >= (1ll << 31)) return false;
   }
+  return true;
 }
 
 template <typename T, typename O>
 static void dropout_run(const T* x, const O* residual, O* y, const DropoutDims& q, const DropoutKey& key, cudaStream_t st) {
   constexpr int V = sizeof(T) == 4 || sizeof(O) == 4 ? 4 : 8;
   const bool flat = q.n == q.D;
-  bool wide = key.some && fits_access(x, sizeof(T) * V) && fits_access(y, sizeof(O) * V) && (residual == nullptr || fits_access(residual, sizeof(O) * V));
-  if (!flat) {
-    wide = wide && q.D % V == 0 && q.n / V < (1ll << 31);
-    const long long n[3] = {q.n / (q.n1 * q.n2 * q.D), q.n1, q.n2};
-    for (const long long* s : {q.xs, q.rs, q.ys}) {   // (without a residual its strides are zero)
-      long long end = q.D / V;
-      for (int k = 0; k < 3; ++k) {
-        wide = wide && s[k] >= 0 && s[k] % V == 0 && s[k] / V <= (1ll << 31);
-        end += (n[k] - 1) * (s[k] / V);
-      }
-      wide = wide && end < (1ll << 31);
-    }
-  }
+  DropoutRows rows{};
+  const bool wide = key.some && fits_access(x, sizeof(T) * V) && fits_access(y, sizeof(O) * V) && (residual == nullptr || fits_access(residual, sizeof(O) * V)) &&
+                    (flat || dropout_rows(q, V, rows));
   if (!wide) {
-    dropout_any<T, O><<<(unsigned)((q.n + 1023) / 1024), 256, 0, st>>>(x, residual, y, q, key);
+    const long long per = 4 * DROP_ANY * DROP_THREADS;
+    auto go = [&](auto lie) {
+      dropout_any<T, O, decltype(lie)::value><<<(unsigned)((q.n + per - 1) / per), DROP_THREADS, 0, st>>>(x, residual, y, q, rows, key);
+    };
+    if (flat) go(std::integral_constant<Lie, Lie::FLAT>{});
+    else if (dropout_rows(q, 1, rows)) go(std::integral_constant<Lie, Lie::ROWS>{});
+    else go(std::integral_constant<Lie, Lie::FAR>{});
     return;
   }
   const long long chunks = (q.n + V - 1) / V, per = DROP_U * DROP_THREADS;
   const unsigned grid = (unsigned)((chunks + per - 1) / per);
-  DropoutRows rows{};
-  if (!flat) {
-    rows = DropoutRows{divide_by(q.D / V), divide_by(q.n2), divide_by(q.n1), {}, {}, {}};
-    for (int k = 0; k < 3; ++k) rows.xs[k] = (unsigned)(q.xs[k] / V), rows.rs[k] = (unsigned)(q.rs[k] / V), rows.ys[k] = (unsigned)(q.ys[k] / V);
-  }
   auto go = [&](auto f, auto r) {
     dropout_wide<T, O, V, decltype(f)::value, decltype(r)::value><<<grid, DROP_THREADS, 0, st>>>(x, residual, y, q.n, rows, key);
   };

@@ -171,6 +171,22 @@ def test_offsets_past_32_bits():
         assert np.array_equal(f64(y[at:at + 5000]) != 0, O.kept((5000,), 0.3, SEED, OFFSET, first=at)), at
 
 
+@pytest.mark.parametrize("n", [(1 << 31) - 5, (1 << 31) + (1 << 20) + 7])
+def test_offsets_past_32_bits_of_any_alignment(n):
+    x = torch.ones(n + 1, dtype=BF16, device="cuda")[1:]
+    y = mk.dropout__b200(x, 0.3, SEED, OFFSET)
+    for at in (0, (1 << 30) - 1003, n - 5000):
+        assert np.array_equal(f64(y[at:at + 5000]) != 0, O.kept((5000,), 0.3, SEED, OFFSET, first=at)), at
+
+
+@pytest.mark.parametrize("n", [1, 5, 31, 127, 128, 129, 1000, 1023, 1025, 4100])
+@pytest.mark.parametrize("dtype,residual", PAIRS)
+def test_lengths_off_the_boundary(n, dtype, residual):
+    rng = np.random.default_rng(n)
+    x = make(rng, n + 1, dtype=TDT[dtype])[1:].requires_grad_(True)
+    case(x, None if residual is None else make(rng, n + 3, dtype=TDT[residual])[3:].requires_grad_(True))
+
+
 def test_captured_with_a_seed_that_counts():
     """A captured step with its seed on the GPU: each replay another mask, the same in forward and backward."""
     rng = np.random.default_rng(4)
