@@ -1,7 +1,7 @@
 // Gated linear recurrence over sequences: forward and backward kernels of one element type (formulas: gated.cuh).
 //
 // A run of tokens acts on the state before it as h -> A h + H (A the product of its factors, H its own end state), and two runs after
-// one another as A2 A1, A2 H1 + H2.  A thread takes GATED_CK tokens of a few channels in registers, the warps of a CTA take runs that
+// one another as A2 A1, A2 H1 + H2.  A thread takes GATED_CK tokens of two channels in registers, the warps of a CTA take runs that
 // follow one another: a unit (gated_units.h).  One pass over the data: every thread reduces its run to (A, H), the CTA's last warp, which
 // takes no tokens, works out the state in front of every run, and every thread takes its tokens again out of its registers.
 //
@@ -9,12 +9,24 @@
 // for has a lower number, so that a CTA that runs has it or has done it: no unit waits for one that is not under way.  A unit
 // publishes its own (A, H) as soon as it has it; the state in front of a group of units is published by the last unit of the group
 // before.  A unit joins the runs of its group in front of it, always in that order, and takes the state in front of the group through
-// them: results do not depend on who ran when.  The last warp looks for these while the others work on their tokens.  Its waits are
-// bounded.  A value in global memory says by itself that it is there: the scratch is zero before, and +0 is
-// published as -0, so that neither fences nor flags stand between two CTAs.
+// them: results do not depend on who ran when.  The last warp looks for these while the others work on their tokens; how often it looks
+// is bounded.  A value in global memory says by itself that it is there: the scratch is zero before, and +0 is published as -0, so
+// that neither fences nor flags stand between two CTAs.
 //
 // The backward is the same in the other direction, on a_t (dyh_t + .): the forward has kept the state in front of every run, so that
 // the states are recomputed without an exchange.
+//
+// What bounds it.  Memory alone would allow 8 x 4096 x 2048 (bf16, i, rate, "variance") 87 us forward and 149 backward.  Its gates take
+// ten results of the special function units for two tokens of a channel, 80 cycles of a scheduler's for every 64 elements, 74 us in
+// all, and about 90 instructions forward, 135 backward.  Forward 163 us (3.5 TB/s) with 54 % of the issue slots and 55 % of the special
+// functions' cycles used, backward 228 (4.3 TB/s) with 55 and 38 %: 24 and 16 warps to an SM, as many as the registers hold, do not fill
+// what latencies and the two barriers of a unit leave.  With few chains the way of the states counts: 1 x 65536 x 2048, twice
+// the elements with 14 units of a chain under way at once, takes 520-560 us; a CTA has a unit for 6.4 us there instead of 3.8.
+//
+// Measured beside it, us forward / backward at 8 x 4096 x 2048: CTAs of a cluster that exchange runs through distributed shared memory
+// 207-248 / 275-513; flags with fences 215 / 360; no warp of its own for the states, eight that take tokens, 283 / 395 (spills); one barrier
+// a unit 160-173 / 300 (spills); two units at once in registers 172; four CTAs of 64 registers 179; three or five warps for tokens 189 / 335,
+// 180 / 280.
 #pragma once
 #include <algorithm>
 
@@ -261,8 +273,10 @@ __device__ __forceinline__ GatedBack gated_token_bw(const M& m, const GatedAbove
 }
 
 // ---- channels in rows of 16 bytes ----------------------------------------------------------------------
-// The operands come by asynchronous copies, a tile ahead: each warp copies its own rows of 64 channels, so that only it waits for
-// them.  Rows behind the sequence and channels behind the last are zeros.
+// The operands come by asynchronous copies, a unit ahead: each warp copies its own rows of 64 channels, so that only it waits for
+// them.  Rows behind the sequence and channels behind the last are zeros.  Three CTAs of 80 registers a thread forward, two of 128
+// backward.  Whole runs go by 32-bit offsets from a base that the warp shares, and without bounds: 171 -> 164 us forward, 260 -> 240
+// backward at 8 x 4096 x 2048; copies that pass L1 by 166 / 245.
 constexpr int GATED_STAGES = 2;
 template <typename T> struct GatedRows {
   static constexpr int CH = 64, CHUNKS = CH * (int)sizeof(T) / 16, PER = 32 / CHUNKS, E = 16 / (int)sizeof(T);   // copies of a row, rows of one instruction
@@ -542,7 +556,9 @@ template <typename T, class M> __global__ void __launch_bounds__(32 * (GATED_WAR
 }
 
 // ---- channels one by one: any width, any alignment -----------------------------------------------------
-// A lane's two channels are 32 apart, so that neighbouring lanes have neighbouring channels of any alignment.
+// A lane's two channels are 32 apart, so that neighbouring lanes have neighbouring channels of any alignment.  Which gates there are is
+// a number of the call here: there is one kernel of a type and direction.  4 x 4096 x 2049 (bf16) takes 154 us forward and 354 backward,
+// 2048 channels in rows 102 and 132: two CTAs to an SM, and loads of single elements, a few of which are under way at once.
 template <typename T> struct GatedApart {
   int c0, c1;        // where to read: the last channel for those behind it
   bool ok0, ok1;

@@ -25,7 +25,9 @@ inline GatedPlan gated_plan(int B, int S, int D, int slots) {
   p.warps = (runs + p.nt - 1) / p.nt;
   p.chains = (long long)B * p.blocks;
   p.units = p.chains * p.nt;
-  // As long as a unit's predecessors in its chain are under way beside it, groups are what keeps them from waiting for one another.
+  // As long as a unit's predecessors in its chain are under way beside it, groups are what keeps them from waiting for one another:
+  // 1 x 65536 x 2048 takes 1117, 742, 641, 606, 553 us with groups of 1, 2, 4, 8, 16, 1 x 65536 x 64 892 with 1, 75 with 16 (and 61
+  // with 32, which every unit of a group would join up to 31 runs for).  Where there are more chains than CTAs a group is two units.
   const long long beside = (slots + p.chains - 1) / p.chains;
   p.group = 1;
   while (p.group < GATED_GROUP && p.group < beside * 2 && p.group < p.nt) p.group *= 2;
