@@ -59,8 +59,8 @@ const char* mlstm_b200_last_cuda_error(void);
 long long mlstm_b200_launch_count(void);
 
 /*
- * Waits for the device to go idle and returns the status word of the tcgen05 kernels: 0, or the
- * code (> 0) of the first bounded wait that ran out (the kernel then stopped and its results are
+ * Waits for the device to go idle and returns the status word of the kernels whose waits are bounded (tcgen05; 301: the gated
+ * linear recurrence): 0, or the code (> 0) of the first such wait that ran out (the kernel then stopped and its results are
  * invalid); a negative MLSTM_ERR_* value if the query itself failed.  reset != 0 clears the word.
  */
 int mlstm_b200_device_status(int reset);

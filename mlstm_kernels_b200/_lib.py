@@ -175,7 +175,7 @@ def profile_read() -> dict:
 
 
 def device_status(reset: bool = True) -> int:
-    """Synchronise and return the status word of the tcgen05 kernels (0 = no bounded wait ran out)."""
+    """Synchronise and return the status word of the kernels whose waits are bounded (0 = none ran out)."""
     rc = int(load().mlstm_b200_device_status(1 if reset else 0))
     if rc < 0:
         check(rc, "mlstm_b200_device_status")

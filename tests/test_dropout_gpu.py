@@ -187,6 +187,18 @@ def test_lengths_off_the_boundary(n, dtype, residual):
     case(x, None if residual is None else make(rng, n + 3, dtype=TDT[residual])[3:].requires_grad_(True))
 
 
+def test_x_as_its_own_residual():
+    x = make(np.random.default_rng(2), 33, 40, dtype=BF16, grad=True)
+    y = mk.dropout__b200(x, 0.3, SEED, OFFSET, x)
+    dy = make(np.random.default_rng(3), 33, 40, dtype=BF16)
+    ref = O.dropout(f64(x), 0.3, SEED, OFFSET, f64(x), f64(dy))
+    check(y, ref["y"], "y")
+    g, = torch.autograd.grad(y, x, dy)
+    alone = x.detach().clone().requires_grad_(True)
+    d, = torch.autograd.grad(mk.dropout__b200(alone, 0.3, SEED, OFFSET), alone, dy)
+    assert torch.equal(g, d + dy)
+
+
 def test_captured_with_a_seed_that_counts():
     """A captured step with its seed on the GPU: each replay another mask, the same in forward and backward."""
     rng = np.random.default_rng(4)
