@@ -12,6 +12,7 @@
 #include "calls.h"
 #include "common.cuh"
 #include "launch.cuh"
+#include "smem_limits.h"
 
 namespace mlstm {
 
@@ -71,6 +72,17 @@ int sm_count() {
     cached[dev] = n;
   }
   return cached[dev];
+}
+
+int allow_smem(const void* kern, size_t smem) {
+  static SmemLimits limits;
+  if (smem <= 32 * 1024) return MLSTM_OK;   // 48 KB, less its static memory, is what every kernel has
+  int dev = 0;
+  MLSTM_CUDA_CHECK(cudaGetDevice(&dev));
+  return limits.allow(dev, kern, smem, [&]() -> int {
+    MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    return MLSTM_OK;
+  });
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -53,6 +53,10 @@ void set_last_cuda_error(cudaError_t e, const char* where);
 constexpr int kB200Sms = 148;
 int sm_count();
 
+// Sees that `kern` may be launched with `smem` bytes of dynamic shared memory on the current device, whatever other threads launch it
+// with (smem_limits.h): for kernels whose need depends on a call's sizes.
+int allow_smem(const void* kern, size_t smem);
+
 // every kernel launch of this library is counted (mlstm_b200_launch_count)
 void note_launch();
 #define MLSTM_LAUNCH_CHECK()                  \

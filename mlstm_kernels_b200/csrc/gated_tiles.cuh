@@ -726,7 +726,7 @@ template <typename T> __global__ void __launch_bounds__(32 * (GATED_WARPS + 1), 
 // ---- launches -----------------------------------------------------------------------------------------
 template <typename T, class M> int gated_launch(void (*kern)(GatedPtrs<T>, GatedDims, M), size_t smem, const GatedPtrs<T>& p, const GatedDims& q, M m,
                                                 cudaStream_t st) {
-  if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem((const void*)kern, smem)) return rc;
   int held = 0;
   MLSTM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, 32 * (q.warps + 1), smem));
   const long long grid = std::min((long long)q.units, (long long)std::max(held, 1) * sm_count());
