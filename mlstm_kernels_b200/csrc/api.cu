@@ -76,7 +76,7 @@ int sm_count() {
 
 int allow_smem(const void* kern, size_t smem) {
   static SmemLimits limits;
-  if (smem <= 32 * 1024) return MLSTM_OK;   // 48 KB, less its static memory, is what every kernel has
+  if (smem <= 32 * 1024) return MLSTM_OK;   // every kernel has as much, also beside its static memory
   int dev = 0;
   MLSTM_CUDA_CHECK(cudaGetDevice(&dev));
   return limits.allow(dev, kern, smem, [&]() -> int {

@@ -733,7 +733,7 @@ static int par_t(ParArgs<T>& a, bool backward, const ChunkwiseDims& d, cudaStrea
   const unsigned grid = (unsigned)(backward ? n_v + 2 * n_k : n_v) * (unsigned)(d.B * d.NH * d.NC) * (unsigned)ceil_div(d.L, TILE);
   auto kern = vec_dims(d) ? (backward ? par_bw_kernel<T, true> : par_fw_kernel<T, true>)
                           : (backward ? par_bw_kernel<T, false> : par_fw_kernel<T, false>);
-  MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem((const void*)kern, smem)) return rc;
   return launch_pdl(grid <= pdl_max_ctas(), kern, grid, NTHR, smem, st, a);
 }
 

@@ -373,7 +373,7 @@ static int step_tv(const void* q, const void* k, const void* v, const void* i, c
   const unsigned grid = (unsigned)ceil_div(DHHV, TV) * (unsigned)(B * NH);
   const size_t smem = sizeof(float) * (2 * (size_t)DHQK + (STEP_THREADS / 32) * TV);
   auto kern = step_kernel<T, TS, TV, PDL>;
-  if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem((const void*)kern, smem)) return rc;
   return launch_pdl(PDL, kern, grid, STEP_THREADS, smem, st, (const T*)q, (const T*)k, (const T*)v, i, f, gate_dtype,
                     (const TS*)c, (const TS*)n, (const TS*)m, (T*)h, (TS*)c_new, (TS*)n_new, (TS*)m_new, DHQK, DHHV, eps);
 }
@@ -421,7 +421,7 @@ int step_seq_t(const void* q, const void* k, const void* v, const void* i, const
   const unsigned sms = (unsigned)sm_count();
   const bool overlap = grid <= pdl_max_ctas() && (2 * grid <= sms || grid > sms || Tn <= 2 * SEQ_TB);
   auto kern = step_sequence_kernel<T, ROWS, FULL, TV, CTAS>;
-  if (smem > 48 * 1024) MLSTM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (int rc = allow_smem((const void*)kern, smem)) return rc;
   return launch_pdl(overlap, kern, grid, STEP_THREADS, smem, st, (const T*)q, (const T*)k, (const T*)v, i, f, gate_dtype, c, n, m,
                     (T*)h, c_new, n_new, m_new, Tn, DHQK, DHHV, eps);
 }

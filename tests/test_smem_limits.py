@@ -60,3 +60,17 @@ def test_gated_scan_takes_its_limit_from_there():
     assert not [name for name, _ in sizes_set() if name.startswith("gated")]
     with open(os.path.join(CSRC, "gated_tiles.cuh")) as f:
         assert "allow_smem((const void*)kern, smem)" in f.read()
+
+
+def test_only_sizes_that_are_constants_of_a_kernel_are_set_elsewhere():
+    """A size that is the same in every call of a kernel can be set by any thread at any time."""
+    constant = {"tensor_maps.cuh", "layer_norm.cu", "short_conv.cu", "ssm.cuh"}   # (a kernel's template arguments give it)
+    assert {name for name, _ in sizes_set()} == constant | {"api.cu"}
+    for name in ("chunkwise_simt.cu", "step.cu"):
+        with open(os.path.join(CSRC, name)) as f:
+            assert "allow_smem((const void*)kern, smem)" in f.read(), name
+    for name, call in (("layer_norm.cu", "ln_run"), ("short_conv.cu", "conv_bw_run"), ("ssm_fw.cu", "ssm_launch"), ("ssm_bw.cu", "ssm_launch")):
+        with open(os.path.join(CSRC, name)) as f:
+            src = f.read()
+        calls = len(re.findall(rf"(?<!int ){call}\(\w+<", src))
+        assert calls > 0 and len(re.findall(rf"(?<!int ){call}\(\w+<[^>]*>, [^;:]*\w+<[^>]*>::BYTES, ", src)) == calls, name

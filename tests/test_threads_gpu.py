@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import mlstm_kernels_b200 as mk
+from mlstm_kernels_b200.recurrent import mlstm_recurrent_step__b200_fw
 from util_layers import make
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +59,40 @@ def test_dropout():
         x = make(np.random.default_rng(n), 300 + n, 1024, dtype=torch.bfloat16)
         return lambda: [mk.dropout__b200(x, 0.3, n, n)]
     at_once([job(n) for n in range(4)], 200)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_portable_chunkwise_of_different_head_dims(backward):
+    def job(DHQK):
+        rng = np.random.default_rng(DHQK)
+        t = [make(rng, 1, 2, 128, n, grad=backward) for n in (DHQK, DHQK, 32)] + [make(rng, 1, 2, 128, grad=backward) for _ in range(2)]
+
+        def run():
+            h = mk.mlstm_chunkwise__b200_xl_chunk(*t, chunk_size=64, impl="simt")
+            return [h.detach(), *torch.autograd.grad(h, t, torch.ones_like(h))] if backward else [h]
+        return run
+    at_once([job(D) for D in (256, 32, 128, 64)], 100 if backward else 500)
+
+
+def step_job(DHQK):
+    rng = np.random.default_rng(DHQK)
+    q, k, v = make(rng, 1, 1, DHQK), make(rng, 1, 1, DHQK), make(rng, 1, 1, 32)
+    i, f, m = (make(rng, 1, 1, 1) for _ in range(3))
+    c, n = make(rng, 1, 1, DHQK, 32), make(rng, 1, 1, DHQK)
+
+    def run():   # (through the C interface, without the GIL)
+        h, new = mlstm_recurrent_step__b200_fw(c, n, m, q, k, v, i, f, *(torch.empty_like(t) for t in (c, n, m)), vecH_out=torch.empty_like(v), validate=False)
+        return [h, *new]
+    return run
+
+
+def test_steps_of_different_head_dims():
+    """Beyond 6000 a step's operands need more shared memory than a kernel has unasked."""
+    at_once([step_job(D) for D in (8192, 6400, 7168, 6144)], 500)
+
+
+def test_step_between_the_limits_with_and_without_static_memory():
+    """Head dims whose operands fit the 48 KB that a kernel has unasked, but not beside its static memory."""
+    for D in (6008, 6012, 6016, 6020):
+        h, c, n, m = step_job(D)()
+        assert all(torch.isfinite(t).all() for t in (h, c, n, m)) and (n != 0).any()
