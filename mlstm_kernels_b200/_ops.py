@@ -384,6 +384,7 @@ def _(x, f, i, z, rate, h_initial, input_scale, keep, want_last):
 def gated_scan_bw(x: Tensor, f: Tensor, i: Optional[Tensor], z: Optional[Tensor], rate: Optional[Tensor], h_initial: Optional[Tensor],
                   input_scale: int, checkpoints: Tensor, dy: Optional[Tensor], dh_last: Optional[Tensor]
                   ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """of h_initial only type and shape are read"""
     g = _lib.host().gated_scan_bw(x, f, i, z, rate, h_initial, input_scale, checkpoints, dy, dh_last)
     return tuple(x.new_empty((0,)) if t is None else t for t in g)
 
@@ -395,16 +396,20 @@ def _(x, f, i, z, rate, h_initial, input_scale, checkpoints, dy, dh_last):
 
 
 def _gated_setup_context(ctx, inputs, output):
-    *tensors, input_scale, keep, want_last = inputs
+    *tensors, h_initial, input_scale, keep, want_last = inputs
+    # h_initial's values are not needed, and its buffer may hold the next state before the backward runs
     ctx.save_for_backward(*tensors, output[2])
-    ctx.cfg = (input_scale, keep, want_last)
+    ctx.cfg = (input_scale, keep, want_last, None if h_initial is None else h_initial.dtype)
 
 
 def _gated_backward(ctx, dy, dh_last, _dck):
     *tensors, checkpoints = ctx.saved_tensors
-    input_scale, keep, want_last = ctx.cfg
+    input_scale, keep, want_last, h_dtype = ctx.cfg
     if not keep:
         raise RuntimeError("mlstm_b200::gated_scan: no gradient without checkpoints (keep=False)")
+    x = tensors[0]
+    # of the initial state's type and shape, without its values
+    tensors.append(None if h_dtype is None else x.new_empty((1, 1), dtype=h_dtype).expand(x.shape[0], x.shape[2]))
     grads = gated_scan_bw(*tensors, input_scale, checkpoints, dy, dh_last if want_last else None)
     return (*(None if t is None else g for t, g in zip(tensors, grads)), None, None, None)
 

@@ -57,7 +57,9 @@ Gated gated_forward(const GatedTensors& t_, bool want_last, bool keep) {
   return o;
 }
 struct GatedGrads { Tensor dx, df, di, dz, drate, dh0; };
-GatedGrads gated_backward(const GatedTensors& t_, const Tensor& ckpt, const Tensor& dy_, const Tensor& dh_last_, bool want_rate, bool want_h0) {
+// h0: the initial state's type, where its gradient is wanted (its values are not needed: the checkpoints have them)
+GatedGrads gated_backward(const GatedTensors& t_, const Tensor& ckpt, const Tensor& dy_, const Tensor& dh_last_, bool want_rate,
+                          std::optional<at::ScalarType> h0) {
   const at::Device dev = t_.x.device();
   const at::ScalarType dt = t_.x.scalar_type();
   const int B = (int)t_.x.size(0), S = (int)t_.x.size(1), D = (int)t_.x.size(2);
@@ -67,12 +69,12 @@ GatedGrads gated_backward(const GatedTensors& t_, const Tensor& ckpt, const Tens
   if (t_.i.defined()) g.di = empty(t_.x.sizes(), dt, dev);
   if (t_.z.defined()) g.dz = empty(t_.x.sizes(), dt, dev);
   if (want_rate) g.drate = empty({D}, at::kFloat, dev);
-  if (want_h0) g.dh0 = empty({B, D}, at::kFloat, dev);
+  if (h0) g.dh0 = empty({B, D}, at::kFloat, dev);
   if (t_.x.numel() == 0) {
     if (want_rate) g.drate.zero_();
-    if (want_h0) { if (dh_last_.defined()) g.dh0.copy_(dh_last_); else g.dh0.zero_(); }
+    if (h0) { if (dh_last_.defined()) g.dh0.copy_(dh_last_); else g.dh0.zero_(); }
   } else {
-    const GatedTensors t = gated_ready(t_);
+    const GatedTensors t = gated_ready({t_.x, t_.f, t_.i, t_.z, t_.rate, Tensor(), t_.scale});
     const Tensor dy = dy_.defined() ? last_dense(to_dtype(dy_, dt)) : zeros(t_.x.sizes(), dt, dev);
     const Tensor dhl = f32c(dh_last_);
     const long long gs[2] = {dy.stride(0), token_stride(dy)};
@@ -86,7 +88,7 @@ GatedGrads gated_backward(const GatedTensors& t_, const Tensor& ckpt, const Tens
           "mlstm_b200_gated_scan_bw");
   }
   if (want_rate) g.drate = to_dtype(g.drate, t_.rate.scalar_type());
-  if (want_h0) g.dh0 = to_dtype(g.dh0, t_.h0.scalar_type());
+  if (h0) g.dh0 = to_dtype(g.dh0, *h0);
   return g;
 }
 
@@ -97,9 +99,10 @@ class GatedFn : public torch::autograd::Function<GatedFn> {
                                int64_t scale, bool want_last) {
     const GatedTensors t{x, f, i.value_or(Tensor()), z.value_or(Tensor()), rate.value_or(Tensor()), h0.value_or(Tensor()), (int)scale};
     Gated o = gated_forward(t, want_last, true);
-    ctx->save_for_backward({t.x, t.f, t.i, t.z, t.rate, t.h0, o.ckpt});
+    ctx->save_for_backward({t.x, t.f, t.i, t.z, t.rate, o.ckpt});   // (not h0: its buffer may hold the next state before the backward runs)
     ctx->set_materialize_grads(false);
-    ctx->saved_data["cfg"] = std::vector<int64_t>{scale, t.rate.defined() && t.rate.requires_grad(), t.h0.defined() && t.h0.requires_grad()};
+    const bool want_h0 = t.h0.defined() && t.h0.requires_grad();
+    ctx->saved_data["cfg"] = std::vector<int64_t>{scale, t.rate.defined() && t.rate.requires_grad(), want_h0, want_h0 ? (int64_t)t.h0.scalar_type() : 0};
     if (want_last) return {o.y, o.h_last};
     return {o.y};
   }
@@ -108,8 +111,9 @@ class GatedFn : public torch::autograd::Function<GatedFn> {
     const auto s = ctx->get_saved_variables();
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
     c10::cuda::OptionalCUDAGuard guard(s[0].device());
-    const GatedTensors t{s[0], s[1], s[2], s[3], s[4], s[5], (int)cfg[0]};
-    const GatedGrads g = gated_backward(t, s[6], grads[0], grads.size() > 1 ? grads[1] : Tensor(), cfg[1] != 0, cfg[2] != 0);
+    const GatedTensors t{s[0], s[1], s[2], s[3], s[4], Tensor(), (int)cfg[0]};
+    const GatedGrads g = gated_backward(t, s[5], grads[0], grads.size() > 1 ? grads[1] : Tensor(), cfg[1] != 0,
+                                        cfg[2] != 0 ? std::optional((at::ScalarType)cfg[3]) : std::nullopt);
     return {g.dx, g.df, g.di, g.dz, g.drate, g.dh0, Tensor(), Tensor()};
   }
 };
@@ -160,7 +164,7 @@ PyObject* py_gated_scan_fw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Py_BuildValue("(NNN)", wrap(o.y), wrap(o.h_last), wrap(o.ckpt));
   END_HANDLE_TH_ERRORS
 }
-// gated_scan_bw(..., checkpoints, dy, dh_last) -> (dx, df, di, dz, drate, dh_initial), None for what was not given
+// gated_scan_bw(..., checkpoints, dy, dh_last) -> (dx, df, di, dz, drate, dh_initial), None for what was not given; h_initial's values are not read
 PyObject* py_gated_scan_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   nargs_are(n, 10);
@@ -174,7 +178,7 @@ PyObject* py_gated_scan_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     C10_THROW_ERROR(ValueError, "gated_scan__b200: checkpoints of another call");
   c10::cuda::OptionalCUDAGuard guard(t.x.device());
   at::AutoDispatchBelowADInplaceOrView below;
-  const GatedGrads g = gated_backward(t, ckpt, dy, dhl, t.rate.defined(), t.h0.defined());
+  const GatedGrads g = gated_backward(t, ckpt, dy, dhl, t.rate.defined(), t.h0.defined() ? std::optional(t.h0.scalar_type()) : std::nullopt);
   return Py_BuildValue("(NNNNNN)", wrap(g.dx), wrap(g.df), wrap(g.di), wrap(g.dz), wrap(g.drate), wrap(g.dh0));
   END_HANDLE_TH_ERRORS
 }
