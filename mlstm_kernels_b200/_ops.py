@@ -312,6 +312,7 @@ def ssm_scan_bw(x: Tensor, dt: Tensor, a: Tensor, b: Tensor, c: Tensor, skip: Op
                 dt_bias: Optional[Tensor], softplus: bool, h_initial: Optional[Tensor], checkpoints: Tensor,
                 dy: Optional[Tensor], dh_last: Optional[Tensor]
                 ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """of h_initial only type and shape are read"""
     g = _lib.host().ssm_scan_bw(x, dt, a, b, c, skip, z, dt_bias, h_initial, softplus, checkpoints, dy, dh_last)
     return tuple(x.new_empty((0,)) if t is None else t for t in g)
 
@@ -324,15 +325,18 @@ def _(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, checkpoints, dy, dh
 
 def _ssm_setup_context(ctx, inputs, output):
     x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial, keep, want_last = inputs
-    ctx.save_for_backward(x, dt, a, b, c, skip, z, dt_bias, h_initial, output[2])
-    ctx.cfg = (softplus, keep, want_last)
+    # h_initial's values are not needed, and its buffer may hold the next state before the backward runs
+    ctx.save_for_backward(x, dt, a, b, c, skip, z, dt_bias, output[2])
+    ctx.cfg = (softplus, keep, want_last, None if h_initial is None else h_initial.dtype)
 
 
 def _ssm_backward(ctx, dy, dh_last, _dck):
-    x, dt, a, b, c, skip, z, dt_bias, h_initial, checkpoints = ctx.saved_tensors
-    softplus, keep, want_last = ctx.cfg
+    x, dt, a, b, c, skip, z, dt_bias, checkpoints = ctx.saved_tensors
+    softplus, keep, want_last, h_dtype = ctx.cfg
     if not keep:
         raise RuntimeError("mlstm_b200::ssm_scan: no gradient without checkpoints (keep=False)")
+    # of the initial state's type and shape, without its values
+    h_initial = None if h_dtype is None else x.new_empty((1, 1, 1), dtype=h_dtype).expand(x.shape[0], x.shape[2], a.shape[1])
     dx, ddt, da, db, dc, dskip, dz, dbias, dh0 = ssm_scan_bw(x, dt, a, b, c, skip, z, dt_bias, softplus, h_initial,
                                                              checkpoints, dy, dh_last if want_last else None)
     return (dx, ddt, da, db, dc, None if skip is None else dskip, None if z is None else dz, None if dt_bias is None else dbias,

@@ -409,7 +409,9 @@ Scanned ssm_forward(const SsmTensors& t_, bool want_last, bool keep) {
   return o;
 }
 struct ScanGrads { Tensor dx, ddt, da, db, dc, dskip, dz, ddt_bias, dh0; };
-ScanGrads ssm_backward(const SsmTensors& t_, const Tensor& ckpt, const Tensor& dy_, const Tensor& dh_last_, bool want_skip, bool want_bias, bool want_h0) {
+// h0: the initial state's type, where its gradient is wanted (its values are not needed: the checkpoints have them)
+ScanGrads ssm_backward(const SsmTensors& t_, const Tensor& ckpt, const Tensor& dy_, const Tensor& dh_last_, bool want_skip, bool want_bias,
+                       std::optional<at::ScalarType> h0) {
   const at::Device dev = t_.x.device();
   const at::ScalarType dt = t_.x.scalar_type();
   const SsmSizes q = ssm_sizes(t_);
@@ -422,13 +424,13 @@ ScanGrads ssm_backward(const SsmTensors& t_, const Tensor& ckpt, const Tensor& d
   g.da = empty({q.D, q.N}, at::kFloat, dev);
   if (want_skip) g.dskip = empty({q.D}, at::kFloat, dev);
   if (want_bias) g.ddt_bias = empty({q.D}, at::kFloat, dev);
-  if (want_h0) g.dh0 = empty({q.B, q.D, q.N}, at::kFloat, dev);
+  if (h0) g.dh0 = empty({q.B, q.D, q.N}, at::kFloat, dev);
   if (t_.x.numel() == 0) {
     for (Tensor* p : {&g.db, &g.dc, &g.da, &g.dskip, &g.ddt_bias})
       if (p->defined()) p->zero_();
-    if (want_h0) { if (dh_last_.defined()) g.dh0.copy_(dh_last_); else g.dh0.zero_(); }
+    if (h0) { if (dh_last_.defined()) g.dh0.copy_(dh_last_); else g.dh0.zero_(); }
   } else {
-    const SsmTensors t = ssm_ready(t_);
+    const SsmTensors t = ssm_ready({t_.x, t_.dt, t_.a, t_.b, t_.c, t_.skip, t_.z, t_.dt_bias, Tensor(), t_.softplus});
     const Tensor dy = dy_.defined() ? tokens_near(to_dtype(dy_, dt)) : zeros(t_.x.sizes(), dt, dev);
     const Tensor dhl = f32c(dh_last_);
     const long long gs[2] = {dy.stride(0), token_stride(dy)};
@@ -444,7 +446,7 @@ ScanGrads ssm_backward(const SsmTensors& t_, const Tensor& ckpt, const Tensor& d
   g.da = to_dtype(g.da, t_.a.scalar_type());
   if (want_skip) g.dskip = to_dtype(g.dskip, t_.skip.scalar_type());
   if (want_bias) g.ddt_bias = to_dtype(g.ddt_bias, t_.dt_bias.scalar_type());
-  if (want_h0) g.dh0 = to_dtype(g.dh0, t_.h0.scalar_type());
+  if (h0) g.dh0 = to_dtype(g.dh0, *h0);
   return g;
 }
 
@@ -455,10 +457,12 @@ class ScanFn : public torch::autograd::Function<ScanFn> {
                                const OptT& z, const OptT& dt_bias, const OptT& h0, bool softplus, bool want_last) {
     const SsmTensors t{x, dt, a, b, c, skip.value_or(Tensor()), z.value_or(Tensor()), dt_bias.value_or(Tensor()), h0.value_or(Tensor()), softplus};
     Scanned o = ssm_forward(t, want_last, true);
-    ctx->save_for_backward({t.x, t.dt, t.a, t.b, t.c, t.skip, t.z, t.dt_bias, t.h0, o.ckpt});
+    // (not h0: its buffer may hold the next state before the backward runs)
+    ctx->save_for_backward({t.x, t.dt, t.a, t.b, t.c, t.skip, t.z, t.dt_bias, o.ckpt});
     ctx->set_materialize_grads(false);
+    const bool want_h0 = t.h0.defined() && t.h0.requires_grad();
     ctx->saved_data["cfg"] = std::vector<int64_t>{softplus, t.skip.defined() && t.skip.requires_grad(), t.dt_bias.defined() && t.dt_bias.requires_grad(),
-                                                  t.h0.defined() && t.h0.requires_grad()};
+                                                  want_h0, want_h0 ? (int64_t)t.h0.scalar_type() : 0};
     if (want_last) return {o.y, o.h_last};
     return {o.y};
   }
@@ -467,8 +471,9 @@ class ScanFn : public torch::autograd::Function<ScanFn> {
     const auto s = ctx->get_saved_variables();
     const auto cfg = ctx->saved_data["cfg"].toIntVector();
     c10::cuda::OptionalCUDAGuard guard(s[0].device());
-    const SsmTensors t{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], cfg[0] != 0};
-    const ScanGrads g = ssm_backward(t, s[9], grads[0], grads.size() > 1 ? grads[1] : Tensor(), cfg[1] != 0, cfg[2] != 0, cfg[3] != 0);
+    const SsmTensors t{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], Tensor(), cfg[0] != 0};
+    const ScanGrads g = ssm_backward(t, s[8], grads[0], grads.size() > 1 ? grads[1] : Tensor(), cfg[1] != 0, cfg[2] != 0,
+                                     cfg[3] != 0 ? std::optional((at::ScalarType)cfg[4]) : std::nullopt);
     return {g.dx, g.ddt, g.da, g.db, g.dc, g.dskip, g.dz, g.ddt_bias, g.dh0, Tensor(), Tensor()};
   }
 };
@@ -514,7 +519,8 @@ PyObject* py_ssm_scan_fw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return Py_BuildValue("(NNN)", wrap(o.y), wrap(o.h_last), wrap(o.ckpt));
   END_HANDLE_TH_ERRORS
 }
-// ssm_scan_bw(..., checkpoints, dy, dh_last) -> (dx, ddt, da, db, dc, dskip, dz, ddt_bias, dh_initial), None for what was not given
+// ssm_scan_bw(..., checkpoints, dy, dh_last) -> (dx, ddt, da, db, dc, dskip, dz, ddt_bias, dh_initial), None for what was not given;
+// h_initial's values are not read
 PyObject* py_ssm_scan_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   nargs_are(n, 13);
@@ -529,7 +535,8 @@ PyObject* py_ssm_scan_bw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     C10_THROW_ERROR(ValueError, "ssm_scan__b200: checkpoints of another call");
   c10::cuda::OptionalCUDAGuard guard(t.x.device());
   at::AutoDispatchBelowADInplaceOrView below;
-  const ScanGrads g = ssm_backward(t, ckpt, dy, dhl, t.skip.defined(), t.dt_bias.defined(), t.h0.defined());
+  const ScanGrads g = ssm_backward(t, ckpt, dy, dhl, t.skip.defined(), t.dt_bias.defined(),
+                                   t.h0.defined() ? std::optional(t.h0.scalar_type()) : std::nullopt);
   return Py_BuildValue("(NNNNNNNNN)", wrap(g.dx), wrap(g.ddt), wrap(g.da), wrap(g.db), wrap(g.dc), wrap(g.dskip), wrap(g.dz), wrap(g.ddt_bias), wrap(g.dh0));
   END_HANDLE_TH_ERRORS
 }
