@@ -3,8 +3,11 @@
 //   log a = log sigmoid(f), or rate sigmoid(f);   s = 1, 1 - a or sqrt(1 - a^2);   u = s sigmoid(i) x
 //   h_t = a_t h_{t-1} + u_t;   y_t = h_t z_t sigmoid(z_t)
 //
-// What a long recurrence remembers hangs on 1 - a: it is computed by itself, with all of f32's digits but the last two, and a near
-// one as 1 - (1 - a).  All on pairs of values, for the packed instructions.
+// 1 - a is computed by itself, with all of f32's digits but the last two, for the input's scale and the gradients, and a near one as
+// 1 - (1 - a).  The state is multiplied by a as f32 has it, off by up to 2^-25, and joined runs by products of such factors, each off by as
+// much: what a state forgets in a token is off by up to 2^-24 of the state, 2^-24 / (1 - a) of itself.  (A complement carried through
+// the runs instead would leave the state's own rounding, 2^-24 of it in every join, and lose the digits of an a near zero.)
+// All on pairs of values, for the packed instructions.
 //
 // Backward, with G_t = dL/dh_t (G_t = dy_t z_t sigmoid(z_t) + a_{t+1} G_{t+1}): everything that goes through a is
 //

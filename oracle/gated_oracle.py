@@ -110,6 +110,22 @@ def gated_scan(x, f, i=None, z=None, rate=None, h_initial=None, input_scale=None
     return r
 
 
+# ---- what a state forgets --------------------------------------------------------------------------------------------
+# Tokens of one factor a = exp(-rho).  f32 holds a to 2^-25 and products of joined runs to 2^-24 of themselves, about one to a token
+# (seven to a run of eight, some to a unit of runs): 2^-23 a token with half of that to spare; rho has 2^-20 of itself (_logistic, a
+# product and a polynomial).
+def kept_state(S, rho):
+    """What S tokens without input leave of a state of one: 1 - it, and by how much of itself that may be off."""
+    gone = -np.expm1(-S * rho)
+    return gone, S * (2.0 ** -23 + rho * 2.0 ** -20) / gone
+
+
+def constant_input(S, rho):
+    """The "convex" state after S inputs of one: its value, and by how much of itself it may be off: a token's input (2^-20), and for
+    each token that is remembered its factor and the sums, which round as often as the products."""
+    return -np.expm1(-S * rho), np.minimum(S, 1 / rho) * 2.0 ** -22 + 2.0 ** -19
+
+
 # ---- the generator --------------------------------------------------------------------------------------------------
 def philox4x32(counter, key, rounds):
     """Salmon, Moraes, Dror, Shaw, Parallel random numbers: as easy as 1, 2, 3 (2011).  counter (..., 4), key (2): 32-bit words."""
