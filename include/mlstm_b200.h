@@ -75,6 +75,14 @@ int mlstm_b200_device_status(int reset);
 int mlstm_b200_selftest_wait_expiry(unsigned int limit_polls, int code, void* stream);
 
 /*
+ * The same for the gated linear recurrence: in the next mlstm_b200_gated_scan_fw or _bw of the calling thread nobody does the first
+ * `units` (1 .. 255) units of work, and those that wait for them give up after limit_looks (1 .. 1,000,000: a second at most; counted
+ * in 256s) looks at memory.  Results of that call are invalid, and the status word is 301 where a unit has waited (sequences of one
+ * unit, up to 56 tokens, wait for nothing).  0, 0 takes it back.
+ */
+int mlstm_b200_selftest_gated_wait_expiry(unsigned int limit_looks, int units);
+
+/*
  * Per-phase device timing.  After mlstm_b200_profile_enable(1) every phase of the entry points
  * below is bracketed by CUDA events on the launching stream; mlstm_b200_profile_read() waits for
  * them, adds up the elapsed milliseconds and the number of occurrences per phase into arrays of

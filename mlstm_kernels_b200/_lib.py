@@ -31,6 +31,7 @@ SIGNATURES = {
     "mlstm_b200_launch_count": (C.c_longlong, []),
     "mlstm_b200_device_status": (_i, [_i]),
     "mlstm_b200_selftest_wait_expiry": (_i, [C.c_uint, _i, _vp]),
+    "mlstm_b200_selftest_gated_wait_expiry": (_i, [C.c_uint, _i]),
     "mlstm_b200_profile_enable": (_i, [_i]),
     "mlstm_b200_profile_phases": (_i, []),
     "mlstm_b200_profile_phase_name": (C.c_char_p, [_i]),

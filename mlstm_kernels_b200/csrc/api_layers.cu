@@ -145,6 +145,8 @@ int mlstm_b200_gated_scan_bw(const void* x, const void* f, const void* i, const 
                          dh_initial, workspace, B, S, D, input_scale, dtype, static_cast<cudaStream_t>(stream));
 }
 
+int mlstm_b200_selftest_gated_wait_expiry(unsigned int limit_looks, int units) { return gated_expiry_selftest(limit_looks, units); }
+
 int mlstm_b200_gated_step(const void* x, const void* f, const void* i, const void* z, const float* rate, const float* h, void* y, float* h_new, int B, int D,
                           int input_scale, int dtype, void* stream) {
   if (!kernel_dtype(dtype)) return MLSTM_ERR_DTYPE;

@@ -23,7 +23,8 @@
 namespace mlstm {
 
 struct GatedDims {
-  int B, S, D, nc;      // nc: kept states of a sequence.  (B is not read: without it the compiler spills in the backward with a rate, 260 us for 228.)
+  unsigned looks;       // how often a wait looks at memory, at most
+  int S, D, nc;         // nc: kept states of a sequence
   int scale;
   int warps, nt, group, groups, units;   // (gated_units.h)
   Divide chains, blocks;

@@ -107,6 +107,16 @@ static bool gated_rows(const GatedVoid& p, const long long* st, const long long*
     if (ins[k / 2] != nullptr && (st[k] % e != 0 || st[k] < 0 || (k % 2 == 1 && st[k] > (1 << 26)))) return false;
   return gs == nullptr || (gs[0] % e == 0 && gs[1] % e == 0 && gs[0] >= 0 && gs[1] >= 0 && gs[1] <= (1 << 26));
 }
+// Looks at memory of a wait: some seconds.  For tests a thread may ask that its next call waits for less, and in vain.
+constexpr unsigned GATED_LOOKS = 1u << 24;
+struct GatedExpiry { unsigned looks; int units; };
+static thread_local GatedExpiry t_expiry{0, 0};
+int gated_expiry_selftest(unsigned looks, int units) {
+  if (looks > 1000000u || units < 0 || units > 255 || (looks == 0) != (units == 0)) return MLSTM_ERR_UNSUPPORTED;
+  t_expiry = GatedExpiry{looks, units};
+  return MLSTM_OK;
+}
+
 static int gated_call(bool back, GatedVoid p, const long long* st, const long long* gs, void* scratch, int B, int S, int D, int scale, int dtype, float* drate,
                       cudaStream_t stream) {
   PhaseScope ps(PH_GATED, stream);
@@ -115,7 +125,10 @@ static int gated_call(bool back, GatedVoid p, const long long* st, const long lo
   const GatedScratch at = gated_scratch(plan, B, D, back);
   unsigned char* const base = static_cast<unsigned char*>(scratch);
   GatedDims q{};
-  q.B = B, q.S = S, q.D = D, q.scale = scale, q.nc = ceil_div(S, GATED_CK);
+  const GatedExpiry expiry = t_expiry;
+  t_expiry = GatedExpiry{0, 0};
+  q.looks = expiry.units > 0 ? expiry.looks : GATED_LOOKS;
+  q.S = S, q.D = D, q.scale = scale, q.nc = ceil_div(S, GATED_CK);
   q.warps = plan.warps, q.nt = plan.nt, q.group = plan.group, q.groups = plan.groups, q.units = (int)plan.units;
   q.chains = divide_by(plan.chains), q.blocks = divide_by(plan.blocks);
   if (plan.nt > 1) {
@@ -124,6 +137,7 @@ static int gated_call(bool back, GatedVoid p, const long long* st, const long lo
     q.state = reinterpret_cast<uint2*>(base + at.state);
     q.agg = reinterpret_cast<uint4*>(base + at.agg);
     MLSTM_CUDA_CHECK(cudaMemsetAsync(base, 0, at.rate, stream));
+    if (expiry.units > 0) MLSTM_CUDA_CHECK(cudaMemsetAsync(q.ticket, expiry.units, 1, stream));   // (its lowest byte: nobody takes the first units)
   }
   if (drate != nullptr) p.rate_parts = reinterpret_cast<float*>(base + at.rate);
   long long* const to[8] = {&q.xb, &q.xt, &q.fb, &q.ft, &q.ib, &q.it, &q.zb, &q.zt};

@@ -46,7 +46,6 @@ constexpr int GL = GATED_CK;
 // ---- units --------------------------------------------------------------------------------------------
 // Code of the first wait that ran out since it was last asked for (0: none), read by the host
 static __device__ int g_gated_status = 0;
-constexpr unsigned kGatedWaitLimit = 1u << 24;   // looks at memory: some seconds
 
 __device__ __forceinline__ uint2 look(const uint2* p) {
   uint2 v;
@@ -179,16 +178,16 @@ __device__ __forceinline__ void gated_hand_on(GatedShared& sh, const GatedDims& 
         gave = true;
       }
       find.look_again();
-      // After kGatedWaitLimit looks, or once another wait of this launch has run out, it goes on without: the results are wrong, the
+      // After q.looks of them, or once another wait of this launch has run out, it goes on without: the results are wrong, the
       // status says so, and every CTA ends.
       if (++looks % 256 == 0) {
         unsigned gone;
         asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(gone) : "l"(q.gave_up) : "memory");
-        if (looks >= kGatedWaitLimit && lane == 0) {
+        if (looks >= q.looks && lane == 0) {
           atomicExch(q.gave_up, 1u);
           atomicCAS(&g_gated_status, 0, 301);
         }
-        if (__any_sync(0xffffffffu, gone != 0 || looks >= kGatedWaitLimit)) find.have = true, find.n = find.pos;
+        if (__any_sync(0xffffffffu, gone != 0 || looks >= q.looks)) find.have = true, find.n = find.pos;
       }
     }
     uint64_t h = find.value();

@@ -128,6 +128,7 @@ bool gated_sizes_ok(int B, int S, int D);
 size_t gated_ckpt_bytes(int B, int S, int D);
 size_t gated_bytes(int B, int S, int D, bool backward);
 int gated_status(int reset, int* status);   // of its bounded waits
+int gated_expiry_selftest(unsigned looks, int units);
 int launch_gated_fw(const GatedIn& in, const long long* strides, void* y, float* h_last, float* ckpt, void* scratch, int B, int S, int D, int scale,
                     int dtype, cudaStream_t st);
 int launch_gated_bw(const GatedIn& in, const long long* strides, const float* ckpt, const void* dy, const long long* gs, const float* dh_last, void* dx,
