@@ -1,4 +1,5 @@
-// Division by a number that is known when a kernel is launched.
+// Division by a number that is known when a kernel is launched, as in Granlund and Montgomery, Division by invariant integers using
+// multiplication (1994).
 #pragma once
 #include <cuda_runtime.h>
 

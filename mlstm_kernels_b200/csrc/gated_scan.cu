@@ -61,7 +61,9 @@ __global__ void __launch_bounds__(256) gated_one(const T* x, const T* f, const T
 }
 
 // ---- calls --------------------------------------------------------------------------------------------
-static int gated_slots() { return 3 * sm_count(); }   // CTAs that run at once
+// CTAs that run at once, by which groups are cut: those of the 16-bit forward for all.  (The backward and the element-by-element kernels
+// hold two to an SM, f32 one to three: their groups are longer than what is under way.)
+static int gated_slots() { return 3 * sm_count(); }
 
 bool gated_sizes_ok(int B, int S, int D) {
   return B > 0 && S > 0 && S <= (1 << 30) && D > 0 && D <= (1 << 30) && gated_plan(B, S, D, gated_slots()).units < (1ll << 31);

@@ -16,12 +16,14 @@
 // The backward is the same in the other direction, on a_t (dyh_t + .): the forward has kept the state in front of every run, so that
 // the states are recomputed without an exchange.
 //
-// What bounds it.  Memory alone would allow 8 x 4096 x 2048 (bf16, i, rate, "variance") 87 us forward and 149 backward.  Its gates take
-// ten results of the special function units for two tokens of a channel, 80 cycles of a scheduler's for every 64 elements, 74 us in
-// all, and about 90 instructions forward, 135 backward.  Forward 163 us (3.5 TB/s) with 54 % of the issue slots and 55 % of the special
-// functions' cycles used, backward 228 (4.3 TB/s) with 55 and 38 %: 24 and 16 warps to an SM, as many as the registers hold, do not fill
-// what latencies and the two barriers of a unit leave.  With few chains the way of the states counts: 1 x 65536 x 2048, twice
-// the elements with 14 units of a chain under way at once, takes 520-560 us; a CTA has a unit for 6.4 us there instead of 3.8.
+// What bounds it: waiting.  8 x 4096 x 2048 (bf16, i, rate, "variance") takes 163 us forward (3.5 TB/s) and 228 backward (4.3), where memory
+// alone would take 87 and 149.  No unit is busy for the whole time: 54 and 55 % of the issue slots are used (about 90 and 135 instructions for 64
+// elements), 55 and 38 % of the special functions' cycles; each of these is about half of the forward's time, and they overlap.  Of
+// the resident warps' time 48 % forward and 30 % backward go to the two barriers of a unit: its warps keep their tokens in registers
+// until the states in front of them come, and have nothing else to do meanwhile.  With few chains the states take longer: 1 x
+// 65536 x 2048, twice the elements with 14 units of a chain under way at once, takes 505-560 us, 59 % of it at barriers (at 16384 tokens).
+// Tokens held in shared memory instead (of an SM's 228 KB three CTAs with i use 156 forward, two 133 backward) would let a CTA reduce its
+// next unit before the states of this one are there; that has not been built.
 //
 // Measured beside it, us forward / backward at 8 x 4096 x 2048: CTAs of a cluster that exchange runs through distributed shared memory
 // 207-248 / 275-513; flags with fences 215 / 360; no warp of its own for the states, eight that take tokens, 283 / 395 (spills); one barrier
@@ -274,7 +276,8 @@ __device__ __forceinline__ GatedBack gated_token_bw(const M& m, const GatedAbove
 // ---- channels in rows of 16 bytes ----------------------------------------------------------------------
 // The operands come by asynchronous copies, a unit ahead: each warp copies its own rows of 64 channels, so that only it waits for
 // them.  Rows behind the sequence and channels behind the last are zeros.  Three CTAs of 80 registers a thread forward, two of 128
-// backward.  Whole runs go by 32-bit offsets from a base that the warp shares, and without bounds: 171 -> 164 us forward, 260 -> 240
+// backward.  (In f32 their operands leave room for two forward with one gate and one with both, and for one backward with any: 8 x 4096 x
+// 2048 with i, rate and "variance" takes 211 us, 5.2 TB/s, and 354, 5.4.)  Whole runs go by 32-bit offsets from a base that the warp shares, and without bounds: 171 -> 164 us forward, 260 -> 240
 // backward at 8 x 4096 x 2048; copies that pass L1 by 166 / 245.
 constexpr int GATED_STAGES = 2;
 template <typename T> struct GatedRows {
