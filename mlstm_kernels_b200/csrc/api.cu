@@ -21,6 +21,9 @@ static thread_local char g_last_cuda_error[512] = "";
 void set_last_cuda_error(cudaError_t e, const char* where) {
   snprintf(g_last_cuda_error, sizeof(g_last_cuda_error), "%s: %s (%s)", cudaGetErrorName(e), cudaGetErrorString(e),
            where);
+  // The error is this call's.  Left with the runtime, the next call to ask behind its launch would take it for its own.  (An error that the
+  // context does not survive stays.)
+  (void)cudaGetLastError();
 }
 
 // ---- launch counter and phase profiler ----------------------------------------------------------
