@@ -251,7 +251,11 @@ rec_body(const CUtensorMap& mapL, const CUtensorMap& mapR, const CUtensorMap& ma
         sc[tb] = *reinterpret_cast<const float2*>(&s_scale[st][8 * tb + tok2]);
         if (BWD) sc2[tb] = *reinterpret_cast<const float2*>(&s_scale2[st][8 * tb + tok2]);
       }
-      if (!JOINT) warp_arrive(&bar_empty[st], ok);
+      // These are reads through the generic proxy, and what refills the stage writes through the async proxy: an arrival alone does not
+      // order the one before the other.  (Without the fence a first launch after its kernels had been loaded, whose warps wait for
+      // instructions between any two, found the stage's next tokens in up to one call of four.  With one ring the values have
+      // been used, and the product with them is done, before the stage can be refilled.)
+      if (!JOINT) { fence_proxy_async_smem(); warp_arrive(&bar_empty[st], ok); }
       uint32_t w[2][16];
       uint64_t ns[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
